@@ -120,6 +120,10 @@ const char* fa_error_string(int err) {
     case FA_ERR_BLOCKS:
       return "a block-sparse layout does not combine with a mask, a bias or key rows that differ "
              "from the query rows, and the backward needs block_cols with block_rows";
+    case FA_ERR_PAGES:
+      return "a paged cache needs a page size that is a power of two, positive sizes, 16-byte "
+             "aligned rows and at most 2^31 - 1 rows, and paged attention takes no option but the "
+             "format, layout, window, ALiBi slopes and scale";
     case FA_ERR_SCRATCH:
       return "fa_bwd_noalloc: 2 * B*Hq*N floats exceed the built-in scratch "
              "(FA_BWD_NOALLOC_SCRATCH_BYTES); use fa_bwd with a workspace";
@@ -556,6 +560,130 @@ int fa_segment_bounds(const void* ids, int wide, int B, int N, long long stride_
   if (!ids || !seg_start || !seg_end) return FA_ERR_NULL;
   return to_code(fa::launch_segment_bounds(ids, wide != 0, B, N, stride_b, stride_n, seg_start,
                                            seg_end, stream));
+}
+
+// The shift of a page size, or -1 where it is not a power of two.
+static int page_shift_of(int page_size) {
+  return page_size > 0 && (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Checks a paged cache's pools and fills the kernels' description of them.
+static int paged_pool(const fa_paged_cache* c, int Hkv, int D, fa::PagedPool& p) {
+  if (!fa::valid_head_dim(D)) return FA_ERR_HEAD_DIM;
+  if (Hkv <= 0) return FA_ERR_HEADS;
+  if (!c || !c->k || !c->v) return FA_ERR_NULL;
+  p.page_shift = page_shift_of(c->page_size);
+  if (p.page_shift < 0 || c->pages <= 0 || (long long)c->pages * c->page_size > INT_MAX)
+    return FA_ERR_PAGES;
+  if (!aligned16(c->k) || !aligned16(c->v) || c->stride_page < 0 || c->stride_head < 0 ||
+      c->stride_row < 0 || ((c->stride_page | c->stride_head | c->stride_row) & 7))
+    return FA_ERR_PAGES;
+  p.k = c->k;
+  p.v = c->v;
+  p.page_stride = c->stride_page;
+  p.head_stride = c->stride_head;
+  p.row_stride = c->stride_row;
+  p.pages = c->pages;
+  return FA_OK;
+}
+
+int fa_paged_tables(int* table, long long table_stride, int table_width, const int* old_len,
+                    const int* new_len, int* free_pages, int n_ring, const int* ring,
+                    int page_size, int B, int max_new, int tokens, int* slots, int* kv_len,
+                    int* ring_out, void* stream) {
+  if (B <= 0) return FA_ERR_BATCH;
+  const int shift = page_shift_of(page_size);
+  if (shift < 0 || table_width <= 0 || table_stride < table_width || n_ring <= 0 ||
+      (tokens < 0 && max_new < 0))
+    return FA_ERR_PAGES;
+  if (B > (1 << 20) || (long long)table_width * page_size > INT_MAX || n_ring > INT_MAX / 2 ||
+      (tokens < 0 && (long long)max_new * B > INT_MAX))
+    return FA_ERR_TOO_LARGE;
+  const bool no_slots = tokens == 0 || (tokens < 0 && max_new == 0);
+  if (!table || !old_len || !new_len || !free_pages || !ring || (!slots && !no_slots) || !kv_len ||
+      !ring_out)
+    return FA_ERR_NULL;
+  fa::TablesArgs a{table, table_stride, table_width, old_len, new_len, free_pages, n_ring, ring,
+                   shift, B, max_new, tokens, slots, kv_len, ring_out};
+  return to_code(fa::launch_paged_tables(a, stream));
+}
+
+int fa_paged_append(const void* k, const void* v, long long k_stride_b, long long k_stride_n,
+                    long long k_stride_h, long long v_stride_b, long long v_stride_n,
+                    long long v_stride_h, const int* slots, const fa_paged_cache* cache, int B,
+                    int N, int Hkv, int D, void* stream) {
+  fa::PagedPool pool{};
+  const int rc = paged_pool(cache, Hkv, D, pool);
+  if (rc != FA_OK) return rc;
+  if (N <= 0) return FA_ERR_SEQLEN;
+  if (B <= 0) return FA_ERR_BATCH;
+  if ((long long)B * N > INT_MAX || (long long)Hkv * D > INT_MAX) return FA_ERR_TOO_LARGE;
+  if (!k || !v || !slots) return FA_ERR_NULL;
+  if (!aligned16(k) || !aligned16(v) ||
+      ((k_stride_b | k_stride_n | k_stride_h | v_stride_b | v_stride_n | v_stride_h) & 7))
+    return FA_ERR_PAGES;
+  return to_code(fa::launch_paged_append(k, v, {k_stride_b, k_stride_n, k_stride_h},
+                                         {v_stride_b, v_stride_n, v_stride_h}, slots, pool, B, N,
+                                         Hkv, D, stream));
+}
+
+// The shapes paged attention takes: the rows of q as in a forward call.
+static int check_paged_shape(int B, int Hq, int Hkv, int N, int D) {
+  if (!fa::valid_head_dim(D)) return FA_ERR_HEAD_DIM;
+  if (N <= 0) return FA_ERR_SEQLEN;
+  if (Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0) return FA_ERR_HEADS;
+  if (B <= 0) return FA_ERR_BATCH;
+  // (rows of a request in one int; a wave or more per row in a 32-bit launch)
+  if ((long long)Hq * N > (1 << 26) || (long long)B * Hq * N > (1 << 26)) return FA_ERR_TOO_LARGE;
+  return FA_OK;
+}
+
+size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D) {
+  if (check_paged_shape(B, Hq, Hkv, N, D) != FA_OK) return 0;
+  return fa::paged_workspace_bytes(B, Hq, Hkv, N, D);
+}
+
+int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
+                  void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int N, int D,
+                  int causal, const fa_options* opts, void* stream) {
+  const fa_options& op = opts ? *opts : kDefaultOpts;
+  int rc = check_opts(op, causal, Hq, N, D, false);
+  if (rc == FA_OK) rc = check_paged_shape(B, Hq, Hkv, N, D);
+  if (rc != FA_OK) return rc;
+  if (op.kv_len || op.seg_start || op.mask || op.drop || op.bias || op.kv_rows || op.block_rows)
+    return FA_ERR_PAGES;
+  fa::PagedArgs a{};
+  rc = paged_pool(cache, Hkv, D, a.pool);
+  if (rc != FA_OK) return rc;
+  if (cache->table_width <= 0 || cache->table_stride < cache->table_width ||
+      (long long)cache->table_width * cache->page_size > INT_MAX)
+    return FA_ERR_PAGES;
+  const size_t need = fa::paged_workspace_bytes(B, Hq, Hkv, N, D);
+  if (!q || !o || !cache->table || !cache->kv_len || (need && !workspace)) return FA_ERR_NULL;
+  if (workspace_bytes < need) return FA_ERR_WORKSPACE;
+  a.q = q;
+  a.o = o;
+  a.lse = lse;
+  a.table = cache->table;
+  a.table_stride = cache->table_stride;
+  a.table_width = cache->table_width;
+  a.kv_len = cache->kv_len;
+  a.workspace = workspace;
+  a.B = B;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.N = N;
+  a.D = D;
+  a.causal = causal != 0;
+  a.stream = stream;
+  a.layout = op.layout;
+  a.dtype = op.dtype;
+  a.window = op.window;
+  a.alibi = op.alibi_slopes;
+  a.scale = op.scale;
+  return to_code(fa::launch_paged(a));
 }
 
 float fa_dropout_scale(float p) {

@@ -269,6 +269,65 @@ hipError_t launch_pack_blocks(const uint8_t* layout, int Bl, int Hl, int B, int 
 hipError_t launch_segment_bounds(const void* ids, bool wide, int B, int N, long long stride_b,
                                  long long stride_n, int* start, int* end, void* stream);
 
+// A pool of pages of K and V rows (fa_paged_cache): element (page, head, row, d)
+// at page * page_stride + head * head_stride + row * row_stride + d of either.
+struct PagedPool {
+  void* k;
+  void* v;
+  long long page_stride, head_stride, row_stride;
+  int pages, page_shift;  // (rows of a page: a power of two)
+};
+
+// Attention of the newest N tokens of B requests over their pages
+// (fa_paged_attn; arguments as FwdArgs).
+struct PagedArgs {
+  const void* q;
+  void* o;
+  float* lse;  // may be null
+  PagedPool pool;
+  const int* table;  // table_stride apart, table_width page indices each
+  long long table_stride;
+  int table_width;
+  const int* kv_len;
+  void* workspace;
+  int B, Hq, Hkv, N, D;
+  bool causal;
+  void* stream;
+  int layout = kBHND;
+  int dtype = kFP16;
+  int window = 0;
+  const float* alibi = nullptr;
+  float scale = 0.f;
+};
+size_t paged_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
+template <int W, bool BF>
+hipError_t launch_paged_w(const PagedArgs& a);
+hipError_t launch_paged(const PagedArgs& a);
+
+// Strides (elements) of the rows that fa_paged_append writes: (b, n, head).
+struct RowStrides {
+  long long b, n, h;
+};
+hipError_t launch_paged_append(const void* k, const void* v, RowStrides sk, RowStrides sv,
+                               const int* slots, const PagedPool& pool, int B, int N, int Hkv,
+                               int D, void* stream);
+// fa_paged_tables' arguments (tokens < 0: slots of max_new per request).
+struct TablesArgs {
+  int* table;
+  long long table_stride;
+  int table_width;
+  const int* old_len;
+  const int* new_len;
+  int* free_pages;
+  int n_ring;
+  const int* ring;
+  int page_shift, B, max_new, tokens;
+  int* slots;
+  int* kv_len;
+  int* ring_out;
+};
+hipError_t launch_paged_tables(const TablesArgs& a, void* stream);
+
 // Work-items (workgroups x threads) of the largest launch each pass makes for
 // a shape (either masking). An AMD dispatch packet counts its grid in
 // work-items in 32-bit fields, and the kernels number their work items with

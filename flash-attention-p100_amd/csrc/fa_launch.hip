@@ -397,6 +397,14 @@ hipError_t launch_bwd_main(const BwdArgs& a) {
   });
 }
 
+size_t paged_workspace_bytes(int, int, int, int, int) { return 0; }
+
+hipError_t launch_paged(const PagedArgs& a) {
+  return by_width(a, a.dtype == kBF16, [](auto w, auto bf, const PagedArgs& a) {
+    return launch_paged_w<decltype(w)::value, decltype(bf)::value>(a);
+  });
+}
+
 unsigned long long fwd_launch_items(int B, int Hq, int N, int D) {
   const unsigned long long tiles = ((unsigned long long)N + kFwdRows - 1) / kFwdRows;
   const unsigned long long wgs = tiles * (unsigned long long)B * (unsigned long long)Hq;

@@ -675,7 +675,206 @@ std::vector<at::Tensor> fa_dropout_bits_t(int64_t seed, double p, int64_t B, int
   return {bits, bits_t};
 }
 
+// ---------------------------------------------------------------------------
+// Paged key/value caches (fa_paged_tables, fa_paged_append, fa_paged_attn).
+
+// An int32 tensor on `dev`, contiguous along its last dimension.
+static void check_ints(const at::Tensor& t, const at::Device& dev, const char* name) {
+  TORCH_CHECK(t.device() == dev, name, " must be on ", dev);
+  TORCH_CHECK(t.scalar_type() == at::kInt, name, " must be int32");
+  TORCH_CHECK(t.dim() >= 1 && (t.size(-1) <= 1 || t.stride(-1) == 1), name,
+              " must be contiguous along its last dimension");
+}
+
+static void check_no_grad(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name,
+              " requires grad, and paged caches have no backward: call under torch.no_grad()");
+}
+
+// The stride of a dimension that is walked (one of size 1 has any stride).
+static int64_t walk(const at::Tensor& t, int64_t dim) { return t.size(dim) == 1 ? 0 : t.stride(dim); }
+
+// Whether 16-byte loads can take t's rows: dense, each on a 16-byte boundary.
+static bool rows_aligned(const at::Tensor& t) {
+  bool ok = (t.size(-1) <= 1 || t.stride(-1) == 1) && ((uintptr_t)t.data_ptr() & 15) == 0;
+  for (int64_t i = 0; i < t.dim() - 1; ++i) ok = ok && walk(t, i) % 8 == 0;
+  return ok;
+}
+
+// The cache of k_cache and v_cache, (pages, Hkv, page_size, D) in any order of
+// the first three dimensions, laid out alike; the tables are left unset.
+static fa_paged_cache paged_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& like) {
+  check_no_grad(k, "k_cache");
+  check_no_grad(v, "v_cache");
+  TORCH_CHECK(k.is_cuda() && k.device() == like.device() && v.device() == like.device(),
+              "k_cache and v_cache must be on ", like.device());
+  TORCH_CHECK(k.scalar_type() == like.scalar_type() && v.scalar_type() == like.scalar_type(),
+              "k_cache and v_cache must be ", like.scalar_type(), " as the tokens are");
+  TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes(),
+              "k_cache and v_cache must both be (pages, Hkv, page_size, D)");
+  const int64_t page_size = k.size(2);
+  TORCH_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0 && k.size(0) > 0 &&
+                  k.size(0) * page_size <= INT32_MAX,
+              "k_cache must hold 1 to 2^31 - 1 rows in pages of a power of two, got ", k.sizes());
+  bool alike = rows_aligned(k) && rows_aligned(v);
+  for (int64_t i = 0; i < 3; ++i) alike = alike && walk(k, i) == walk(v, i);
+  TORCH_CHECK(alike,
+              "k_cache and v_cache must be laid out alike, with dense rows and every row 16-byte "
+              "aligned");
+  fa_paged_cache c{};
+  c.k = k.data_ptr();
+  c.v = v.data_ptr();
+  c.stride_page = walk(k, 0);
+  c.stride_head = walk(k, 1);
+  c.stride_row = walk(k, 2);
+  c.pages = (int)k.size(0);
+  c.page_size = (int)page_size;
+  return c;
+}
+
+// [slots (B, max_new) or (tokens,), kv_len (B,), ring (2,)]; block_table and
+// free_pages in place (fa_paged_tables).
+std::vector<at::Tensor> fa_paged_tables_t(const at::Tensor& block_table, const at::Tensor& old_len,
+                                          const at::Tensor& new_len, const at::Tensor& free_pages,
+                                          const at::Tensor& ring, int64_t page_size,
+                                          const c10::optional<int64_t>& max_new,
+                                          const c10::optional<int64_t>& tokens) {
+  TORCH_CHECK(block_table.is_cuda(), "block_table must be a CUDA tensor");
+  const at::Device dev = block_table.device();
+  check_ints(block_table, dev, "block_table");
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) > 0 && block_table.size(1) > 0,
+              "block_table must be (B, pages per request)");
+  const int64_t B = block_table.size(0), M = block_table.size(1);
+  TORCH_CHECK(B == 1 || block_table.stride(0) >= M, "block_table's rows must not overlap");
+  check_ints(old_len, dev, "old_len");
+  check_ints(new_len, dev, "new_len");
+  check_ints(free_pages, dev, "free_pages");
+  check_ints(ring, dev, "ring");
+  TORCH_CHECK(old_len.dim() == 1 && old_len.size(0) == B && new_len.sizes() == old_len.sizes(),
+              "old_len and new_len must be (", B, ",)");
+  TORCH_CHECK(free_pages.dim() == 1 && free_pages.size(0) > 0 && free_pages.size(0) <= INT32_MAX / 2,
+              "free_pages must be a ring of one page index or more");
+  TORCH_CHECK(ring.dim() == 1 && ring.size(0) == 2, "ring must be (2,): head and count");
+  TORCH_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0 && M * page_size <= INT32_MAX,
+              "page_size must be a power of two, and a request's pages hold at most 2^31 - 1 tokens");
+  TORCH_CHECK(max_new.has_value() != tokens.has_value(),
+              "one of max_new (slots per request) and tokens (packed slots) must be given");
+  const int64_t want = tokens ? *tokens : *max_new;
+  TORCH_CHECK(want >= 0 && B <= (1 << 20) && (tokens ? want : want * B) <= INT32_MAX,
+              "max_new and tokens must not be negative, and the slots at most 2^31 - 1");
+  c10::DeviceGuard guard(dev);
+  const auto opts = old_len.options();
+  at::Tensor slots = tokens ? at::empty({want}, opts) : at::empty({B, want}, opts);
+  at::Tensor kv_len = at::empty({B}, opts), ring_out = at::empty({2}, opts);
+  check_rc(fa_paged_tables(block_table.data_ptr<int>(), B == 1 ? M : block_table.stride(0), (int)M,
+                           old_len.data_ptr<int>(), new_len.data_ptr<int>(),
+                           free_pages.data_ptr<int>(), (int)free_pages.size(0), ring.data_ptr<int>(),
+                           (int)page_size, (int)B, tokens ? 0 : (int)want, tokens ? (int)want : -1,
+                           slots.data_ptr<int>(), kv_len.data_ptr<int>(), ring_out.data_ptr<int>(),
+                           current_stream(block_table)),
+           "fa_paged_tables");
+  return {slots, kv_len, ring_out};
+}
+
+// k, v (T, Hkv, D) with slots (T,), or (B, Hkv, N, D) with slots (B, N), into
+// the caches (fa_paged_append).
+void fa_paged_append_t(at::Tensor k, at::Tensor v, const at::Tensor& k_cache,
+                       const at::Tensor& v_cache, at::Tensor slots) {
+  for (auto& tn : {std::make_pair(&k, "k"), std::make_pair(&v, "v")}) {
+    const at::Tensor& t = *tn.first;
+    TORCH_CHECK(t.is_cuda(), tn.second, " must be a CUDA tensor");
+    TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, tn.second,
+                " must be fp16 or bf16");
+    check_no_grad(t, tn.second);
+  }
+  TORCH_CHECK((k.dim() == 3 || k.dim() == 4) && k.sizes() == v.sizes(),
+              "k and v must both be (T, Hkv, D) or (B, Hkv, N, D)");
+  const bool flat = k.dim() == 3;  // (T, Hkv, D): T entries of one row
+  const int64_t B = k.size(0), Hkv = k.size(1), N = flat ? 1 : k.size(2), D = k.size(-1);
+  TORCH_CHECK(D >= 8 && D <= 256 && D % 8 == 0, "head dim must be a multiple of 8 from 8 to 256, got ", D);
+  TORCH_CHECK(v.device() == k.device(), "k and v must be on the same device");
+  const fa_paged_cache cache = paged_cache(k_cache, v_cache, k);
+  TORCH_CHECK(k_cache.size(1) == Hkv && k_cache.size(3) == D && v.scalar_type() == k.scalar_type(),
+              "k, v, k_cache and v_cache must have the same heads, head dim and format");
+  TORCH_CHECK(slots.device() == k.device() && slots.scalar_type() == at::kInt,
+              "slots must be int32 on ", k.device());
+  TORCH_CHECK(slots.dim() == (flat ? 1 : 2) && slots.size(0) == B && (flat || slots.size(1) == N),
+              "slots must be (T,) for k of (T, Hkv, D) and (B, N) for k of (B, Hkv, N, D)");
+  if (B * N * Hkv == 0) return;
+  c10::DeviceGuard guard(k.device());
+  if (!rows_aligned(k)) k = k.clone(at::MemoryFormat::Contiguous);
+  if (!rows_aligned(v)) v = v.clone(at::MemoryFormat::Contiguous);
+  slots = slots.contiguous();
+  check_rc(fa_paged_append(k.data_ptr(), v.data_ptr(), walk(k, 0), flat ? 0 : walk(k, 2), walk(k, 1),
+                           walk(v, 0), flat ? 0 : walk(v, 2), walk(v, 1), slots.data_ptr<int>(),
+                           &cache, (int)B, (int)N, (int)Hkv, (int)D, current_stream(k)),
+           "fa_paged_append");
+}
+
+// [o] or [o, lse]: attention of the newest N tokens over the caches
+// (fa_paged_attn). q as forward_dt's, or a (B, H, N, D) view of a dense (B, N,
+// H, D) tensor, whose layout o then has too.
+std::vector<at::Tensor> fa_paged_attn_t(at::Tensor q, const at::Tensor& k_cache,
+                                        const at::Tensor& v_cache, const at::Tensor& block_table,
+                                        const at::Tensor& kv_len, bool causal, int64_t window,
+                                        const c10::optional<at::Tensor>& alibi_slopes, double scale,
+                                        bool want_lse) {
+  check_in16(q, "q");
+  check_no_grad(q, "q");
+  fa_paged_cache cache = paged_cache(k_cache, v_cache, q);
+  const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3);
+  const int64_t Hkv = k_cache.size(1);
+  TORCH_CHECK(D >= 8 && D <= 256 && D % 8 == 0, "head dim must be a multiple of 8 from 8 to 256, got ", D);
+  TORCH_CHECK(B > 0 && N > 0, "B and N must be positive");
+  TORCH_CHECK(Hkv > 0 && H > 0 && H % Hkv == 0, "query heads (", H,
+              ") must be a multiple of key/value heads (", Hkv, ")");
+  TORCH_CHECK(k_cache.size(3) == D, "k_cache must be (pages, Hkv, page_size, ", D, ") as q's head dim is");
+  check_ints(block_table, q.device(), "block_table");
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == B && block_table.size(1) > 0 &&
+                  (B == 1 || block_table.stride(0) >= block_table.size(1)),
+              "block_table must be (", B, ", pages per request)");
+  TORCH_CHECK(block_table.size(1) * cache.page_size <= INT32_MAX,
+              "a request's pages hold at most 2^31 - 1 tokens");
+  check_ints(kv_len, q.device(), "kv_len");
+  TORCH_CHECK(kv_len.dim() == 1 && kv_len.size(0) == B, "kv_len must be (", B, ",)");
+  TORCH_CHECK(B * H * N <= (1 << 26), "shape exceeds the kernels' index range");
+  c10::DeviceGuard guard(q.device());
+  fa_options op{};
+  op.dtype = dtype_code(q);
+  op.window = (int)window;
+  op.alibi_slopes = alibi_ptr(alibi_slopes, q, (int)H);
+  op.scale = (float)scale;
+  if (!q.is_contiguous()) {
+    if (q.transpose(1, 2).is_contiguous()) op.layout = FA_LAYOUT_BNHD;
+    else q = q.contiguous();
+  }
+  if ((uintptr_t)q.data_ptr() & 15) q = q.clone();  // (keeps the strides)
+  cache.table = block_table.data_ptr<int>();
+  cache.table_stride = B == 1 ? block_table.size(1) : block_table.stride(0);
+  cache.table_width = (int)block_table.size(1);
+  cache.kv_len = kv_len.data_ptr<int>();
+  at::Tensor o = at::empty_like(q), lse, ws;
+  if (want_lse) lse = at::empty({B, H, N}, q.options().dtype(at::kFloat));
+  const size_t bytes = fa_paged_attn_workspace_bytes((int)B, (int)H, (int)Hkv, (int)N, (int)D);
+  if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check_rc(fa_paged_attn(q.data_ptr(), o.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr,
+                         &cache, bytes ? ws.data_ptr() : nullptr, bytes, (int)B, (int)H, (int)Hkv,
+                         (int)N, (int)D, causal ? 1 : 0, &op, current_stream(q)),
+           "fa_paged_attn");
+  if (want_lse) return {o, lse};
+  return {o};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("paged_tables", &fa_paged_tables_t, "Block tables and slots from request lengths",
+        py::arg("block_table"), py::arg("old_len"), py::arg("new_len"), py::arg("free_pages"),
+        py::arg("ring"), py::arg("page_size"), py::arg("max_new"), py::arg("tokens"));
+  m.def("paged_append", &fa_paged_append_t, "Writes tokens' keys and values into a paged cache",
+        py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"));
+  m.def("paged_attn", &fa_paged_attn_t, "Attention of the newest tokens over a paged cache",
+        py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"),
+        py::arg("kv_len"), py::arg("causal"), py::arg("window"), py::arg("alibi_slopes"),
+        py::arg("scale"), py::arg("want_lse"));
   m.def("dropout_bits", &fa_dropout_bits_t,
         "Dropout keep bits (B, H, N, ceil(N/32)) and their transpose for drop / drop_t",
         py::arg("seed"), py::arg("p"), py::arg("B"), py::arg("H"), py::arg("N"),

@@ -1,0 +1,222 @@
+// Paged key/value caches: the block tables and slots of a step from the
+// requests' lengths, and the writes of new rows into their slots. No counterpart
+// in the reference, which has no cache. (The attention over them: fa_paged.hip.)
+#include <algorithm>
+
+#include "fa_device.h"
+#include "fa_launch.h"
+
+namespace fa {
+namespace {
+
+// ---------------------------------------------------------------------------
+// Tables and slots. With p rows per page, request b of old and new lengths o, n
+// owns ceil(o / p) pages and wants ceil(n / p): the pages it takes are the free
+// ring's entries from head + (what the requests before it take) on, those it
+// gives back go behind the ring's last free entry likewise. Everything follows
+// from three prefix sums over the requests (pages taken, pages returned, tokens
+// added), which every workgroup computes for itself, a tile of requests at a
+// time: the lengths are a few KB in L2, and a launch apart for the sums would
+// cost more than the call. The workgroups then share the tile's pages and
+// tokens evenly, finding a page's or token's request by bisection in LDS, so one
+// long prompt is spread like many short ones. Nothing that a workgroup reads is
+// written in the launch: taken pages come from the ring (a token's slot looks
+// there too, not into the table), returned ones from table entries that no
+// taken page replaces, and the free entries they overwrite are none of the
+// ring's.
+constexpr int kTabThreads = 256;  // and requests per tile
+
+struct Sums {
+  long long need, gone, grown;  // pages to take and to return, tokens added
+};
+__device__ __forceinline__ Sums operator+(Sums a, Sums b) {
+  return {a.need + b.need, a.gone + b.gone, a.grown + b.grown};
+}
+__device__ __forceinline__ Sums shfl_up(Sums s, int d) {
+  return {__shfl_up(s.need, d), __shfl_up(s.gone, d), __shfl_up(s.grown, d)};
+}
+
+struct Request {
+  int old, have, want, capped;  // tokens and pages before, pages and tokens wanted
+  long long grown;
+  __device__ __forceinline__ Request(const TablesArgs& a, int b) : old(0), have(0), want(0), capped(0), grown(0) {
+    if (b >= a.B) return;
+    const int cap = a.table_width << a.page_shift, n = max(a.new_len[b], 0);
+    old = min(max(a.old_len[b], 0), cap);
+    capped = min(n, cap);
+    have = pages(a, old);
+    want = pages(a, capped);
+    grown = max(n - old, 0);
+  }
+  __device__ __forceinline__ static int pages(const TablesArgs& a, int len) {
+    return (int)(((unsigned)len + (1u << a.page_shift) - 1u) >> a.page_shift);
+  }
+};
+
+// The first of `n` ascending values that is greater than x (n if none is).
+__device__ __forceinline__ int first_above(const long long* v, int n, long long x) {
+  int lo = 0;
+  for (int hi = n; lo < hi;) {
+    const int mid = (lo + hi) >> 1;
+    if (v[mid] > x) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kTabThreads) void tables_kernel(const TablesArgs a) {
+  // Of the tile's requests: the sums through each, and what a token needs.
+  __shared__ long long need_end[kTabThreads], gone_end[kTabThreads], grown_end[kTabThreads];
+  __shared__ int olds[kTabThreads], haves[kTabThreads], wants[kTabThreads], lens[kTabThreads];
+  __shared__ Sums waves[kTabThreads / 64];
+  const int tid = threadIdx.x, C = a.n_ring;
+  const int head = (int)((((long long)a.ring[0] % C) + C) % C), count = min(max(a.ring[1], 0), C);
+  const int page_mask = (1 << a.page_shift) - 1;
+  const bool packed = a.tokens >= 0;
+  Sums carry{0, 0, 0};  // of the tiles before
+  // The page index at free entry i past the head.
+  auto ring_at = [&](long long i) { return (int)((head + i) % C); };
+  // This workgroup's share of n items.
+  auto share = [&](long long n, auto&& f) {
+    const long long per = (n + gridDim.x - 1) / gridDim.x, end = min(n, (blockIdx.x + 1) * per);
+    for (long long i = blockIdx.x * per + tid; i < end; i += kTabThreads) f(i);
+  };
+  // The slot of request r's (of the tile) token j, or -1.
+  auto slot_of = [&](int b, int r, long long j) {
+    if (j >= lens[r]) return -1;
+    const int p = (int)(j >> a.page_shift);
+    const long long before = r ? need_end[r - 1] : carry.need;
+    const int page = p < haves[r] ? a.table[b * a.table_stride + p]
+                                  : a.free_pages[ring_at(before + p - haves[r])];
+    const long long slot = ((long long)page << a.page_shift) + (j & page_mask);
+    return page < 0 || slot > 0x7fffffffLL ? -1 : (int)slot;
+  };
+  for (int b0 = 0; b0 < a.B; b0 += kTabThreads) {
+    const int b = b0 + tid;
+    const Request q(a, b);
+    Sums s{max(q.want - q.have, 0), max(q.have - q.want, 0), q.grown};
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const Sums t = shfl_up(s, d);
+      if ((tid & 63) >= d) s = s + t;
+    }
+    if ((tid & 63) == 63) waves[tid >> 6] = s;
+    __syncthreads();
+    s = s + carry;
+    for (int w = 0; w < (tid >> 6); ++w) s = s + waves[w];
+    need_end[tid] = s.need;
+    gone_end[tid] = s.gone;
+    grown_end[tid] = s.grown;
+    olds[tid] = q.old;
+    haves[tid] = q.have;
+    wants[tid] = q.want;
+    const int need = max(q.want - q.have, 0);
+    const int given = (int)min((long long)need, max((long long)count - (s.need - need), 0LL));
+    const long long held = ((long long)q.have + given) << a.page_shift;
+    lens[tid] = q.capped > q.old ? (int)min((long long)q.capped, held) : q.capped;
+    if (b < a.B && blockIdx.x == 0) a.kv_len[b] = lens[tid];
+    __syncthreads();
+    const int n = min(kTabThreads, a.B - b0);
+    // Pages taken, up to the free ones.
+    const long long taken = min(need_end[n - 1], (long long)count);
+    share(max(taken - carry.need, 0LL), [&](long long i) {
+      const long long x = carry.need + i;
+      const int r = first_above(need_end, n, x);
+      const int p = haves[r] + (int)(x - (r ? need_end[r - 1] : carry.need));
+      a.table[(b0 + r) * a.table_stride + p] = a.free_pages[ring_at(x)];
+    });
+    // Pages returned, as far as the ring has room.
+    share(max(min(gone_end[n - 1], (long long)(C - count)) - carry.gone, 0LL), [&](long long i) {
+      const long long x = carry.gone + i;
+      const int r = first_above(gone_end, n, x);
+      const int p = wants[r] + (int)(x - (r ? gone_end[r - 1] : carry.gone));
+      a.free_pages[ring_at(count + x)] = a.table[(b0 + r) * a.table_stride + p];
+    });
+    if (packed) {
+      share(max(min(grown_end[n - 1], (long long)a.tokens) - carry.grown, 0LL), [&](long long i) {
+        const long long x = carry.grown + i;
+        const int r = first_above(grown_end, n, x);
+        const long long first = r ? grown_end[r - 1] : carry.grown;
+        a.slots[x] = slot_of(b0 + r, r, olds[r] + (x - first));
+      });
+    } else if (a.max_new > 0) {
+      share((long long)n * a.max_new, [&](long long i) {
+        const int r = (int)((unsigned)i / (unsigned)a.max_new);
+        a.slots[(long long)b0 * a.max_new + i] = slot_of(b0 + r, r, olds[r] + (i - (long long)r * a.max_new));
+      });
+    }
+    carry = {need_end[n - 1], gone_end[n - 1], grown_end[n - 1]};
+    __syncthreads();
+  }
+  if (packed)
+    share(max(a.tokens - carry.grown, 0LL), [&](long long i) { a.slots[carry.grown + i] = -1; });
+  if (blockIdx.x == 0 && tid == 0) {
+    const long long taken = min(carry.need, (long long)count);
+    a.ring_out[0] = (int)((head + taken) % C);
+    a.ring_out[1] = (int)(count - taken + min(carry.gone, (long long)(C - count)));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Cache writes: a copy of each token's K and V rows to its slot, a thread per
+// 16-byte chunk of both. Bound by HBM at prompts, by latency at a step.
+constexpr int kAppThreads = 256;
+
+struct AppendArgs {
+  const half_t* k;
+  const half_t* v;
+  RowStrides sk, sv;
+  const int* slots;
+  PagedPool pool;
+  int N, row_chunks, chunks;  // 16-byte chunks of a row, and of a token's heads
+  long long items;            // tokens * chunks
+};
+
+__global__ __launch_bounds__(kAppThreads) void append_kernel(const AppendArgs a) {
+  const long long step = (long long)gridDim.x * kAppThreads;
+  for (long long i = (long long)blockIdx.x * kAppThreads + threadIdx.x; i < a.items; i += step) {
+    const int t = (int)(i / a.chunks), x = (int)(i - (long long)t * a.chunks);
+    const int slot = a.slots[t], page = slot >> a.pool.page_shift;
+    if (slot < 0 || page >= a.pool.pages) continue;
+    const int h = x / a.row_chunks, c = (x - h * a.row_chunks) * 8;
+    const int b = t / a.N, n = t - b * a.N;
+    const long long to = page * a.pool.page_stride + h * a.pool.head_stride +
+                         (slot - (page << a.pool.page_shift)) * a.pool.row_stride + c;
+    const u32x4 k = *reinterpret_cast<const u32x4*>(a.k + b * a.sk.b + n * a.sk.n + h * a.sk.h + c);
+    const u32x4 v = *reinterpret_cast<const u32x4*>(a.v + b * a.sv.b + n * a.sv.n + h * a.sv.h + c);
+    *reinterpret_cast<u32x4*>((half_t*)a.pool.k + to) = k;
+    *reinterpret_cast<u32x4*>((half_t*)a.pool.v + to) = v;
+  }
+}
+
+}  // namespace
+
+hipError_t launch_paged_tables(const TablesArgs& a, void* stream) {
+  // A workgroup per 1024 slots: the requests' sums are done again in each.
+  const long long slots = a.tokens >= 0 ? a.tokens : (long long)a.B * a.max_new;
+  const unsigned blocks = (unsigned)std::min(std::max(slots / 1024, 1LL), 512LL);
+  hipLaunchKernelGGL(tables_kernel, dim3(blocks), dim3(kTabThreads), 0, (hipStream_t)stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_append(const void* k, const void* v, RowStrides sk, RowStrides sv,
+                               const int* slots, const PagedPool& pool, int B, int N, int Hkv,
+                               int D, void* stream) {
+  AppendArgs a{};
+  a.k = (const half_t*)k;
+  a.v = (const half_t*)v;
+  a.sk = sk;
+  a.sv = sv;
+  a.slots = slots;
+  a.pool = pool;
+  a.N = N;
+  a.row_chunks = D / 8;
+  a.chunks = Hkv * a.row_chunks;
+  a.items = (long long)B * N * a.chunks;
+  const long long blocks = (a.items + kAppThreads - 1) / kAppThreads;
+  hipLaunchKernelGGL(append_kernel, dim3((unsigned)std::min(blocks, 1LL << 20)), dim3(kAppThreads), 0,
+                     (hipStream_t)stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace fa

@@ -479,6 +479,116 @@ def segment_bounds(segment_ids):
     return seg_start.to(torch.int32).contiguous(), seg_end.to(torch.int32).contiguous()
 
 
+def _paged_inputs(name, *tensors):
+    """Refuses what the paged entries cannot see through: a tracer, a dispatch mode,
+    a functorch transform or a tensor subclass. (A compiler breaks its graph at the
+    binding's call and runs it as it is.)"""
+    if not _is_compiling() and (_is_tracing() or is_in_torch_dispatch_mode()
+                                or _functorch_level() is not None):
+        raise RuntimeError(f"{name} writes and reads caches in place and cannot be traced or "
+                           "transformed")
+    for t in tensors:
+        if type(t) not in _PLAIN:
+            raise TypeError(f"{name} takes plain tensors, got {type(t).__name__}")
+
+
+def paged_tables(block_table, old_len, new_len, free_pages, ring, page_size, max_new=None,
+                 tokens=None):
+    """(slots, kv_len, ring) of a serving step over a paged key/value cache: pages
+    and slots for the requests' new lengths, by one HIP kernel without a copy to
+    the host.
+
+    A paged cache is a pool of pages of `page_size` rows (a power of two). Token j
+    of request b lies in row j % page_size of page block_table[b, j // page_size],
+    and its slot is that page times page_size plus that row. All tensors are int32
+    on one GPU:
+
+      * block_table (B, pages per request), updated in place: pages taken are
+        entered behind the request's own, everything else keeps its value;
+      * old_len, new_len (B,): each request's tokens before and after the step
+        (old_len clamped to what its table holds, a negative new_len is 0). A
+        request that grows takes pages, one that shrinks (a rejected draft, a
+        finished request: 0) gives pages back;
+      * free_pages (C,), updated in place: a ring of free page indices, and ring
+        (2,): its first free entry and the number of free ones. Start with
+        torch.arange(P) and [0, P) for a pool of P pages. Pages given back are
+        written behind the free ones and not taken again in the same call.
+
+    Returned: kv_len (B,), new_len as far as there were pages (in the order of the
+    requests; a request that got fewer has the tokens that its pages hold), the new
+    ring (2,), and the slots of the tokens from old_len on, -1 for tokens without
+    one: (B, max_new), token old_len[b] + i at [b, i], or, with `tokens` instead,
+    (tokens,) packed, the new tokens of one request behind those of the one
+    before (as flash_attn takes packed prompts), -1 behind the last.
+
+    Hand kv_len and ring to the next step as old_len and ring. Under HIP graph
+    capture copy them into the captured inputs (old_len.copy_(kv_len)).
+    """
+    _paged_inputs("paged_tables", block_table, old_len, new_len, free_pages, ring)
+    return tuple(_ext.paged_tables(block_table, old_len, new_len, free_pages, ring, page_size,
+                                   max_new, tokens))
+
+
+def paged_append(k, v, k_cache, v_cache, slots):
+    """Writes new tokens' keys and values into a paged cache, in place.
+
+    k and v (fp16 or bf16) are (T, Hkv, D) with slots (T,), or (B, Hkv, N, D) with
+    slots (B, N) (int32, from paged_tables; negative ones and ones past the pool
+    are left out, and each may occur once: the rows of a slot given twice are
+    undefined). k_cache and v_cache are (pages, Hkv, page_size, D) in k's
+    format, laid out alike, their first three dimensions in any order of storage
+    (a transposed view of (pages, page_size, Hkv, D), or halves of one
+    (pages, 2, Hkv, page_size, D) pool). One HIP kernel; no gradient.
+    """
+    _paged_inputs("paged_append", k, v, k_cache, v_cache, slots)
+    _ext.paged_append(k, v, k_cache, v_cache, slots)
+
+
+def paged_attn(q, k_cache, v_cache, block_table, kv_len, causal=True, sliding_window=None,
+               alibi_slopes=None, softmax_scale=None, return_lse=False):
+    """Attention of each request's newest tokens over its paged cache: o (B, Hq, N, D),
+    or (o, lse) with lse (B, Hq, N) fp32 when return_lse is set.
+
+    q (B, Hq, N, D), fp16 or bf16, holds the newest N tokens of each of B requests
+    (N = 1 for a decoding step; a few for drafted tokens checked at once):
+    row n of request b is its token kv_len[b] - N + n, whose key and value the
+    cache holds already (paged_append). k_cache and v_cache are as paged_append
+    takes them, Hq a multiple of their Hkv and D a multiple of 8 up to 256;
+    block_table (B, pages per request) and kv_len (B,), int32, are as paged_tables
+    gives them. A (B, Hq, N, D) view of a dense (B, N, Hq, D) tensor is read in
+    place and o comes back the same way.
+
+    causal, sliding_window (causal only), alibi_slopes and softmax_scale are
+    flash_attn's, counted from each row's own token; without causal every row sees
+    all of its request's tokens. A row without a key (an unused entry of the
+    batch with kv_len 0, or the first rows of one with kv_len < N) gets o = 0 and
+    lse = +inf. Keys in pages whose index is outside the pool are hidden.
+
+    The requests' keys are dealt evenly to the GPU's compute units, so a batch of
+    ragged lengths costs what its keys cost. Results are deterministic; the last
+    bits of one request may depend on the lengths of the others. No gradient.
+    """
+    _paged_inputs("paged_attn", q, k_cache, v_cache, block_table, kv_len)
+    window = 0
+    if sliding_window is not None:
+        window = int(sliding_window)
+        if window <= 0 or not causal:
+            raise ValueError("sliding_window must be positive and needs causal=True")
+    if alibi_slopes is not None:
+        if alibi_slopes.dim() != 1 or alibi_slopes.numel() != q.size(1):
+            raise ValueError(f"alibi_slopes must have shape ({q.size(1)},), got "
+                             f"{tuple(alibi_slopes.shape)}")
+        alibi_slopes = alibi_slopes.detach().float().contiguous()
+    scale = 0.0
+    if softmax_scale is not None:
+        scale = float(softmax_scale)
+        if not (scale > 0.0 and math.isfinite(scale)):
+            raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
+    out = _ext.paged_attn(q, k_cache, v_cache, block_table, kv_len, bool(causal), window,
+                          alibi_slopes, scale, return_lse)
+    return tuple(out) if return_lse else out[0]
+
+
 def _expand_kv(k, n_head):
     """Repeat each K/V head across the query heads that share it (fa_p100.py:58-62)."""
     if k.size(1) == n_head:

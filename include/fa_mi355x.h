@@ -65,9 +65,12 @@ enum {
                                 N > 2^22 or a head dim above 128 */
   FA_ERR_KV_ROWS = 10017,    /* kv_rows < 0, or kv_rows != N together with packed sequences,
                                 a mask, dropout or a bias */
-  FA_ERR_BLOCKS = 10018      /* a block-sparse layout with a mask, a bias or kv_rows != N, a
+  FA_ERR_BLOCKS = 10018,     /* a block-sparse layout with a mask, a bias or kv_rows != N, a
                                 backward without block_cols, block_cols without block_rows,
                                 or (fa_pack_blocks) layout planes not 1 or B by 1 or Hq */
+  FA_ERR_PAGES = 10019       /* a paged cache whose page size is not a power of two, whose
+                                sizes are not positive, whose rows are not 16-byte aligned, or
+                                with an option that paged attention does not take */
 };
 
 /* Memory layouts of the 16-bit tensors, for the entry points that take one:
@@ -419,6 +422,105 @@ float fa_dropout_scale(float p);
  */
 int fa_pack_blocks(const uint8_t* layout, int layout_b, int layout_h, int B, int Hq, int Hkv,
                    int N, int causal, int* block_rows, int* block_cols, void* stream);
+
+/*
+ * Paged key/value caches: the tokens of all requests lie in one pool of pages of
+ * `page_size` rows, and a table per request says which page holds which run of
+ * its tokens. Token j of request b is row j % page_size of page
+ * table[b * table_stride + j / page_size], and its slot is that page's index
+ * times page_size plus that row. No counterpart in the reference, which has no
+ * cache. A serving step is fa_paged_tables (pages and slots for the new
+ * tokens), fa_paged_append (their keys and values) and fa_paged_attn, all on one
+ * stream; none reads anything back to the host, so a step can be captured.
+ *   - k, v: the two pools, 16-byte aligned: element (page, kv head, row, d) at
+ *     page * stride_page + head * stride_head + row * stride_row + d, strides in
+ *     elements, multiples of 8 and the same for both (so (pages, Hkv, page_size,
+ *     D), (pages, page_size, Hkv, D) and pools that interleave k and v will do);
+ *   - pages, page_size: pages of the pool, and rows of a page, a power of two;
+ *     pages * page_size <= 2^31 - 1;
+ *   - table, table_stride, table_width: int32 page indices, table_width >= 1 of
+ *     them per request; table_width * page_size <= 2^31 - 1. Entries past a
+ *     request's last page are never read;
+ *   - kv_len: B int32, the tokens of each request, the newest included (values
+ *     are clamped to [0, table_width * page_size]).
+ * fa_paged_append uses the pools only, and fa_paged_tables takes its own arguments.
+ */
+typedef struct fa_paged_cache {
+  void* k;
+  void* v;
+  long long stride_page;
+  long long stride_head;
+  long long stride_row;
+  int pages;
+  int page_size;
+  const int* table;
+  long long table_stride;
+  int table_width;
+  const int* kv_len;
+} fa_paged_cache;
+
+/*
+ * Pages and slots for the lengths of this step, on the device. Request b has
+ * old_len[b] tokens in the pages of its table (clamped to [0, table_width *
+ * page_size]) and is to have new_len[b] (negative: 0): growing takes pages
+ * from the free ones, in the order of the requests, shrinking (a rejected draft,
+ * a request that ended: 0) gives pages back. `free_pages` is a ring of n_ring
+ * page indices, ring[0] its first free entry and ring[1] the number of free
+ * ones from there on (ring[0] is taken modulo n_ring, ring[1] clamped to
+ * [0, n_ring]); pages that come back are written behind them, and are not taken
+ * again in the same call. Writes
+ *   - table: the pages taken, behind the request's own (nothing else changes:
+ *     the entries of returned pages keep their values);
+ *   - kv_len[b]: new_len[b], or, where the free pages ran out or the table is
+ *     full, the tokens that the request's pages hold;
+ *   - ring_out (2 values): the ring after the call;
+ *   - slots: the slot of each token from old_len on, -1 where there is none.
+ *     With tokens < 0, max_new per request: slots[b * max_new + i] for token
+ *     old_len[b] + i. Otherwise `tokens` of them, packed: the max(new_len -
+ *     old_len, 0) new tokens of one request behind those of the one before.
+ * A call with the same inputs again gives the same results (what it overwrites
+ * it does not read), so kv_len, ring_out and slots must not overlap its inputs.
+ * B <= 2^20, max_new * B and tokens <= 2^31 - 1.
+ */
+int fa_paged_tables(int* table, long long table_stride, int table_width, const int* old_len,
+                    const int* new_len, int* free_pages, int n_ring, const int* ring,
+                    int page_size, int B, int max_new, int tokens, int* slots, int* kv_len,
+                    int* ring_out, void* stream);
+
+/*
+ * Writes rows into a paged cache: row n of entry b of k and v (fp16 or bf16
+ * alike), Hkv heads of D values, to the slot slots[b * N + n]. Element (b, n, h,
+ * d) of k is at b * k_stride_b + n * k_stride_n + h * k_stride_h + d (strides in
+ * elements, multiples of 8; k and v 16-byte aligned). Slots that are negative or
+ * past the pool are left out. Each slot may occur once; the rows of a slot given
+ * twice are undefined.
+ */
+int fa_paged_append(const void* k, const void* v, long long k_stride_b, long long k_stride_n,
+                    long long k_stride_h, long long v_stride_b, long long v_stride_n,
+                    long long v_stride_h, const int* slots, const fa_paged_cache* cache, int B,
+                    int N, int Hkv, int D, void* stream);
+
+/*
+ * Attention of the newest N tokens of each request over its paged cache (N = 1:
+ * a decoding step; a few: drafted tokens checked at once). q, o and lse as in
+ * fa_fwd_ex (lse may be NULL); row n of entry b is token kv_len[b] - N + n, whose
+ * own keys and values the cache holds already, and with `causal` it sees the
+ * keys up to itself, else all of them. Rows without a key (kv_len[b] = 0, or
+ * kv_len[b] < N: the first rows under causal masking) get o = 0, lse = +inf. Of
+ * `opts`, dtype, layout, window (counted from the row's token), alibi_slopes and
+ * scale are taken (NULL: the defaults); anything else set is refused. With a
+ * window the table entries of pages wholly outside it are not read. Keys in
+ * pages whose index is outside [0, pages) are hidden like masked ones. The keys
+ * of a batch are shared evenly among the GPU's compute units whatever their
+ * lengths; partial results meet in `workspace`, of at least
+ * fa_paged_attn_workspace_bytes() bytes (0 for invalid arguments), which may hold
+ * anything. Calls that overlap in time need workspaces of their own. The
+ * results are deterministic; a request's last bits may depend on the lengths of
+ * the others in its batch. */
+size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
+int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
+                  void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int N, int D,
+                  int causal, const fa_options* opts, void* stream);
 
 /*
  * fa_bwd without a workspace argument and without any allocation. No
