@@ -598,7 +598,7 @@ int fa_paged_tables(int* table, long long table_stride, int table_width, const i
   if (shift < 0 || table_width <= 0 || table_stride < table_width || n_ring <= 0 ||
       (tokens < 0 && max_new < 0))
     return FA_ERR_PAGES;
-  if (B > (1 << 20) || (long long)table_width * page_size > INT_MAX || n_ring > INT_MAX / 2 ||
+  if (B > (1 << 20) || (long long)table_width * page_size > (1 << 30) || n_ring > INT_MAX / 2 ||
       (tokens < 0 && (long long)max_new * B > INT_MAX))
     return FA_ERR_TOO_LARGE;
   const bool no_slots = tokens == 0 || (tokens < 0 && max_new == 0);
@@ -635,14 +635,14 @@ static int check_paged_shape(int B, int Hq, int Hkv, int N, int D) {
   if (N <= 0) return FA_ERR_SEQLEN;
   if (Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0) return FA_ERR_HEADS;
   if (B <= 0) return FA_ERR_BATCH;
-  // (rows of a request in one int; a wave or more per row in a 32-bit launch)
-  if ((long long)Hq * N > (1 << 26) || (long long)B * Hq * N > (1 << 26)) return FA_ERR_TOO_LARGE;
+  // (256 threads per 32 rows of a request's kv head in a 32-bit launch)
+  if ((long long)Hq * N > (1 << 23) || (long long)B * Hq * N > (1 << 23)) return FA_ERR_TOO_LARGE;
   return FA_OK;
 }
 
 size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D) {
   if (check_paged_shape(B, Hq, Hkv, N, D) != FA_OK) return 0;
-  return fa::paged_workspace_bytes(B, Hq, Hkv, N, D);
+  return fa::paged_workspace_bytes(D);
 }
 
 int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
@@ -658,9 +658,13 @@ int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cach
   rc = paged_pool(cache, Hkv, D, a.pool);
   if (rc != FA_OK) return rc;
   if (cache->table_width <= 0 || cache->table_stride < cache->table_width ||
-      (long long)cache->table_width * cache->page_size > INT_MAX)
+      (long long)cache->table_width * cache->page_size > (1 << 30))
     return FA_ERR_PAGES;
-  const size_t need = fa::paged_workspace_bytes(B, Hq, Hkv, N, D);
+  // The key blocks of all row tiles are counted in 32 bits.
+  const long long tiles = (long long)B * Hkv * (((long long)Hq / Hkv * N + 31) / 32);
+  if (tiles * ((long long)cache->table_width * cache->page_size / 32 + 2) > (1 << 30))
+    return FA_ERR_TOO_LARGE;
+  const size_t need = fa::paged_workspace_bytes(D);
   if (!q || !o || !cache->table || !cache->kv_len || (need && !workspace)) return FA_ERR_NULL;
   if (workspace_bytes < need) return FA_ERR_WORKSPACE;
   a.q = q;

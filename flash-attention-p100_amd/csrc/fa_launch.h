@@ -299,7 +299,9 @@ struct PagedArgs {
   const float* alibi = nullptr;
   float scale = 0.f;
 };
-size_t paged_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
+size_t paged_workspace_bytes(int D);
+template <int W, bool BF>
+size_t paged_workspace_w();
 template <int W, bool BF>
 hipError_t launch_paged_w(const PagedArgs& a);
 hipError_t launch_paged(const PagedArgs& a);

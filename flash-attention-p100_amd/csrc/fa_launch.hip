@@ -397,7 +397,16 @@ hipError_t launch_bwd_main(const BwdArgs& a) {
   });
 }
 
-size_t paged_workspace_bytes(int, int, int, int, int) { return 0; }
+size_t paged_workspace_bytes(int D) {
+  FwdArgs a{};
+  a.D = D;
+  size_t n = 0;
+  (void)by_width(a, false, [&](auto w, auto bf, const FwdArgs&) {
+    n = paged_workspace_w<decltype(w)::value, decltype(bf)::value>();
+    return hipSuccess;
+  });
+  return n;
+}
 
 hipError_t launch_paged(const PagedArgs& a) {
   return by_width(a, a.dtype == kBF16, [](auto w, auto bf, const PagedArgs& a) {

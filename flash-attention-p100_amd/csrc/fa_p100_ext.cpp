@@ -755,8 +755,8 @@ std::vector<at::Tensor> fa_paged_tables_t(const at::Tensor& block_table, const a
   TORCH_CHECK(free_pages.dim() == 1 && free_pages.size(0) > 0 && free_pages.size(0) <= INT32_MAX / 2,
               "free_pages must be a ring of one page index or more");
   TORCH_CHECK(ring.dim() == 1 && ring.size(0) == 2, "ring must be (2,): head and count");
-  TORCH_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0 && M * page_size <= INT32_MAX,
-              "page_size must be a power of two, and a request's pages hold at most 2^31 - 1 tokens");
+  TORCH_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0 && M * page_size <= (1 << 30),
+              "page_size must be a power of two, and a request's pages hold at most 2^30 tokens");
   TORCH_CHECK(max_new.has_value() != tokens.has_value(),
               "one of max_new (slots per request) and tokens (packed slots) must be given");
   const int64_t want = tokens ? *tokens : *max_new;
@@ -833,11 +833,11 @@ std::vector<at::Tensor> fa_paged_attn_t(at::Tensor q, const at::Tensor& k_cache,
   TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == B && block_table.size(1) > 0 &&
                   (B == 1 || block_table.stride(0) >= block_table.size(1)),
               "block_table must be (", B, ", pages per request)");
-  TORCH_CHECK(block_table.size(1) * cache.page_size <= INT32_MAX,
-              "a request's pages hold at most 2^31 - 1 tokens");
+  TORCH_CHECK(block_table.size(1) * cache.page_size <= (1 << 30),
+              "a request's pages hold at most 2^30 tokens");
   check_ints(kv_len, q.device(), "kv_len");
   TORCH_CHECK(kv_len.dim() == 1 && kv_len.size(0) == B, "kv_len must be (", B, ",)");
-  TORCH_CHECK(B * H * N <= (1 << 26), "shape exceeds the kernels' index range");
+  TORCH_CHECK(B * H * N <= (1 << 23), "shape exceeds the kernels' index range");
   c10::DeviceGuard guard(q.device());
   fa_options op{};
   op.dtype = dtype_code(q);

@@ -439,7 +439,7 @@ int fa_pack_blocks(const uint8_t* layout, int layout_b, int layout_h, int B, int
  *   - pages, page_size: pages of the pool, and rows of a page, a power of two;
  *     pages * page_size <= 2^31 - 1;
  *   - table, table_stride, table_width: int32 page indices, table_width >= 1 of
- *     them per request; table_width * page_size <= 2^31 - 1. Entries past a
+ *     them per request; table_width * page_size <= 2^30. Entries past a
  *     request's last page are never read;
  *   - kv_len: B int32, the tokens of each request, the newest included (values
  *     are clamped to [0, table_width * page_size]).
@@ -480,7 +480,7 @@ typedef struct fa_paged_cache {
  *     old_len, 0) new tokens of one request behind those of the one before.
  * A call with the same inputs again gives the same results (what it overwrites
  * it does not read), so kv_len, ring_out and slots must not overlap its inputs.
- * B <= 2^20, max_new * B and tokens <= 2^31 - 1.
+ * B <= 2^20, max_new * B and tokens <= 2^31 - 1, table_width * page_size <= 2^30.
  */
 int fa_paged_tables(int* table, long long table_stride, int table_width, const int* old_len,
                     const int* new_len, int* free_pages, int n_ring, const int* ring,
@@ -514,8 +514,9 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
  * of a batch are shared evenly among the GPU's compute units whatever their
  * lengths; partial results meet in `workspace`, of at least
  * fa_paged_attn_workspace_bytes() bytes (0 for invalid arguments), which may hold
- * anything. Calls that overlap in time need workspaces of their own. The
- * results are deterministic; a request's last bits may depend on the lengths of
+ * anything. Calls that overlap in time need workspaces of their own. B * Hq * N <=
+ * 2^23, and the 32-key blocks of full tables, times Hkv and the 32-row tiles of Hq /
+ * Hkv * N, at most 2^30. The results are deterministic; a request's last bits may depend on the lengths of
  * the others in its batch. */
 size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
 int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
