@@ -580,6 +580,8 @@ static int paged_pool(const fa_paged_cache* c, int Hkv, int D, fa::PagedPool& p)
   if (!aligned16(c->k) || !aligned16(c->v) || c->stride_page < 0 || c->stride_head < 0 ||
       c->stride_row < 0 || ((c->stride_page | c->stride_head | c->stride_row) & 7))
     return FA_ERR_PAGES;
+  // (pages and rows are found by products of 32 bits)
+  if (c->stride_page >= 1LL << 31 || c->stride_row >= 1LL << 31) return FA_ERR_TOO_LARGE;
   p.k = c->k;
   p.v = c->v;
   p.page_stride = c->stride_page;
@@ -635,14 +637,13 @@ static int check_paged_shape(int B, int Hq, int Hkv, int N, int D) {
   if (N <= 0) return FA_ERR_SEQLEN;
   if (Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0) return FA_ERR_HEADS;
   if (B <= 0) return FA_ERR_BATCH;
-  // (256 threads per 32 rows of a request's kv head in a 32-bit launch)
-  if ((long long)Hq * N > (1 << 23) || (long long)B * Hq * N > (1 << 23)) return FA_ERR_TOO_LARGE;
+  if ((long long)Hq * N > (1 << 24)) return FA_ERR_TOO_LARGE;  // (rows of a request in an int)
   return FA_OK;
 }
 
 size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D) {
   if (check_paged_shape(B, Hq, Hkv, N, D) != FA_OK) return 0;
-  return fa::paged_workspace_bytes(D);
+  return fa::paged_workspace_bytes(Hq / Hkv * N, D);
 }
 
 int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
@@ -664,7 +665,7 @@ int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cach
   const long long tiles = (long long)B * Hkv * (((long long)Hq / Hkv * N + 31) / 32);
   if (tiles * ((long long)cache->table_width * cache->page_size / 32 + 2) > (1 << 30))
     return FA_ERR_TOO_LARGE;
-  const size_t need = fa::paged_workspace_bytes(D);
+  const size_t need = fa::paged_workspace_bytes(Hq / Hkv * N, D);
   if (!q || !o || !cache->table || !cache->kv_len || (need && !workspace)) return FA_ERR_NULL;
   if (workspace_bytes < need) return FA_ERR_WORKSPACE;
   a.q = q;

@@ -270,7 +270,7 @@ __device__ __forceinline__ void lds_direct_buf(void* lds, rsrc_t r, uint32_t vof
 //
 // Row r occupies 2*D contiguous bytes and keeps its 16-byte chunk c at position
 // c ^ g(r), where g permutes the low row bits:
-//   D = 128 (a row spans all 16 bank groups): g(r) = perm16(r & 15);
+//   D = 128, 256 (a row spans all 16 bank groups): g(r) = perm16(r & 15);
 //   D = 64 (two rows per 256 bytes): g(r) = ((r >> 1) & 1) << 2 | (r >> 2) & 3.
 // The 16-byte operand reads (16 consecutive rows at one chunk) and the
 // transpose reads (per half-wave: 4 consecutive rows x 4 consecutive chunks)
@@ -285,7 +285,7 @@ struct Swz {
   static constexpr int kRowBytes = 2 * D;
   static constexpr int kRowsPerInst = 1024 / kRowBytes;
   __host__ __device__ static constexpr int g(int r) {
-    return D == 128 ? perm16(r & 15) : ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
+    return D >= 128 ? perm16(r & 15) : ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
   }
   template <int ROWS>
   static constexpr int bytes() { return ROWS * kRowBytes; }

@@ -299,9 +299,10 @@ struct PagedArgs {
   const float* alibi = nullptr;
   float scale = 0.f;
 };
-size_t paged_workspace_bytes(int D);
+// rows: of a kv head (Hq / Hkv * N).
+size_t paged_workspace_bytes(int rows, int D);
 template <int W, bool BF>
-size_t paged_workspace_w();
+size_t paged_workspace_w(int rows);
 template <int W, bool BF>
 hipError_t launch_paged_w(const PagedArgs& a);
 hipError_t launch_paged(const PagedArgs& a);

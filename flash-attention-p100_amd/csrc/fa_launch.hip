@@ -397,12 +397,12 @@ hipError_t launch_bwd_main(const BwdArgs& a) {
   });
 }
 
-size_t paged_workspace_bytes(int D) {
+size_t paged_workspace_bytes(int rows, int D) {
   FwdArgs a{};
   a.D = D;
   size_t n = 0;
   (void)by_width(a, false, [&](auto w, auto bf, const FwdArgs&) {
-    n = paged_workspace_w<decltype(w)::value, decltype(bf)::value>();
+    n = paged_workspace_w<decltype(w)::value, decltype(bf)::value>(rows);
     return hipSuccess;
   });
   return n;

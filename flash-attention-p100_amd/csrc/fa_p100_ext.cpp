@@ -837,7 +837,7 @@ std::vector<at::Tensor> fa_paged_attn_t(at::Tensor q, const at::Tensor& k_cache,
               "a request's pages hold at most 2^30 tokens");
   check_ints(kv_len, q.device(), "kv_len");
   TORCH_CHECK(kv_len.dim() == 1 && kv_len.size(0) == B, "kv_len must be (", B, ",)");
-  TORCH_CHECK(B * H * N <= (1 << 23), "shape exceeds the kernels' index range");
+  TORCH_CHECK(B <= INT32_MAX && H * N <= (1 << 24), "shape exceeds the kernels' index range");
   c10::DeviceGuard guard(q.device());
   fa_options op{};
   op.dtype = dtype_code(q);

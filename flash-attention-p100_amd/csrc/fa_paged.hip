@@ -9,15 +9,19 @@
 // different is where the keys are and how they are dealt out:
 //   * the lengths are known on the device only, and differ. So all key blocks of
 //     the call, request after request, kv head after kv head, tile after tile, lie
-//     on one line, which the workgroups divide evenly: each finds its stretch from
-//     the sum of the lengths, walks the items (a row tile of a request's kv head)
-//     in it, and writes the result of an item that it has whole; the parts of the
-//     others meet in paged_merge_kernel. No workgroup waits for a longer one;
+//     on one line, which the waves divide evenly: each finds its stretch from the
+//     sum of the lengths, walks the items (a row tile of a request's kv head) in
+//     it, and writes the result of an item that it has whole; the parts of the
+//     others meet in paged_merge_kernel. No wave waits for a longer request. Where
+//     a workgroup's stretch lies within one item, its waves' parts meet in LDS
+//     first: long requests then leave an eighth of the parts;
 //   * a wave's lanes hold the next 64 page indices of its stretch; a block's rows
 //     take theirs from there by a lane permutation, so the table is read once in
 //     64 pages and the K/V loads (direct to LDS, an address per lane) wait for
 //     nothing. Rows outside the request's keys read one of its rows instead: a
 //     masked key's P is zero, but zero times what an unused row holds may be NaN.
+#include <type_traits>
+
 #include "fa_device.h"
 #include "fa_launch.h"
 
@@ -31,18 +35,21 @@ template <int D>
 struct Paged {
   static constexpr int kWaves = D > 128 ? 4 : 8;
   static constexpr int kThreads = 64 * kWaves;
-  using S = Stream<D>;
+  static constexpr bool kSwz = kSwizzled<D> || D == 256;
+  using S = std::conditional_t<kSwz, Swz<D>, Pad<D>>;
   static constexpr int kParts = (S::template bytes<kKeys>() + 1023) / 1024;  // loads of a tile
   static constexpr int kTileBytes = kParts * 1024;
   static constexpr int kFloats = kRows * D;  // a partial O
   // Workgroups that share a CU's 160 KB of LDS.
   static constexpr int kPerCu = kWaves * kTileBytes * 2 > 80 * 1024 ? 1 : 2;
   static constexpr int kGrid = kCUs * kPerCu;
+  // The least stretch whose waves meet in LDS.
+  static constexpr int kJoinFrom = 4;
   static_assert(kWaves / 2 * kFloats * 4 <= kWaves * kTileBytes, "merge area exceeds the tiles");
 
   // The row and 16-byte chunk that lane `lane` of load u brings in.
   __device__ __forceinline__ static void place(int u, int lane, int& row, int& chunk) {
-    if constexpr (kSwizzled<D>) {
+    if constexpr (kSwz) {
       row = S::kRowsPerInst * u + lane / S::kChunks;
       chunk = (lane % S::kChunks) ^ S::g(row);
     } else {
@@ -65,10 +72,14 @@ struct PagedKernelArgs {
   long long table_stride;
   int cap;  // tokens that a table holds
   const int* kv_len;
-  float* part_o;    // (workgroup, 2) x kRows x D: unscaled partial O
-  float2* part_ml;  // (workgroup, 2) x kRows: running max (log2 units), row sum
+  float* part_o;    // (wave, 2) x part_rows x D: unscaled partial O
+  float2* part_ml;  // (wave, 2) x part_rows: running max (log2 units), row sum
+  int4* owned;      // (wave): the item that it begins and does not end (see Owned)
+  int* sizes;       // Line's stretch and total
+  int part_rows;    // of a tile: kRows, or all of a kv head's
   int B, Hq, group, N, n_tiles, heads_tiles, causal, window, dr;
-  float scale_log2;
+  int runs;  // of 64 float4 columns in a tile's rows
+  float scale_log2, rescale, alibi_unit;  // (the last two in units of q . k)
   const float* alibi;
   Strides stq;
 };
@@ -85,59 +96,87 @@ struct Keys {
   }
 };
 
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  return x;
-}
-__device__ __forceinline__ int wave_prefix(int x, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  return x;
-}
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
-// Blocks that a workgroup takes of `total`: a round of its waves at least.
-template <int D>
-__device__ __forceinline__ int share_of(int total) {
-  return max(Paged<D>::kWaves, (total + Paged<D>::kGrid - 1) / Paged<D>::kGrid);
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int plus_dpp(int x) {  // x + the lane that CTRL names (none: 0)
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+// The sum over the lanes up to each.
+__device__ __forceinline__ int wave_prefix(int x) {
+  x = plus_dpp<0x111, 0xf>(x);  // 1, 2, 4 and 8 lanes before, within rows of 16
+  x = plus_dpp<0x112, 0xf>(x);
+  x = plus_dpp<0x114, 0xf>(x);
+  x = plus_dpp<0x118, 0xf>(x);
+  x = plus_dpp<0x142, 0xa>(x);  // row 0's last lane to row 1, 2's to 3
+  return plus_dpp<0x143, 0xc>(x);  // row 1's last lane to rows 2 and 3
 }
 
-// Where the line's position `pos` lies: request b, which begins at `start`. The
-// lanes sum runs of `per` requests each, then look at the run that holds pos.
-// Sets the line's length; false when pos is past it.
+// The line of key blocks and its division. A request's items are equally long.
 template <int D>
-__device__ __forceinline__ bool locate(const PagedKernelArgs& a, int lane, int wg, int& pos,
-                                       int& end, int& b, int& start) {
-  const int per = (a.B + 63) / 64;
-  int mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int c = lane * per + i;
-    if (c < a.B) mine += Keys(a, a.kv_len[c]).blocks * a.heads_tiles;
-  }
-  const int through = wave_prefix(mine, lane), total = uniform(__shfl(through, 63));
-  const int share = share_of<D>(total);
-  pos = wg * share;
-  if (pos >= total) return false;
-  end = min(pos + share, total);
-  const int run = 63 - __clzll(__ballot(through - mine <= pos));
-  start = uniform(__shfl(through - mine, run));
-  for (int c0 = run * per;; c0 += 64) {
-    const int c = c0 + lane;
-    const int x = c < min(a.B, (run + 1) * per) ? Keys(a, a.kv_len[c]).blocks * a.heads_tiles : 0;
-    const int sum = wave_prefix(x, lane), all = uniform(__shfl(sum, 63));
-    if (pos < start + all) {
-      const int l = __ffsll(__ballot(start + sum > pos)) - 1;
-      b = uniform(c0 + l);
-      start = uniform(start + __shfl(sum - x, l));
-      return true;
+struct Line {
+  using T = Paged<D>;
+  const PagedKernelArgs& a;
+  const int lane;
+  int lens, c0;      // kv_len of the requests c0 + lane (c0 < 0: none yet)
+  int per, through;  // blocks of the requests up to (lane + 1) * per
+  int total, stretch;  // all blocks, and those of a workgroup
+
+  __device__ __forceinline__ Line(const PagedKernelArgs& a, int lane)
+      : a(a), lane(lane), lens(0), c0(a.B > 64 ? -64 : 0), per((a.B + 63) / 64) {
+    int mine = 0;
+    for (int i = 0; i < per; ++i) {
+      const int c = lane * per + i;
+      if (c < a.B) {
+        lens = a.kv_len[c];
+        mine += Keys(a, lens).blocks * a.heads_tiles;
+      }
     }
-    start += all;
+    through = wave_prefix(mine);
+    total = __builtin_amdgcn_readlane(through, 63);
+    stretch = (total + T::kGrid - 1) / T::kGrid;
   }
-}
+  // The request that holds position pos (< total), and where it starts.
+  __device__ __forceinline__ void locate(int pos, int& b, int& start) {
+    const int upto = __shfl_up(through, 1), before = lane ? upto : 0;
+    const int run = 63 - __clzll(__ballot(before <= pos));
+    start = __builtin_amdgcn_readlane(before, run);
+    b = run * per;
+    if (per == 1) return;
+    for (c0 = b;; c0 += 64) {
+      const int c = c0 + lane;
+      lens = a.kv_len[min(c, a.B - 1)];
+      const int x = c < min(a.B, (run + 1) * per) ? Keys(a, lens).blocks * a.heads_tiles : 0;
+      const int sum = wave_prefix(x), all = __builtin_amdgcn_readlane(sum, 63);
+      if (pos < start + all) {
+        const int l = __ffsll(__ballot(start + sum > pos)) - 1;
+        b = c0 + l;
+        start += __builtin_amdgcn_readlane(sum - x, l);
+        return;
+      }
+      start += all;
+    }
+  }
+  __device__ __forceinline__ Keys keys(int b) {
+    if ((unsigned)(b - c0) >= 64u) {
+      c0 = b;
+      lens = a.kv_len[min(b + lane, a.B - 1)];
+    }
+    return Keys(a, __builtin_amdgcn_readlane(lens, b - c0));
+  }
+};
+
+// A lane's row of an item's tile.
+struct Row {
+  bool ok;
+  int hq, n;
+  __device__ __forceinline__ Row(const PagedKernelArgs& a, int hkv, int tile, int row) {
+    const int rows = a.group * a.N, r = tile * kRows + row, rc = min(r, rows - 1);
+    const int g = a.N == 1 ? rc : rc / a.N;
+    ok = r < rows;
+    hq = hkv * a.group + g;
+    n = rc - g * a.N;
+  }
+};
 
 // A wave's LDS reads so far are done: its tile may be loaded again.
 __device__ __forceinline__ void wait_lds() {
@@ -152,7 +191,29 @@ __device__ __forceinline__ void lds_direct(void* lds, const char* from, uint32_t
                                    (__attribute__((address_space(3))) void*)p, 16, 0, 0);
 }
 
-template <int D, bool BF>
+// 16 bytes each at two or four LDS addresses. In assembly, with their wait: ahead
+// of an ordinary LDS read the compiler waits for every global_load_lds under way,
+// whatever array it fills (of buffer loads to LDS it keeps them apart), which would
+// hold K's products up for V's block.
+typedef __attribute__((address_space(3))) const char lds_char;
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+  return (uint32_t)(uintptr_t)(lds_char*)p;
+}
+__device__ __forceinline__ void lds_read(const uint32_t (&at)[2], u32x4 (&out)[2]) {
+  asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(out[0]), "=&v"(out[1])
+               : "v"(at[0]), "v"(at[1])
+               : "memory");
+}
+__device__ __forceinline__ void lds_read(const uint32_t (&at)[4], u32x4 (&out)[4]) {
+  asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\t"
+               "ds_read_b128 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(out[0]), "=&v"(out[1]), "=&v"(out[2]), "=&v"(out[3])
+               : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+               : "memory");
+}
+
+template <int D, bool BF, bool FULL>  // FULL: the head dim is the width
 __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const PagedKernelArgs a) {
   using T = Paged<D>;
   using S = typename T::S;
@@ -165,59 +226,74 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
   __builtin_assume(wave >= 0 && wave < kWaves);
   const int h = lane >> 5, l32 = lane & 31;
   const int wg = xcd_work_index(T::kGrid);
-  int pos, end, b, start;
-  if (!locate<D>(a, lane, wg, pos, end, b, start)) return;
+  Line<D> line(a, lane);
+  if (wg == 0 && tid == 0) {
+    a.sizes[0] = line.stretch;
+    a.sizes[1] = line.total;
+  }
+  // The workgroup's stretch [wg0, wg1), and this wave's of it [pos, end): wave w
+  // begins at floor(w * stretch / kWaves).
+  const int wg0 = wg * line.stretch, wg1 = min(wg0 + line.stretch, line.total);
+  int4 owned = make_int4(0, 0, 0, 0);  // request, item, its start and blocks (none: 0)
+  if (wg0 >= wg1) {
+    if (lane == 0) a.owned[wg * kWaves + wave] = owned;
+    return;
+  }
+  int pos = min(wg0 + wave * line.stretch / kWaves, wg1);
+  const int end = min(wg0 + (wave + 1) * line.stretch / kWaves, wg1);
+  int b, start;
+  line.locate(min(pos, wg1 - 1), b, start);
+  Keys keys = line.keys(b);
+  int item = (min(pos, wg1 - 1) - start) / keys.blocks;
+  start += item * keys.blocks;  // of the item, from here on
+  const bool join = line.stretch >= T::kJoinFrom && start <= wg0 && wg1 <= start + keys.blocks;
+  if (!join && pos == end) {
+    if (lane == 0) a.owned[wg * kWaves + wave] = owned;
+    return;
+  }
 
-  const int Hkv = a.Hq / a.group, rows = a.group * a.N;
   typename S::Offsets off;
   off.init(lane, 0);
-  char* const my_k = kt + wave * T::kTileBytes;
+  const uint32_t k_at = lds_address(kt) + wave * T::kTileBytes;
   char* const my_v = vt + wave * T::kTileBytes;
-  int row[kParts], col[kParts];  // (of this lane's loads; columns in bytes)
-#pragma unroll
-  for (int u = 0; u < kParts; ++u) {
-    int chunk;
-    T::place(u, lane, row[u], chunk);
-    col[u] = chunk < a.dr / 8 ? 16 * chunk : 0;  // (columns past the head dim: never used)
-  }
-  const float c = a.scale_log2, thr_raw = kRescaleLog2 / c;
+  const uint32_t page_bytes = 2u * (uint32_t)a.page_stride, row_bytes = 2u * (uint32_t)a.row_stride;
+  const int page_mask = (1 << a.page_shift) - 1, dr = FULL ? D : a.dr, chunks = dr / 8;
+  const float c = a.scale_log2, thr_raw = a.rescale;
   constexpr int kWaitOlder = 0x0F70 | (kParts & 15) | ((kParts >> 4) << 14);
 
-  while (pos < end) {
-    const Keys keys(a, a.kv_len[b]);
-    const int item = (pos - start) / keys.blocks;
-    const int from = pos - start - item * keys.blocks, upto = min(from + end - pos, keys.blocks);
-    const int hkv = item / a.n_tiles, tile = item - hkv * a.n_tiles;
-    const int r = tile * kRows + l32;  // this lane's row of the kv head
-    const bool row_ok = r < rows;
-    const int rc = min(r, rows - 1);
-    const int hq = hkv * a.group + rc / a.N, n = rc % a.N;
-    const half_t* qrow = a.q + b * a.stq.b + hq * a.stq.h + (size_t)n * a.stq.n;
+  do {
+    const int from = pos - start, upto = min(from + end - pos, keys.blocks);
+    const int hkv = a.n_tiles == 1 ? item : item / a.n_tiles, tile = item - hkv * a.n_tiles;
+    const Row row(a, hkv, tile, l32);
+    const half_t* qrow = a.q + b * a.stq.b + row.hq * a.stq.h + (size_t)row.n * a.stq.n;
     half8 qb[D / 16];
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk)
-      qb[kk] = as_half8(load16(qrow + kk * 16 + h * 8, kk * 16 + h * 8 < a.dr));
-    const float alibi_raw = a.alibi ? a.alibi[hq] * kLog2e / c : 0.f;
+      qb[kk] = as_half8(load16(qrow + kk * 16 + h * 8, FULL || kk * 16 + h * 8 < dr));
+    const float alibi_raw = a.alibi ? a.alibi[row.hq] * a.alibi_unit : 0.f;
 
     // Keys [lo, hi) of this lane's row, and those that every row sees.
-    const int at = keys.len - a.N + n, at0 = keys.len - a.N;
+    const int at0 = keys.len - a.N, at = at0 + row.n;
     const int lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
     const int hi = a.causal ? min(keys.len, at + 1) : keys.len;
     const int all_lo = a.window > 0 ? max(0, keys.len - a.window) : 0;
     const int all_hi = a.causal ? at0 + 1 : keys.len;
 
-    // This wave's blocks [j, j1), and the page indices around them.
-    const int n_blocks = upto - from, per = (n_blocks + kWaves - 1) / kWaves;
-    const int j0 = keys.first + from + wave * per;
-    const int j1 = keys.len > keys.lo ? min(j0 + per, keys.first + upto) : 0;
+    // The blocks [j0, j1), and the page indices around them.
+    const int j0 = keys.first + from, j1 = keys.len > keys.lo ? keys.first + upto : j0;
     const int* table = a.table + b * a.table_stride;
     const int last_page = max(keys.len - 1, 0) >> a.page_shift;
-    int p0 = 0, held = 0;         // pages p0 .. p0 + 63 are in the lanes' `held`
+    int p0 = 0, held = 0;           // pages p0 .. p0 + 63 are in the lanes' `held`
     unsigned long long hidden = 0;  // of those, the ones outside the pool
     const char* base_k = (const char*)(a.k + hkv * a.head_stride);
     const char* base_v = (const char*)(a.v + hkv * a.head_stride);
-    long long offs[kParts];  // of the loaded block's rows
-    auto key_of = [&](int j, int u) { return min(max(j * kKeys + row[u], keys.lo), keys.len - 1); };
+    unsigned long long offs[kParts];  // of the loaded block's rows
+    // The key that lane `ln` brings in with load u of block j.
+    auto key_of = [&](int j, int u, int ln, int& chunk) {
+      int r;
+      T::place(u, ln, r, chunk);
+      return min(max(j * kKeys + r, keys.lo), keys.len - 1);
+    };
     auto fetch = [&](int j) {  // pages for block j
       p0 = max(j * kKeys, keys.lo) >> a.page_shift;
       const int page = table[min(p0 + lane, last_page)];
@@ -228,11 +304,27 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
     };
     auto place = [&](int j) {
       if ((min(j * kKeys + kKeys, keys.len) - 1) >> a.page_shift > p0 + 63) fetch(j);
+      int ln = lane;
+      asm("" : "+v"(ln));  // (the rows and columns are worked out again: registers are scarcer)
+      constexpr int kAtOnce = kParts < 8 ? kParts : 8;
 #pragma unroll
-      for (int u = 0; u < kParts; ++u) {
-        const int key = key_of(j, u);
-        const int page = __shfl(held, (key >> a.page_shift) - p0);
-        offs[u] = 2 * (page * a.page_stride + (key & ((1 << a.page_shift) - 1)) * a.row_stride) + col[u];
+      for (int u0 = 0; u0 < kParts; u0 += kAtOnce) {
+        uint32_t page[kAtOnce];
+        int key[kAtOnce], chunk;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          key[i] = key_of(j, u0 + i, ln, chunk);
+          page[i] = (uint32_t)__shfl(held, (key[i] >> a.page_shift) - p0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          (void)key_of(j, u0 + i, ln, chunk);
+          // (past the head dim: unused)
+          const uint32_t col = FULL || chunk < chunks ? 16u * (uint32_t)chunk : 0u;
+          offs[u0 + i] = (unsigned long long)page[i] * page_bytes +
+                         (unsigned long long)(uint32_t)(key[i] & page_mask) * row_bytes + col;
+        }
       }
     };
     auto load = [&](char* array, const char* base) {
@@ -246,200 +338,320 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
     for (int cb = 0; cb < D / 32; ++cb) oacc[cb] = zero16();
     float m_raw = -INFINITY, l = 0.f;
     if (j0 < j1) {
-      fetch(j0);
+      fetch(j0);  // (and waits for q: the loop's waits count K's and V's loads only)
       place(j0);
       load(kt, base_k);
       load(vt, base_v);
-    }
-    for (int j = j0; j < j1; ++j) {
-      const unsigned long long hide = hidden;  // (of block j's pages, from page hide0 on)
-      const int hide0 = p0;
-      __builtin_amdgcn_s_waitcnt(kWaitOlder);  // K's block is here, V's may be under way
-      floatx16 s = zero16();
+      for (int j = j0; j < j1; ++j) {
+        const unsigned long long hide = hidden;  // (of block j's pages, from page hide0 on)
+        const int hide0 = p0;
+        __builtin_amdgcn_s_waitcnt(kWaitOlder);  // K's block is here, V's may be under way
+        // (two sums, each product waiting for the one before of its own, where there
+        // are registers for them)
+        constexpr bool kTwo = D <= 128;
+        floatx16 s = zero16(), s2 = zero16();
+        constexpr int kRead = D % 64 == 0 ? 4 : 2;  // operands at a time
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) s = mfma16<BF>(S::read16(my_k, off, kk), qb[kk], s);
-      wait_lds();
-      const bool more = j + 1 < j1;
-      if (more) {
-        place(j + 1);
+        for (int k0 = 0; k0 < D / 16; k0 += kRead) {
+          uint32_t lds[kRead];
+          u32x4 x[kRead];
+#pragma unroll
+          for (int i = 0; i < kRead; ++i) lds[i] = k_at + off.rd[k0 + i];
+          lds_read(lds, x);
+#pragma unroll
+          for (int i = 0; i < kRead; i += 2) {
+            s = mfma16<BF>(as_half8(x[i]), qb[k0 + i], s);
+            floatx16& t = kTwo ? s2 : s;
+            t = mfma16<BF>(as_half8(x[i + 1]), qb[k0 + i + 1], t);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // (Loads behind the last block are one row again and again, and not used: a
+        // branch around them would leave their number unknown, and every wait full.)
+        if (j + 1 < j1) {
+          place(j + 1);
+        } else {
+#pragma unroll
+          for (int u = 0; u < kParts; ++u) offs[u] = 0;
+        }
         load(kt, base_k);
-      }
-      const int base = j * kKeys + 4 * h;
-      if (alibi_raw != 0.f) {
-        const float d0 = (float)(at - base);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          s[e] = fmaf(-alibi_raw, fabsf(d0 - (float)(8 * (e >> 2) + (e & 3))), s[e]);
-      }
-      if (j * kKeys < all_lo || (j + 1) * kKeys > all_hi) {
+        for (int e = 0; e < 16; ++e) s[e] += kTwo ? s2[e] : 0.f;
+        const int base = j * kKeys + 4 * h;
+        if (alibi_raw != 0.f) {
+          const float d0 = (float)(at - base);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            s[e] = fmaf(-alibi_raw, fabsf(d0 - (float)(8 * (e >> 2) + (e & 3))), s[e]);
+        }
+        if (j * kKeys < all_lo || (j + 1) * kKeys > all_hi) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int key = base + 8 * (e >> 2) + (e & 3);
+            if (key < lo || key >= hi) s[e] = -INFINITY;
+          }
+        }
+        if (hide) {  // pages outside the pool: their keys masked, their values zero
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int key = min(max(base + 8 * (e >> 2) + (e & 3), keys.lo), keys.len - 1);
+            if ((hide >> ((key >> a.page_shift) - hide0)) & 1) s[e] = -INFINITY;
+          }
+        }
+        float mloc = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mloc = fmaxf(mloc, s[e]);
+        mloc = max_halves(mloc);
+        if (__any(mloc > m_raw + thr_raw)) {
+          const float m_new = fmaxf(m_raw, mloc);
+          const float corr = m_raw == -INFINITY ? 0.f : fast_exp2((m_raw - m_new) * c);
+          l *= corr;
+#pragma unroll
+          for (int cb = 0; cb < D / 32; ++cb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) oacc[cb][e] *= corr;
+          m_raw = m_new;
+        }
+        const float neg = m_raw == -INFINITY ? 0.f : -m_raw * c;
+        half8 pb[2];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int key = base + 8 * (e >> 2) + (e & 3);
-          if (key < lo || key >= hi) s[e] = -INFINITY;
+          const float p = fast_exp2(fmaf(s[e], c, neg));
+          l += p;
+          pb[e >> 3][e & 7] = to16<BF>(p);
         }
-      }
-      if (hide) {  // pages outside the pool: their keys masked, their values zero
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int key = min(max(base + 8 * (e >> 2) + (e & 3), keys.lo), keys.len - 1);
-          if ((hide >> ((key >> a.page_shift) - hide0)) & 1) s[e] = -INFINITY;
+        __builtin_amdgcn_s_waitcnt(kWaitOlder);  // V's block is here, K's next may be under way
+        if (hide) {
+#pragma unroll 1
+          for (int u = 0; u < kParts; ++u) {
+            int chunk;
+            if ((hide >> ((key_of(j, u, lane, chunk) >> a.page_shift) - hide0)) & 1)
+              *reinterpret_cast<u32x4*>(my_v + u * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
+          }
+          wait_lds();
         }
-      }
-      float mloc = s[0];
 #pragma unroll
-      for (int e = 1; e < 16; ++e) mloc = fmaxf(mloc, s[e]);
-      mloc = max_halves(mloc);
-      if (__any(mloc > m_raw + thr_raw)) {
-        const float m_new = fmaxf(m_raw, mloc);
-        const float corr = m_raw == -INFINITY ? 0.f : fast_exp2((m_raw - m_new) * c);
-        l *= corr;
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int cb = 0; cb < D / 32; ++cb)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) oacc[cb][e] *= corr;
-        m_raw = m_new;
-      }
-      const float neg = m_raw == -INFINITY ? 0.f : -m_raw * c;
-      half8 pb[2];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p = fast_exp2(fmaf(s[e], c, neg));
-        l += p;
-        pb[e >> 3][e & 7] = to16<BF>(p);
-      }
-      if (more) __builtin_amdgcn_s_waitcnt(kWaitOlder);  // V's block is here, K's next may be under way
-      else wait_vmem();
-      if (hide) {
-#pragma unroll
-        for (int u = 0; u < kParts; ++u)
-          if ((hide >> ((key_of(j, u) >> a.page_shift) - hide0)) & 1)
-            *reinterpret_cast<u32x4*>(my_v + u * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
+          for (int cb = 0; cb < D / 32; ++cb)
+            oacc[cb] = mfma16<BF>(S::tr_operand(my_v, q, off, cb), pb[q], oacc[cb]);
         wait_lds();
+        load(vt, base_v);
       }
+    }
+    wait_vmem();
+
+    // The rows' results, or the part's: unscaled O, maximum and sum. Part slots: 0
+    // of a wave for the item that it does not begin, 1 for the one that it does; 0
+    // of its first wave for a workgroup's.
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // (addresses are worked out here, not kept through the loop)
+    const int lh = ln >> 5, lr = ln & 31;
+    const int n_blocks = upto - from;
+    if (from == 0 && n_blocks > 0 && n_blocks < keys.blocks) owned = make_int4(b, item, start, keys.blocks);
+    size_t slot = 2 * (size_t)(wg * kWaves + wave) + (from > 0 ? 0 : 1);
+    half_t* orow = a.o + b * a.stq.b + row.hq * a.stq.h + (size_t)row.n * a.stq.n;
+    auto finish = [&](bool whole, float m, float sum) {
+      if (!whole) a.part_ml[slot * a.part_rows + lr] = make_float2(m * c, sum);
+      else if (a.lse)
+        a.lse[((size_t)b * a.Hq + row.hq) * a.N + row.n] =
+            sum > 0.f ? (m * c + __log2f(sum)) * kLn2 : INFINITY;
+    };
+    // Columns col .. col + 3 (a row without keys: O = 0).
+    auto put = [&](bool whole, float inv, int col, floatx4 v) {
+      if (!whole) {
+        *reinterpret_cast<floatx4*>(a.part_o + (slot * a.part_rows + lr) * D + col) = v;
+      } else if (FULL || col < dr) {
+        half4 o4;
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
+        for (int e = 0; e < 4; ++e) o4[e] = to16<BF>(v[e] * inv);
+        *reinterpret_cast<half4*>(orow + col) = o4;
+      }
+    };
+    if (!join) {
+      const bool whole = n_blocks == keys.blocks;
+      const float sum = l + xor32(l), inv = sum > 0.f ? 1.f / sum : 0.f;
+      if (row.ok && n_blocks > 0) {
 #pragma unroll
         for (int cb = 0; cb < D / 32; ++cb)
-          oacc[cb] = mfma16<BF>(S::tr_operand(my_v, q, off, cb), pb[q], oacc[cb]);
-      wait_lds();
-      if (more) load(vt, base_v);
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            put(whole, inv, 32 * cb + 8 * g + 4 * lh,
+                floatx4{oacc[cb][4 * g], oacc[cb][4 * g + 1], oacc[cb][4 * g + 2], oacc[cb][4 * g + 3]});
+        if (lh == 0) finish(whole, m_raw, sum);
+      }
+      pos += n_blocks;
+      start += keys.blocks;
+      if (++item == a.heads_tiles && pos < end) {
+        item = 0;
+        keys = line.keys(++b);
+      }
+      continue;
     }
-
-    // The waves' partials meet in LDS.
+    // One item: the waves' parts meet in LDS (the rows that there are), in the
+    // accumulator's order: float4 (cb * 4 + g) * 64 + lane.
+    if (wg1 - wg0 == keys.blocks) owned.w = 0;
+    if (lane == 0) a.owned[wg * kWaves + wave] = owned;
     __syncthreads();
     auto part_of = [&](int src) {
       return reinterpret_cast<float*>(src < kWaves / 2 ? kt : vt) + src % (kWaves / 2) * T::kFloats;
     };
+    if (row.ok) {
 #pragma unroll
-    for (int cb = 0; cb < D / 32; ++cb)
+      for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const floatx4 v = {oacc[cb][4 * g], oacc[cb][4 * g + 1], oacc[cb][4 * g + 2],
-                           oacc[cb][4 * g + 3]};
-        *reinterpret_cast<floatx4*>(part_of(wave) + ((cb * 4 + g) * 64 + lane) * 4) = v;
-      }
-    ml[wave * 64 + lane] = make_float2(m_raw, l);
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<floatx4*>(part_of(wave) + ((cb * 4 + g) * 64 + ln) * 4) =
+              floatx4{oacc[cb][4 * g], oacc[cb][4 * g + 1], oacc[cb][4 * g + 2], oacc[cb][4 * g + 3]};
+    }
+    ml[wave * 64 + ln] = make_float2(m_raw, l);
     __syncthreads();
+    if (!row.ok) return;
     float m_star = -INFINITY, l_star = 0.f, wk[kWaves];
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) m_star = fmaxf(m_star, ml[k * 64 + lane].x);
+    for (int k = 0; k < kWaves; ++k) m_star = fmaxf(m_star, ml[k * 64 + ln].x);
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) {
-      const float2 x = ml[k * 64 + lane];
+      const float2 x = ml[k * 64 + ln];
       wk[k] = x.x == -INFINITY ? 0.f : fast_exp2((x.x - m_star) * c);
-      l_star += wk[k] * (x.y + ml[k * 64 + (lane ^ 32)].y);
+      l_star += wk[k] * (x.y + ml[k * 64 + (ln ^ 32)].y);
     }
-    const bool whole = n_blocks == keys.blocks;
-    const float inv_l = l_star > 0.f ? 1.f / l_star : 0.f;  // a row without keys: O = 0
-    const size_t slot = 2 * (size_t)wg + (from > 0 ? 0 : 1);
-    half_t* orow = a.o + b * a.stq.b + hq * a.stq.h + (size_t)n * a.stq.n;
+    const bool whole = wg1 - wg0 == keys.blocks;
+    const float inv = l_star > 0.f ? 1.f / l_star : 0.f;
+    slot = 2 * (size_t)(wg * kWaves);
     constexpr int kRuns = D / 8;  // float4 runs per lane, dealt to the waves
 #pragma unroll
     for (int i = 0; i < (kRuns + kWaves - 1) / kWaves; ++i) {
       const int run = i * kWaves + wave;
-      if (run >= kRuns || !row_ok) break;
+      if (run >= kRuns) break;
       floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < kWaves; ++k)
-        acc += *reinterpret_cast<const floatx4*>(part_of(k) + (run * 64 + lane) * 4) * wk[k];
-      if (!whole) {
-        *reinterpret_cast<floatx4*>(a.part_o + (slot * kRows + l32) * D + 8 * run + 4 * h) = acc;
-      } else if (8 * run + 4 * h < a.dr) {
-        half4 o4;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o4[e] = to16<BF>(acc[e] * inv_l);
-        *reinterpret_cast<half4*>(orow + 8 * run + 4 * h) = o4;
-      }
+        acc += *reinterpret_cast<const floatx4*>(part_of(k) + (run * 64 + ln) * 4) * wk[k];
+      put(whole, inv, 8 * run + 4 * lh, acc);
     }
-    if (wave == 0 && h == 0 && row_ok) {
-      if (!whole) a.part_ml[slot * kRows + l32] = make_float2(m_star * c, l_star);
-      else if (a.lse)
-        a.lse[((size_t)b * a.Hq + hq) * a.N + n] =
-            l_star > 0.f ? (m_star * c + __log2f(l_star)) * kLn2 : INFINITY;
-    }
-    pos += n_blocks;
-    if (pos - start == keys.blocks * a.heads_tiles) {
-      start = pos;
-      ++b;
-    }
-    __syncthreads();  // (the merge area is the tiles)
-  }
+    if (wave == 0 && lh == 0) finish(whole, m_star, l_star);
+    return;
+  } while (pos < end);
+  if (lane == 0) a.owned[wg * kWaves + wave] = owned;
 }
 
-// Joins the parts of the items that several workgroups share.
-template <int D, bool BF>
-__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedKernelArgs a) {
-  const int b = blockIdx.x / a.heads_tiles, item = blockIdx.x - b * a.heads_tiles;
-  const int lane = threadIdx.x & 63;
-  int before = 0, total = 0;
-  for (int i = lane; i < a.B; i += 64) {
-    const int x = Keys(a, a.kv_len[i]).blocks;
-    total += x;
-    if (i < b) before += x;
-  }
-  before = wave_sum(before);
-  total = wave_sum(total);
-  const int blocks = Keys(a, a.kv_len[b]).blocks, share = share_of<D>(total * a.heads_tiles);
-  const int first = before * a.heads_tiles + item * blocks;
-  const int w0 = first / share, w1 = (first + blocks - 1) / share;
-  if (w0 == w1) return;  // (its workgroup has written it)
-  const int hkv = item / a.n_tiles, tile = item - hkv * a.n_tiles;
-  const int rows = min(kRows, a.group * a.N - tile * kRows);
-  for (int f = threadIdx.x; f < rows * (D / 4); f += 256) {
-    const int rr = f / (D / 4), col = 4 * (f - rr * (D / 4));
-    const int r = tile * kRows + rr, hq = hkv * a.group + r / a.N, n = r % a.N;
-    // Parts: the second slot of the first workgroup, the first slots of the others.
-    const float2* ml = a.part_ml + rr;
-    float m = ml[(2 * (size_t)w0 + 1) * kRows].x;
-#pragma unroll 4
-    for (int w = w0 + 1; w <= w1; ++w) m = fmaxf(m, ml[2 * (size_t)w * kRows].x);
+// Joins the parts of the items that several waves share. A workgroup takes the
+// items that one of paged_kernel's workgroups begins and others end (one of each
+// wave at most); its waves are dealt to these items' runs of 64 float4 columns and
+// then to their parts, so that one long request's parts are read in a few rounds.
+constexpr int kMergeWaves = 16;
+
+// x / y for 0 <= x < 2^20, y >= 1: (x + 0.5) / y is 0.5 / y or more from a whole
+// number, and off by less than 2^-22 of itself.
+__device__ __forceinline__ int small_div(int x, int y) {
+  return (int)(((float)x + 0.5f) * __builtin_amdgcn_rcpf((float)y));
+}
+
+template <int D, bool BF, bool FULL>
+__global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const PagedKernelArgs a) {
+  constexpr int kWaves = Paged<D>::kWaves;
+  __shared__ floatx4 accs[kMergeWaves][64];
+  __shared__ float2 mls[kMergeWaves][64];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int stretch = a.sizes[0], total = a.sizes[1];
+  const int4 mine = lane < kWaves ? a.owned[blockIdx.x * kWaves + lane] : make_int4(0, 0, 0, 0);
+  const unsigned long long some = __ballot(mine.w > 0);
+  if (some == 0) return;
+  const int items = __popcll(some), tasks = items * a.runs;
+  const int groups = max(1, small_div(kMergeWaves, tasks));  // waves that share a task's parts
+  for (int t0 = 0; t0 < tasks; t0 += kMergeWaves) {
+    const int per_round = min(tasks, kMergeWaves), group = small_div(wave, per_round);
+    const int task = t0 + wave - group * per_round;
+    const bool active = task < tasks && group < groups;
+    const int nth = active ? small_div(task, a.runs) : 0, run = active ? task - nth * a.runs : 0;
+    unsigned long long left = some;
+    for (int i = 0; i < nth; ++i) left &= left - 1;
+    const int owner = __ffsll(left) - 1, w0 = blockIdx.x * kWaves + owner;
+    const int b = __builtin_amdgcn_readlane(mine.x, owner), item = __builtin_amdgcn_readlane(mine.y, owner);
+    const int start = __builtin_amdgcn_readlane(mine.z, owner);
+    const int end = start + __builtin_amdgcn_readlane(mine.w, owner);
+    // A workgroup that has joined its waves has left one part, the others one of
+    // each wave with a block of the item: of blocks [x0, x1) of its stretch,
+    // counted from its begin.
+    const int g0 = blockIdx.x, g1 = (end - 1) / stretch;
+    const bool joins = stretch >= Paged<D>::kJoinFrom, single = stretch <= kWaves;
+    auto whole = [&](int g) { return joins && start <= g * stretch && min((g + 1) * stretch, total) <= end; };
+    auto wave_of = [&](int x) {  // (the last w with floor(w * stretch / kWaves) <= x)
+      return single ? small_div(kWaves * (x + 1) - 1, stretch) : (kWaves * (x + 1) - 1) / stretch;
+    };
+    const bool whole0 = whole(g0), whole1 = whole(g1);
+    const int x0 = start - g0 * stretch, x1 = end - g1 * stretch;  // (of g0, and of g1)
+    const int upto0 = g0 == g1 ? x1 : stretch;
+    const int head = whole0 ? 1 : single ? upto0 - x0 : (g0 == g1 ? wave_of(x1 - 1) : kWaves - 1) - owner + 1;
+    const int tail = g0 == g1 ? 0 : whole1 ? 1 : single ? x1 : wave_of(x1 - 1) + 1;
+    const int middle = max(g1 - g0 - 1, 0) * (joins ? 1 : stretch);
+    const int parts = head + middle + tail;
+    auto slot_of = [&](int p) {
+      if (p < head) {
+        const int w = whole0 ? 0 : single ? wave_of(x0 + p) : owner + p;
+        return 2 * (g0 * kWaves + w) + (p == 0 && !whole0 ? 1 : 0);
+      }
+      p -= head;
+      if (p < middle) {
+        const int k = joins ? p : small_div(p, stretch);
+        return 2 * ((g0 + 1 + k) * kWaves + (joins ? 0 : wave_of(p - k * stretch)));
+      }
+      p -= middle;
+      return 2 * (g1 * kWaves + (single && !whole1 ? wave_of(p) : p));
+    };
+    const int hkv = a.n_tiles == 1 ? item : item / a.n_tiles, tile = item - hkv * a.n_tiles;
+    const int rows = min(kRows, a.group * a.N - tile * kRows);
+    const int f = run * 64 + lane, rr = min(f / (D / 4), rows - 1), col = 4 * (f % (D / 4));
+    float m = -INFINITY, l = 0.f;
     floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
+    auto join = [&](float mo, float lo, floatx4 o) {
+      const float m_new = fmaxf(m, mo);
+      const float keep = m == -INFINITY ? 0.f : fast_exp2(m - m_new);  // (no key: zeros)
+      const float add = mo == -INFINITY ? 0.f : fast_exp2(mo - m_new);
+      l = l * keep + lo * add;
+      acc = acc * keep + o * add;
+      m = m_new;
+    };
+    if (active) {
 #pragma unroll 4
-    for (int w = w0; w <= w1; ++w) {
-      const size_t slot = 2 * (size_t)w + (w == w0 ? 1 : 0);
-      const float2 x = ml[slot * kRows];
-      const float f = x.x == -INFINITY ? 0.f : fast_exp2(x.x - m);  // (no key: zeros)
-      l += f * x.y;
-      acc += *reinterpret_cast<const floatx4*>(a.part_o + (slot * kRows + rr) * D + col) * f;
+      for (int p = group; p < parts; p += groups) {
+        const size_t at = (size_t)slot_of(p) * a.part_rows + rr;
+        const float2 x = a.part_ml[at];
+        join(x.x, x.y, *reinterpret_cast<const floatx4*>(a.part_o + at * D + col));
+      }
+      accs[wave][lane] = acc;
+      mls[wave][lane] = make_float2(m, l);
     }
-    const float inv_l = l > 0.f ? 1.f / l : 0.f;
-    if (col < a.dr) {
-      half4 o4;
+    __syncthreads();
+    if (active && group == 0 && f < rows * (D / 4)) {
+      for (int k = 1; k < min(groups, parts); ++k) {
+        const int w = wave + k * per_round;
+        join(mls[w][lane].x, mls[w][lane].y, accs[w][lane]);
+      }
+      const Row row(a, hkv, tile, rr);
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      if (FULL || col < a.dr) {
+        half4 o4;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o4[e] = to16<BF>(acc[e] * inv_l);
-      *reinterpret_cast<half4*>(a.o + b * a.stq.b + hq * a.stq.h + (size_t)n * a.stq.n + col) = o4;
+        for (int e = 0; e < 4; ++e) o4[e] = to16<BF>(acc[e] * inv);
+        *reinterpret_cast<half4*>(a.o + b * a.stq.b + row.hq * a.stq.h + (size_t)row.n * a.stq.n + col) = o4;
+      }
+      if (col == 0 && a.lse)
+        a.lse[((size_t)b * a.Hq + row.hq) * a.N + row.n] =
+            l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
     }
-    if (col == 0 && a.lse)
-      a.lse[((size_t)b * a.Hq + hq) * a.N + n] = l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
+    __syncthreads();
   }
 }
 
 }  // namespace
 
 template <>
-size_t paged_workspace_w<FA_WIDTH, FA_BF>() {
-  return (size_t)Paged<FA_WIDTH>::kGrid * 2 * kRows * (FA_WIDTH * sizeof(float) + sizeof(float2));
+size_t paged_workspace_w<FA_WIDTH, FA_BF>(int rows) {
+  constexpr size_t kAll = (size_t)Paged<FA_WIDTH>::kGrid * Paged<FA_WIDTH>::kWaves;
+  return kAll * 2 * min(rows, kRows) * (FA_WIDTH * sizeof(float) + sizeof(float2)) +
+         kAll * sizeof(int4) + 2 * sizeof(int);
 }
 
 template <>
@@ -460,27 +672,38 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
   d.table_stride = a.table_stride;
   d.cap = a.table_width << a.pool.page_shift;
   d.kv_len = a.kv_len;
-  d.part_o = (float*)a.workspace;
-  d.part_ml = (float2*)(d.part_o + (size_t)Paged<D>::kGrid * 2 * kRows * D);
   d.B = a.B;
   d.Hq = a.Hq;
   d.group = a.Hq / a.Hkv;
   d.N = a.N;
+  d.part_rows = min(d.group * a.N, kRows);
+  d.part_o = (float*)a.workspace;
+  constexpr size_t kAll = (size_t)Paged<D>::kGrid * Paged<D>::kWaves;
+  d.part_ml = (float2*)(d.part_o + kAll * 2 * d.part_rows * D);
+  d.owned = (int4*)(d.part_ml + kAll * 2 * d.part_rows);
+  d.sizes = (int*)(d.owned + kAll);
+  d.runs = (d.part_rows * (D / 4) + 63) / 64;
   d.n_tiles = (d.group * a.N + kRows - 1) / kRows;
   d.heads_tiles = a.Hkv * d.n_tiles;
   d.causal = a.causal;
   d.window = a.window < d.cap ? a.window : 0;  // (a wider one hides nothing)
   d.dr = a.D;
   d.scale_log2 = kLog2e * (a.scale > 0.f ? a.scale : 1.f / sqrtf((float)a.D));
+  d.rescale = kRescaleLog2 / d.scale_log2;
+  d.alibi_unit = kLog2e / d.scale_log2;
   d.alibi = a.alibi;
   d.stq = make_strides(a.layout, a.Hq, a.N, a.D);
-  hipLaunchKernelGGL((paged_kernel<D, FA_BF>), dim3(Paged<D>::kGrid), dim3(Paged<D>::kThreads), 0,
-                     (hipStream_t)a.stream, d);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((paged_merge_kernel<D, FA_BF>), dim3((unsigned)(a.B * d.heads_tiles)), dim3(256),
-                     0, (hipStream_t)a.stream, d);
-  return hipGetLastError();
+  auto launch = [&](auto full) {
+    constexpr bool kFull = decltype(full)::value;
+    hipLaunchKernelGGL((paged_kernel<D, FA_BF, kFull>), dim3(Paged<D>::kGrid), dim3(Paged<D>::kThreads),
+                       0, (hipStream_t)a.stream, d);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((paged_merge_kernel<D, FA_BF, kFull>), dim3(Paged<D>::kGrid),
+                       dim3(64 * kMergeWaves), 0, (hipStream_t)a.stream, d);
+    return hipGetLastError();
+  };
+  return a.D == D ? launch(std::true_type{}) : launch(std::false_type{});
 }
 
 }  // namespace fa

@@ -435,7 +435,8 @@ int fa_pack_blocks(const uint8_t* layout, int layout_b, int layout_h, int B, int
  *   - k, v: the two pools, 16-byte aligned: element (page, kv head, row, d) at
  *     page * stride_page + head * stride_head + row * stride_row + d, strides in
  *     elements, multiples of 8 and the same for both (so (pages, Hkv, page_size,
- *     D), (pages, page_size, Hkv, D) and pools that interleave k and v will do);
+ *     D), (pages, page_size, Hkv, D) and pools that interleave k and v will do),
+ *     stride_page and stride_row below 2^31;
  *   - pages, page_size: pages of the pool, and rows of a page, a power of two;
  *     pages * page_size <= 2^31 - 1;
  *   - table, table_stride, table_width: int32 page indices, table_width >= 1 of
@@ -514,9 +515,9 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
  * of a batch are shared evenly among the GPU's compute units whatever their
  * lengths; partial results meet in `workspace`, of at least
  * fa_paged_attn_workspace_bytes() bytes (0 for invalid arguments), which may hold
- * anything. Calls that overlap in time need workspaces of their own. B * Hq * N <=
- * 2^23, and the 32-key blocks of full tables, times Hkv and the 32-row tiles of Hq /
- * Hkv * N, at most 2^30. The results are deterministic; a request's last bits may depend on the lengths of
+ * anything. Calls that overlap in time need workspaces of their own. Hq * N <=
+ * 2^24, and the 32-key blocks of full tables, times B, Hkv and the 32-row tiles of
+ * Hq / Hkv * N, at most 2^30. The results are deterministic; a request's last bits may depend on the lengths of
  * the others in its batch. */
 size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
 int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,

@@ -89,7 +89,8 @@ def test_attn_refusals():
     for bad in (dict(page_size=48), dict(stride_head=100), dict(table_width=0), dict(table_stride=2),
                 dict(table_width=1 << 28, table_stride=1 << 28)):
         assert call(c=cache(**bad)) == 10019, bad
-    assert call(B=1 << 20, Hq=128, Hkv=2) == 10007
+    assert call(N=1 << 23) == 10007  # rows of a request
+    assert call(B=1 << 16, c=cache(table_width=1 << 20, table_stride=1 << 20)) == 10007  # key blocks
     for bad in (fa_opts(kv_len=1), fa_opts(seg_start=1, seg_end=1), fa_opts(mask=1, mask_heads=1),
                 fa_opts(drop=1, drop_scale=1.0), fa_opts(bias=1), fa_opts(kv_rows=9),
                 fa_opts(block_rows=1)):
