@@ -78,7 +78,7 @@ struct PagedKernelArgs {
   int* sizes;       // Line's stretch and total
   int part_rows;    // of a tile: kRows, or all of a kv head's
   int B, Hq, group, N, n_tiles, heads_tiles, causal, window, dr;
-  int runs;  // of 64 float4 columns in a tile's rows
+  int runs;  // of 64 float4 columns in a tile's rows, a join's workgroup taking kMergeRuns
   float scale_log2, rescale, alibi_unit;  // (the last two in units of q . k)
   const float* alibi;
   Strides stq;
@@ -224,7 +224,6 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
   __builtin_assume(wave >= 0 && wave < kWaves);
-  const int h = lane >> 5, l32 = lane & 31;
   const int wg = xcd_work_index(T::kGrid);
   Line<D> line(a, lane);
   if (wg == 0 && tid == 0) {
@@ -232,28 +231,28 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
     a.sizes[1] = line.total;
   }
   // The workgroup's stretch [wg0, wg1), and this wave's of it [pos, end): wave w
-  // begins at floor(w * stretch / kWaves).
+  // has block w of a stretch below kWaves, else begins at floor(w * stretch / kWaves).
   const int wg0 = wg * line.stretch, wg1 = min(wg0 + line.stretch, line.total);
   int4 owned = make_int4(0, 0, 0, 0);  // request, item, its start and blocks (none: 0)
   if (wg0 >= wg1) {
     if (lane == 0) a.owned[wg * kWaves + wave] = owned;
     return;
   }
-  int pos = min(wg0 + wave * line.stretch / kWaves, wg1);
-  const int end = min(wg0 + (wave + 1) * line.stretch / kWaves, wg1);
+  const bool single = line.stretch < kWaves;
+  int pos = min(wg0 + (single ? wave : wave * line.stretch / kWaves), wg1);
+  const int end = min(wg0 + (single ? wave + 1 : (wave + 1) * line.stretch / kWaves), wg1);
   int b, start;
   line.locate(min(pos, wg1 - 1), b, start);
   Keys keys = line.keys(b);
   int item = (min(pos, wg1 - 1) - start) / keys.blocks;
   start += item * keys.blocks;  // of the item, from here on
-  const bool join = line.stretch >= T::kJoinFrom && start <= wg0 && wg1 <= start + keys.blocks;
+  const bool joins = line.stretch >= T::kJoinFrom;
+  const bool join = joins && start <= wg0 && wg1 <= start + keys.blocks;
   if (!join && pos == end) {
     if (lane == 0) a.owned[wg * kWaves + wave] = owned;
     return;
   }
 
-  typename S::Offsets off;
-  off.init(lane, 0);
   const uint32_t k_at = lds_address(kt) + wave * T::kTileBytes;
   char* const my_v = vt + wave * T::kTileBytes;
   const uint32_t page_bytes = 2u * (uint32_t)a.page_stride, row_bytes = 2u * (uint32_t)a.row_stride;
@@ -264,21 +263,6 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
   do {
     const int from = pos - start, upto = min(from + end - pos, keys.blocks);
     const int hkv = a.n_tiles == 1 ? item : item / a.n_tiles, tile = item - hkv * a.n_tiles;
-    const Row row(a, hkv, tile, l32);
-    const half_t* qrow = a.q + b * a.stq.b + row.hq * a.stq.h + (size_t)row.n * a.stq.n;
-    half8 qb[D / 16];
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk)
-      qb[kk] = as_half8(load16(qrow + kk * 16 + h * 8, FULL || kk * 16 + h * 8 < dr));
-    const float alibi_raw = a.alibi ? a.alibi[row.hq] * a.alibi_unit : 0.f;
-
-    // Keys [lo, hi) of this lane's row, and those that every row sees.
-    const int at0 = keys.len - a.N, at = at0 + row.n;
-    const int lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
-    const int hi = a.causal ? min(keys.len, at + 1) : keys.len;
-    const int all_lo = a.window > 0 ? max(0, keys.len - a.window) : 0;
-    const int all_hi = a.causal ? at0 + 1 : keys.len;
-
     // The blocks [j0, j1), and the page indices around them.
     const int j0 = keys.first + from, j1 = keys.len > keys.lo ? keys.first + upto : j0;
     const int* table = a.table + b * a.table_stride;
@@ -333,15 +317,39 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
         lds_direct(array, base + offs[u], (uint32_t)(wave * T::kTileBytes + u * 1024));
     };
 
+    // The way to the first loads is what a short call waits for: nothing that they
+    // do not need comes before them. (q between K and V: the waits for K are its too.)
+    if (j0 < j1) {
+      fetch(j0);
+      place(j0);
+      load(kt, base_k);
+    }
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    __builtin_amdgcn_sched_barrier(0);
+    const int h = ln >> 5, l32 = ln & 31;
+    const Row row(a, hkv, tile, l32);
     floatx16 oacc[D / 32];
 #pragma unroll
     for (int cb = 0; cb < D / 32; ++cb) oacc[cb] = zero16();
     float m_raw = -INFINITY, l = 0.f;
     if (j0 < j1) {
-      fetch(j0);  // (and waits for q: the loop's waits count K's and V's loads only)
-      place(j0);
-      load(kt, base_k);
+      const half_t* qrow = a.q + b * a.stq.b + row.hq * a.stq.h + (size_t)row.n * a.stq.n;
+      half8 qb[D / 16];
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        qb[kk] = as_half8(load16(qrow + kk * 16 + h * 8, FULL || kk * 16 + h * 8 < dr));
+      const float alibi_raw = a.alibi ? a.alibi[row.hq] * a.alibi_unit : 0.f;
+      __builtin_amdgcn_sched_barrier(0);
       load(vt, base_v);
+      // Keys [lo, hi) of this lane's row, and those that every row sees.
+      const int at0 = keys.len - a.N, at = at0 + row.n;
+      const int lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
+      const int hi = a.causal ? min(keys.len, at + 1) : keys.len;
+      const int all_lo = a.window > 0 ? max(0, keys.len - a.window) : 0;
+      const int all_hi = a.causal ? at0 + 1 : keys.len;
+      typename S::Offsets off;
+      off.init(ln, 0);
       for (int j = j0; j < j1; ++j) {
         const unsigned long long hide = hidden;  // (of block j's pages, from page hide0 on)
         const int hide0 = p0;
@@ -441,15 +449,15 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
     }
     wait_vmem();
 
-    // The rows' results, or the part's: unscaled O, maximum and sum. Part slots: 0
-    // of a wave for the item that it does not begin, 1 for the one that it does; 0
-    // of its first wave for a workgroup's.
-    int ln = lane;
+    // The rows' results, or the part's: unscaled O, maximum and sum. Part slots:
+    // two of a wave, the first for the item that it does not begin and the second
+    // for the one that it does; the first of its first wave for a workgroup's; the
+    // block's position where no stretch is joined (a block is a part there).
     asm volatile("" : "+v"(ln));  // (addresses are worked out here, not kept through the loop)
     const int lh = ln >> 5, lr = ln & 31;
     const int n_blocks = upto - from;
     if (from == 0 && n_blocks > 0 && n_blocks < keys.blocks) owned = make_int4(b, item, start, keys.blocks);
-    size_t slot = 2 * (size_t)(wg * kWaves + wave) + (from > 0 ? 0 : 1);
+    size_t slot = joins ? 2 * (wg * kWaves + wave) + (from > 0 ? 0 : 1) : pos;
     half_t* orow = a.o + b * a.stq.b + row.hq * a.stq.h + (size_t)row.n * a.stq.n;
     auto finish = [&](bool whole, float m, float sum) {
       if (!whole) a.part_ml[slot * a.part_rows + lr] = make_float2(m * c, sum);
@@ -538,14 +546,17 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
 
 // Joins the parts of the items that several waves share. A workgroup takes the
 // items that one of paged_kernel's workgroups begins and others end (one of each
-// wave at most); its waves are dealt to these items' runs of 64 float4 columns and
-// then to their parts, so that one long request's parts are read in a few rounds.
-constexpr int kMergeWaves = 16;
+// wave at most) and two of their runs of 64 float4 columns; its waves are dealt to
+// these and then to the parts, so that one long request's parts are read in a few rounds.
+// Bound by latency (the parts' list, then the parts), so it divides in floats and
+// leaves the list to paged_kernel.
+constexpr int kMergeWaves = 8;
+constexpr int kMergeRuns = 2;
 
 // x / y for 0 <= x < 2^20, y >= 1: (x + 0.5) / y is 0.5 / y or more from a whole
 // number, and off by less than 2^-22 of itself.
 __device__ __forceinline__ int small_div(int x, int y) {
-  return (int)(((float)x + 0.5f) * __builtin_amdgcn_rcpf((float)y));
+  return uniform((int)(((float)x + 0.5f) * __builtin_amdgcn_rcpf((float)y)));
 }
 
 template <int D, bool BF, bool FULL>
@@ -558,47 +569,48 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
   const int4 mine = lane < kWaves ? a.owned[blockIdx.x * kWaves + lane] : make_int4(0, 0, 0, 0);
   const unsigned long long some = __ballot(mine.w > 0);
   if (some == 0) return;
-  const int items = __popcll(some), tasks = items * a.runs;
-  const int groups = max(1, small_div(kMergeWaves, tasks));  // waves that share a task's parts
+  auto div = [&](int x, int y) { return total < 1 << 17 ? small_div(x, y) : x / y; };
+  const int run0 = blockIdx.y * kMergeRuns, runs = min(kMergeRuns, a.runs - run0);
+  const int tasks = __popcll(some) * runs;
+  const int per_round = min(tasks, kMergeWaves);
+  const int groups = small_div(kMergeWaves, per_round);  // waves that share a task's parts
+  const int group = small_div(wave, per_round);
   for (int t0 = 0; t0 < tasks; t0 += kMergeWaves) {
-    const int per_round = min(tasks, kMergeWaves), group = small_div(wave, per_round);
     const int task = t0 + wave - group * per_round;
     const bool active = task < tasks && group < groups;
-    const int nth = active ? small_div(task, a.runs) : 0, run = active ? task - nth * a.runs : 0;
+    const int nth = active ? (runs > 1 ? task / kMergeRuns : task) : 0, run = run0 + (active ? task - nth * runs : 0);
     unsigned long long left = some;
     for (int i = 0; i < nth; ++i) left &= left - 1;
-    const int owner = __ffsll(left) - 1, w0 = blockIdx.x * kWaves + owner;
+    const int owner = __ffsll(left) - 1;
     const int b = __builtin_amdgcn_readlane(mine.x, owner), item = __builtin_amdgcn_readlane(mine.y, owner);
     const int start = __builtin_amdgcn_readlane(mine.z, owner);
     const int end = start + __builtin_amdgcn_readlane(mine.w, owner);
-    // A workgroup that has joined its waves has left one part, the others one of
-    // each wave with a block of the item: of blocks [x0, x1) of its stretch,
-    // counted from its begin.
-    const int g0 = blockIdx.x, g1 = (end - 1) / stretch;
-    const bool joins = stretch >= Paged<D>::kJoinFrom, single = stretch <= kWaves;
-    auto whole = [&](int g) { return joins && start <= g * stretch && min((g + 1) * stretch, total) <= end; };
-    auto wave_of = [&](int x) {  // (the last w with floor(w * stretch / kWaves) <= x)
-      return single ? small_div(kWaves * (x + 1) - 1, stretch) : (kWaves * (x + 1) - 1) / stretch;
-    };
-    const bool whole0 = whole(g0), whole1 = whole(g1);
-    const int x0 = start - g0 * stretch, x1 = end - g1 * stretch;  // (of g0, and of g1)
-    const int upto0 = g0 == g1 ? x1 : stretch;
-    const int head = whole0 ? 1 : single ? upto0 - x0 : (g0 == g1 ? wave_of(x1 - 1) : kWaves - 1) - owner + 1;
-    const int tail = g0 == g1 ? 0 : whole1 ? 1 : single ? x1 : wave_of(x1 - 1) + 1;
-    const int middle = max(g1 - g0 - 1, 0) * (joins ? 1 : stretch);
+    // The item's parts: of the waves from `owner` on in its first workgroup (or of
+    // the workgroup), of the workgroups between, of the last one's first waves (or
+    // of it). Where no stretch is joined, of each block.
+    int head = end - start, middle = 0, tail = 0;
+    int head_slot = start, first = start, step = 1, middle_slot = 0, tail_slot = 0;
+    if (stretch >= Paged<D>::kJoinFrom) {
+      const int g0 = blockIdx.x, g1 = div(end - 1, stretch);
+      const int x1 = end - g1 * stretch;  // (blocks of the item in g1's stretch, if not all)
+      const int last = stretch < kWaves ? x1 - 1 : div(kWaves * x1 - 1, stretch);  // (their last wave)
+      const bool whole0 = start == g0 * stretch && g0 < g1, whole1 = end == min((g1 + 1) * stretch, total);
+      const int waves = min(kWaves, stretch);
+      head = whole0 ? 1 : (g0 == g1 ? last + 1 : waves) - owner;
+      middle = max(g1 - g0 - 1, 0);
+      tail = g0 == g1 ? 0 : whole1 ? 1 : last + 1;
+      head_slot = 2 * (g0 * kWaves + owner);
+      first = head_slot + (whole0 ? 0 : 1);
+      step = 2;
+      middle_slot = 2 * (g0 + 1) * kWaves;
+      tail_slot = 2 * g1 * kWaves;
+    }
     const int parts = head + middle + tail;
     auto slot_of = [&](int p) {
-      if (p < head) {
-        const int w = whole0 ? 0 : single ? wave_of(x0 + p) : owner + p;
-        return 2 * (g0 * kWaves + w) + (p == 0 && !whole0 ? 1 : 0);
-      }
+      if (p == 0) return first;
+      if (p < head) return head_slot + p * step;
       p -= head;
-      if (p < middle) {
-        const int k = joins ? p : small_div(p, stretch);
-        return 2 * ((g0 + 1 + k) * kWaves + (joins ? 0 : wave_of(p - k * stretch)));
-      }
-      p -= middle;
-      return 2 * (g1 * kWaves + (single && !whole1 ? wave_of(p) : p));
+      return p < middle ? middle_slot + p * 2 * kWaves : tail_slot + (p - middle) * 2;
     };
     const int hkv = a.n_tiles == 1 ? item : item / a.n_tiles, tile = item - hkv * a.n_tiles;
     const int rows = min(kRows, a.group * a.N - tile * kRows);
@@ -614,21 +626,36 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
       m = m_new;
     };
     if (active) {
-#pragma unroll 4
-      for (int p = group; p < parts; p += groups) {
-        const size_t at = (size_t)slot_of(p) * a.part_rows + rr;
-        const float2 x = a.part_ml[at];
-        join(x.x, x.y, *reinterpret_cast<const floatx4*>(a.part_o + at * D + col));
+      const float2* ml = a.part_ml + rr;
+      const float* po = a.part_o + rr * D + col;
+      constexpr int kAtOnce = 4;
+      for (int p0 = group; p0 < parts; p0 += kAtOnce * groups) {
+        float2 x[kAtOnce];
+        floatx4 o[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {  // (past the last: the last again, not added)
+          const size_t slot = (size_t)slot_of(min(p0 + i * groups, parts - 1)) * a.part_rows;
+          x[i] = ml[slot];
+          o[i] = *reinterpret_cast<const floatx4*>(po + slot * D);
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+          if (p0 + i * groups < parts) join(x[i].x, x[i].y, o[i]);
       }
-      accs[wave][lane] = acc;
-      mls[wave][lane] = make_float2(m, l);
     }
-    __syncthreads();
-    if (active && group == 0 && f < rows * (D / 4)) {
-      for (int k = 1; k < min(groups, parts); ++k) {
-        const int w = wave + k * per_round;
-        join(mls[w][lane].x, mls[w][lane].y, accs[w][lane]);
+    if (groups > 1) {
+      if (active) {
+        accs[wave][lane] = acc;
+        mls[wave][lane] = make_float2(m, l);
       }
+      __syncthreads();
+      if (active && group == 0)
+        for (int k = 1; k < min(groups, parts); ++k) {
+          const int w = wave + k * per_round;
+          join(mls[w][lane].x, mls[w][lane].y, accs[w][lane]);
+        }
+    }
+    if (active && group == 0 && f < rows * (D / 4)) {
       const Row row(a, hkv, tile, rr);
       const float inv = l > 0.f ? 1.f / l : 0.f;
       if (FULL || col < a.dr) {
@@ -641,7 +668,6 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
         a.lse[((size_t)b * a.Hq + row.hq) * a.N + row.n] =
             l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
     }
-    __syncthreads();
   }
 }
 
@@ -699,7 +725,8 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
                        0, (hipStream_t)a.stream, d);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_merge_kernel<D, FA_BF, kFull>), dim3(Paged<D>::kGrid),
+    hipLaunchKernelGGL((paged_merge_kernel<D, FA_BF, kFull>),
+                       dim3(Paged<D>::kGrid, (unsigned)((d.runs + kMergeRuns - 1) / kMergeRuns)),
                        dim3(64 * kMergeWaves), 0, (hipStream_t)a.stream, d);
     return hipGetLastError();
   };
