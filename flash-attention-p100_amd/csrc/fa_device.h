@@ -84,6 +84,22 @@ __device__ __forceinline__ half8 as_half8(u32x4 v) {
 // Swap with the lane 32 positions away (the other half of the wave).
 __device__ __forceinline__ float xor32(float v) { return __shfl_xor(v, 32, 64); }
 
+// Inclusive prefix over the lanes of an associative op(x, y) whose neutral element
+// is 0: steps of 1, 2, 4 and 8 lanes within rows of 16, then the rows' totals.
+template <int CTRL, int ROWS, class Op>
+__device__ __forceinline__ int prefix_step(int x, const Op& op) {
+  return op(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false));
+}
+template <class Op>
+__device__ __forceinline__ int wave_prefix(int x, const Op& op) {
+  x = prefix_step<0x111, 0xf>(x, op);
+  x = prefix_step<0x112, 0xf>(x, op);
+  x = prefix_step<0x114, 0xf>(x, op);
+  x = prefix_step<0x118, 0xf>(x, op);
+  x = prefix_step<0x142, 0xa>(x, op);     // row 0's last lane to row 1, 2's to 3
+  return prefix_step<0x143, 0xc>(x, op);  // row 1's last lane to rows 2 and 3
+}
+
 // Row max over the two half-waves: lanes l and l ^ 32 hold the same query row.
 __device__ __forceinline__ float max_halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,

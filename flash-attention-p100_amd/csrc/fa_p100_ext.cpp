@@ -763,6 +763,7 @@ std::vector<at::Tensor> fa_paged_tables_t(const at::Tensor& block_table, const a
   TORCH_CHECK(want >= 0 && B <= (1 << 20) && (tokens ? want : want * B) <= INT32_MAX,
               "max_new and tokens must not be negative, and the slots at most 2^31 - 1");
   c10::DeviceGuard guard(dev);
+  at::AutoDispatchBelowADInplaceOrView below;  // (no gradient: the allocations skip its layers)
   const auto opts = old_len.options();
   at::Tensor slots = tokens ? at::empty({want}, opts) : at::empty({B, want}, opts);
   at::Tensor kv_len = at::empty({B}, opts), ring_out = at::empty({2}, opts);
@@ -839,9 +840,10 @@ std::vector<at::Tensor> fa_paged_attn_t(at::Tensor q, const at::Tensor& k_cache,
   TORCH_CHECK(kv_len.dim() == 1 && kv_len.size(0) == B, "kv_len must be (", B, ",)");
   TORCH_CHECK(B <= INT32_MAX && H * N <= (1 << 24), "shape exceeds the kernels' index range");
   c10::DeviceGuard guard(q.device());
+  at::AutoDispatchBelowADInplaceOrView below;
   fa_options op{};
   op.dtype = dtype_code(q);
-  op.window = (int)window;
+  op.window = (int)std::min<int64_t>(window, INT32_MAX);
   op.alibi_slopes = alibi_ptr(alibi_slopes, q, (int)H);
   op.scale = (float)scale;
   if (!q.is_contiguous()) {

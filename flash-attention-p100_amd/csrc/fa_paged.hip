@@ -78,6 +78,7 @@ struct PagedKernelArgs {
   int* sizes;       // Line's stretch and total
   int part_rows;    // of a tile: kRows, or all of a kv head's
   int B, Hq, group, N, n_tiles, heads_tiles, causal, window, dr;
+  bool by_item;  // the join's workgroups take an item each
   int runs;  // of 64 float4 columns in a tile's rows, a join's workgroup taking kMergeRuns
   float scale_log2, rescale, alibi_unit;  // (the last two in units of q . k)
   const float* alibi;
@@ -97,18 +98,9 @@ struct Keys {
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int plus_dpp(int x) {  // x + the lane that CTRL names (none: 0)
-  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
-}
 // The sum over the lanes up to each.
 __device__ __forceinline__ int wave_prefix(int x) {
-  x = plus_dpp<0x111, 0xf>(x);  // 1, 2, 4 and 8 lanes before, within rows of 16
-  x = plus_dpp<0x112, 0xf>(x);
-  x = plus_dpp<0x114, 0xf>(x);
-  x = plus_dpp<0x118, 0xf>(x);
-  x = plus_dpp<0x142, 0xa>(x);  // row 0's last lane to row 1, 2's to 3
-  return plus_dpp<0x143, 0xc>(x);  // row 1's last lane to rows 2 and 3
+  return fa::wave_prefix(x, [](int a, int b) { return a + b; });
 }
 
 // The line of key blocks and its division. A request's items are equally long.
@@ -155,6 +147,13 @@ struct Line {
       }
       start += all;
     }
+  }
+  // Where request b starts.
+  __device__ __forceinline__ int before(int b) const {
+    if (per == 1) return b ? __builtin_amdgcn_readlane(through, b - 1) : 0;
+    int sum = 0;
+    for (int i = lane; i < b; i += 64) sum += Keys(a, a.kv_len[i]).blocks * a.heads_tiles;
+    return __builtin_amdgcn_readlane(wave_prefix(sum), 63);
   }
   __device__ __forceinline__ Keys keys(int b) {
     if ((unsigned)(b - c0) >= 64u) {
@@ -339,7 +338,7 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
         qb[kk] = as_half8(load16(qrow + kk * 16 + h * 8, FULL || kk * 16 + h * 8 < dr));
-      const float alibi_raw = a.alibi ? a.alibi[row.hq] * a.alibi_unit : 0.f;
+      const float slope = a.alibi ? a.alibi[row.hq] : 0.f;
       __builtin_amdgcn_sched_barrier(0);
       load(vt, base_v);
       // Keys [lo, hi) of this lane's row, and those that every row sees.
@@ -350,6 +349,7 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
       const int all_hi = a.causal ? at0 + 1 : keys.len;
       typename S::Offsets off;
       off.init(ln, 0);
+      const float alibi_raw = slope * a.alibi_unit;
       for (int j = j0; j < j1; ++j) {
         const unsigned long long hide = hidden;  // (of block j's pages, from page hide0 on)
         const int hide0 = p0;
@@ -544,12 +544,12 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
   if (lane == 0) a.owned[wg * kWaves + wave] = owned;
 }
 
-// Joins the parts of the items that several waves share. A workgroup takes the
-// items that one of paged_kernel's workgroups begins and others end (one of each
-// wave at most) and two of their runs of 64 float4 columns; its waves are dealt to
+// Joins the parts of the items that several waves share. A workgroup takes an item
+// (by_item), or those that one of paged_kernel's
+// workgroups begins and others end (one of each wave at most), and two of their runs of 64 float4 columns; its waves are dealt to
 // these and then to the parts, so that one long request's parts are read in a few rounds.
-// Bound by latency (the parts' list, then the parts), so it divides in floats and
-// leaves the list to paged_kernel.
+// Bound by latency (the lengths or the list of items that paged_kernel left, then
+// the parts), so it divides in floats.
 constexpr int kMergeWaves = 8;
 constexpr int kMergeRuns = 2;
 
@@ -565,11 +565,37 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
   __shared__ floatx4 accs[kMergeWaves][64];
   __shared__ float2 mls[kMergeWaves][64];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int stretch = a.sizes[0], total = a.sizes[1];
-  const int4 mine = lane < kWaves ? a.owned[blockIdx.x * kWaves + lane] : make_int4(0, 0, 0, 0);
+  int stretch, total;
+  auto div = [&](int x, int y) { return total < 1 << 17 ? small_div(x, y) : x / y; };
+  // The last of a stretch's waves that begins at or before its block x.
+  auto wave_of = [&](int x) { return stretch < kWaves ? x : div(kWaves * (x + 1) - 1, stretch); };
+  int4 mine = make_int4(0, 0, 0, 0);
+  int g0 = blockIdx.x;
+  if (a.by_item) {
+    Line<D> line(a, lane);
+    const int b = blockIdx.x / a.heads_tiles;
+    int start = line.before(b);
+    const Keys keys = line.keys(b);
+    stretch = line.stretch;
+    total = line.total;
+    const int item = blockIdx.x - b * a.heads_tiles;
+    start += item * keys.blocks;
+    const int last = start + keys.blocks - 1;
+    g0 = div(start, stretch);
+    const int owner = wave_of(start - g0 * stretch);
+    if (last < (g0 + 1) * stretch &&
+        (wave_of(last - g0 * stretch) == owner ||
+         (stretch >= Paged<D>::kJoinFrom && start == g0 * stretch &&
+          last + 1 == min((g0 + 1) * stretch, total))))
+      return;  // (written by its wave or workgroup)
+    if (lane == owner) mine = make_int4(b, item, start, keys.blocks);
+  } else {
+    stretch = a.sizes[0];
+    total = a.sizes[1];
+    if (lane < kWaves) mine = a.owned[blockIdx.x * kWaves + lane];
+  }
   const unsigned long long some = __ballot(mine.w > 0);
   if (some == 0) return;
-  auto div = [&](int x, int y) { return total < 1 << 17 ? small_div(x, y) : x / y; };
   const int run0 = blockIdx.y * kMergeRuns, runs = min(kMergeRuns, a.runs - run0);
   const int tasks = __popcll(some) * runs;
   const int per_round = min(tasks, kMergeWaves);
@@ -591,9 +617,9 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
     int head = end - start, middle = 0, tail = 0;
     int head_slot = start, first = start, step = 1, middle_slot = 0, tail_slot = 0;
     if (stretch >= Paged<D>::kJoinFrom) {
-      const int g0 = blockIdx.x, g1 = div(end - 1, stretch);
+      const int g1 = div(end - 1, stretch);
       const int x1 = end - g1 * stretch;  // (blocks of the item in g1's stretch, if not all)
-      const int last = stretch < kWaves ? x1 - 1 : div(kWaves * x1 - 1, stretch);  // (their last wave)
+      const int last = wave_of(x1 - 1);  // (their last wave)
       const bool whole0 = start == g0 * stretch && g0 < g1, whole1 = end == min((g1 + 1) * stretch, total);
       const int waves = min(kWaves, stretch);
       head = whole0 ? 1 : (g0 == g1 ? last + 1 : waves) - owner;
@@ -633,11 +659,12 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
         float2 x[kAtOnce];
         floatx4 o[kAtOnce];
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {  // (past the last: the last again, not added)
-          const size_t slot = (size_t)slot_of(min(p0 + i * groups, parts - 1)) * a.part_rows;
-          x[i] = ml[slot];
-          o[i] = *reinterpret_cast<const floatx4*>(po + slot * D);
-        }
+        for (int i = 0; i < kAtOnce; ++i)
+          if (p0 + i * groups < parts) {
+            const size_t slot = (size_t)slot_of(p0 + i * groups) * a.part_rows;
+            x[i] = ml[slot];
+            o[i] = *reinterpret_cast<const floatx4*>(po + slot * D);
+          }
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i)
           if (p0 + i * groups < parts) join(x[i].x, x[i].y, o[i]);
@@ -719,6 +746,13 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
   d.alibi_unit = kLog2e / d.scale_log2;
   d.alibi = a.alibi;
   d.stq = make_strides(a.layout, a.Hq, a.N, a.D);
+  // A join workgroup per item where that launches fewer and they are several per
+  // stretch (B=8 H=16/4 D=64, 5 tokens: 4.9 us against 6.0, where 1536 workgroups
+  // would start for 96 with work); else the list, a shorter way to the parts (B=1
+  // H=16/8 D=128: 3.5 us against 3.9).
+  const long long items = (long long)a.B * d.heads_tiles;
+  const unsigned slices = (unsigned)((d.runs + kMergeRuns - 1) / kMergeRuns);
+  d.by_item = slices > 1 && items <= Paged<D>::kGrid;
   auto launch = [&](auto full) {
     constexpr bool kFull = decltype(full)::value;
     hipLaunchKernelGGL((paged_kernel<D, FA_BF, kFull>), dim3(Paged<D>::kGrid), dim3(Paged<D>::kThreads),
@@ -726,7 +760,7 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((paged_merge_kernel<D, FA_BF, kFull>),
-                       dim3(Paged<D>::kGrid, (unsigned)((d.runs + kMergeRuns - 1) / kMergeRuns)),
+                       dim3(d.by_item ? (unsigned)items : Paged<D>::kGrid, slices),
                        dim3(64 * kMergeWaves), 0, (hipStream_t)a.stream, d);
     return hipGetLastError();
   };

@@ -26,20 +26,21 @@ namespace {
 // ring's.
 constexpr int kTabThreads = 256;  // and requests per tile
 
+// Sums saturate at 2^31 - 1, which is past every ring, table and slot array.
+__device__ __forceinline__ int sat_add(int a, int b) {
+  return (int)min((unsigned)a + (unsigned)b, 0x7fffffffu);
+}
 struct Sums {
-  long long need, gone, grown;  // pages to take and to return, tokens added
+  int need, gone, grown;  // pages to take and to return, tokens added
 };
 __device__ __forceinline__ Sums operator+(Sums a, Sums b) {
-  return {a.need + b.need, a.gone + b.gone, a.grown + b.grown};
-}
-__device__ __forceinline__ Sums shfl_up(Sums s, int d) {
-  return {__shfl_up(s.need, d), __shfl_up(s.gone, d), __shfl_up(s.grown, d)};
+  return {sat_add(a.need, b.need), sat_add(a.gone, b.gone), sat_add(a.grown, b.grown)};
 }
 
 struct Request {
-  int old, have, want, capped;  // tokens and pages before, pages and tokens wanted
-  long long grown;
-  __device__ __forceinline__ Request(const TablesArgs& a, int b) : old(0), have(0), want(0), capped(0), grown(0) {
+  int old, have, want, capped, grown;  // tokens and pages before, pages and tokens wanted, new ones
+  __device__ __forceinline__ Request(const TablesArgs& a, int b)
+      : old(0), have(0), want(0), capped(0), grown(0) {
     if (b >= a.B) return;
     const int cap = a.table_width << a.page_shift, n = max(a.new_len[b], 0);
     old = min(max(a.old_len[b], 0), cap);
@@ -54,7 +55,7 @@ struct Request {
 };
 
 // The first of `n` ascending values that is greater than x (n if none is).
-__device__ __forceinline__ int first_above(const long long* v, int n, long long x) {
+__device__ __forceinline__ int first_above(const int* v, int n, int x) {
   int lo = 0;
   for (int hi = n; lo < hi;) {
     const int mid = (lo + hi) >> 1;
@@ -66,40 +67,38 @@ __device__ __forceinline__ int first_above(const long long* v, int n, long long 
 
 __global__ __launch_bounds__(kTabThreads) void tables_kernel(const TablesArgs a) {
   // Of the tile's requests: the sums through each, and what a token needs.
-  __shared__ long long need_end[kTabThreads], gone_end[kTabThreads], grown_end[kTabThreads];
+  __shared__ int need_end[kTabThreads], gone_end[kTabThreads], grown_end[kTabThreads];
   __shared__ int olds[kTabThreads], haves[kTabThreads], wants[kTabThreads], lens[kTabThreads];
   __shared__ Sums waves[kTabThreads / 64];
   const int tid = threadIdx.x, C = a.n_ring;
-  const int head = (int)((((long long)a.ring[0] % C) + C) % C), count = min(max(a.ring[1], 0), C);
+  const int behind = a.ring[0] % C, head = behind < 0 ? behind + C : behind;
+  const int count = min(max(a.ring[1], 0), C);
   const int page_mask = (1 << a.page_shift) - 1;
   const bool packed = a.tokens >= 0;
   Sums carry{0, 0, 0};  // of the tiles before
-  // The page index at free entry i past the head.
-  auto ring_at = [&](long long i) { return (int)((head + i) % C); };
+  // The ring's entry i (below C) past the head.
+  auto ring_at = [&](int i) { return head + i < C ? head + i : head + i - C; };
   // This workgroup's share of n items.
-  auto share = [&](long long n, auto&& f) {
-    const long long per = (n + gridDim.x - 1) / gridDim.x, end = min(n, (blockIdx.x + 1) * per);
-    for (long long i = blockIdx.x * per + tid; i < end; i += kTabThreads) f(i);
+  auto share = [&](int n, auto&& f) {
+    const unsigned per = ((unsigned)n + gridDim.x - 1) / gridDim.x;
+    const unsigned end = min((unsigned)n, (blockIdx.x + 1) * per);
+    for (unsigned i = blockIdx.x * per + tid; i < end; i += kTabThreads) f((int)i);
   };
   // The slot of request r's (of the tile) token j, or -1.
-  auto slot_of = [&](int b, int r, long long j) {
-    if (j >= lens[r]) return -1;
+  auto slot_of = [&](int b, int r, unsigned j) {
+    if (j >= (unsigned)lens[r]) return -1;
     const int p = (int)(j >> a.page_shift);
-    const long long before = r ? need_end[r - 1] : carry.need;
+    const int before = r ? need_end[r - 1] : carry.need;
     const int page = p < haves[r] ? a.table[b * a.table_stride + p]
                                   : a.free_pages[ring_at(before + p - haves[r])];
-    const long long slot = ((long long)page << a.page_shift) + (j & page_mask);
+    const long long slot = ((long long)page << a.page_shift) + (int)(j & page_mask);
     return page < 0 || slot > 0x7fffffffLL ? -1 : (int)slot;
   };
   for (int b0 = 0; b0 < a.B; b0 += kTabThreads) {
     const int b = b0 + tid;
     const Request q(a, b);
     Sums s{max(q.want - q.have, 0), max(q.have - q.want, 0), q.grown};
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const Sums t = shfl_up(s, d);
-      if ((tid & 63) >= d) s = s + t;
-    }
+    s = {wave_prefix(s.need, sat_add), wave_prefix(s.gone, sat_add), wave_prefix(s.grown, sat_add)};
     if ((tid & 63) == 63) waves[tid >> 6] = s;
     __syncthreads();
     s = s + carry;
@@ -111,49 +110,47 @@ __global__ __launch_bounds__(kTabThreads) void tables_kernel(const TablesArgs a)
     haves[tid] = q.have;
     wants[tid] = q.want;
     const int need = max(q.want - q.have, 0);
-    const int given = (int)min((long long)need, max((long long)count - (s.need - need), 0LL));
-    const long long held = ((long long)q.have + given) << a.page_shift;
-    lens[tid] = q.capped > q.old ? (int)min((long long)q.capped, held) : q.capped;
+    // (past saturation nothing is left to give)
+    const int given = min(need, max(count - (s.need - need), 0));
+    const int held = (q.have + given) << a.page_shift;  // (at most the table's tokens)
+    lens[tid] = q.capped > q.old ? min(q.capped, held) : q.capped;
     if (b < a.B && blockIdx.x == 0) a.kv_len[b] = lens[tid];
     __syncthreads();
     const int n = min(kTabThreads, a.B - b0);
     // Pages taken, up to the free ones.
-    const long long taken = min(need_end[n - 1], (long long)count);
-    share(max(taken - carry.need, 0LL), [&](long long i) {
-      const long long x = carry.need + i;
+    share(max(min(need_end[n - 1], count) - carry.need, 0), [&](int i) {
+      const int x = carry.need + i;
       const int r = first_above(need_end, n, x);
-      const int p = haves[r] + (int)(x - (r ? need_end[r - 1] : carry.need));
+      const int p = haves[r] + x - (r ? need_end[r - 1] : carry.need);
       a.table[(b0 + r) * a.table_stride + p] = a.free_pages[ring_at(x)];
     });
     // Pages returned, as far as the ring has room.
-    share(max(min(gone_end[n - 1], (long long)(C - count)) - carry.gone, 0LL), [&](long long i) {
-      const long long x = carry.gone + i;
+    share(max(min(gone_end[n - 1], C - count) - carry.gone, 0), [&](int i) {
+      const int x = carry.gone + i;
       const int r = first_above(gone_end, n, x);
-      const int p = wants[r] + (int)(x - (r ? gone_end[r - 1] : carry.gone));
+      const int p = wants[r] + x - (r ? gone_end[r - 1] : carry.gone);
       a.free_pages[ring_at(count + x)] = a.table[(b0 + r) * a.table_stride + p];
     });
     if (packed) {
-      share(max(min(grown_end[n - 1], (long long)a.tokens) - carry.grown, 0LL), [&](long long i) {
-        const long long x = carry.grown + i;
-        const int r = first_above(grown_end, n, x);
-        const long long first = r ? grown_end[r - 1] : carry.grown;
-        a.slots[x] = slot_of(b0 + r, r, olds[r] + (x - first));
+      share(max(min(grown_end[n - 1], a.tokens) - carry.grown, 0), [&](int i) {
+        const int x = carry.grown + i, r = first_above(grown_end, n, x);
+        a.slots[x] = slot_of(b0 + r, r, (unsigned)olds[r] + (unsigned)(x - (r ? grown_end[r - 1] : carry.grown)));
       });
     } else if (a.max_new > 0) {
-      share((long long)n * a.max_new, [&](long long i) {
-        const int r = (int)((unsigned)i / (unsigned)a.max_new);
-        a.slots[(long long)b0 * a.max_new + i] = slot_of(b0 + r, r, olds[r] + (i - (long long)r * a.max_new));
+      share(n * a.max_new, [&](int i) {
+        const int r = a.max_new == 1 ? i : (int)((unsigned)i / (unsigned)a.max_new);
+        a.slots[b0 * a.max_new + i] = slot_of(b0 + r, r, (unsigned)olds[r] + (unsigned)(i - r * a.max_new));
       });
     }
     carry = {need_end[n - 1], gone_end[n - 1], grown_end[n - 1]};
     __syncthreads();
   }
   if (packed)
-    share(max(a.tokens - carry.grown, 0LL), [&](long long i) { a.slots[carry.grown + i] = -1; });
+    share(max(a.tokens - carry.grown, 0), [&](int i) { a.slots[carry.grown + i] = -1; });
   if (blockIdx.x == 0 && tid == 0) {
-    const long long taken = min(carry.need, (long long)count);
-    a.ring_out[0] = (int)((head + taken) % C);
-    a.ring_out[1] = (int)(count - taken + min(carry.gone, (long long)(C - count)));
+    const int taken = min(carry.need, count);
+    a.ring_out[0] = taken < C ? ring_at(taken) : head;
+    a.ring_out[1] = count - taken + min(carry.gone, C - count);
   }
 }
 
@@ -172,14 +169,15 @@ struct AppendArgs {
   long long items;            // tokens * chunks
 };
 
+template <class Index>  // (division of 64 bits takes longer than a step's copy)
 __global__ __launch_bounds__(kAppThreads) void append_kernel(const AppendArgs a) {
-  const long long step = (long long)gridDim.x * kAppThreads;
-  for (long long i = (long long)blockIdx.x * kAppThreads + threadIdx.x; i < a.items; i += step) {
-    const int t = (int)(i / a.chunks), x = (int)(i - (long long)t * a.chunks);
+  const Index step = (Index)gridDim.x * kAppThreads, items = (Index)a.items;
+  for (Index i = (Index)blockIdx.x * kAppThreads + threadIdx.x; i < items; i += step) {
+    const int t = (int)(i / (Index)a.chunks), x = (int)(i - (Index)t * a.chunks);
     const int slot = a.slots[t], page = slot >> a.pool.page_shift;
     if (slot < 0 || page >= a.pool.pages) continue;
     const int h = x / a.row_chunks, c = (x - h * a.row_chunks) * 8;
-    const int b = t / a.N, n = t - b * a.N;
+    const int b = a.N == 1 ? t : t / a.N, n = t - b * a.N;
     const long long to = page * a.pool.page_stride + h * a.pool.head_stride +
                          (slot - (page << a.pool.page_shift)) * a.pool.row_stride + c;
     const u32x4 k = *reinterpret_cast<const u32x4*>(a.k + b * a.sk.b + n * a.sk.n + h * a.sk.h + c);
@@ -213,9 +211,11 @@ hipError_t launch_paged_append(const void* k, const void* v, RowStrides sk, RowS
   a.row_chunks = D / 8;
   a.chunks = Hkv * a.row_chunks;
   a.items = (long long)B * N * a.chunks;
-  const long long blocks = (a.items + kAppThreads - 1) / kAppThreads;
-  hipLaunchKernelGGL(append_kernel, dim3((unsigned)std::min(blocks, 1LL << 20)), dim3(kAppThreads), 0,
-                     (hipStream_t)stream, a);
+  const unsigned blocks = (unsigned)std::min((a.items + kAppThreads - 1) / kAppThreads, 1LL << 20);
+  if (a.items <= 1LL << 31)  // (i + step stays below 2^32)
+    hipLaunchKernelGGL(append_kernel<uint32_t>, dim3(blocks), dim3(kAppThreads), 0, (hipStream_t)stream, a);
+  else
+    hipLaunchKernelGGL(append_kernel<uint64_t>, dim3(blocks), dim3(kAppThreads), 0, (hipStream_t)stream, a);
   return hipGetLastError();
 }
 
