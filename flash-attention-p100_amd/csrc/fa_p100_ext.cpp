@@ -855,12 +855,13 @@ std::vector<at::Tensor> fa_paged_attn_t(at::Tensor q, const at::Tensor& k_cache,
   cache.table_stride = B == 1 ? block_table.size(1) : block_table.stride(0);
   cache.table_width = (int)block_table.size(1);
   cache.kv_len = kv_len.data_ptr<int>();
-  at::Tensor o = at::empty_like(q), lse, ws;
+  at::Tensor o = at::empty_like(q), lse;
   if (want_lse) lse = at::empty({B, H, N}, q.options().dtype(at::kFloat));
   const size_t bytes = fa_paged_attn_workspace_bytes((int)B, (int)H, (int)Hkv, (int)N, (int)D);
-  if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  // (from torch's allocator as a tensor's memory is, without the tensor)
+  const c10::DataPtr ws = c10::GetAllocator(c10::DeviceType::CUDA)->allocate(bytes);
   check_rc(fa_paged_attn(q.data_ptr(), o.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr,
-                         &cache, bytes ? ws.data_ptr() : nullptr, bytes, (int)B, (int)H, (int)Hkv,
+                         &cache, ws.get(), bytes, (int)B, (int)H, (int)Hkv,
                          (int)N, (int)D, causal ? 1 : 0, &op, current_stream(q)),
            "fa_paged_attn");
   if (want_lse) return {o, lse};
