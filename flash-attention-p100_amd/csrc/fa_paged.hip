@@ -183,11 +183,16 @@ __device__ __forceinline__ void wait_lds() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// 16 bytes per lane from `from` to LDS at lds + byte_off + 16 * lane.
+// 16 bytes per lane from `from` to LDS at lds + byte_off + 16 * lane. STREAM: with
+// the nontemporal hint. K and V that one row tile reads are read once, and hinted
+// so they come at 6.5 TB/s (403 us at B=64 H=32/8 D=128, up to 16384 keys; 5.8 and
+// 449 without); several tiles find them in L2, where the hint takes them out (32 us
+// without it and 42 with it at 16 tiles, B=4 H=32/8 N=16, up to 8192 keys).
+template <bool STREAM>
 __device__ __forceinline__ void lds_direct(void* lds, const char* from, uint32_t byte_off) {
   auto* p = (__attribute__((address_space(3))) char*)lds + byte_off;
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                   (__attribute__((address_space(3))) void*)p, 16, 0, 0);
+                                   (__attribute__((address_space(3))) void*)p, 16, 0, STREAM ? 2 : 0);
 }
 
 // 16 bytes each at two or four LDS addresses. In assembly, with their wait: ahead
@@ -212,7 +217,8 @@ __device__ __forceinline__ void lds_read(const uint32_t (&at)[4], u32x4 (&out)[4
                : "memory");
 }
 
-template <int D, bool BF, bool FULL>  // FULL: the head dim is the width
+// FULL: the head dim is the width. ONE: one row tile per kv head.
+template <int D, bool BF, bool FULL, bool ONE>
 __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const PagedKernelArgs a) {
   using T = Paged<D>;
   using S = typename T::S;
@@ -261,7 +267,7 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
 
   do {
     const int from = pos - start, upto = min(from + end - pos, keys.blocks);
-    const int hkv = a.n_tiles == 1 ? item : item / a.n_tiles, tile = item - hkv * a.n_tiles;
+    const int hkv = ONE ? item : item / a.n_tiles, tile = ONE ? 0 : item - hkv * a.n_tiles;
     // The blocks [j0, j1), and the page indices around them.
     const int j0 = keys.first + from, j1 = keys.len > keys.lo ? keys.first + upto : j0;
     const int* table = a.table + b * a.table_stride;
@@ -313,7 +319,7 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
     auto load = [&](char* array, const char* base) {
 #pragma unroll
       for (int u = 0; u < kParts; ++u)
-        lds_direct(array, base + offs[u], (uint32_t)(wave * T::kTileBytes + u * 1024));
+        lds_direct<ONE>(array, base + offs[u], (uint32_t)(wave * T::kTileBytes + u * 1024));
     };
 
     // The way to the first loads is what a short call waits for: nothing that they
@@ -755,7 +761,9 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
   d.by_item = slices > 1 && items <= Paged<D>::kGrid;
   auto launch = [&](auto full) {
     constexpr bool kFull = decltype(full)::value;
-    hipLaunchKernelGGL((paged_kernel<D, FA_BF, kFull>), dim3(Paged<D>::kGrid), dim3(Paged<D>::kThreads),
+    const auto kernel = d.n_tiles == 1 ? paged_kernel<D, FA_BF, kFull, true>
+                                       : paged_kernel<D, FA_BF, kFull, false>;
+    hipLaunchKernelGGL(kernel, dim3(Paged<D>::kGrid), dim3(Paged<D>::kThreads),
                        0, (hipStream_t)a.stream, d);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
