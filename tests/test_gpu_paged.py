@@ -176,6 +176,25 @@ def test_append_matches_indexing(T, Hkv, D, page, dtype, layout):
         assert torch.equal(kc, want[0]) and torch.equal(vc, want[1]), form
 
 
+@pytest.mark.parametrize("Hkv,D,dtype", [(8, 128, torch.bfloat16), (3, 200, torch.half)])
+def test_append_of_many_tokens(Hkv, D, dtype):
+    """Prompts of more rows than L2 holds, with padding behind them: every row of the
+    pool either written or as it was."""
+    T, page = 20011, 32
+    g = torch.Generator(device=DEV).manual_seed(D)
+    P = T // page + 60
+    slots = torch.randperm(P * page, device=DEV, generator=g)[:T].to(torch.int32)
+    slots[-77:] = -1
+    kc, vc = (torch.randn(P, Hkv, page, D, device=DEV, generator=g).to(dtype) for _ in range(2))
+    k, v = (torch.randn(T, Hkv, D, device=DEV, generator=g).to(dtype) for _ in range(2))
+    want = [kc.clone(), vc.clone()]
+    at = slots[:-77].long()
+    for c, x in zip(want, (k, v)):
+        c[at // page, :, at % page] = x[:-77]
+    fa().paged_append(k, v, kc, vc, slots)
+    assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+
+
 def test_append_of_nothing_and_refusals():
     f = fa().paged_append
     kc, vc = pool_of(4, 2, 16, 64, torch.half, "bhnd")
