@@ -156,9 +156,10 @@ __global__ __launch_bounds__(kTabThreads) void tables_kernel(const TablesArgs a)
 
 // ---------------------------------------------------------------------------
 // Cache writes: a copy of each token's K and V rows to its slot, a thread per
-// 16-byte chunk of both. Bound by HBM at prompts (88 us for 65536 tokens of 8 heads
-// of 128, 529 MB moved at 6.0 TB/s; a copy of 2 GiB moves 4.95), by latency at a
-// step (2.7 us for 64 tokens).
+// 16-byte chunk, workgroups of K and of V in turn (both in one thread: 96 us where
+// this takes 88, into pages that hold the rows before the heads). Bound by HBM at
+// prompts (88 us for 65536 tokens of 8 heads of 128, 529 MB moved at 6.0 TB/s; a
+// copy of 2 GiB moves 4.95), by latency at a step (2.7 us for 64 tokens).
 constexpr int kAppThreads = 256;
 // Chunks from which loads and stores carry the nontemporal hint: 32 MB written, what
 // the L2s hold. Above, the hint takes 98 to 88 us at 268 MB and 27.4 to 24.3 at 67;
@@ -167,39 +168,34 @@ constexpr int kAppThreads = 256;
 constexpr long long kAppStream = 1LL << 20;
 
 struct AppendArgs {
-  const half_t* k;
-  const half_t* v;
-  RowStrides sk, sv;
+  const half_t* from[2];  // k and v, their strides and their pools
+  RowStrides strides[2];
+  half_t* to[2];
   const int* slots;
-  PagedPool pool;
+  long long page_stride, head_stride, row_stride;
+  int pages, page_shift;
   int N, row_chunks, chunks;  // 16-byte chunks of a row, and of a token's heads
   long long items;            // tokens * chunks
 };
 
 template <class Index, bool STREAM>  // (division of 64 bits takes longer than a step's copy)
 __global__ __launch_bounds__(kAppThreads) void append_kernel(const AppendArgs a) {
-  const Index step = (Index)gridDim.x * kAppThreads, items = (Index)a.items;
-  for (Index i = (Index)blockIdx.x * kAppThreads + threadIdx.x; i < items; i += step) {
+  const bool v = blockIdx.x & 1;
+  const half_t* const from = v ? a.from[1] : a.from[0];
+  const RowStrides s = v ? a.strides[1] : a.strides[0];
+  half_t* const to = v ? a.to[1] : a.to[0];
+  const Index step = (Index)(gridDim.x / 2) * kAppThreads, items = (Index)a.items;
+  for (Index i = (Index)(blockIdx.x / 2) * kAppThreads + threadIdx.x; i < items; i += step) {
     const int t = (int)(i / (Index)a.chunks), x = (int)(i - (Index)t * a.chunks);
-    const int slot = a.slots[t], page = slot >> a.pool.page_shift;
-    if (slot < 0 || page >= a.pool.pages) continue;
+    const int slot = a.slots[t], page = slot >> a.page_shift;
+    if (slot < 0 || page >= a.pages) continue;
     const int h = x / a.row_chunks, c = (x - h * a.row_chunks) * 8;
     const int b = a.N == 1 ? t : t / a.N, n = t - b * a.N;
-    const long long to = page * a.pool.page_stride + h * a.pool.head_stride +
-                         (slot - (page << a.pool.page_shift)) * a.pool.row_stride + c;
-    auto from = [](const half_t* p) {
-      const u32x4* x = reinterpret_cast<const u32x4*>(p);
-      return STREAM ? __builtin_nontemporal_load(x) : *x;
-    };
-    auto put = [](void* pool, long long at, u32x4 x) {
-      u32x4* y = reinterpret_cast<u32x4*>((half_t*)pool + at);
-      if constexpr (STREAM) __builtin_nontemporal_store(x, y);
-      else *y = x;
-    };
-    const u32x4 k = from(a.k + b * a.sk.b + n * a.sk.n + h * a.sk.h + c);
-    const u32x4 v = from(a.v + b * a.sv.b + n * a.sv.n + h * a.sv.h + c);
-    put(a.pool.k, to, k);
-    put(a.pool.v, to, v);
+    const u32x4* src = reinterpret_cast<const u32x4*>(from + b * s.b + n * s.n + h * s.h + c);
+    u32x4* dst = reinterpret_cast<u32x4*>(to + page * a.page_stride + h * a.head_stride +
+                                          (slot - (page << a.page_shift)) * a.row_stride + c);
+    if constexpr (STREAM) __builtin_nontemporal_store(__builtin_nontemporal_load(src), dst);
+    else *dst = *src;
   }
 }
 
@@ -216,18 +212,17 @@ hipError_t launch_paged_tables(const TablesArgs& a, void* stream) {
 hipError_t launch_paged_append(const void* k, const void* v, RowStrides sk, RowStrides sv,
                                const int* slots, const PagedPool& pool, int B, int N, int Hkv,
                                int D, void* stream) {
-  AppendArgs a{};
-  a.k = (const half_t*)k;
-  a.v = (const half_t*)v;
-  a.sk = sk;
-  a.sv = sv;
-  a.slots = slots;
-  a.pool = pool;
+  AppendArgs a{{(const half_t*)k, (const half_t*)v}, {sk, sv}, {(half_t*)pool.k, (half_t*)pool.v}, slots};
+  a.page_stride = pool.page_stride;
+  a.head_stride = pool.head_stride;
+  a.row_stride = pool.row_stride;
+  a.pages = pool.pages;
+  a.page_shift = pool.page_shift;
   a.N = N;
   a.row_chunks = D / 8;
   a.chunks = Hkv * a.row_chunks;
   a.items = (long long)B * N * a.chunks;
-  const unsigned blocks = (unsigned)std::min((a.items + kAppThreads - 1) / kAppThreads, 1LL << 20);
+  const unsigned blocks = 2 * (unsigned)std::min((a.items + kAppThreads - 1) / kAppThreads, 1LL << 20);
   // (32 bits while i + step stays below 2^32)
   const auto kernel = a.items < kAppStream    ? append_kernel<uint32_t, false>
                       : a.items <= 1LL << 31 ? append_kernel<uint32_t, true>
