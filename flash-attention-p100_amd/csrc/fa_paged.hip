@@ -79,7 +79,8 @@ struct PagedKernelArgs {
   int part_rows;    // of a tile: kRows, or all of a kv head's
   int B, Hq, group, N, n_tiles, heads_tiles, causal, window, dr;
   bool by_item;  // the join's workgroups take an item each
-  int runs;  // of 64 float4 columns in a tile's rows, a join's workgroup taking kMergeRuns
+  int runs;  // of 64 float4 columns in a tile's rows, slice (1 or 2) a join's workgroup
+  int slice;
   float scale_log2, rescale, alibi_unit;  // (the last two in units of q . k)
   const float* alibi;
   Strides stq;
@@ -557,7 +558,6 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
 // Bound by latency (the lengths or the list of items that paged_kernel left, then
 // the parts), so it divides in floats.
 constexpr int kMergeWaves = 8;
-constexpr int kMergeRuns = 2;
 
 // x / y for 0 <= x < 2^20, y >= 1: (x + 0.5) / y is 0.5 / y or more from a whole
 // number, and off by less than 2^-22 of itself.
@@ -602,7 +602,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
   }
   const unsigned long long some = __ballot(mine.w > 0);
   if (some == 0) return;
-  const int run0 = blockIdx.y * kMergeRuns, runs = min(kMergeRuns, a.runs - run0);
+  const int run0 = blockIdx.y * a.slice, runs = min(a.slice, a.runs - run0);
   const int tasks = __popcll(some) * runs;
   const int per_round = min(tasks, kMergeWaves);
   const int groups = small_div(kMergeWaves, per_round);  // waves that share a task's parts
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
   for (int t0 = 0; t0 < tasks; t0 += kMergeWaves) {
     const int task = t0 + wave - group * per_round;
     const bool active = task < tasks && group < groups;
-    const int nth = active ? (runs > 1 ? task / kMergeRuns : task) : 0, run = run0 + (active ? task - nth * runs : 0);
+    const int nth = active ? task >> (runs - 1) : 0, run = run0 + (active ? task - nth * runs : 0);
     unsigned long long left = some;
     for (int i = 0; i < nth; ++i) left &= left - 1;
     const int owner = __ffsll(left) - 1;
@@ -752,13 +752,14 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
   d.alibi_unit = kLog2e / d.scale_log2;
   d.alibi = a.alibi;
   d.stq = make_strides(a.layout, a.Hq, a.N, a.D);
-  // A join workgroup per item where that launches fewer and they are several per
-  // stretch (B=8 H=16/4 D=64, 5 tokens: 4.9 us against 6.0, where 1536 workgroups
-  // would start for 96 with work); else the list, a shorter way to the parts (B=1
-  // H=16/8 D=128: 3.5 us against 3.9).
+  // A join workgroup per item and run where that launches fewer (B=8 H=16/4 D=64, 5
+  // tokens: 4.9 us against 6.0, where 1536 workgroups would start for 96 with work);
+  // else the list, a shorter way to the parts (B=1 H=16/8 D=128: 3.5 us against 3.9),
+  // with two runs each (B=250 H=32/4 D=128: 47.2 us in all, 48.5 with one).
   const long long items = (long long)a.B * d.heads_tiles;
-  const unsigned slices = (unsigned)((d.runs + kMergeRuns - 1) / kMergeRuns);
-  d.by_item = slices > 1 && items <= Paged<D>::kGrid;
+  d.by_item = d.runs > 1 && items <= Paged<D>::kGrid;
+  d.slice = d.by_item ? 1 : 2;
+  const unsigned slices = (unsigned)((d.runs + d.slice - 1) / d.slice);
   auto launch = [&](auto full) {
     constexpr bool kFull = decltype(full)::value;
     const auto kernel = d.n_tiles == 1 ? paged_kernel<D, FA_BF, kFull, true>
