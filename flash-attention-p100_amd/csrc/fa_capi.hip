@@ -661,9 +661,10 @@ int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cach
   if (cache->table_width <= 0 || cache->table_stride < cache->table_width ||
       (long long)cache->table_width * cache->page_size > (1 << 30))
     return FA_ERR_PAGES;
-  // The key blocks of all row tiles are counted in 32 bits.
+  // The key blocks of all row tiles, with up to three more of each, are counted in
+  // 32 bits.
   const long long tiles = (long long)B * Hkv * (((long long)Hq / Hkv * N + 31) / 32);
-  if (tiles * ((long long)cache->table_width * cache->page_size / 32 + 2) > (1 << 30))
+  if (tiles * ((long long)cache->table_width * cache->page_size / 32 + 4) > (1 << 30))
     return FA_ERR_TOO_LARGE;
   const size_t need = fa::paged_workspace_bytes(Hq / Hkv * N, D);
   if (!q || !o || !cache->table || !cache->kv_len || (need && !workspace)) return FA_ERR_NULL;

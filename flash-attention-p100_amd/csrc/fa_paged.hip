@@ -104,7 +104,12 @@ __device__ __forceinline__ int wave_prefix(int x) {
   return fa::wave_prefix(x, [](int a, int b) { return a + b; });
 }
 
-// The line of key blocks and its division. A request's items are equally long.
+// The line of key blocks and its division. A request's items are equally long: a
+// unit per block and, where every wave has a block or more, `lead` of two before
+// them for the item's begin, whose loads nothing runs ahead of. (Of the waves of
+// B=250 H=32/4 D=128, up to 600 keys, those with one item took 23 us, with three 30,
+// at as many blocks. In all 47 us without the lead, 41 with it; 84 and 64 at B=200
+// H=16, up to 400 keys; 27.1 and 25.5 at B=24 H=12 D=64, window 1024.)
 template <int D>
 struct Line {
   using T = Paged<D>;
@@ -112,7 +117,8 @@ struct Line {
   const int lane;
   int lens, c0;      // kv_len of the requests c0 + lane (c0 < 0: none yet)
   int per, through;  // blocks of the requests up to (lane + 1) * per
-  int total, stretch;  // all blocks, and those of a workgroup
+  int lead;            // units of an item beside its blocks
+  int total, stretch;  // all units, and those of a workgroup
 
   __device__ __forceinline__ Line(const PagedKernelArgs& a, int lane)
       : a(a), lane(lane), lens(0), c0(a.B > 64 ? -64 : 0), per((a.B + 63) / 64) {
@@ -127,7 +133,14 @@ struct Line {
     through = wave_prefix(mine);
     total = __builtin_amdgcn_readlane(through, 63);
     stretch = (total + T::kGrid - 1) / T::kGrid;
+    lead = stretch >= T::kWaves ? 2 : 0;
+    if (lead) {
+      through += lead * min((lane + 1) * per, a.B) * a.heads_tiles;
+      total += lead * a.B * a.heads_tiles;
+      stretch = (total + T::kGrid - 1) / T::kGrid;
+    }
   }
+  __device__ __forceinline__ int units(const Keys& k) const { return k.blocks + lead; }
   // The request that holds position pos (< total), and where it starts.
   __device__ __forceinline__ void locate(int pos, int& b, int& start) {
     const int upto = __shfl_up(through, 1), before = lane ? upto : 0;
@@ -138,7 +151,7 @@ struct Line {
     for (c0 = b;; c0 += 64) {
       const int c = c0 + lane;
       lens = a.kv_len[min(c, a.B - 1)];
-      const int x = c < min(a.B, (run + 1) * per) ? Keys(a, lens).blocks * a.heads_tiles : 0;
+      const int x = c < min(a.B, (run + 1) * per) ? units(Keys(a, lens)) * a.heads_tiles : 0;
       const int sum = wave_prefix(x), all = __builtin_amdgcn_readlane(sum, 63);
       if (pos < start + all) {
         const int l = __ffsll(__ballot(start + sum > pos)) - 1;
@@ -153,7 +166,7 @@ struct Line {
   __device__ __forceinline__ int before(int b) const {
     if (per == 1) return b ? __builtin_amdgcn_readlane(through, b - 1) : 0;
     int sum = 0;
-    for (int i = lane; i < b; i += 64) sum += Keys(a, a.kv_len[i]).blocks * a.heads_tiles;
+    for (int i = lane; i < b; i += 64) sum += units(Keys(a, a.kv_len[i])) * a.heads_tiles;
     return __builtin_amdgcn_readlane(wave_prefix(sum), 63);
   }
   __device__ __forceinline__ Keys keys(int b) {
@@ -239,7 +252,7 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
   // The workgroup's stretch [wg0, wg1), and this wave's of it [pos, end): wave w
   // has block w of a stretch below kWaves, else begins at floor(w * stretch / kWaves).
   const int wg0 = wg * line.stretch, wg1 = min(wg0 + line.stretch, line.total);
-  int4 owned = make_int4(0, 0, 0, 0);  // request, item, its start and blocks (none: 0)
+  int4 owned = make_int4(0, 0, 0, 0);  // request, item, its start and units (none: 0)
   if (wg0 >= wg1) {
     if (lane == 0) a.owned[wg * kWaves + wave] = owned;
     return;
@@ -250,10 +263,10 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
   int b, start;
   line.locate(min(pos, wg1 - 1), b, start);
   Keys keys = line.keys(b);
-  int item = (min(pos, wg1 - 1) - start) / keys.blocks;
-  start += item * keys.blocks;  // of the item, from here on
+  int item = (min(pos, wg1 - 1) - start) / line.units(keys);
+  start += item * line.units(keys);  // of the item, from here on
   const bool joins = line.stretch >= T::kJoinFrom;
-  const bool join = joins && start <= wg0 && wg1 <= start + keys.blocks;
+  const bool join = joins && start <= wg0 && wg1 <= start + line.units(keys);
   if (!join && pos == end) {
     if (lane == 0) a.owned[wg * kWaves + wave] = owned;
     return;
@@ -267,10 +280,11 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
   constexpr int kWaitOlder = 0x0F70 | (kParts & 15) | ((kParts >> 4) << 14);
 
   do {
-    const int from = pos - start, upto = min(from + end - pos, keys.blocks);
+    const int units = line.units(keys), from = pos - start, upto = min(from + end - pos, units);
     const int hkv = ONE ? item : item / a.n_tiles, tile = ONE ? 0 : item - hkv * a.n_tiles;
     // The blocks [j0, j1), and the page indices around them.
-    const int j0 = keys.first + from, j1 = keys.len > keys.lo ? keys.first + upto : j0;
+    const int j0 = keys.first + max(from - line.lead, 0);
+    const int j1 = keys.len > keys.lo ? keys.first + max(upto - line.lead, 0) : j0;
     const int* table = a.table + b * a.table_stride;
     const int last_page = max(keys.len - 1, 0) >> a.page_shift;
     int p0 = 0, held = 0;           // pages p0 .. p0 + 63 are in the lanes' `held`
@@ -462,8 +476,8 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
     // block's position where no stretch is joined (a block is a part there).
     asm volatile("" : "+v"(ln));  // (addresses are worked out here, not kept through the loop)
     const int lh = ln >> 5, lr = ln & 31;
-    const int n_blocks = upto - from;
-    if (from == 0 && n_blocks > 0 && n_blocks < keys.blocks) owned = make_int4(b, item, start, keys.blocks);
+    const int n = upto - from;
+    if (from == 0 && n > 0 && n < units) owned = make_int4(b, item, start, units);
     size_t slot = joins ? 2 * (wg * kWaves + wave) + (from > 0 ? 0 : 1) : pos;
     half_t* orow = a.o + b * a.stq.b + row.hq * a.stq.h + (size_t)row.n * a.stq.n;
     auto finish = [&](bool whole, float m, float sum) {
@@ -484,9 +498,9 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
       }
     };
     if (!join) {
-      const bool whole = n_blocks == keys.blocks;
+      const bool whole = n == units;
       const float sum = l + xor32(l), inv = sum > 0.f ? 1.f / sum : 0.f;
-      if (row.ok && n_blocks > 0) {
+      if (row.ok && n > 0) {
 #pragma unroll
         for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
@@ -495,8 +509,8 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
                 floatx4{oacc[cb][4 * g], oacc[cb][4 * g + 1], oacc[cb][4 * g + 2], oacc[cb][4 * g + 3]});
         if (lh == 0) finish(whole, m_raw, sum);
       }
-      pos += n_blocks;
-      start += keys.blocks;
+      pos += n;
+      start += units;
       if (++item == a.heads_tiles && pos < end) {
         item = 0;
         keys = line.keys(++b);
@@ -505,7 +519,7 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
     }
     // One item: the waves' parts meet in LDS (the rows that there are), in the
     // accumulator's order: float4 (cb * 4 + g) * 64 + lane.
-    if (wg1 - wg0 == keys.blocks) owned.w = 0;
+    if (wg1 - wg0 == units) owned.w = 0;
     if (lane == 0) a.owned[wg * kWaves + wave] = owned;
     __syncthreads();
     auto part_of = [&](int src) {
@@ -531,7 +545,7 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
       wk[k] = x.x == -INFINITY ? 0.f : fast_exp2((x.x - m_star) * c);
       l_star += wk[k] * (x.y + ml[k * 64 + (ln ^ 32)].y);
     }
-    const bool whole = wg1 - wg0 == keys.blocks;
+    const bool whole = wg1 - wg0 == units;
     const float inv = l_star > 0.f ? 1.f / l_star : 0.f;
     slot = 2 * (size_t)(wg * kWaves);
     constexpr int kRuns = D / 8;  // float4 runs per lane, dealt to the waves
@@ -581,12 +595,12 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
     Line<D> line(a, lane);
     const int b = blockIdx.x / a.heads_tiles;
     int start = line.before(b);
-    const Keys keys = line.keys(b);
+    const int units = line.units(line.keys(b));
     stretch = line.stretch;
     total = line.total;
     const int item = blockIdx.x - b * a.heads_tiles;
-    start += item * keys.blocks;
-    const int last = start + keys.blocks - 1;
+    start += item * units;
+    const int last = start + units - 1;
     g0 = div(start, stretch);
     const int owner = wave_of(start - g0 * stretch);
     if (last < (g0 + 1) * stretch &&
@@ -594,7 +608,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
          (stretch >= Paged<D>::kJoinFrom && start == g0 * stretch &&
           last + 1 == min((g0 + 1) * stretch, total))))
       return;  // (written by its wave or workgroup)
-    if (lane == owner) mine = make_int4(b, item, start, keys.blocks);
+    if (lane == owner) mine = make_int4(b, item, start, units);
   } else {
     stretch = a.sizes[0];
     total = a.sizes[1];
