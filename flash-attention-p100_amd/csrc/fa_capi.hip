@@ -122,8 +122,8 @@ const char* fa_error_string(int err) {
              "from the query rows, and the backward needs block_cols with block_rows";
     case FA_ERR_PAGES:
       return "a paged cache needs a page size that is a power of two, positive sizes, 16-byte "
-             "aligned rows and at most 2^31 - 1 rows, and paged attention takes no option but the "
-             "format, layout, window, ALiBi slopes and scale";
+             "aligned rows and at most 2^31 - 1 rows, and paged attention 16-byte aligned buffers "
+             "and no option but the format, layout, window, ALiBi slopes and scale";
     case FA_ERR_SCRATCH:
       return "fa_bwd_noalloc: 2 * B*Hq*N floats exceed the built-in scratch "
              "(FA_BWD_NOALLOC_SCRATCH_BYTES); use fa_bwd with a workspace";
@@ -653,7 +653,8 @@ int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cach
   int rc = check_opts(op, causal, Hq, N, D, false);
   if (rc == FA_OK) rc = check_paged_shape(B, Hq, Hkv, N, D);
   if (rc != FA_OK) return rc;
-  if (op.kv_len || op.seg_start || op.mask || op.drop || op.bias || op.kv_rows || op.block_rows)
+  if (op.kv_len || op.seg_start || op.mask || op.mask_t || op.drop || op.drop_t || op.bias ||
+      op.kv_rows || op.block_rows)
     return FA_ERR_PAGES;
   fa::PagedArgs a{};
   rc = paged_pool(cache, Hkv, D, a.pool);
@@ -669,6 +670,7 @@ int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cach
   const size_t need = fa::paged_workspace_bytes(Hq / Hkv * N, D);
   if (!q || !o || !cache->table || !cache->kv_len || (need && !workspace)) return FA_ERR_NULL;
   if (workspace_bytes < need) return FA_ERR_WORKSPACE;
+  if (!aligned16(q) || !aligned16(o) || !aligned16(workspace)) return FA_ERR_PAGES;
   a.q = q;
   a.o = o;
   a.lse = lse;

@@ -691,6 +691,11 @@ static void check_no_grad(const at::Tensor& t, const char* name) {
               " requires grad, and paged caches have no backward: call under torch.no_grad()");
 }
 
+// A tensor has been written behind autograd's back: what was saved of it is stale.
+static void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // The stride of a dimension that is walked (one of size 1 has any stride).
 static int64_t walk(const at::Tensor& t, int64_t dim) { return t.size(dim) == 1 ? 0 : t.stride(dim); }
 
@@ -774,6 +779,8 @@ std::vector<at::Tensor> fa_paged_tables_t(const at::Tensor& block_table, const a
                            slots.data_ptr<int>(), kv_len.data_ptr<int>(), ring_out.data_ptr<int>(),
                            current_stream(block_table)),
            "fa_paged_tables");
+  written(block_table);
+  written(free_pages);
   return {slots, kv_len, ring_out};
 }
 
@@ -810,6 +817,8 @@ void fa_paged_append_t(at::Tensor k, at::Tensor v, const at::Tensor& k_cache,
                            walk(v, 0), flat ? 0 : walk(v, 2), walk(v, 1), slots.data_ptr<int>(),
                            &cache, (int)B, (int)N, (int)Hkv, (int)D, current_stream(k)),
            "fa_paged_append");
+  written(k_cache);
+  written(v_cache);
 }
 
 // [o] or [o, lse]: attention of the newest N tokens over the caches

@@ -148,7 +148,8 @@ struct Line {
     start = __builtin_amdgcn_readlane(before, run);
     b = run * per;
     if (per == 1) return;
-    for (c0 = b;; c0 += 64) {
+    // (the bounds hold for lengths that another stream changes meanwhile, too)
+    for (c0 = b; c0 < a.B; c0 += 64) {
       const int c = c0 + lane;
       lens = a.kv_len[min(c, a.B - 1)];
       const int x = c < min(a.B, (run + 1) * per) ? units(Keys(a, lens)) * a.heads_tiles : 0;
@@ -161,6 +162,8 @@ struct Line {
       }
       start += all;
     }
+    b = a.B - 1;
+    start = pos;
   }
   // Where request b starts.
   __device__ __forceinline__ int before(int b) const {
@@ -178,11 +181,23 @@ struct Line {
   }
 };
 
+// The kernel's arguments, read from memory where this stands. They take about as
+// many scalar registers as there are: held from the start, those that the rows and
+// results need were spilled ahead of the first loads, 100 instructions that a short
+// call waited for (19.5 us in all at B=8 H=16/4 D=64, 5 tokens, 18.7 without them).
+typedef __attribute__((address_space(4))) const PagedKernelArgs LateArgs;
+__device__ __forceinline__ LateArgs& late_args() {
+  auto* p = (LateArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+}
+
 // A lane's row of an item's tile.
 struct Row {
   bool ok;
   int hq, n;
-  __device__ __forceinline__ Row(const PagedKernelArgs& a, int hkv, int tile, int row) {
+  template <class Args>
+  __device__ __forceinline__ Row(const Args& a, int hkv, int tile, int row) {
     const int rows = a.group * a.N, r = tile * kRows + row, rc = min(r, rows - 1);
     const int g = a.N == 1 ? rc : rc / a.N;
     ok = r < rows;
@@ -276,7 +291,6 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
   char* const my_v = vt + wave * T::kTileBytes;
   const uint32_t page_bytes = 2u * (uint32_t)a.page_stride, row_bytes = 2u * (uint32_t)a.row_stride;
   const int page_mask = (1 << a.page_shift) - 1, dr = FULL ? D : a.dr, chunks = dr / 8;
-  const float c = a.scale_log2, thr_raw = a.rescale;
   constexpr int kWaitOlder = 0x0F70 | (kParts & 15) | ((kParts >> 4) << 14);
 
   do {
@@ -348,29 +362,30 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
     asm volatile("" : "+v"(ln));
     __builtin_amdgcn_sched_barrier(0);
     const int h = ln >> 5, l32 = ln & 31;
-    const Row row(a, hkv, tile, l32);
+    LateArgs& qa = late_args();
+    const Row row(qa, hkv, tile, l32);
     floatx16 oacc[D / 32];
 #pragma unroll
     for (int cb = 0; cb < D / 32; ++cb) oacc[cb] = zero16();
     float m_raw = -INFINITY, l = 0.f;
     if (j0 < j1) {
-      const half_t* qrow = a.q + b * a.stq.b + row.hq * a.stq.h + (size_t)row.n * a.stq.n;
+      const half_t* qrow = qa.q + b * qa.stq.b + row.hq * qa.stq.h + (size_t)row.n * qa.stq.n;
       half8 qb[D / 16];
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
         qb[kk] = as_half8(load16(qrow + kk * 16 + h * 8, FULL || kk * 16 + h * 8 < dr));
-      const float slope = a.alibi ? a.alibi[row.hq] : 0.f;
+      const float slope = qa.alibi ? qa.alibi[row.hq] : 0.f;
       __builtin_amdgcn_sched_barrier(0);
       load(vt, base_v);
       // Keys [lo, hi) of this lane's row, and those that every row sees.
-      const int at0 = keys.len - a.N, at = at0 + row.n;
-      const int lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
-      const int hi = a.causal ? min(keys.len, at + 1) : keys.len;
-      const int all_lo = a.window > 0 ? max(0, keys.len - a.window) : 0;
-      const int all_hi = a.causal ? at0 + 1 : keys.len;
+      const int at0 = keys.len - qa.N, at = at0 + row.n, window = qa.window;
+      const int lo = window > 0 ? max(0, at - window + 1) : 0;
+      const int hi = qa.causal ? min(keys.len, at + 1) : keys.len;
+      const int all_lo = window > 0 ? max(0, keys.len - window) : 0;
+      const int all_hi = qa.causal ? at0 + 1 : keys.len;
       typename S::Offsets off;
       off.init(ln, 0);
-      const float alibi_raw = slope * a.alibi_unit;
+      const float alibi_raw = slope * qa.alibi_unit, c = qa.scale_log2, thr_raw = qa.rescale;
       for (int j = j0; j < j1; ++j) {
         const unsigned long long hide = hidden;  // (of block j's pages, from page hide0 on)
         const int hide0 = p0;
@@ -476,20 +491,22 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
     // block's position where no stretch is joined (a block is a part there).
     asm volatile("" : "+v"(ln));  // (addresses are worked out here, not kept through the loop)
     const int lh = ln >> 5, lr = ln & 31;
+    LateArgs& ra = late_args();
+    const float c = ra.scale_log2;
     const int n = upto - from;
     if (from == 0 && n > 0 && n < units) owned = make_int4(b, item, start, units);
     size_t slot = joins ? 2 * (wg * kWaves + wave) + (from > 0 ? 0 : 1) : pos;
-    half_t* orow = a.o + b * a.stq.b + row.hq * a.stq.h + (size_t)row.n * a.stq.n;
+    half_t* orow = ra.o + b * ra.stq.b + row.hq * ra.stq.h + (size_t)row.n * ra.stq.n;
     auto finish = [&](bool whole, float m, float sum) {
-      if (!whole) a.part_ml[slot * a.part_rows + lr] = make_float2(m * c, sum);
-      else if (a.lse)
-        a.lse[((size_t)b * a.Hq + row.hq) * a.N + row.n] =
+      if (!whole) ra.part_ml[slot * ra.part_rows + lr] = make_float2(m * c, sum);
+      else if (ra.lse)
+        ra.lse[((size_t)b * ra.Hq + row.hq) * ra.N + row.n] =
             sum > 0.f ? (m * c + __log2f(sum)) * kLn2 : INFINITY;
     };
     // Columns col .. col + 3 (a row without keys: O = 0).
     auto put = [&](bool whole, float inv, int col, floatx4 v) {
       if (!whole) {
-        *reinterpret_cast<floatx4*>(a.part_o + (slot * a.part_rows + lr) * D + col) = v;
+        *reinterpret_cast<floatx4*>(ra.part_o + (slot * ra.part_rows + lr) * D + col) = v;
       } else if (FULL || col < dr) {
         half4 o4;
 #pragma unroll
@@ -512,15 +529,16 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
       pos += n;
       start += units;
       if (++item == a.heads_tiles && pos < end) {
+        if (++b == a.B) break;
         item = 0;
-        keys = line.keys(++b);
+        keys = line.keys(b);
       }
       continue;
     }
     // One item: the waves' parts meet in LDS (the rows that there are), in the
     // accumulator's order: float4 (cb * 4 + g) * 64 + lane.
     if (wg1 - wg0 == units) owned.w = 0;
-    if (lane == 0) a.owned[wg * kWaves + wave] = owned;
+    if (lane == 0) ra.owned[wg * kWaves + wave] = owned;
     __syncthreads();
     auto part_of = [&](int src) {
       return reinterpret_cast<float*>(src < kWaves / 2 ? kt : vt) + src % (kWaves / 2) * T::kFloats;
@@ -562,15 +580,15 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
     if (wave == 0 && lh == 0) finish(whole, m_star, l_star);
     return;
   } while (pos < end);
-  if (lane == 0) a.owned[wg * kWaves + wave] = owned;
+  if (lane == 0) late_args().owned[wg * kWaves + wave] = owned;
 }
 
 // Joins the parts of the items that several waves share. A workgroup takes an item
-// (by_item), or those that one of paged_kernel's
-// workgroups begins and others end (one of each wave at most), and two of their runs of 64 float4 columns; its waves are dealt to
-// these and then to the parts, so that one long request's parts are read in a few rounds.
-// Bound by latency (the lengths or the list of items that paged_kernel left, then
-// the parts), so it divides in floats.
+// (by_item), or those that one of paged_kernel's workgroups begins and others end
+// (one of each wave at most), and one or two of their runs of 64 float4 columns; its
+// waves are dealt to these and then to the parts, so that a long request's parts are
+// read in a few rounds. Bound by latency (the lengths, or the list of items that
+// paged_kernel left, then the parts: 3.6 to 7 us), so it divides in floats.
 constexpr int kMergeWaves = 8;
 
 // x / y for 0 <= x < 2^20, y >= 1: (x + 0.5) / y is 0.5 / y or more from a whole
@@ -651,7 +669,8 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
       middle_slot = 2 * (g0 + 1) * kWaves;
       tail_slot = 2 * g1 * kWaves;
     }
-    const int parts = head + middle + tail;
+    constexpr int kSlots = Paged<D>::kGrid * kWaves * 2;
+    const int parts = min(head + middle + tail, kSlots);
     auto slot_of = [&](int p) {
       if (p == 0) return first;
       if (p < head) return head_slot + p * step;
@@ -681,7 +700,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i)
           if (p0 + i * groups < parts) {
-            const size_t slot = (size_t)slot_of(p0 + i * groups) * a.part_rows;
+            const size_t slot = (size_t)min(slot_of(p0 + i * groups), kSlots - 1) * a.part_rows;
             x[i] = ml[slot];
             o[i] = *reinterpret_cast<const floatx4*>(po + slot * D);
           }

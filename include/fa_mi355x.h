@@ -70,7 +70,8 @@ enum {
                                 or (fa_pack_blocks) layout planes not 1 or B by 1 or Hq */
   FA_ERR_PAGES = 10019       /* a paged cache whose page size is not a power of two, whose
                                 sizes are not positive, whose rows are not 16-byte aligned, or
-                                with an option that paged attention does not take */
+                                with an option that paged attention does not take, or a
+                                buffer of its that is not 16-byte aligned */
 };
 
 /* Memory layouts of the 16-bit tensors, for the entry points that take one:
@@ -515,10 +516,12 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
  * of a batch are shared evenly among the GPU's compute units whatever their
  * lengths; partial results meet in `workspace`, of at least
  * fa_paged_attn_workspace_bytes() bytes (0 for invalid arguments), which may hold
- * anything. Calls that overlap in time need workspaces of their own. Hq * N <=
- * 2^24, and the 32-key blocks of full tables, times B, Hkv and the 32-row tiles of
- * Hq / Hkv * N, at most 2^30. The results are deterministic; a request's last bits may depend on the lengths of
- * the others in its batch. */
+ * anything. Calls that overlap in time need workspaces of their own. q, o and the
+ * workspace are 16-byte aligned; Hq * N <= 2^24, and the 32-key blocks of full
+ * tables, times B, Hkv and the 32-row tiles of Hq / Hkv * N, at most 2^30. The
+ * results are deterministic; a request's last bits may depend on the lengths of
+ * the others in its batch.
+ */
 size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
 int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
                   void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int N, int D,

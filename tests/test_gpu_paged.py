@@ -213,8 +213,10 @@ def test_append_of_nothing_and_refusals():
                 (k[None], k[None], kc, vc, s), (k.requires_grad_(), k, kc, vc, s)):
         with pytest.raises(RuntimeError):
             f(*bad)
+    versions = kc._version, vc._version
     with torch.no_grad():
         f(k, k, kc, vc, s)  # (requires grad)
+    assert kc._version > versions[0] and vc._version > versions[1]
     assert torch.equal(kc[0, :, :3].transpose(0, 1), k)
 
 

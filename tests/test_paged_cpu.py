@@ -93,15 +93,17 @@ def test_attn_refusals():
     assert call(B=1 << 16, c=cache(table_width=1 << 20, table_stride=1 << 20)) == 10007  # key blocks
     for bad in (fa_opts(kv_len=1), fa_opts(seg_start=1, seg_end=1), fa_opts(mask=1, mask_heads=1),
                 fa_opts(drop=1, drop_scale=1.0), fa_opts(bias=1), fa_opts(kv_rows=9),
-                fa_opts(block_rows=1)):
+                fa_opts(block_rows=1), fa_opts(mask_t=1), fa_opts(drop_t=1)):
         assert call(opts=bad) == 10019
     assert call(causal=0, opts=fa_opts(window=4)) == 10010
     assert call(opts=fa_opts(window=-1)) == 10010
     assert call(opts=fa_opts(scale=float("nan"))) == 10012
     assert call(opts=fa_opts(dtype=2)) == 10009 and call(opts=fa_opts(layout=2)) == 10008
     need = lib.fa_paged_attn_workspace_bytes(1, 4, 2, 1, 64)
-    if need:
-        assert call(nbytes=need - 1) == 10006 and call(ws=None) == 10005
+    assert need > 0 and call(nbytes=need - 1) == 10006 and call(ws=None) == 10005
+    for bad in (dict(q=24), dict(o=8), dict(ws=20)):  # alignment
+        assert call(**bad) == 10019, bad
+    assert call(c=cache(stride_page=1 << 31)) == 10007
     assert lib.fa_paged_attn_workspace_bytes(1, 4, 3, 1, 64) == 0
 
 
