@@ -322,6 +322,39 @@ def test_attn_batches_split_and_joined(lens, Hq, Hkv):
     check_attn(attn_inputs(lens, Hq, Hkv, 1, 64, 16, torch.half, seed=len(lens)))
 
 
+@pytest.mark.parametrize("lens,Hq,Hkv,N,D", [
+    ([9000, 3, 700], 32, 1, 1, 256),                     # 32 rows of 256: every part run of a join
+    ([5000, 1, 40], 7, 1, 5, 256),                       # 35 rows: a tile of three
+    ([13 * i % 400 for i in range(300)], 8, 1, 1, 128),  # more items than stretches' workgroups
+    ([3 * i % 50 for i in range(4500)], 1, 1, 1, 32),    # requests past 64 runs of 64
+    ([40000] * 3, 16, 2, 4, 64)])
+def test_attn_wide_tiles_and_large_batches(lens, Hq, Hkv, N, D):
+    check_attn(attn_inputs(lens, Hq, Hkv, N, D, 16, torch.bfloat16, seed=D))
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_attn_random_calls(seed):
+    """Every option crossed at random, requests shorter than N and pages outside the
+    pool among them."""
+    import random
+    r = random.Random(seed)
+    Hkv = r.choice([1, 1, 2, 3, 8])
+    Hq, N = Hkv * r.choice([1, 2, 5, 8]), r.choice([1, 1, 1, 2, 6, 33])
+    D, page = r.choice([16, 32, 64, 72, 96, 128, 128, 256]), 2 ** r.randint(0, 7)
+    top = r.choice([3, 90, 1200, 6000])
+    lens = [r.randint(0, top) for _ in range(r.choice([1, 2, 5, 20]))]
+    causal = r.random() < 0.7
+    window = r.choice([None, None, 1, 30, 700]) if causal else None
+    alibi = torch.tensor([r.random() for _ in range(Hq)], device=DEV) if r.random() < 0.3 else None
+    print(seed, lens, Hq, Hkv, N, D, page, causal, window, flush=True)
+    args = attn_inputs(lens, Hq, Hkv, N, D, page, r.choice([torch.half, torch.bfloat16]),
+                       r.choice(["bhnd", "bnhd", "halves", "wide"]), seed, r.randint(0, 3),
+                       r.choice([1.0, 1.0, 8.0]))
+    if r.random() < 0.3:
+        args[3][torch.rand(args[3].shape, generator=torch.Generator().manual_seed(seed)).to(DEV) < 0.1] = -1
+    check_attn(args, causal, window, alibi, r.choice([None, 0.05]))
+
+
 def test_attn_pages_outside_the_pool_hide_their_keys():
     q, kc, vc, table, kv_len = attn_inputs([640, 100, 33], 4, 2, 2, 64, 16, torch.half, seed=6)
     bad = table.clone()
@@ -425,6 +458,75 @@ def test_on_a_side_stream_and_in_two_threads():
         t.join()
     for outs, w in zip(got, want):
         assert all(torch.equal(o, w) for o in outs)
+
+
+def test_two_captured_graphs_replayed_at_once():
+    """Each captured call has a workspace of its own: replays overlap on two streams."""
+    calls = [attn_inputs([6000, 900], 8, 2, 1, 128, 16, torch.half, seed=3),
+             attn_inputs([200, 3000, 77], 16, 2, 3, 64, 32, torch.bfloat16, seed=4)]
+    want = [fa().paged_attn(*c) for c in calls]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for c in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(fa().paged_attn(*c))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        for o in outs:
+            o.fill_(float("nan"))
+        fa().paged_attn(*calls[0])  # eager work between the replays
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_capi_step_with_a_poisoned_workspace():
+    """The three entries through the C ABI: a NaN-filled workspace of the size asked
+    for, slots that are not 16-byte aligned, nothing written around either."""
+    from test_paged_cpu import Cache, capi
+    from helpers import fa_opts
+    import ctypes
+    lib, page, P, B, M, Hq, Hkv, D = capi(), 16, 4000, 6, 700, 8, 2, 128
+    g = torch.Generator().manual_seed(11)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    table, free = torch.full((B, M), -1, **i32), torch.randperm(P, generator=g).to(**i32)
+    old, ring = torch.zeros(B, **i32), torch.tensor([P - 5, P], **i32)
+    new = torch.tensor([9000, 0, 1, 700, 33, 5001], **i32)
+    T = int(new.sum())
+    slots = torch.full((T + 9,), -77, **i32)
+    kv_len, ring_out = torch.empty(B, **i32), torch.empty(2, **i32)
+    at = lambda t: t.data_ptr()
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.fa_paged_tables(at(table), M, M, at(old), at(new), at(free), P, at(ring), page, B, 0,
+                               T + 3, at(slots) + 4, at(kv_len), at(ring_out), stream) == 0
+    assert torch.equal(kv_len, new) and slots[0] == -77 and slots[T + 4:].tolist() == [-77] * 5
+    assert slots[T + 1:T + 4].tolist() == [-1] * 3
+    want = paged_ref.tables(*(x.cpu() for x in (torch.full_like(table, -1), old, new, free, ring)),
+                            page, tokens=T)
+    assert torch.equal(table.cpu(), want[0]) and torch.equal(slots[1:T + 1].cpu(), want[2])
+    k, v = (torch.randn(T, Hkv, D, generator=g).half().to(DEV) for _ in range(2))
+    kc, vc = (torch.full((P, Hkv, page, D), float("nan"), dtype=torch.half, device=DEV) for _ in range(2))
+    c = ctypes.pointer(Cache(at(kc), at(vc), kc.stride(0), kc.stride(1), kc.stride(2), P, page,
+                             at(table), M, M, at(kv_len)))
+    row = Hkv * D
+    assert lib.fa_paged_append(at(k), at(v), row, 0, D, row, 0, D, at(slots) + 4, c, T, 1, Hkv, D,
+                               stream) == 0
+    q = torch.randn(B, Hq, 1, D, generator=g).half().to(DEV)
+    o, lse = torch.full_like(q, float("nan")), torch.full((B, Hq, 1), float("nan"), device=DEV)
+    size = lib.fa_paged_attn_workspace_bytes(B, Hq, Hkv, 1, D)
+    ws = torch.full((size // 4 + 64,), float("nan"), device=DEV)
+    assert lib.fa_paged_attn(at(q), at(o), at(lse), c, at(ws), size, B, Hq, Hkv, 1, D, 1, fa_opts(),
+                             stream) == 0
+    torch.cuda.synchronize()
+    assert bool(torch.isnan(ws[size // 4:]).all())
+    paged_ref.check(o, lse, paged_ref.attention(q, kc, vc, table, kv_len))
+    assert torch.equal(fa().paged_attn(q, kc, vc, table, kv_len), o)
 
 
 # ------------------------------------------------------- the three together
