@@ -637,7 +637,8 @@ static int check_paged_shape(int B, int Hq, int Hkv, int N, int D) {
   if (N <= 0) return FA_ERR_SEQLEN;
   if (Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0) return FA_ERR_HEADS;
   if (B <= 0) return FA_ERR_BATCH;
-  if ((long long)Hq * N > (1 << 24)) return FA_ERR_TOO_LARGE;  // (rows of a request in an int)
+  // (rows of a request, and a token's elements, in an int)
+  if ((long long)Hq * N > (1 << 24) || (long long)Hq * D > INT_MAX) return FA_ERR_TOO_LARGE;
   return FA_OK;
 }
 
@@ -665,7 +666,8 @@ int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cach
   // The key blocks of all row tiles, with up to three more of each, are counted in
   // 32 bits.
   const long long tiles = (long long)B * Hkv * (((long long)Hq / Hkv * N + 31) / 32);
-  if (tiles * ((long long)cache->table_width * cache->page_size / 32 + 4) > (1 << 30))
+  const long long blocks = (long long)cache->table_width * cache->page_size / 32 + 4;
+  if (tiles > (1 << 30) / blocks)
     return FA_ERR_TOO_LARGE;
   const size_t need = fa::paged_workspace_bytes(Hq / Hkv * N, D);
   if (!q || !o || !cache->table || !cache->kv_len || (need && !workspace)) return FA_ERR_NULL;

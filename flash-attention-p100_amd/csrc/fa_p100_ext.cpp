@@ -719,7 +719,7 @@ static fa_paged_cache paged_cache(const at::Tensor& k, const at::Tensor& v, cons
               "k_cache and v_cache must both be (pages, Hkv, page_size, D)");
   const int64_t page_size = k.size(2);
   TORCH_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0 && k.size(0) > 0 &&
-                  k.size(0) * page_size <= INT32_MAX,
+                  k.size(0) <= INT32_MAX / page_size,
               "k_cache must hold 1 to 2^31 - 1 rows in pages of a power of two, got ", k.sizes());
   bool alike = rows_aligned(k) && rows_aligned(v);
   for (int64_t i = 0; i < 3; ++i) alike = alike && walk(k, i) == walk(v, i);
@@ -760,12 +760,12 @@ std::vector<at::Tensor> fa_paged_tables_t(const at::Tensor& block_table, const a
   TORCH_CHECK(free_pages.dim() == 1 && free_pages.size(0) > 0 && free_pages.size(0) <= INT32_MAX / 2,
               "free_pages must be a ring of one page index or more");
   TORCH_CHECK(ring.dim() == 1 && ring.size(0) == 2, "ring must be (2,): head and count");
-  TORCH_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0 && M * page_size <= (1 << 30),
+  TORCH_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0 && M <= (1 << 30) / page_size,
               "page_size must be a power of two, and a request's pages hold at most 2^30 tokens");
   TORCH_CHECK(max_new.has_value() != tokens.has_value(),
               "one of max_new (slots per request) and tokens (packed slots) must be given");
   const int64_t want = tokens ? *tokens : *max_new;
-  TORCH_CHECK(want >= 0 && B <= (1 << 20) && (tokens ? want : want * B) <= INT32_MAX,
+  TORCH_CHECK(want >= 0 && B <= (1 << 20) && want <= INT32_MAX / (tokens ? 1 : B),
               "max_new and tokens must not be negative, and the slots at most 2^31 - 1");
   c10::DeviceGuard guard(dev);
   at::AutoDispatchBelowADInplaceOrView below;  // (no gradient: the allocations skip its layers)
@@ -808,6 +808,8 @@ void fa_paged_append_t(at::Tensor k, at::Tensor v, const at::Tensor& k_cache,
               "slots must be int32 on ", k.device());
   TORCH_CHECK(slots.dim() == (flat ? 1 : 2) && slots.size(0) == B && (flat || slots.size(1) == N),
               "slots must be (T,) for k of (T, Hkv, D) and (B, N) for k of (B, Hkv, N, D)");
+  at::assert_no_internal_overlap(k_cache);  // (expanded ones, whose rows are several tokens')
+  at::assert_no_internal_overlap(v_cache);
   if (B * N * Hkv == 0) return;
   c10::DeviceGuard guard(k.device());
   if (!rows_aligned(k)) k = k.clone(at::MemoryFormat::Contiguous);
@@ -843,11 +845,11 @@ std::vector<at::Tensor> fa_paged_attn_t(at::Tensor q, const at::Tensor& k_cache,
   TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == B && block_table.size(1) > 0 &&
                   (B == 1 || block_table.stride(0) >= block_table.size(1)),
               "block_table must be (", B, ", pages per request)");
-  TORCH_CHECK(block_table.size(1) * cache.page_size <= (1 << 30),
+  TORCH_CHECK(block_table.size(1) <= (1 << 30) / cache.page_size,
               "a request's pages hold at most 2^30 tokens");
   check_ints(kv_len, q.device(), "kv_len");
   TORCH_CHECK(kv_len.dim() == 1 && kv_len.size(0) == B, "kv_len must be (", B, ",)");
-  TORCH_CHECK(B <= INT32_MAX && H * N <= (1 << 24), "shape exceeds the kernels' index range");
+  TORCH_CHECK(B <= INT32_MAX && H * N <= (1 << 24) && H * D <= INT32_MAX, "shape exceeds the kernels' index range");
   c10::DeviceGuard guard(q.device());
   at::AutoDispatchBelowADInplaceOrView below;
   fa_options op{};

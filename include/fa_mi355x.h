@@ -517,7 +517,7 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
  * lengths; partial results meet in `workspace`, of at least
  * fa_paged_attn_workspace_bytes() bytes (0 for invalid arguments), which may hold
  * anything. Calls that overlap in time need workspaces of their own. q, o and the
- * workspace are 16-byte aligned; Hq * N <= 2^24, and the 32-key blocks of full
+ * workspace are 16-byte aligned; Hq * N <= 2^24, Hq * D < 2^31, and the 32-key blocks of full
  * tables, times B, Hkv and the 32-row tiles of Hq / Hkv * N, at most 2^30. The
  * results are deterministic; a request's last bits may depend on the lengths of
  * the others in its batch.

@@ -118,6 +118,10 @@ def test_tables_refusals():
                 (t, old, new, free, ring, 1 << 30)):
         with pytest.raises(RuntimeError):
             f(*bad, max_new=1)
+    for kw in (dict(page_size=1 << 62, max_new=1), dict(page_size=16, max_new=1 << 62),
+               dict(page_size=16, tokens=1 << 62)):  # (products past 64 bits)
+        with pytest.raises(RuntimeError, match="2\\^30|2\\^31"):
+            f(t, old, new, free, ring, **kw)
 
 
 # ------------------------------------------------------------------ append
@@ -218,6 +222,16 @@ def test_append_of_nothing_and_refusals():
         f(k, k, kc, vc, s)  # (requires grad)
     assert kc._version > versions[0] and vc._version > versions[1]
     assert torch.equal(kc[0, :, :3].transpose(0, 1), k)
+
+
+def test_append_refuses_caches_whose_rows_are_shared():
+    k = torch.zeros(3, 2, 64, dtype=torch.half, device=DEV)
+    s = torch.arange(3, dtype=torch.int32, device=DEV)
+    one, whole = pool_of(1, 2, 16, 64, torch.half, "bhnd", fill=1.0)[0], pool_of(4, 1, 16, 64, torch.half, "bhnd")[0]
+    for kc in (one.expand(4, -1, -1, -1), whole.expand(-1, 2, -1, -1), whole[:, :, :1].expand(-1, 2, 16, -1)):
+        with pytest.raises(RuntimeError, match="single memory location"):
+            fa().paged_append(k, k, kc, kc, s)
+    assert bool((one == 1).all())
 
 
 # --------------------------------------------------------------- attention

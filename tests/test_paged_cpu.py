@@ -91,6 +91,10 @@ def test_attn_refusals():
         assert call(c=cache(**bad)) == 10019, bad
     assert call(N=1 << 23) == 10007  # rows of a request
     assert call(B=1 << 16, c=cache(table_width=1 << 20, table_stride=1 << 20)) == 10007  # key blocks
+    # (2^54 tiles of 2^10 blocks: their product in 64 bits is 0)
+    assert call(B=1 << 30, Hq=1 << 24, Hkv=1 << 24, D=8,
+                c=cache(table_width=1020, table_stride=1020, page_size=32)) == 10007
+    assert call(Hq=1 << 23, Hkv=1, N=2, D=256, opts=fa_opts(layout=1)) == 10007  # a token's elements
     for bad in (fa_opts(kv_len=1), fa_opts(seg_start=1, seg_end=1), fa_opts(mask=1, mask_heads=1),
                 fa_opts(drop=1, drop_scale=1.0), fa_opts(bias=1), fa_opts(kv_rows=9),
                 fa_opts(block_rows=1), fa_opts(mask_t=1), fa_opts(drop_t=1)):
