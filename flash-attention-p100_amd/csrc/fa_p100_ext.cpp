@@ -16,6 +16,8 @@
 // the backward its gradient buffer `dbias`). segment_bounds finds packed
 // sequences' bounds, and flash_attn is the autograd Function over these entries
 // for the calls that need no packed mask, dropout, bias or block lists.
+// paged_tables, paged_append and paged_attn are a serving step over a paged
+// key/value cache, without gradients.
 //
 // Plain C++ (no device code): every launch goes through the C ABI of
 // libfa_mi355x.so (include/fa_mi355x.h). Unlike the reference, which uses the

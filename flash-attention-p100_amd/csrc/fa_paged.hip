@@ -20,6 +20,9 @@
 //     64 pages and the K/V loads (direct to LDS, an address per lane) wait for
 //     nothing. Rows outside the request's keys read one of its rows instead: a
 //     masked key's P is zero, but zero times what an unused row holds may be NaN.
+// Measured at D=128, bf16: 399 us and 7 for the join at B=64 H=32/8, up to 16384
+// keys (2.6 GB, 6.5 TB/s; a large read reaches 6.3); 6.4 and 3.6 us for one request
+// of 1021 keys, H=16/8, most of it the way to the first keys.
 #include <type_traits>
 
 #include "fa_device.h"
@@ -460,6 +463,10 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
         half8 pb[2];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
+          // P is rounded to the inputs' format, half a step, as the second product's
+          // operand, whose matrix instruction takes no wider one; its sum, as S and O,
+          // is not. (Off the 64-bit results by 0.0019 to 0.0023 of their norm in bf16
+          // and 0.00029 in fp16; rounding the results alone is 0.0017 and 0.00021.)
           const float p = fast_exp2(fmaf(s[e], c, neg));
           l += p;
           pb[e >> 3][e & 7] = to16<BF>(p);

@@ -512,7 +512,8 @@ def paged_tables(block_table, old_len, new_len, free_pages, ring, page_size, max
       * free_pages (C,), updated in place: a ring of free page indices, and ring
         (2,): its first free entry and the number of free ones. Start with
         torch.arange(P) and [0, P) for a pool of P pages. Pages given back are
-        written behind the free ones and not taken again in the same call.
+        written behind the free ones and not taken again in the same call. A page is
+        one request's: one that stands in several tables would come back from each.
 
     Returned: kv_len (B,), new_len as far as there were pages (in the order of the
     requests; a request that got fewer has the tokens that its pages hold), the new
@@ -562,7 +563,8 @@ def paged_attn(q, k_cache, v_cache, block_table, kv_len, causal=True, sliding_wi
     flash_attn's, counted from each row's own token; without causal every row sees
     all of its request's tokens. A row without a key (an unused entry of the
     batch with kv_len 0, or the first rows of one with kv_len < N) gets o = 0 and
-    lse = +inf. Keys in pages whose index is outside the pool are hidden.
+    lse = +inf. Keys in pages whose index is outside the pool are hidden, and what
+    lies in rows that no row of q sees reaches no output.
 
     The requests' keys are dealt evenly to the GPU's compute units, so a batch of
     ragged lengths costs what its keys cost. Results are deterministic; the last

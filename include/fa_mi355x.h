@@ -480,8 +480,10 @@ typedef struct fa_paged_cache {
  *     With tokens < 0, max_new per request: slots[b * max_new + i] for token
  *     old_len[b] + i. Otherwise `tokens` of them, packed: the max(new_len -
  *     old_len, 0) new tokens of one request behind those of the one before.
- * A call with the same inputs again gives the same results (what it overwrites
- * it does not read), so kv_len, ring_out and slots must not overlap its inputs.
+ * A page is one request's: a page that stands in several tables would come back
+ * once from each. A call with the same inputs again gives the same results (what it
+ * overwrites it does not read), so kv_len, ring_out and slots must not overlap its
+ * inputs.
  * B <= 2^20, max_new * B and tokens <= 2^31 - 1, table_width * page_size <= 2^30.
  */
 int fa_paged_tables(int* table, long long table_stride, int table_width, const int* old_len,
@@ -508,8 +510,9 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
  * fa_fwd_ex (lse may be NULL); row n of entry b is token kv_len[b] - N + n, whose
  * own keys and values the cache holds already, and with `causal` it sees the
  * keys up to itself, else all of them. Rows without a key (kv_len[b] = 0, or
- * kv_len[b] < N: the first rows under causal masking) get o = 0, lse = +inf. Of
- * `opts`, dtype, layout, window (counted from the row's token), alibi_slopes and
+ * kv_len[b] < N: the first rows under causal masking) get o = 0, lse = +inf. What
+ * lies in rows of the pool that no row of q sees reaches no output, NaN included.
+ * Of `opts`, dtype, layout, window (counted from the row's token), alibi_slopes and
  * scale are taken (NULL: the defaults); anything else set is refused. With a
  * window the table entries of pages wholly outside it are not read. Keys in
  * pages whose index is outside [0, pages) are hidden like masked ones. The keys
@@ -517,10 +520,10 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
  * lengths; partial results meet in `workspace`, of at least
  * fa_paged_attn_workspace_bytes() bytes (0 for invalid arguments), which may hold
  * anything. Calls that overlap in time need workspaces of their own. q, o and the
- * workspace are 16-byte aligned; Hq * N <= 2^24, Hq * D < 2^31, and the 32-key blocks of full
- * tables, times B, Hkv and the 32-row tiles of Hq / Hkv * N, at most 2^30. The
- * results are deterministic; a request's last bits may depend on the lengths of
- * the others in its batch.
+ * workspace are 16-byte aligned; Hq * N <= 2^24, Hq * D < 2^31, and the 32-key
+ * blocks of full tables, times B, Hkv and the 32-row tiles of Hq / Hkv * N, at most
+ * 2^30. The results are deterministic; a request's last bits may depend on the
+ * lengths of the others in its batch.
  */
 size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
 int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
