@@ -43,9 +43,11 @@ struct Paged {
   static constexpr int kParts = (S::template bytes<kKeys>() + 1023) / 1024;  // loads of a tile
   static constexpr int kTileBytes = kParts * 1024;
   static constexpr int kFloats = kRows * D;  // a partial O
-  // Workgroups that share a CU's 160 KB of LDS.
-  static constexpr int kPerCu = kWaves * kTileBytes * 2 > 80 * 1024 ? 1 : 2;
-  static constexpr int kGrid = kCUs * kPerCu;
+  // One workgroup per CU. Its waves have 48 to 128 KB of K and V under way, as much as
+  // HBM needs: two per CU at D=64 read 5.4 TB/s where one reads 6.4 (B=32 H=32, up to
+  // 8000 keys), and one after another they begin twice (19.8 us for 15.0 at B=8 H=16/4
+  // D=64, 5 tokens, up to 4003 keys).
+  static constexpr int kGrid = kCUs;
   // The least stretch whose waves meet in LDS.
   static constexpr int kJoinFrom = 4;
   static_assert(kWaves / 2 * kFloats * 4 <= kWaves * kTileBytes, "merge area exceeds the tiles");
@@ -112,7 +114,7 @@ __device__ __forceinline__ int wave_prefix(int x) {
 // them for the item's begin, whose loads nothing runs ahead of. (Of the waves of
 // B=250 H=32/4 D=128, up to 600 keys, those with one item took 23 us, with three 30,
 // at as many blocks. In all 47 us without the lead, 41 with it; 84 and 64 at B=200
-// H=16, up to 400 keys; 27.1 and 25.5 at B=24 H=12 D=64, window 1024.)
+// H=16, up to 400 keys; 22.2 and 21.0 at B=24 H=12 D=64, window 1024.)
 template <int D>
 struct Line {
   using T = Paged<D>;
@@ -604,8 +606,10 @@ __device__ __forceinline__ int small_div(int x, int y) {
   return uniform((int)(((float)x + 0.5f) * __builtin_amdgcn_rcpf((float)y)));
 }
 
+// (Six waves per SIMD: up to 80 registers. Left to itself it takes 93, and where the list
+// is 1024 workgroups they come in more rounds: 5.0 us against 6.4 at B=60 H=16/2 D=256.)
 template <int D, bool BF, bool FULL>
-__global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const PagedKernelArgs a) {
+__global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const PagedKernelArgs a) {
   constexpr int kWaves = Paged<D>::kWaves;
   __shared__ floatx4 accs[kMergeWaves][64];
   __shared__ float2 mls[kMergeWaves][64];
@@ -792,12 +796,14 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
   d.alibi_unit = kLog2e / d.scale_log2;
   d.alibi = a.alibi;
   d.stq = make_strides(a.layout, a.Hq, a.N, a.D);
-  // A join workgroup per item and run where that launches fewer (B=8 H=16/4 D=64, 5
-  // tokens: 4.9 us against 6.0, where 1536 workgroups would start for 96 with work);
-  // else the list, a shorter way to the parts (B=1 H=16/8 D=128: 3.5 us against 3.9),
-  // with two runs each (B=250 H=32/4 D=128: 47.2 us in all, 48.5 with one).
+  // A join workgroup per item and run where these are at most half as many as the
+  // list's (3.8 us against 4.8 at B=8 H=16/4 D=64, 5 tokens: 160 and 768 workgroups;
+  // 4.6 against 6.1 at B=30 H=16/2 D=256: 480 and 1024); else the list, a shorter way to
+  // the parts (4.3 against 7.8 at B=40 H=16/4 D=64, 4 tokens: 512 and 640; 6.5 against
+  // 13.4 at B=100 H=16/2 D=256: 1024 and 1600), with two runs each (B=250 H=32/4
+  // D=128: 47.2 us in all, 48.5 with one).
   const long long items = (long long)a.B * d.heads_tiles;
-  d.by_item = d.runs > 1 && items <= Paged<D>::kGrid;
+  d.by_item = d.runs > 1 && 2 * items * d.runs <= Paged<D>::kGrid * ((d.runs + 1) / 2);
   d.slice = d.by_item ? 1 : 2;
   const unsigned slices = (unsigned)((d.runs + d.slice - 1) / d.slice);
   auto launch = [&](auto full) {
