@@ -48,8 +48,13 @@ struct Paged {
   // 8000 keys), and one after another they begin twice (19.8 us for 15.0 at B=8 H=16/4
   // D=64, 5 tokens, up to 4003 keys).
   static constexpr int kGrid = kCUs;
-  // The least stretch whose waves meet in LDS.
-  static constexpr int kJoinFrom = 4;
+  // Whether a workgroup's waves meet in LDS: from a stretch of four blocks on, or two
+  // where a part per block would be 64 or more for the items' mean (at D=128: 19.0 us
+  // against 29.5 for one item of 625 blocks, 13.8 and 14.3 for 8 of 94; 13.3 and 12.6
+  // for 32 of 19, 13.0 and 12.6 for 8 of 63).
+  __device__ __forceinline__ static bool joins(int stretch, int total, int items) {
+    return stretch >= 4 || (stretch >= 2 && total / 64 >= items);
+  }
   static_assert(kWaves / 2 * kFloats * 4 <= kWaves * kTileBytes, "merge area exceeds the tiles");
 
   // The row and 16-byte chunk that lane `lane` of load u brings in.
@@ -285,7 +290,7 @@ __global__ __launch_bounds__((Paged<D>::kThreads)) void paged_kernel(const Paged
   Keys keys = line.keys(b);
   int item = (min(pos, wg1 - 1) - start) / line.units(keys);
   start += item * line.units(keys);  // of the item, from here on
-  const bool joins = line.stretch >= T::kJoinFrom;
+  const bool joins = T::joins(line.stretch, line.total, a.B * a.heads_tiles);
   const bool join = joins && start <= wg0 && wg1 <= start + line.units(keys);
   if (!join && pos == end) {
     if (lane == 0) a.owned[wg * kWaves + wave] = owned;
@@ -634,7 +639,7 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const 
     const int owner = wave_of(start - g0 * stretch);
     if (last < (g0 + 1) * stretch &&
         (wave_of(last - g0 * stretch) == owner ||
-         (stretch >= Paged<D>::kJoinFrom && start == g0 * stretch &&
+         (Paged<D>::joins(stretch, total, a.B * a.heads_tiles) && start == g0 * stretch &&
           last + 1 == min((g0 + 1) * stretch, total))))
       return;  // (written by its wave or workgroup)
     if (lane == owner) mine = make_int4(b, item, start, units);
@@ -665,7 +670,7 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const 
     // of it). Where no stretch is joined, of each block.
     int head = end - start, middle = 0, tail = 0;
     int head_slot = start, first = start, step = 1, middle_slot = 0, tail_slot = 0;
-    if (stretch >= Paged<D>::kJoinFrom) {
+    if (Paged<D>::joins(stretch, total, a.B * a.heads_tiles)) {
       const int g1 = div(end - 1, stretch);
       const int x1 = end - g1 * stretch;  // (blocks of the item in g1's stretch, if not all)
       const int last = wave_of(x1 - 1);  // (their last wave)

@@ -346,6 +346,17 @@ def test_attn_wide_tiles_and_large_batches(lens, Hq, Hkv, N, D):
     check_attn(attn_inputs(lens, Hq, Hkv, N, D, 16, torch.bfloat16, seed=D))
 
 
+@pytest.mark.parametrize("lens,Hkv,D", [
+    # 256 workgroups of one to three blocks: few requests, whose workgroups' parts are
+    # joined first, and many, whose blocks are
+    ([8100], 1, 128), ([12000], 1, 64), ([20000], 1, 128), ([24500], 1, 32), ([30, 24000], 1, 96),
+    ([8000], 2, 256), ([5000, 5100, 4900], 1, 256), ([2040] * 8, 1, 128), ([2060] * 8, 1, 128),
+    ([600] * 8, 4, 64), ([1, 700, 0, 650, 33] * 4, 2, 128), ([31 * i for i in range(40)], 1, 64)])
+def test_attn_short_stretches(lens, Hkv, D):
+    for N in (1, 3):
+        check_attn(attn_inputs(lens, 4 * Hkv, Hkv, N, D, 32, torch.half, seed=N))
+
+
 @pytest.mark.parametrize("seed", range(48))
 def test_attn_random_calls(seed):
     """Every option crossed at random, requests shorter than N and pages outside the
