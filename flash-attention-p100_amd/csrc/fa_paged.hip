@@ -89,7 +89,7 @@ struct PagedKernelArgs {
   int part_rows;    // of a tile: kRows, or all of a kv head's
   int B, Hq, group, N, n_tiles, heads_tiles, causal, window, dr;
   bool by_item;  // the join's workgroups take an item each
-  int runs;  // of 64 float4 columns in a tile's rows, slice (1 or 2) a join's workgroup
+  int runs;  // of 64 or 16 float4 columns in a tile's rows, slice (1 or 2) a join's workgroup
   int slice;
   float scale_log2, rescale, alibi_unit;  // (the last two in units of q . k)
   const float* alibi;
@@ -613,7 +613,8 @@ __device__ __forceinline__ int small_div(int x, int y) {
 
 // (Six waves per SIMD: up to 80 registers. Left to itself it takes 93, and where the list
 // is 1024 workgroups they come in more rounds: 5.0 us against 6.4 at B=60 H=16/2 D=256.)
-template <int D, bool BF, bool FULL>
+// RUN: float4 columns of a run. Where they are 16, quarters of a wave take a part each.
+template <int D, bool BF, bool FULL, int RUN>
 __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const PagedKernelArgs a) {
   constexpr int kWaves = Paged<D>::kWaves;
   __shared__ floatx4 accs[kMergeWaves][64];
@@ -695,7 +696,9 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const 
     };
     const int hkv = a.n_tiles == 1 ? item : item / a.n_tiles, tile = item - hkv * a.n_tiles;
     const int rows = min(kRows, a.group * a.N - tile * kRows);
-    const int f = run * 64 + lane, rr = min(f / (D / 4), rows - 1), col = 4 * (f % (D / 4));
+    constexpr int kSubs = 64 / RUN;
+    const int sub = lane / RUN, f = run * RUN + lane % RUN;
+    const int rr = min(f / (D / 4), rows - 1), col = 4 * (f % (D / 4));
     float m = -INFINITY, l = 0.f;
     floatx4 acc = {0.f, 0.f, 0.f, 0.f};
     auto join = [&](float mo, float lo, floatx4 o) {
@@ -710,19 +713,26 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const 
       const float2* ml = a.part_ml + rr;
       const float* po = a.part_o + rr * D + col;
       constexpr int kAtOnce = 4;
-      for (int p0 = group; p0 < parts; p0 += kAtOnce * groups) {
+      const int step = groups * kSubs;
+      for (int p0 = group * kSubs + sub; p0 < parts; p0 += kAtOnce * step) {
         float2 x[kAtOnce];
         floatx4 o[kAtOnce];
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i)
-          if (p0 + i * groups < parts) {
-            const size_t slot = (size_t)min(slot_of(p0 + i * groups), kSlots - 1) * a.part_rows;
+          if (p0 + i * step < parts) {
+            const size_t slot = (size_t)min(slot_of(p0 + i * step), kSlots - 1) * a.part_rows;
             x[i] = ml[slot];
             o[i] = *reinterpret_cast<const floatx4*>(po + slot * D);
           }
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i)
-          if (p0 + i * groups < parts) join(x[i].x, x[i].y, o[i]);
+          if (p0 + i * step < parts) join(x[i].x, x[i].y, o[i]);
+      }
+#pragma unroll
+      for (int x = RUN; x < 64; x <<= 1) {
+        const floatx4 o = {__shfl_xor(acc[0], x), __shfl_xor(acc[1], x), __shfl_xor(acc[2], x),
+                           __shfl_xor(acc[3], x)};
+        join(__shfl_xor(m, x), __shfl_xor(l, x), o);
       }
     }
     if (groups > 1) {
@@ -732,12 +742,12 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const 
       }
       __syncthreads();
       if (active && group == 0)
-        for (int k = 1; k < min(groups, parts); ++k) {
+        for (int k = 1; k < min(groups, (parts + kSubs - 1) / kSubs); ++k) {
           const int w = wave + k * per_round;
           join(mls[w][lane].x, mls[w][lane].y, accs[w][lane]);
         }
     }
-    if (active && group == 0 && f < rows * (D / 4)) {
+    if (active && group == 0 && sub == 0 && f < rows * (D / 4)) {
       const Row row(a, hkv, tile, rr);
       const float inv = l > 0.f ? 1.f / l : 0.f;
       if (FULL || col < a.dr) {
@@ -790,7 +800,6 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
   d.part_ml = (float2*)(d.part_o + kAll * 2 * d.part_rows * D);
   d.owned = (int4*)(d.part_ml + kAll * 2 * d.part_rows);
   d.sizes = (int*)(d.owned + kAll);
-  d.runs = (d.part_rows * (D / 4) + 63) / 64;
   d.n_tiles = (d.group * a.N + kRows - 1) / kRows;
   d.heads_tiles = a.Hkv * d.n_tiles;
   d.causal = a.causal;
@@ -806,9 +815,17 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
   // 4.6 against 6.1 at B=30 H=16/2 D=256: 480 and 1024); else the list, a shorter way to
   // the parts (4.3 against 7.8 at B=40 H=16/4 D=64, 4 tokens: 512 and 640; 6.5 against
   // 13.4 at B=100 H=16/2 D=256: 1024 and 1600), with two runs each (B=250 H=32/4
-  // D=128: 47.2 us in all, 48.5 with one).
+  // D=128: 47.2 us in all, 48.5 with one). The list too for items of one run, but for
+  // up to four of them, whose parts can be many (at B=1 H=16/4 D=64: 4.2 us against
+  // 4.9 at 4000 keys, 3.9 and 3.4 at 1000).
   const long long items = (long long)a.B * d.heads_tiles;
-  d.by_item = d.runs > 1 && 2 * items * d.runs <= Paged<D>::kGrid * ((d.runs + 1) / 2);
+  const int columns = d.part_rows * (D / 4);
+  d.runs = (columns + 63) / 64;
+  d.by_item = (d.runs > 1 || items <= 4) && 2 * items * d.runs <= Paged<D>::kGrid * ((d.runs + 1) / 2);
+  // Of 16 columns where few workgroups would join many parts: 5.8 us for 9.0 at B=1 H=8/1
+  // D=128, 20000 keys (4 workgroups, 16 with shorter runs).
+  const bool narrow = d.by_item && items * d.runs <= 64;
+  if (narrow) d.runs = (columns + 15) / 16;
   d.slice = d.by_item ? 1 : 2;
   const unsigned slices = (unsigned)((d.runs + d.slice - 1) / d.slice);
   auto launch = [&](auto full) {
@@ -819,7 +836,9 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
                        0, (hipStream_t)a.stream, d);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_merge_kernel<D, FA_BF, kFull>),
+    const auto merge = narrow ? paged_merge_kernel<D, FA_BF, kFull, 16>
+                              : paged_merge_kernel<D, FA_BF, kFull, 64>;
+    hipLaunchKernelGGL(merge,
                        dim3(d.by_item ? (unsigned)items : Paged<D>::kGrid, slices),
                        dim3(64 * kMergeWaves), 0, (hipStream_t)a.stream, d);
     return hipGetLastError();

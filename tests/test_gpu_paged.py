@@ -351,7 +351,9 @@ def test_attn_wide_tiles_and_large_batches(lens, Hq, Hkv, N, D):
     # joined first, and many, whose blocks are
     ([8100], 1, 128), ([12000], 1, 64), ([20000], 1, 128), ([24500], 1, 32), ([30, 24000], 1, 96),
     ([8000], 2, 256), ([5000, 5100, 4900], 1, 256), ([2040] * 8, 1, 128), ([2060] * 8, 1, 128),
-    ([600] * 8, 4, 64), ([1, 700, 0, 650, 33] * 4, 2, 128), ([31 * i for i in range(40)], 1, 64)])
+    ([600] * 8, 4, 64), ([1, 700, 0, 650, 33] * 4, 2, 128), ([31 * i for i in range(40)], 1, 64),
+    # (the join's narrow runs: one item of few and of many parts, a tile of few columns)
+    ([50000], 1, 128), ([90000, 0], 1, 64), ([300, 7000], 2, 32), ([100, 90], 1, 16), ([40000], 2, 256)])
 def test_attn_short_stretches(lens, Hkv, D):
     for N in (1, 3):
         check_attn(attn_inputs(lens, 4 * Hkv, Hkv, N, D, 32, torch.half, seed=N))
