@@ -38,6 +38,13 @@ template <int D>
 struct Paged {
   static constexpr int kWaves = D > 128 ? 4 : 8;
   static constexpr int kThreads = 64 * kWaves;
+  // Row tiles of a kv head that waves abreast take, over the same keys, and the waves
+  // of each: what one brings in the others find in L2. (In all 113 us for 146 at B=20
+  // H=64/8 D=128, 7 tokens, up to 8000 keys, and 208 for 296 at D=256; tiles apart on
+  // the line read from HBM each, and are better where L2 holds all: 14.1 for 14.6 at
+  // B=1 H=64/8 D=128, 5 tokens, 2000 keys.)
+  template <int TILES>
+  static constexpr int kLine = kWaves / TILES;
   // Waves per SIMD that the compiler is to allow for. More than run, but asked for less
   // it spills scalar registers, 33 instead of 3 at D=64 (15.6 us in all for 15.2 at
   // B=60 H=16/4, up to 1000 keys).
@@ -56,8 +63,10 @@ struct Paged {
   // where a part per block would be 64 or more for the items' mean (at D=128: 19.0 us
   // against 29.5 for one item of 625 blocks, 13.8 and 14.3 for 8 of 94; 13.3 and 12.6
   // for 32 of 19, 13.0 and 12.6 for 8 of 63).
+  template <int TILES>
   __device__ __forceinline__ static bool joins(int stretch, int total, int items) {
-    return stretch >= 4 || (stretch >= 2 && total / 64 >= items);
+    constexpr int kFrom = kLine<TILES> < 4 ? kLine<TILES> : 4;  // (a wave's stretch is a block below)
+    return stretch >= kFrom || (stretch >= 2 && total / (64 / TILES) >= items);
   }
   static_assert(kWaves / 2 * kFloats * 4 <= kWaves * kTileBytes, "merge area exceeds the tiles");
 
@@ -91,7 +100,8 @@ struct PagedKernelArgs {
   int4* owned;      // (wave): the item that it begins and does not end (see Owned)
   int* sizes;       // Line's stretch and total
   int part_rows;    // of a tile: kRows, or all of a kv head's
-  int B, Hq, group, N, n_tiles, heads_tiles, causal, window, dr;
+  // items: of a request, groups of row tiles of each kv head
+  int B, Hq, group, N, n_groups, items, causal, window, dr;
   bool by_item;  // the join's workgroups take an item each
   int runs;  // of 64 or 16 float4 columns in a tile's rows, slice (1 or 2) a join's workgroup
   int slice;
@@ -124,7 +134,7 @@ __device__ __forceinline__ int wave_prefix(int x) {
 // B=250 H=32/4 D=128, up to 600 keys, those with one item took 23 us, with three 30,
 // at as many blocks. In all 47 us without the lead, 41 with it; 84 and 64 at B=200
 // H=16, up to 400 keys; 22.2 and 21.0 at B=24 H=12 D=64, window 1024.)
-template <int D>
+template <int D, int TILES>
 struct Line {
   using T = Paged<D>;
   const PagedKernelArgs& a;
@@ -141,16 +151,16 @@ struct Line {
       const int c = lane * per + i;
       if (c < a.B) {
         lens = a.kv_len[c];
-        mine += Keys(a, lens).blocks * a.heads_tiles;
+        mine += Keys(a, lens).blocks * a.items;
       }
     }
     through = wave_prefix(mine);
     total = __builtin_amdgcn_readlane(through, 63);
     stretch = (total + T::kGrid - 1) / T::kGrid;
-    lead = stretch >= T::kWaves ? 2 : 0;
+    lead = stretch >= T::template kLine<TILES> ? 2 : 0;
     if (lead) {
-      through += lead * min((lane + 1) * per, a.B) * a.heads_tiles;
-      total += lead * a.B * a.heads_tiles;
+      through += lead * min((lane + 1) * per, a.B) * a.items;
+      total += lead * a.B * a.items;
       stretch = (total + T::kGrid - 1) / T::kGrid;
     }
   }
@@ -166,7 +176,7 @@ struct Line {
     for (c0 = b; c0 < a.B; c0 += 64) {
       const int c = c0 + lane;
       lens = a.kv_len[min(c, a.B - 1)];
-      const int x = c < min(a.B, (run + 1) * per) ? units(Keys(a, lens)) * a.heads_tiles : 0;
+      const int x = c < min(a.B, (run + 1) * per) ? units(Keys(a, lens)) * a.items : 0;
       const int sum = wave_prefix(x), all = __builtin_amdgcn_readlane(sum, 63);
       if (pos < start + all) {
         const int l = __ffsll(__ballot(start + sum > pos)) - 1;
@@ -183,7 +193,7 @@ struct Line {
   __device__ __forceinline__ int before(int b) const {
     if (per == 1) return b ? __builtin_amdgcn_readlane(through, b - 1) : 0;
     int sum = 0;
-    for (int i = lane; i < b; i += 64) sum += units(Keys(a, a.kv_len[i])) * a.heads_tiles;
+    for (int i = lane; i < b; i += 64) sum += units(Keys(a, a.kv_len[i])) * a.items;
     return __builtin_amdgcn_readlane(wave_prefix(sum), 63);
   }
   __device__ __forceinline__ Keys keys(int b) {
@@ -230,7 +240,7 @@ __device__ __forceinline__ void wait_lds() {
 // the nontemporal hint. K and V that one row tile reads are read once, and hinted
 // so they come at 6.5 TB/s (403 us at B=64 H=32/8 D=128, up to 16384 keys; 5.8 and
 // 449 without); several tiles find them in L2, where the hint takes them out (32 us
-// without it and 42 with it at 16 tiles, B=4 H=32/8 N=16, up to 8192 keys).
+// without it and 42 with it at B=4 H=32/8 D=128, 16 tokens, up to 8192 keys).
 template <bool STREAM>
 __device__ __forceinline__ void lds_direct(void* lds, const char* from, uint32_t byte_off) {
   auto* p = (__attribute__((address_space(3))) char*)lds + byte_off;
@@ -260,12 +270,13 @@ __device__ __forceinline__ void lds_read(const uint32_t (&at)[4], u32x4 (&out)[4
                : "memory");
 }
 
-// FULL: the head dim is the width. ONE: one row tile per kv head.
-template <int D, bool BF, bool FULL, bool ONE>
+// FULL: the head dim is the width. TILES: row tiles that waves abreast take. STREAM:
+// there is one per kv head.
+template <int D, bool BF, bool FULL, int TILES, bool STREAM>
 __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_kernel(const PagedKernelArgs a) {
   using T = Paged<D>;
   using S = typename T::S;
-  constexpr int kWaves = T::kWaves, kParts = T::kParts;
+  constexpr int kWaves = T::kWaves, kLine = T::template kLine<TILES>, kParts = T::kParts;
   __shared__ __align__(1024) char kt[kWaves * T::kTileBytes];
   __shared__ __align__(1024) char vt[kWaves * T::kTileBytes];
   __shared__ float2 ml[kWaves * 64];
@@ -273,31 +284,32 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
   const int wave = uniform(tid >> 6);
   __builtin_assume(wave >= 0 && wave < kWaves);
   const int wg = xcd_work_index(T::kGrid);
-  Line<D> line(a, lane);
+  const int on = wave / TILES, beside = wave % TILES;  // (of the waves on the line, of the tiles)
+  Line<D, TILES> line(a, lane);
   if (wg == 0 && tid == 0) {
     a.sizes[0] = line.stretch;
     a.sizes[1] = line.total;
   }
   // The workgroup's stretch [wg0, wg1), and this wave's of it [pos, end): wave w
-  // has block w of a stretch below kWaves, else begins at floor(w * stretch / kWaves).
+  // has block w of a stretch below kLine, else begins at floor(w * stretch / kLine).
   const int wg0 = wg * line.stretch, wg1 = min(wg0 + line.stretch, line.total);
   int4 owned = make_int4(0, 0, 0, 0);  // request, item, its start and units (none: 0)
   if (wg0 >= wg1) {
-    if (lane == 0) a.owned[wg * kWaves + wave] = owned;
+    if (lane == 0 && beside == 0) a.owned[wg * kLine + on] = owned;
     return;
   }
-  const bool single = line.stretch < kWaves;
-  int pos = min(wg0 + (single ? wave : wave * line.stretch / kWaves), wg1);
-  const int end = min(wg0 + (single ? wave + 1 : (wave + 1) * line.stretch / kWaves), wg1);
+  const bool single = line.stretch < kLine;
+  int pos = min(wg0 + (single ? on : on * line.stretch / kLine), wg1);
+  const int end = min(wg0 + (single ? on + 1 : (on + 1) * line.stretch / kLine), wg1);
   int b, start;
   line.locate(min(pos, wg1 - 1), b, start);
   Keys keys = line.keys(b);
   int item = (min(pos, wg1 - 1) - start) / line.units(keys);
   start += item * line.units(keys);  // of the item, from here on
-  const bool joins = T::joins(line.stretch, line.total, a.B * a.heads_tiles);
+  const bool joins = T::template joins<TILES>(line.stretch, line.total, a.B * a.items);
   const bool join = joins && start <= wg0 && wg1 <= start + line.units(keys);
   if (!join && pos == end) {
-    if (lane == 0) a.owned[wg * kWaves + wave] = owned;
+    if (lane == 0 && beside == 0) a.owned[wg * kLine + on] = owned;
     return;
   }
 
@@ -309,10 +321,12 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
 
   do {
     const int units = line.units(keys), from = pos - start, upto = min(from + end - pos, units);
-    const int hkv = ONE ? item : item / a.n_tiles, tile = ONE ? 0 : item - hkv * a.n_tiles;
+    const int hkv = STREAM || a.n_groups == 1 ? item : item / a.n_groups;
+    const int tile = STREAM ? 0 : (item - hkv * a.n_groups) * TILES + beside;
     // The blocks [j0, j1), and the page indices around them.
     const int j0 = keys.first + max(from - line.lead, 0);
-    const int j1 = keys.len > keys.lo ? keys.first + max(upto - line.lead, 0) : j0;
+    const bool some = keys.len > keys.lo && tile * kRows < a.group * a.N;  // (keys and rows)
+    const int j1 = some ? keys.first + max(upto - line.lead, 0) : j0;
     const int* table = a.table + b * a.table_stride;
     const int last_page = max(keys.len - 1, 0) >> a.page_shift;
     int p0 = 0, held = 0;           // pages p0 .. p0 + 63 are in the lanes' `held`
@@ -362,7 +376,7 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
     auto load = [&](char* array, const char* base) {
 #pragma unroll
       for (int u = 0; u < kParts; ++u)
-        lds_direct<ONE>(array, base + offs[u], (uint32_t)(wave * T::kTileBytes + u * 1024));
+        lds_direct<STREAM>(array, base + offs[u], (uint32_t)(wave * T::kTileBytes + u * 1024));
     };
 
     // The way to the first loads is what a short call waits for: nothing that they
@@ -513,7 +527,7 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
     const float c = ra.scale_log2;
     const int n = upto - from;
     if (from == 0 && n > 0 && n < units) owned = make_int4(b, item, start, units);
-    size_t slot = joins ? 2 * (wg * kWaves + wave) + (from > 0 ? 0 : 1) : pos;
+    size_t slot = (joins ? 2 * (wg * kLine + on) + (from > 0 ? 0 : 1) : pos) * TILES + beside;
     half_t* orow = ra.o + b * ra.stq.b + row.hq * ra.stq.h + (size_t)row.n * ra.stq.n;
     auto finish = [&](bool whole, float m, float sum) {
       if (!whole) ra.part_ml[slot * ra.part_rows + lr] = make_float2(m * c, sum);
@@ -546,7 +560,7 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
       }
       pos += n;
       start += units;
-      if (++item == a.heads_tiles && pos < end) {
+      if (++item == a.items && pos < end) {
         if (++b == a.B) break;
         item = 0;
         keys = line.keys(b);
@@ -556,7 +570,7 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
     // One item: the waves' parts meet in LDS (the rows that there are), in the
     // accumulator's order: float4 (cb * 4 + g) * 64 + lane.
     if (wg1 - wg0 == units) owned.w = 0;
-    if (lane == 0) ra.owned[wg * kWaves + wave] = owned;
+    if (lane == 0 && beside == 0) ra.owned[wg * kLine + on] = owned;
     __syncthreads();
     auto part_of = [&](int src) {
       return reinterpret_cast<float*>(src < kWaves / 2 ? kt : vt) + src % (kWaves / 2) * T::kFloats;
@@ -572,33 +586,34 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
     ml[wave * 64 + ln] = make_float2(m_raw, l);
     __syncthreads();
     if (!row.ok) return;
-    float m_star = -INFINITY, l_star = 0.f, wk[kWaves];
+    float m_star = -INFINITY, l_star = 0.f, wk[kLine];
+    const float2* const mine = ml + beside * 64;
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) m_star = fmaxf(m_star, ml[k * 64 + ln].x);
+    for (int k = 0; k < kLine; ++k) m_star = fmaxf(m_star, mine[k * TILES * 64 + ln].x);
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-      const float2 x = ml[k * 64 + ln];
+    for (int k = 0; k < kLine; ++k) {
+      const float2 x = mine[k * TILES * 64 + ln];
       wk[k] = x.x == -INFINITY ? 0.f : fast_exp2((x.x - m_star) * c);
-      l_star += wk[k] * (x.y + ml[k * 64 + (ln ^ 32)].y);
+      l_star += wk[k] * (x.y + mine[k * TILES * 64 + (ln ^ 32)].y);
     }
     const bool whole = wg1 - wg0 == units;
     const float inv = l_star > 0.f ? 1.f / l_star : 0.f;
-    slot = 2 * (size_t)(wg * kWaves);
+    slot = 2 * (size_t)(wg * kLine) * TILES + beside;
     constexpr int kRuns = D / 8;  // float4 runs per lane, dealt to the waves
 #pragma unroll
-    for (int i = 0; i < (kRuns + kWaves - 1) / kWaves; ++i) {
-      const int run = i * kWaves + wave;
+    for (int i = 0; i < (kRuns + kLine - 1) / kLine; ++i) {
+      const int run = i * kLine + on;
       if (run >= kRuns) break;
       floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k)
-        acc += *reinterpret_cast<const floatx4*>(part_of(k) + (run * 64 + ln) * 4) * wk[k];
+      for (int k = 0; k < kLine; ++k)
+        acc += *reinterpret_cast<const floatx4*>(part_of(k * TILES + beside) + (run * 64 + ln) * 4) * wk[k];
       put(whole, inv, 8 * run + 4 * lh, acc);
     }
-    if (wave == 0 && lh == 0) finish(whole, m_star, l_star);
+    if (on == 0 && lh == 0) finish(whole, m_star, l_star);
     return;
   } while (pos < end);
-  if (lane == 0) late_args().owned[wg * kWaves + wave] = owned;
+  if (lane == 0 && beside == 0) late_args().owned[wg * kLine + on] = owned;
 }
 
 // Joins the parts of the items that several waves share. A workgroup takes an item
@@ -618,9 +633,9 @@ __device__ __forceinline__ int small_div(int x, int y) {
 // (Six waves per SIMD: up to 80 registers. Left to itself it takes 93, and where the list
 // is 1024 workgroups they come in more rounds: 5.0 us against 6.4 at B=60 H=16/2 D=256.)
 // RUN: float4 columns of a run. Where they are 16, quarters of a wave take a part each.
-template <int D, bool BF, bool FULL, int RUN>
+template <int D, bool BF, bool FULL, int TILES, int RUN>
 __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const PagedKernelArgs a) {
-  constexpr int kWaves = Paged<D>::kWaves;
+  constexpr int kLine = Paged<D>::template kLine<TILES>;
   __shared__ floatx4 accs[kMergeWaves][64];
   __shared__ float2 mls[kMergeWaves][64];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -629,43 +644,44 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const 
   int stretch, total;
   auto div = [&](int x, int y) { return total < 1 << 17 ? small_div(x, y) : x / y; };
   // The last of a stretch's waves that begins at or before its block x.
-  auto wave_of = [&](int x) { return stretch < kWaves ? x : div(kWaves * (x + 1) - 1, stretch); };
+  auto wave_of = [&](int x) { return stretch < kLine ? x : div(kLine * (x + 1) - 1, stretch); };
   int4 mine = make_int4(0, 0, 0, 0);
   int g0 = blockIdx.x;
   if (a.by_item) {
-    Line<D> line(a, lane);
-    const int b = blockIdx.x / a.heads_tiles;
+    Line<D, TILES> line(a, lane);
+    const int b = blockIdx.x / a.items;
     int start = line.before(b);
     const int units = line.units(line.keys(b));
     stretch = line.stretch;
     total = line.total;
-    const int item = blockIdx.x - b * a.heads_tiles;
+    const int item = blockIdx.x - b * a.items;
     start += item * units;
     const int last = start + units - 1;
     g0 = div(start, stretch);
     const int owner = wave_of(start - g0 * stretch);
     if (last < (g0 + 1) * stretch &&
         (wave_of(last - g0 * stretch) == owner ||
-         (Paged<D>::joins(stretch, total, a.B * a.heads_tiles) && start == g0 * stretch &&
+         (Paged<D>::template joins<TILES>(stretch, total, a.B * a.items) && start == g0 * stretch &&
           last + 1 == min((g0 + 1) * stretch, total))))
       return;  // (written by its wave or workgroup)
     if (lane == owner) mine = make_int4(b, item, start, units);
   } else {
     stretch = a.sizes[0];
     total = a.sizes[1];
-    if (lane < kWaves) mine = a.owned[blockIdx.x * kWaves + lane];
+    if (lane < kLine) mine = a.owned[blockIdx.x * kLine + lane];
   }
   const unsigned long long some = __ballot(mine.w > 0);
   if (some == 0) return;
-  const int run0 = blockIdx.y * a.slice, runs = min(a.slice, a.runs - run0);
+  const int run0 = blockIdx.y * a.slice, runs = min(a.slice, a.runs * TILES - run0);
   const int tasks = __popcll(some) * runs;
   const int per_round = min(tasks, kMergeWaves);
   const int groups = small_div(kMergeWaves, per_round);  // waves that share a task's parts
   const int group = small_div(wave, per_round);
   for (int t0 = 0; t0 < tasks; t0 += kMergeWaves) {
     const int task = t0 + wave - group * per_round;
-    const bool active = task < tasks && group < groups;
-    const int nth = active ? task >> (runs - 1) : 0, run = run0 + (active ? task - nth * runs : 0);
+    bool active = task < tasks && group < groups;
+    const int nth = active ? TILES == 1 ? task >> (runs - 1) : small_div(task, runs) : 0, part_run = run0 + (active ? task - nth * runs : 0);
+    const int beside = TILES == 1 ? 0 : part_run / a.runs, run = part_run - beside * a.runs;
     unsigned long long left = some;
     for (int i = 0; i < nth; ++i) left &= left - 1;
     const int owner = __ffsll(left) - 1;
@@ -677,31 +693,33 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const 
     // of it). Where no stretch is joined, of each block.
     int head = end - start, middle = 0, tail = 0;
     int head_slot = start, first = start, step = 1, middle_slot = 0, tail_slot = 0;
-    if (Paged<D>::joins(stretch, total, a.B * a.heads_tiles)) {
+    if (Paged<D>::template joins<TILES>(stretch, total, a.B * a.items)) {
       const int g1 = div(end - 1, stretch);
       const int x1 = end - g1 * stretch;  // (blocks of the item in g1's stretch, if not all)
       const int last = wave_of(x1 - 1);  // (their last wave)
       const bool whole0 = start == g0 * stretch && g0 < g1, whole1 = end == min((g1 + 1) * stretch, total);
-      const int waves = min(kWaves, stretch);
+      const int waves = min(kLine, stretch);
       head = whole0 ? 1 : (g0 == g1 ? last + 1 : waves) - owner;
       middle = max(g1 - g0 - 1, 0);
       tail = g0 == g1 ? 0 : whole1 ? 1 : last + 1;
-      head_slot = 2 * (g0 * kWaves + owner);
+      head_slot = 2 * (g0 * kLine + owner);
       first = head_slot + (whole0 ? 0 : 1);
       step = 2;
-      middle_slot = 2 * (g0 + 1) * kWaves;
-      tail_slot = 2 * g1 * kWaves;
+      middle_slot = 2 * (g0 + 1) * kLine;
+      tail_slot = 2 * g1 * kLine;
     }
-    constexpr int kSlots = Paged<D>::kGrid * kWaves * 2;
+    constexpr int kSlots = Paged<D>::kGrid * kLine * 2;
     const int parts = min(head + middle + tail, kSlots);
     auto slot_of = [&](int p) {
       if (p == 0) return first;
       if (p < head) return head_slot + p * step;
       p -= head;
-      return p < middle ? middle_slot + p * 2 * kWaves : tail_slot + (p - middle) * 2;
+      return p < middle ? middle_slot + p * 2 * kLine : tail_slot + (p - middle) * 2;
     };
-    const int hkv = a.n_tiles == 1 ? item : item / a.n_tiles, tile = item - hkv * a.n_tiles;
+    const int hkv = a.n_groups == 1 ? item : item / a.n_groups;
+    const int tile = (item - hkv * a.n_groups) * TILES + beside;
     const int rows = min(kRows, a.group * a.N - tile * kRows);
+    active = active && rows > 0;
     constexpr int kSubs = 64 / RUN;
     const int sub = lane / RUN, f = run * RUN + lane % RUN;
     const int rr = min(f / (D / 4), rows - 1), col = 4 * (f % (D / 4));
@@ -726,7 +744,8 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const 
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i)
           if (p0 + i * step < parts) {
-            const size_t slot = (size_t)min(slot_of(p0 + i * step), kSlots - 1) * a.part_rows;
+            const size_t slot =
+                (size_t)(min(slot_of(p0 + i * step), kSlots - 1) * TILES + beside) * a.part_rows;
             x[i] = ml[slot];
             o[i] = *reinterpret_cast<const floatx4*>(po + slot * D);
           }
@@ -806,8 +825,15 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
   d.part_ml = (float2*)(d.part_o + kAll * 2 * d.part_rows * D);
   d.owned = (int4*)(d.part_ml + kAll * 2 * d.part_rows);
   d.sizes = (int*)(d.owned + kAll);
-  d.n_tiles = (d.group * a.N + kRows - 1) / kRows;
-  d.heads_tiles = a.Hkv * d.n_tiles;
+  const int n_tiles = (d.group * a.N + kRows - 1) / kRows;
+  // Several row tiles per kv head go abreast, two or four, but where full tables are
+  // 16 MB, which L2 holds anyway, and where a half of two pairs would be idle.
+  const bool small = (long long)a.B * d.cap * a.Hkv * a.D * 4 <= 16 << 20;
+  const int tiles = n_tiles == 1 || small || (D > 128 && n_tiles == 3) ? 1
+                    : n_tiles == 2 || D > 128                           ? 2
+                                                                        : 4;
+  d.n_groups = (n_tiles + tiles - 1) / tiles;
+  d.items = a.Hkv * d.n_groups;
   d.causal = a.causal;
   d.window = a.window < d.cap ? a.window : 0;  // (a wider one hides nothing)
   d.dr = a.D;
@@ -824,32 +850,40 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
   // D=128: 47.2 us in all, 48.5 with one). The list too for items of one run, but for
   // up to four of them, whose parts can be many (at B=1 H=16/4 D=64: 4.2 us against
   // 4.9 at 4000 keys, 3.9 and 3.4 at 1000).
-  const long long items = (long long)a.B * d.heads_tiles;
+  const long long items = (long long)a.B * d.items;
   const int columns = d.part_rows * (D / 4);
   d.runs = (columns + 63) / 64;
-  d.by_item = (d.runs > 1 || items <= 4) && 2 * items * d.runs <= Paged<D>::kGrid * ((d.runs + 1) / 2);
+  d.by_item = (d.runs > 1 || items <= 4) &&
+              2 * items * d.runs * tiles <= Paged<D>::kGrid * ((d.runs * tiles + 1) / 2);
   // Of 16 columns where few workgroups would join many parts: 5.8 us for 9.0 at B=1 H=8/1
   // D=128, 20000 keys (4 workgroups, 16 with shorter runs).
-  const bool narrow = d.by_item && items * d.runs <= 64;
+  const bool narrow = d.by_item && items * d.runs * tiles <= 64;
   if (narrow) d.runs = (columns + 15) / 16;
-  d.slice = d.by_item ? 1 : 2;
-  const unsigned slices = (unsigned)((d.runs + d.slice - 1) / d.slice);
-  auto launch = [&](auto full) {
-    constexpr bool kFull = decltype(full)::value;
-    const auto kernel = d.n_tiles == 1 ? paged_kernel<D, FA_BF, kFull, true>
-                                       : paged_kernel<D, FA_BF, kFull, false>;
-    hipLaunchKernelGGL(kernel, dim3(Paged<D>::kGrid), dim3(Paged<D>::kThreads),
-                       0, (hipStream_t)a.stream, d);
+  d.slice = d.by_item ? 1 : 2 * tiles;
+  const unsigned slices = (unsigned)((d.runs * tiles + d.slice - 1) / d.slice);
+  auto launch = [&](auto full, auto abreast, auto stream) {
+    constexpr bool kFull = decltype(full)::value, kStream = decltype(stream)::value;
+    constexpr int kTiles = decltype(abreast)::value;
+    hipLaunchKernelGGL((paged_kernel<D, FA_BF, kFull, kTiles, kStream>), dim3(Paged<D>::kGrid),
+                       dim3(Paged<D>::kThreads), 0, (hipStream_t)a.stream, d);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const auto merge = narrow ? paged_merge_kernel<D, FA_BF, kFull, 16>
-                              : paged_merge_kernel<D, FA_BF, kFull, 64>;
+    const auto merge = narrow ? paged_merge_kernel<D, FA_BF, kFull, kTiles, 16>
+                              : paged_merge_kernel<D, FA_BF, kFull, kTiles, 64>;
     hipLaunchKernelGGL(merge,
                        dim3(d.by_item ? (unsigned)items : Paged<D>::kGrid, slices),
                        dim3(64 * kMergeWaves), 0, (hipStream_t)a.stream, d);
     return hipGetLastError();
   };
-  return a.D == D ? launch(std::true_type{}) : launch(std::false_type{});
+  auto by_tiles = [&](auto full) {
+    using std::false_type, std::true_type;
+    if (n_tiles == 1) return launch(full, std::integral_constant<int, 1>{}, true_type{});
+    if (tiles == 1) return launch(full, std::integral_constant<int, 1>{}, false_type{});
+    if constexpr (D <= 128)
+      if (tiles == 4) return launch(full, std::integral_constant<int, 4>{}, false_type{});
+    return launch(full, std::integral_constant<int, 2>{}, false_type{});
+  };
+  return a.D == D ? by_tiles(std::true_type{}) : by_tiles(std::false_type{});
 }
 
 }  // namespace fa

@@ -359,6 +359,23 @@ def test_attn_short_stretches(lens, Hkv, D):
         check_attn(attn_inputs(lens, 4 * Hkv, Hkv, N, D, 32, torch.half, seed=N))
 
 
+@pytest.mark.parametrize("D", [32, 64, 80, 128, 256])
+@pytest.mark.parametrize("lens,Hq,Hkv,N", [
+    ([9000, 3, 700], 7, 1, 5),                  # two row tiles, the second of three rows
+    ([5000], 33, 1, 2), ([50, 0, 1300], 48, 2, 3),  # three
+    ([40, 2000, 333], 8, 1, 15), ([70000], 16, 1, 10),  # four, five
+    ([3, 800, 90], 4, 2, 100),                  # seven, and requests shorter than N
+    ([41 * i for i in range(24)], 16, 2, 5), ([300] * 100, 40, 1, 1)])
+def test_attn_row_tiles_abreast(lens, Hq, Hkv, N, D):
+    """Full tables past 16 MB: the row tiles of a kv head go side by side."""
+    spare = (16 << 20) // (4 * Hkv * D * 16) // len(lens) + 2
+    args = attn_inputs(lens, Hq, Hkv, N, D, 16, torch.bfloat16, seed=N, spare=spare)
+    check_attn(args)
+    if N > 1:
+        check_attn(args, causal=False)
+        check_attn(args, window=60, alibi=torch.rand(Hq, device=DEV))
+
+
 @pytest.mark.parametrize("seed", range(48))
 def test_attn_random_calls(seed):
     """Every option crossed at random, requests shorter than N and pages outside the
