@@ -2,7 +2,7 @@
 // (tables and cache writes: fa_pages.hip). No counterpart in the reference,
 // which has no cache.
 //
-// Bound: HBM, each K/V row is read once per 32 query rows. As in fa_dec.hip a row
+// Bound: HBM, each K/V row is read once per 32 to 128 query rows. As in fa_dec.hip a row
 // tile is 32 rows of one kv head (the rows of the query heads of its group, head
 // after head), a wave's step is a block of 32 keys of its own LDS tiles, and the
 // products are S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16. What is
@@ -14,15 +14,16 @@
 //     it, and writes the result of an item that it has whole; the parts of the
 //     others meet in paged_merge_kernel. No wave waits for a longer request. Where
 //     a workgroup's stretch lies within one item, its waves' parts meet in LDS
-//     first: long requests then leave an eighth of the parts;
+//     first: long requests then leave an eighth of the parts. Several row tiles of a
+//     kv head go side by side, as many waves over the same stretch;
 //   * a wave's lanes hold the next 64 page indices of its stretch; a block's rows
 //     take theirs from there by a lane permutation, so the table is read once in
 //     64 pages and the K/V loads (direct to LDS, an address per lane) wait for
 //     nothing. Rows outside the request's keys read one of its rows instead: a
 //     masked key's P is zero, but zero times what an unused row holds may be NaN.
-// Measured at D=128, bf16: 399 us and 7 for the join at B=64 H=32/8, up to 16384
-// keys (2.6 GB, 6.5 TB/s; a large read reaches 6.3); 6.4 and 3.6 us for one request
-// of 1021 keys, H=16/8, most of it the way to the first keys.
+// Measured at D=128, bf16: 396 us and 6 for the join at B=64 H=32/8, up to 16384
+// keys (2.6 GB, 6.6 TB/s; a large read reaches 6.3); 6.2 and 3.8 us for one request
+// of 1021 keys, H=16/8, most of it the way to the first keys and to the parts.
 #include <type_traits>
 
 #include "fa_device.h"
@@ -208,7 +209,7 @@ struct Line {
 // The kernel's arguments, read from memory where this stands. They take about as
 // many scalar registers as there are: held from the start, those that the rows and
 // results need were spilled ahead of the first loads, 100 instructions that a short
-// call waited for (19.5 us in all at B=8 H=16/4 D=64, 5 tokens, 18.7 without them).
+// call waited for (0.8 us at B=8 H=16/4 D=64, 5 tokens).
 typedef __attribute__((address_space(4))) const PagedKernelArgs LateArgs;
 __device__ __forceinline__ LateArgs& late_args() {
   auto* p = (LateArgs*)__builtin_amdgcn_kernarg_segment_ptr();
@@ -846,8 +847,8 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
   // list's (3.8 us against 4.8 at B=8 H=16/4 D=64, 5 tokens: 160 and 768 workgroups;
   // 4.6 against 6.1 at B=30 H=16/2 D=256: 480 and 1024); else the list, a shorter way to
   // the parts (4.3 against 7.8 at B=40 H=16/4 D=64, 4 tokens: 512 and 640; 6.5 against
-  // 13.4 at B=100 H=16/2 D=256: 1024 and 1600), with two runs each (B=250 H=32/4
-  // D=128: 47.2 us in all, 48.5 with one). The list too for items of one run, but for
+  // 13.4 at B=100 H=16/2 D=256: 1024 and 1600), with two runs each (1.3 us less
+  // than with one at B=250 H=32/4 D=128). The list too for items of one run, but for
   // up to four of them, whose parts can be many (at B=1 H=16/4 D=64: 4.2 us against
   // 4.9 at 4000 keys, 3.9 and 3.4 at 1000).
   const long long items = (long long)a.B * d.items;

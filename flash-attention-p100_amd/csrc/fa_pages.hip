@@ -191,8 +191,8 @@ __global__ __launch_bounds__(kTabThreads) void tables_kernel(const TablesArgs a)
 // Cache writes: a copy of each token's K and V rows to its slot, a thread per
 // 16-byte chunk, workgroups of K and of V in turn (both in one thread: 96 us where
 // this takes 88, into pages that hold the rows before the heads). Bound by HBM at
-// prompts (88 us for 65536 tokens of 8 heads of 128, 529 MB moved at 6.0 TB/s; a
-// copy of 2 GiB moves 4.95), by latency at a step (2.7 us for 64 tokens).
+// prompts (88 to 92 us for 65536 tokens of 8 heads of 128, 529 MB moved at 5.8 TB/s
+// or more; a copy of 2 GiB moves 4.95), by latency at a step (2.7 us for 64 tokens).
 constexpr int kAppThreads = 256;
 // Chunks from which loads and stores carry the nontemporal hint: 32 MB written, what
 // the L2s hold. Above, the hint takes 98 to 88 us at 268 MB and 27.4 to 24.3 at 67;

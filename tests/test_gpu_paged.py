@@ -399,6 +399,24 @@ def test_attn_random_calls(seed):
     check_attn(args, causal, window, alibi, r.choice([None, 0.05]))
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_attn_random_row_tiles(seed):
+    """Two to nine row tiles per kv head, in tables large enough to take them abreast."""
+    import random
+    r = random.Random(100 + seed)
+    Hkv, group, N = r.choice([(1, 8, 5), (1, 3, 33), (2, 16, 4), (1, 64, 1), (3, 5, 17), (1, 16, 16), (2, 2, 65)])
+    D, page = r.choice([16, 64, 72, 128, 128, 256]), 2 ** r.randint(0, 6)
+    top = r.choice([20, 300, 3000, 12000])
+    lens = [r.randint(0, top) for _ in range(r.choice([1, 3, 12, 90 if top < 1000 else 6]))]
+    causal = r.random() < 0.7
+    window = r.choice([None, None, 40, 900]) if causal else None
+    print(seed, lens, Hkv, group, N, D, page, causal, window, flush=True)
+    spare = (16 << 20) // (4 * Hkv * D * page) // len(lens) + 2
+    args = attn_inputs(lens, Hkv * group, Hkv, N, D, page, r.choice([torch.half, torch.bfloat16]),
+                       r.choice(["bhnd", "bnhd"]), seed, spare)
+    check_attn(args, causal, window)
+
+
 def test_attn_pages_outside_the_pool_hide_their_keys():
     q, kc, vc, table, kv_len = attn_inputs([640, 100, 33], 4, 2, 2, 64, 16, torch.half, seed=6)
     bad = table.clone()
