@@ -511,12 +511,13 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
  * own keys and values the cache holds already, and with `causal` it sees the
  * keys up to itself, else all of them. Rows without a key (kv_len[b] = 0, or
  * kv_len[b] < N: the first rows under causal masking) get o = 0, lse = +inf. What
- * lies in rows of the pool that no row of q sees reaches no output, NaN included.
- * Of `opts`, dtype, layout, window (counted from the row's token), alibi_slopes and
- * scale are taken (NULL: the defaults); anything else set is refused. With a
- * window the table entries of pages wholly outside it are not read. Keys in
- * pages whose index is outside [0, pages) are hidden like masked ones. The keys
- * of a batch are shared evenly among the GPU's compute units whatever their
+ * lies in rows of the pool that no row of q sees reaches no output, NaN included;
+ * an infinity or NaN that one row sees may come out as NaN in it and in the others
+ * of its kv head (masked values are multiplied by zero). Of `opts`, dtype, layout,
+ * window (counted from the row's token), alibi_slopes and scale are taken (NULL:
+ * the defaults); anything else set is refused. With a window the table entries of
+ * pages wholly outside it are not read. Keys in pages whose index is outside [0,
+ * pages) are hidden like masked ones. The keys of a batch are shared evenly among the GPU's compute units whatever their
  * lengths; partial results meet in `workspace`, of at least
  * fa_paged_attn_workspace_bytes() bytes (0 for invalid arguments), which may hold
  * anything. Calls that overlap in time need workspaces of their own. q, o and the
