@@ -517,14 +517,14 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
  * window (counted from the row's token), alibi_slopes and scale are taken (NULL:
  * the defaults); anything else set is refused. With a window the table entries of
  * pages wholly outside it are not read. Keys in pages whose index is outside [0,
- * pages) are hidden like masked ones. The keys of a batch are shared evenly among the GPU's compute units whatever their
- * lengths; partial results meet in `workspace`, of at least
- * fa_paged_attn_workspace_bytes() bytes (0 for invalid arguments), which may hold
- * anything. Calls that overlap in time need workspaces of their own. q, o and the
- * workspace are 16-byte aligned; Hq * N <= 2^24, Hq * D < 2^31, and the 32-key
- * blocks of full tables, times B, Hkv and the 32-row tiles of Hq / Hkv * N, at most
- * 2^30. The results are deterministic; a request's last bits may depend on the
- * lengths of the others in its batch.
+ * pages) are hidden like masked ones. The keys of a batch are shared evenly among
+ * the GPU's compute units whatever their lengths; partial results meet in
+ * `workspace`, of at least fa_paged_attn_workspace_bytes() bytes (0 for invalid
+ * arguments), which may hold anything. Calls that overlap in time need workspaces of
+ * their own. q, o and the workspace are 16-byte aligned; Hq * N <= 2^24, Hq * D <
+ * 2^31, and the 32-key blocks of full tables, times B, Hkv and the 32-row tiles of
+ * Hq / Hkv * N, at most 2^30. The results are deterministic; a request's last bits
+ * may depend on the lengths of the others in its batch.
  */
 size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
 int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
