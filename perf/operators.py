@@ -25,18 +25,12 @@ own = False
 _DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
 
 
-_loaded = None
-
-
 def _fa():
-    global _loaded
-    if _loaded is None:  # once, as a program imports it
-        path = os.path.abspath("flash-attention-p100_amd")
-        if path not in sys.path:
-            sys.path.insert(0, path)
-        import fa_p100
-        _loaded = fa_p100
-    return _loaded
+    path = os.path.abspath("flash-attention-p100_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import fa_p100
+    return fa_p100
 
 
 # ------------------------------------------------------------------ the cases
