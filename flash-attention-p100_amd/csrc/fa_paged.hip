@@ -35,6 +35,23 @@ namespace {
 constexpr int kRows = 32;  // query rows of a tile
 constexpr int kKeys = 32;  // keys of a wave's block
 
+// P = 2^(kPScale + log2 units of a score below its row's maximum) is rounded to the
+// inputs' format, half a step of itself, as the operand of the second product. (A second
+// product of the remainders would leave the results' own rounding alone; they are off
+// the 64-bit ones by 0.0019 to 0.0023 of their norm in bf16 and 0.00025 to 0.00029 in
+// fp16, where that is 0.0017 and 0.00021.) bf16 has fp32's exponents. fp16's end at
+// 2^-24, which the many small weights behind one large one (an attention sink) may be
+// below, so P is 2^15 there for the row's largest and the maximum is never behind: half a
+// step holds down to 2^-29 of the largest, and 2^-40 of it below. (Of 1 without the
+// scale a tail of 16384 keys at 2^-24.5 came out a half too large.)
+template <bool BF>
+constexpr int kPScale = BF ? 0 : 15;
+template <bool BF>
+constexpr float kPUnit = BF ? 1.f : 0x1p-15f;
+// The maximum's growth, in log2 units, that leaves it where it was.
+template <bool BF>
+constexpr float kPRescale = BF ? kRescaleLog2 : 0.f;
+
 template <int D>
 struct Paged {
   static constexpr int kWaves = D > 128 ? 4 : 8;
@@ -485,18 +502,18 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
             for (int e = 0; e < 16; ++e) oacc[cb][e] *= corr;
           m_raw = m_new;
         }
-        const float neg = m_raw == -INFINITY ? 0.f : -m_raw * c;
+        // (s - m first: exact near the maximum, so that P is at most its scale's)
+        const float m_use = m_raw == -INFINITY ? 0.f : m_raw;
         half8 pb[2];
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          // P is rounded to the inputs' format, half a step, as the second product's
-          // operand, whose matrix instruction takes no wider one; its sum, as S and O,
-          // is not. (Off the 64-bit results by 0.0019 to 0.0023 of their norm in bf16
-          // and 0.00029 in fp16; rounding the results alone is 0.0017 and 0.00021.)
-          const float p = fast_exp2(fmaf(s[e], c, neg));
-          l += p;
+          const float p = fast_exp2(fmaf(s[e] - m_use, c, (float)kPScale<BF>));
+          ls[e & 3] += p;
           pb[e >> 3][e & 7] = to16<BF>(p);
         }
+        // (a block's sum at a time: a sum near 1 does not feel single weights below 2^-25)
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
         __builtin_amdgcn_s_waitcnt(kWaitOlder);  // V's block is here, K's next may be under way
         if (hide) {
 #pragma unroll 1
@@ -534,7 +551,7 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
       if (!whole) ra.part_ml[slot * ra.part_rows + lr] = make_float2(m * c, sum);
       else if (ra.lse)
         ra.lse[((size_t)b * ra.Hq + row.hq) * ra.N + row.n] =
-            sum > 0.f ? (m * c + __log2f(sum)) * kLn2 : INFINITY;
+            sum > 0.f ? (m * c + __log2f(sum * kPUnit<BF>)) * kLn2 : INFINITY;
     };
     // Columns col .. col + 3 (a row without keys: O = 0).
     auto put = [&](bool whole, float inv, int col, floatx4 v) {
@@ -784,7 +801,7 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const 
       }
       if (col == 0 && a.lse)
         a.lse[((size_t)b * a.Hq + row.hq) * a.N + row.n] =
-            l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
+            l > 0.f ? (m + __log2f(l * kPUnit<BF>)) * kLn2 : INFINITY;
     }
   }
 }
@@ -839,7 +856,7 @@ hipError_t launch_paged_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
   d.window = a.window < d.cap ? a.window : 0;  // (a wider one hides nothing)
   d.dr = a.D;
   d.scale_log2 = kLog2e * (a.scale > 0.f ? a.scale : 1.f / sqrtf((float)a.D));
-  d.rescale = kRescaleLog2 / d.scale_log2;
+  d.rescale = kPRescale<FA_BF> / d.scale_log2;
   d.alibi_unit = kLog2e / d.scale_log2;
   d.alibi = a.alibi;
   d.stq = make_strides(a.layout, a.Hq, a.N, a.D);
