@@ -36,14 +36,23 @@ constexpr int kRows = 32;  // query rows of a tile
 constexpr int kKeys = 32;  // keys of a wave's block
 
 // P = 2^(kPScale + log2 units of a score below its row's maximum) is rounded to the
-// inputs' format, half a step of itself, as the operand of the second product. (A second
-// product of the remainders would leave the results' own rounding alone; they are off
-// the 64-bit ones by 0.0019 to 0.0023 of their norm in bf16 and 0.00025 to 0.00029 in
-// fp16, where that is 0.0017 and 0.00021.) bf16 has fp32's exponents. fp16's end at
-// 2^-24, which the many small weights behind one large one (an attention sink) may be
-// below, so P is 2^15 there for the row's largest and the maximum is never behind: half a
-// step holds down to 2^-29 of the largest, and 2^-40 of it below. (Of 1 without the
-// scale a tail of 16384 keys at 2^-24.5 came out a half too large.)
+// inputs' format as the second product's operand. Up to 32 rows per kv head a second
+// matrix instruction adds the product of what that rounding left, so the results are
+// off the 64-bit ones by their own rounding (0.0017 of their norm in bf16, 0.00021 in
+// fp16; 0.0020 to 0.0023 and 0.00024 to 0.00027 without). HBM bounds these calls:
+// 0.2 to 0.3 us of 10 to 40, 1 of 160, none of 400. With more rows the instructions
+// bound, and P is rounded once, as in the other forward kernels (another product
+// would take 113 us to 115 at B=20 H=64/8 D=128, 8 tokens, and 51 to 57 at D=64; 146 to
+// 157 at 16 tokens; 490 to 580 for 2048 tokens of H=32/8 D=128 over 8192).
+//
+// bf16 has fp32's exponents. fp16's end at 2^-24, which the many small weights behind
+// one large one (an attention sink) may be below, so P is 2^15 there for the row's
+// largest and the maximum is never behind: half a step holds down to 2^-29 of the
+// largest, and 2^-40 of it below. (With P up to 2^8 and none of the scale, as in the
+// other forward kernels, a tail of 16384 keys at 2^-24.5 came out 1.5 times too large.)
+// Each time that a row's maximum grows O is multiplied; where the products bound, that
+// took 1 to 3% (140 us for 138 and 503 for 487 at 512 and 2048 tokens of H=32/8 D=128
+// over 8192).
 template <bool BF>
 constexpr int kPScale = BF ? 0 : 15;
 template <bool BF>
@@ -504,13 +513,14 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
         }
         // (s - m first: exact near the maximum, so that P is at most its scale's)
         const float m_use = m_raw == -INFINITY ? 0.f : m_raw;
-        half8 pb[2];
+        half8 pb[2], rest[2];
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float p = fast_exp2(fmaf(s[e] - m_use, c, (float)kPScale<BF>));
           ls[e & 3] += p;
           pb[e >> 3][e & 7] = to16<BF>(p);
+          if constexpr (STREAM) rest[e >> 3][e & 7] = to16<BF>(p - from16<BF>(pb[e >> 3][e & 7]));
         }
         // (a block's sum at a time: a sum near 1 does not feel single weights below 2^-25)
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
@@ -527,8 +537,11 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
-          for (int cb = 0; cb < D / 32; ++cb)
-            oacc[cb] = mfma16<BF>(S::tr_operand(my_v, q, off, cb), pb[q], oacc[cb]);
+          for (int cb = 0; cb < D / 32; ++cb) {
+            const half8 v = S::tr_operand(my_v, q, off, cb);
+            oacc[cb] = mfma16<BF>(v, pb[q], oacc[cb]);
+            if constexpr (STREAM) oacc[cb] = mfma16<BF>(v, rest[q], oacc[cb]);
+          }
         wait_lds();
         load(vt, base_v);
       }

@@ -44,3 +44,24 @@ def test_a_sink_over_a_long_flat_tail(peak, B, D, Hq, N, dtype):
                                       softmax_scale=1.0, return_lse=True)
     ref = [x.expand(B, *x.shape[1:]) for x in (o, lse, o_tol, lse_tol)]
     paged_ref.check(got, got_lse, ref)
+
+
+@pytest.mark.parametrize("dtype", [torch.half, torch.bfloat16])
+@pytest.mark.parametrize("lens,Hq,Hkv,N,D", [
+    ([1, 33, 1000, 5000], 8, 1, 1, 128), ([20000], 8, 2, 4, 64), ([700] * 40, 32, 1, 1, 256),
+    ([9000, 3, 700], 16, 4, 8, 96), ([300 * i for i in range(30)], 4, 4, 1, 32), ([4000], 31, 1, 1, 80)])
+def test_up_to_32_rows_of_a_kv_head_are_rounded_once(lens, Hq, Hkv, N, D, dtype):
+    """paged_ref's bound without the probabilities' rounding u A (A = sum_j p_j |v_j|, its
+    result of |v|): they are two numbers of q's format, whose sum is off by u^2 of it, in
+    fp16 by 2^-40 of the row's largest where it is below 2^-29 of that (see above)."""
+    from test_gpu_paged import attn_inputs, fa
+    args = attn_inputs(lens, Hq, Hkv, N, D, 16, dtype, seed=D)
+    o, lse, o_tol, lse_tol = paged_ref.attention(*args)
+    a = paged_ref.attention(args[0], args[1], args[2].abs(), *args[3:])[0]
+    u = torch.finfo(dtype).eps / 2
+    o_tol = o_tol - (u - u * u) * a
+    if dtype == torch.half:
+        values = args[2].double()
+        o_tol = o_tol + max(lens) * 2.0 ** -40 * values[torch.isfinite(values)].abs().max()
+    got, got_lse = fa().paged_attn(*args, return_lse=True)
+    paged_ref.check(got, got_lse, (o, lse, o_tol, lse_tol))
