@@ -560,11 +560,12 @@ __global__ __launch_bounds__(Paged<D>::kThreads, Paged<D>::kPerSimd) void paged_
     if (from == 0 && n > 0 && n < units) owned = make_int4(b, item, start, units);
     size_t slot = (joins ? 2 * (wg * kLine + on) + (from > 0 ? 0 : 1) : pos) * TILES + beside;
     half_t* orow = ra.o + b * ra.stq.b + row.hq * ra.stq.h + (size_t)row.n * ra.stq.n;
+    // (a sum of 0: no key. NaN stays NaN, and does not say that there was none.)
     auto finish = [&](bool whole, float m, float sum) {
       if (!whole) ra.part_ml[slot * ra.part_rows + lr] = make_float2(m * c, sum);
       else if (ra.lse)
         ra.lse[((size_t)b * ra.Hq + row.hq) * ra.N + row.n] =
-            sum > 0.f ? (m * c + __log2f(sum * kPUnit<BF>)) * kLn2 : INFINITY;
+            sum == 0.f ? INFINITY : (m * c + __log2f(sum * kPUnit<BF>)) * kLn2;
     };
     // Columns col .. col + 3 (a row without keys: O = 0).
     auto put = [&](bool whole, float inv, int col, floatx4 v) {
@@ -814,7 +815,7 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const 
       }
       if (col == 0 && a.lse)
         a.lse[((size_t)b * a.Hq + row.hq) * a.N + row.n] =
-            l > 0.f ? (m + __log2f(l * kPUnit<BF>)) * kLn2 : INFINITY;
+            l == 0.f ? INFINITY : (m + __log2f(l * kPUnit<BF>)) * kLn2;
     }
   }
 }

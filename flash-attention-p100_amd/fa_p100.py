@@ -565,7 +565,8 @@ def paged_attn(q, k_cache, v_cache, block_table, kv_len, causal=True, sliding_wi
     batch with kv_len 0, or the first rows of one with kv_len < N) gets o = 0 and
     lse = +inf. Keys in pages whose index is outside the pool are hidden, and what
     lies in rows that no row of q sees reaches no output; an infinity or NaN that one
-    row sees may come out as NaN in the request's others too.
+    row sees may come out as NaN in o for the others of its request and kv head too,
+    while lse is NaN only for rows whose own scores hold a NaN or +inf.
 
     The requests' keys are dealt evenly to the GPU's compute units, so a batch of
     ragged lengths costs what its keys cost. Results are deterministic; the last

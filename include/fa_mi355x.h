@@ -513,7 +513,9 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
  * kv_len[b] < N: the first rows under causal masking) get o = 0, lse = +inf. What
  * lies in rows of the pool that no row of q sees reaches no output, NaN included;
  * an infinity or NaN that one row sees may come out as NaN in it and in the others
- * of its kv head (masked values are multiplied by zero). Of `opts`, dtype, layout,
+ * of its kv head (masked values are multiplied by zero). Their lse is theirs alone:
+ * NaN for a row whose own scores hold a NaN or +inf, +inf for rows without a key
+ * and (their weights being zero) for those whose scores are all -inf. Of `opts`, dtype, layout,
  * window (counted from the row's token), alibi_slopes and scale are taken (NULL:
  * the defaults); anything else set is refused. With a window the table entries of
  * pages wholly outside it are not read. Keys in pages whose index is outside [0,
