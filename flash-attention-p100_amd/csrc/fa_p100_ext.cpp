@@ -691,6 +691,8 @@ static void check_ints(const at::Tensor& t, const at::Device& dev, const char* n
 static void check_no_grad(const at::Tensor& t, const char* name) {
   TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name,
               " requires grad, and paged caches have no backward: call under torch.no_grad()");
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), name,
+              " has a forward-mode tangent, and paged caches have no derivative");
 }
 
 // A tensor has been written behind autograd's back: what was saved of it is stale.
@@ -711,8 +713,6 @@ static bool rows_aligned(const at::Tensor& t) {
 // The cache of k_cache and v_cache, (pages, Hkv, page_size, D) in any order of
 // the first three dimensions, laid out alike; the tables are left unset.
 static fa_paged_cache paged_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& like) {
-  check_no_grad(k, "k_cache");
-  check_no_grad(v, "v_cache");
   TORCH_CHECK(k.is_cuda() && k.device() == like.device() && v.device() == like.device(),
               "k_cache and v_cache must be on ", like.device());
   TORCH_CHECK(k.scalar_type() == like.scalar_type() && v.scalar_type() == like.scalar_type(),
@@ -790,12 +790,15 @@ std::vector<at::Tensor> fa_paged_tables_t(const at::Tensor& block_table, const a
 // the caches (fa_paged_append).
 void fa_paged_append_t(at::Tensor k, at::Tensor v, const at::Tensor& k_cache,
                        const at::Tensor& v_cache, at::Tensor slots) {
+  check_no_grad(k, "k");
+  check_no_grad(v, "v");
+  check_no_grad(k_cache, "k_cache");
+  check_no_grad(v_cache, "v_cache");
   for (auto& tn : {std::make_pair(&k, "k"), std::make_pair(&v, "v")}) {
     const at::Tensor& t = *tn.first;
     TORCH_CHECK(t.is_cuda(), tn.second, " must be a CUDA tensor");
     TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, tn.second,
                 " must be fp16 or bf16");
-    check_no_grad(t, tn.second);
   }
   TORCH_CHECK((k.dim() == 3 || k.dim() == 4) && k.sizes() == v.sizes(),
               "k and v must both be (T, Hkv, D) or (B, Hkv, N, D)");
@@ -831,10 +834,16 @@ void fa_paged_append_t(at::Tensor k, at::Tensor v, const at::Tensor& k_cache,
 std::vector<at::Tensor> fa_paged_attn_t(at::Tensor q, const at::Tensor& k_cache,
                                         const at::Tensor& v_cache, const at::Tensor& block_table,
                                         const at::Tensor& kv_len, bool causal, int64_t window,
-                                        const c10::optional<at::Tensor>& alibi_slopes, double scale,
+                                        c10::optional<at::Tensor> alibi_slopes, double scale,
                                         bool want_lse) {
-  check_in16(q, "q");
   check_no_grad(q, "q");
+  check_no_grad(k_cache, "k_cache");
+  check_no_grad(v_cache, "v_cache");
+  if (alibi_slopes) {
+    check_no_grad(*alibi_slopes, "alibi_slopes");
+    alibi_slopes = alibi_slopes->to(at::kFloat).contiguous();
+  }
+  check_in16(q, "q");
   fa_paged_cache cache = paged_cache(k_cache, v_cache, q);
   const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3);
   const int64_t Hkv = k_cache.size(1);

@@ -539,7 +539,8 @@ def paged_append(k, v, k_cache, v_cache, slots):
     undefined). k_cache and v_cache are (pages, Hkv, page_size, D) in k's
     format, laid out alike, their first three dimensions in any order of storage
     (a transposed view of (pages, page_size, Hkv, D), or halves of one
-    (pages, 2, Hkv, page_size, D) pool). One HIP kernel; no gradient.
+    (pages, 2, Hkv, page_size, D) pool). One HIP kernel; no gradient: tensors that
+    require grad are refused outside torch.no_grad(), and duals of forward mode.
     """
     _paged_inputs("paged_append", k, v, k_cache, v_cache, slots)
     _ext.paged_append(k, v, k_cache, v_cache, slots)
@@ -570,9 +571,13 @@ def paged_attn(q, k_cache, v_cache, block_table, kv_len, causal=True, sliding_wi
 
     The requests' keys are dealt evenly to the GPU's compute units, so a batch of
     ragged lengths costs what its keys cost. Results are deterministic; the last
-    bits of one request may depend on the lengths of the others. No gradient.
+    bits of one request may depend on the lengths of the others. No gradient: tensors
+    that require grad (the slopes too) are refused outside torch.no_grad(), and duals
+    of forward mode.
     """
     _paged_inputs("paged_attn", q, k_cache, v_cache, block_table, kv_len)
+    if alibi_slopes is not None:
+        _paged_inputs("paged_attn", alibi_slopes)
     window = 0
     if sliding_window is not None:
         window = int(sliding_window)
@@ -582,7 +587,6 @@ def paged_attn(q, k_cache, v_cache, block_table, kv_len, causal=True, sliding_wi
         if alibi_slopes.dim() != 1 or alibi_slopes.numel() != q.size(1):
             raise ValueError(f"alibi_slopes must have shape ({q.size(1)},), got "
                              f"{tuple(alibi_slopes.shape)}")
-        alibi_slopes = alibi_slopes.detach().float().contiguous()
     scale = 0.0
     if softmax_scale is not None:
         scale = float(softmax_scale)
