@@ -813,6 +813,8 @@ void fa_paged_append_t(at::Tensor k, at::Tensor v, const at::Tensor& k_cache,
               "slots must be int32 on ", k.device());
   TORCH_CHECK(slots.dim() == (flat ? 1 : 2) && slots.size(0) == B && (flat || slots.size(1) == N),
               "slots must be (T,) for k of (T, Hkv, D) and (B, N) for k of (B, Hkv, N, D)");
+  TORCH_CHECK(B <= INT32_MAX && N <= INT32_MAX && B * N <= INT32_MAX && Hkv * D <= INT32_MAX,
+              "k and v may hold at most 2^31 - 1 tokens, of 2^31 - 1 elements");
   at::assert_no_internal_overlap(k_cache);  // (expanded ones, whose rows are several tokens')
   at::assert_no_internal_overlap(v_cache);
   if (B * N * Hkv == 0) return;
