@@ -7,6 +7,7 @@
 // state: every kernel's LDS is static, so launches need no attributes set.
 #include <limits.h>
 
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 
@@ -122,8 +123,9 @@ const char* fa_error_string(int err) {
              "from the query rows, and the backward needs block_cols with block_rows";
     case FA_ERR_PAGES:
       return "a paged cache needs a page size that is a power of two, positive sizes, 16-byte "
-             "aligned rows and at most 2^31 - 1 rows, and paged attention 16-byte aligned buffers "
-             "and no option but the format, layout, window, ALiBi slopes and scale";
+             "aligned rows and at most 2^31 - 1 rows, which do not overlap where it is written, "
+             "and paged attention 16-byte aligned buffers and no option but the format, layout, "
+             "window, ALiBi slopes and scale";
     case FA_ERR_SCRATCH:
       return "fa_bwd_noalloc: 2 * B*Hq*N floats exceed the built-in scratch "
              "(FA_BWD_NOALLOC_SCRATCH_BYTES); use fa_bwd with a workspace";
@@ -591,6 +593,42 @@ static int paged_pool(const fa_paged_cache* c, int Hkv, int D, fa::PagedPool& p)
   return FA_OK;
 }
 
+// Whether two elements of a paged cache's pools share a place: of one pool, or of k's and
+// v's. The sizes and strides of the pool's dimensions that are walked, the innermost
+// first: each stride has to pass all that lies within it. same: k's rows are v's, and
+// both are written from the same ones.
+static bool pools_overlap(const fa::PagedPool& p, int Hkv, int page_size, int D, bool same) {
+  struct Dim {
+    long long size, stride;
+  } dims[4] = {{D, 1}};
+  int n = 1;
+  for (const Dim& d : {Dim{p.pages, p.page_stride}, Dim{Hkv, p.head_stride}, Dim{page_size, p.row_stride}})
+    if (d.size > 1) dims[n++] = d;
+  std::sort(dims, dims + n, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+  long long reach[4], last = 0;  // the last element within dimension i's steps
+  for (int i = 0; i < n; ++i) {
+    if (dims[i].stride <= last || dims[i].stride > (1LL << 62) / dims[i].size - last) return true;
+    reach[i] = last;
+    last += (dims[i].size - 1) * dims[i].stride;
+  }
+  if (same) return false;
+  // v's element x lies on k's y where their offsets differ by the pools' distance: by
+  // steps of the outermost dimension (two numbers of them leave little enough), and so on.
+  const long long bytes = (const char*)p.v - (const char*)p.k;
+  auto meet = [&](auto&& self, long long apart, int i) -> bool {
+    apart = apart < 0 ? -apart : apart;
+    if (i < 0) return apart == 0;
+    const long long steps = apart / dims[i].stride;
+    for (long long a = steps; a <= steps + 1; ++a) {
+      const long long rest = apart - a * dims[i].stride;
+      if (a < dims[i].size && rest <= reach[i] && rest >= -reach[i] && self(self, rest, i - 1)) return true;
+    }
+    return false;
+  };
+  const long long apart = (bytes < 0 ? -bytes : bytes) / 2;
+  return apart <= last && meet(meet, apart, n - 1);
+}
+
 int fa_paged_tables(int* table, long long table_stride, int table_width, const int* old_len,
                     const int* new_len, int* free_pages, int n_ring, const int* ring,
                     int page_size, int B, int max_new, int tokens, int* slots, int* kv_len,
@@ -626,6 +664,9 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
   if (!aligned16(k) || !aligned16(v) ||
       ((k_stride_b | k_stride_n | k_stride_h | v_stride_b | v_stride_n | v_stride_h) & 7))
     return FA_ERR_PAGES;
+  const bool same = pool.k == pool.v && k == v && k_stride_b == v_stride_b &&
+                    k_stride_n == v_stride_n && k_stride_h == v_stride_h;
+  if (pools_overlap(pool, Hkv, cache->page_size, D, same)) return FA_ERR_PAGES;
   return to_code(fa::launch_paged_append(k, v, {k_stride_b, k_stride_n, k_stride_h},
                                          {v_stride_b, v_stride_n, v_stride_h}, slots, pool, B, N,
                                          Hkv, D, stream));

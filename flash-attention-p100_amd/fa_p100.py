@@ -539,7 +539,8 @@ def paged_append(k, v, k_cache, v_cache, slots):
     undefined). k_cache and v_cache are (pages, Hkv, page_size, D) in k's
     format, laid out alike, their first three dimensions in any order of storage
     (a transposed view of (pages, page_size, Hkv, D), or halves of one
-    (pages, 2, Hkv, page_size, D) pool). One HIP kernel; no gradient: tensors that
+    (pages, 2, Hkv, page_size, D) pool), no two rows overlapping; k and v must not lie
+    in rows that are written. One HIP kernel; no gradient: tensors that
     require grad are refused outside torch.no_grad(), and duals of forward mode.
     """
     _paged_inputs("paged_append", k, v, k_cache, v_cache, slots)

@@ -69,9 +69,10 @@ enum {
                                 backward without block_cols, block_cols without block_rows,
                                 or (fa_pack_blocks) layout planes not 1 or B by 1 or Hq */
   FA_ERR_PAGES = 10019       /* a paged cache whose page size is not a power of two, whose
-                                sizes are not positive, whose rows are not 16-byte aligned, or
-                                with an option that paged attention does not take, or a
-                                buffer of its that is not 16-byte aligned */
+                                sizes are not positive, whose rows are not 16-byte aligned or
+                                (where they are written) overlap, or with an option that paged
+                                attention does not take, or a buffer of its that is not
+                                16-byte aligned */
 };
 
 /* Memory layouts of the 16-bit tensors, for the entry points that take one:
@@ -497,7 +498,9 @@ int fa_paged_tables(int* table, long long table_stride, int table_width, const i
  * d) of k is at b * k_stride_b + n * k_stride_n + h * k_stride_h + d (strides in
  * elements, multiples of 8; k and v 16-byte aligned). Slots that are negative or
  * past the pool are left out. Each slot may occur once; the rows of a slot given
- * twice are undefined.
+ * twice are undefined. The pools' rows must lie apart, k's from v's too unless both
+ * pools are one and k is v (strides that pass what lies within them; anything else is
+ * refused), and k and v outside the rows that are written.
  */
 int fa_paged_append(const void* k, const void* v, long long k_stride_b, long long k_stride_n,
                     long long k_stride_h, long long v_stride_b, long long v_stride_n,
