@@ -38,12 +38,6 @@ struct Dec {
   static_assert(kWaves / 2 * kFloats * 4 <= kWaves * kTileHalves * 2, "merge area exceeds the tiles");
 };
 
-// A wave's LDS reads so far are done: its tile may be loaded again.
-__device__ __forceinline__ void wait_lds() {
-  __builtin_amdgcn_s_waitcnt(0xC07F);
-  __builtin_amdgcn_sched_barrier(0);
-}
-
 struct DecArgs {
   const half_t* q;
   const half_t* k;

@@ -425,6 +425,11 @@ using Stream = std::conditional_t<kSwizzled<D>, Swz<D>, Pad<D>>;
 
 // Wait until this wave's direct-to-LDS (and other vector memory) loads landed.
 __device__ __forceinline__ void wait_vmem() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+// Wait until this wave's LDS reads are done: its tile may be loaded again.
+__device__ __forceinline__ void wait_lds() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 // Direct loads of logical rows [r0, r0 + ROWS) of a row-major (N, D) fp16
 // matrix into a tile by the NW waves of a workgroup: kInsts 1 KB instructions

@@ -14,16 +14,18 @@
 //     it, and writes the result of an item that it has whole; the parts of the
 //     others meet in paged_merge_kernel. No wave waits for a longer request. Where
 //     a workgroup's stretch lies within one item, its waves' parts meet in LDS
-//     first: long requests then leave an eighth of the parts. Several row tiles of a
-//     kv head go side by side, as many waves over the same stretch;
+//     first: long requests then leave one where the kLine waves that divide the
+//     stretch (8, 4 at D=256, less with tiles abreast) would leave one each. Several
+//     row tiles of a kv head go side by side, as many waves over the same stretch;
 //   * a wave's lanes hold the next 64 page indices of its stretch; a block's rows
 //     take theirs from there by a lane permutation, so the table is read once in
 //     64 pages and the K/V loads (direct to LDS, an address per lane) wait for
 //     nothing. Rows outside the request's keys read one of its rows instead: a
 //     masked key's P is zero, but zero times what an unused row holds may be NaN.
-// Measured at D=128, bf16: 396 us and 6 for the join at B=64 H=32/8, up to 16384
-// keys (2.6 GB, 6.6 TB/s; a large read reaches 6.3); 6.2 and 3.8 us for one request
-// of 1021 keys, H=16/8, most of it the way to the first keys and to the parts.
+// Measured at D=128, bf16: 399 us and 7 for the join at B=64 H=32/8, up to 16384
+// keys (2.6 GB, 6.5 TB/s; the fastest large read found reaches 7.1, most others 6);
+// 6.6 and 3.8 us for one request of 1021 keys, H=16/8, most of it the way to the first
+// keys and to the parts.
 #include <type_traits>
 
 #include "fa_device.h"
@@ -256,12 +258,6 @@ struct Row {
     n = rc - g * a.N;
   }
 };
-
-// A wave's LDS reads so far are done: its tile may be loaded again.
-__device__ __forceinline__ void wait_lds() {
-  __builtin_amdgcn_s_waitcnt(0xC07F);
-  __builtin_amdgcn_sched_barrier(0);
-}
 
 // 16 bytes per lane from `from` to LDS at lds + byte_off + 16 * lane. STREAM: with
 // the nontemporal hint. K and V that one row tile reads are read once, and hinted
@@ -712,7 +708,8 @@ __global__ __launch_bounds__(64 * kMergeWaves, 6) void paged_merge_kernel(const 
   for (int t0 = 0; t0 < tasks; t0 += kMergeWaves) {
     const int task = t0 + wave - group * per_round;
     bool active = task < tasks && group < groups;
-    const int nth = active ? TILES == 1 ? task >> (runs - 1) : small_div(task, runs) : 0, part_run = run0 + (active ? task - nth * runs : 0);
+    const int nth = !active ? 0 : TILES == 1 ? task >> (runs - 1) : small_div(task, runs);
+    const int part_run = run0 + (active ? task - nth * runs : 0);
     const int beside = TILES == 1 ? 0 : part_run / a.runs, run = part_run - beside * a.runs;
     unsigned long long left = some;
     for (int i = 0; i < nth; ++i) left &= left - 1;

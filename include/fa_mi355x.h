@@ -470,8 +470,9 @@ typedef struct fa_paged_cache {
  * a request that ended: 0) gives pages back. `free_pages` is a ring of n_ring
  * page indices, ring[0] its first free entry and ring[1] the number of free
  * ones from there on (ring[0] is taken modulo n_ring, ring[1] clamped to
- * [0, n_ring]); pages that come back are written behind them, and are not taken
- * again in the same call. Writes
+ * [0, n_ring]); pages that come back are written behind them as far as the ring has
+ * room (one of at least the pool's pages has), and are not taken again in the same
+ * call. Writes
  *   - table: the pages taken, behind the request's own (nothing else changes:
  *     the entries of returned pages keep their values);
  *   - kv_len[b]: new_len[b], or, where the free pages ran out or the table is
@@ -525,11 +526,15 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
  * pages) are hidden like masked ones. The keys of a batch are shared evenly among
  * the GPU's compute units whatever their lengths; partial results meet in
  * `workspace`, of at least fa_paged_attn_workspace_bytes() bytes (0 for invalid
- * arguments), which may hold anything. Calls that overlap in time need workspaces of
+ * arguments; whatever the lengths, about 2.1 MB for each of the Hq / Hkv * N rows of a kv
+ * head up to 32, less at small D: 68 MB at most), which may hold anything. Calls that overlap in time need workspaces of
  * their own. q, o and the workspace are 16-byte aligned; Hq * N <= 2^24, Hq * D <
  * 2^31, and the 32-key blocks of full tables, times B, Hkv and the 32-row tiles of
- * Hq / Hkv * N, at most 2^30. The results are deterministic; a request's last bits
- * may depend on the lengths of the others in its batch.
+ * Hq / Hkv * N, at most 2^30. Sums, maxima and scores are fp32, and so are the
+ * probabilities where Hq / Hkv * N <= 32; with more rows they are rounded to q's format
+ * as operands, as in fa_fwd (in fp16 below 2^-29 of a row's largest to multiples of
+ * 2^-39 of it, with fewer rows too). The results are deterministic; a request's last
+ * bits may depend on the lengths of the others in its batch.
  */
 size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
 int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
