@@ -39,7 +39,8 @@ constexpr int kKeys = 32;  // keys of a wave's block
 
 // P = 2^(kPScale + log2 units of a score below its row's maximum) is rounded to the
 // inputs' format as the second product's operand. Up to 32 rows per kv head a second
-// matrix instruction adds the product of what that rounding left, so the results are
+// matrix instruction adds the product of what that rounding left, itself rounded (P is
+// off by 2^-16 of itself in bf16 and 2^-22 in fp16), so the results are
 // off the 64-bit ones by their own rounding (0.0017 of their norm in bf16, 0.00021 in
 // fp16; 0.0020 to 0.0023 and 0.00024 to 0.00027 without). HBM bounds these calls:
 // 0.2 to 0.3 us of 10 to 40, 1 of 160, none of 400. With more rows the instructions

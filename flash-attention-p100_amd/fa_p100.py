@@ -571,9 +571,9 @@ def paged_attn(q, k_cache, v_cache, block_table, kv_len, causal=True, sliding_wi
     while lse is NaN only for rows whose own scores hold a NaN or +inf.
 
     The requests' keys are dealt evenly to the GPU's compute units, so a batch of
-    ragged lengths costs what its keys cost. With up to 32 rows per kv head (Hq / Hkv * N)
-    the softmax is fp32 throughout; with more its probabilities are rounded to q's
-    format for the product with v, as flash_attn's are. Results are deterministic; the last
+    ragged lengths costs what its keys cost. The softmax is fp32; its
+    probabilities enter the product with v as two numbers of q's format with up to 32
+    rows per kv head (Hq / Hkv * N), with more as one, as flash_attn's do. Results are deterministic; the last
     bits of one request may depend on the lengths of the others. No gradient: tensors
     that require grad (the slopes too) are refused outside torch.no_grad(), and duals
     of forward mode.

@@ -530,10 +530,10 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
  * head up to 32, less at small D: 68 MB at most), which may hold anything. Calls that overlap in time need workspaces of
  * their own. q, o and the workspace are 16-byte aligned; Hq * N <= 2^24, Hq * D <
  * 2^31, and the 32-key blocks of full tables, times B, Hkv and the 32-row tiles of
- * Hq / Hkv * N, at most 2^30. Sums, maxima and scores are fp32, and so are the
- * probabilities where Hq / Hkv * N <= 32; with more rows they are rounded to q's format
- * as operands, as in fa_fwd (in fp16 below 2^-29 of a row's largest to multiples of
- * 2^-39 of it, with fewer rows too). The results are deterministic; a request's last
+ * Hq / Hkv * N, at most 2^30. Sums, maxima and scores are fp32; the
+ * probabilities enter the product with v as two numbers of q's format (off by 2^-16 of
+ * themselves in bf16, 2^-22 in fp16) where Hq / Hkv * N <= 32, with more rows as one,
+ * as in fa_fwd (in fp16, below 2^-29 of a row's largest, as multiples of 2^-39 of it). The results are deterministic; a request's last
  * bits may depend on the lengths of the others in its batch.
  */
 size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
