@@ -40,13 +40,13 @@ constexpr int kKeys = 32;  // keys of a wave's block
 // P = 2^(kPScale + log2 units of a score below its row's maximum) is rounded to the
 // inputs' format as the second product's operand. Up to 32 rows per kv head a second
 // matrix instruction adds the product of what that rounding left, itself rounded (P is
-// off by 2^-16 of itself in bf16 and 2^-22 in fp16), so the results are
-// off the 64-bit ones by their own rounding (0.0017 of their norm in bf16, 0.00021 in
-// fp16; 0.0020 to 0.0023 and 0.00024 to 0.00027 without). HBM bounds these calls:
-// 0.2 to 0.3 us of 10 to 40, 1 of 160, none of 400. With more rows the instructions
-// bound, and P is rounded once, as in the other forward kernels (another product
-// would take 113 us to 115 at B=20 H=64/8 D=128, 8 tokens, and 51 to 57 at D=64; 146 to
-// 157 at 16 tokens; 490 to 580 for 2048 tokens of H=32/8 D=128 over 8192).
+// off by 2^-16 of itself in bf16 and 2^-22 in fp16), so the results are off the 64-bit
+// ones by their own rounding (0.0017 of their norm in bf16, 0.00021 in fp16; 0.0020 to
+// 0.0023 and 0.00024 to 0.00027 without). HBM bounds these calls: 0.2 to 0.5 us of 10
+// to 40, 1 of 160, none of 400. With more rows the instructions bound, and P is rounded
+// once, as in the other forward kernels (another product would take 113 us to 115 at
+// B=20 H=64/8 D=128, 8 tokens, and 51 to 57 at D=64; 146 to 157 at 16 tokens; 490 to 580
+// for 2048 tokens of H=32/8 D=128 over 8192).
 //
 // bf16 has fp32's exponents. fp16's end at 2^-24, which the many small weights behind
 // one large one (an attention sink) may be below, so P is 2^15 there for the row's

@@ -567,16 +567,16 @@ def paged_attn(q, k_cache, v_cache, block_table, kv_len, causal=True, sliding_wi
     batch with kv_len 0, or the first rows of one with kv_len < N) gets o = 0 and
     lse = +inf. Keys in pages whose index is outside the pool are hidden, and what
     lies in rows that no row of q sees reaches no output; an infinity or NaN that one
-    row sees may come out as NaN in o for the others of its request and kv head too,
-    while lse is NaN only for rows whose own scores hold a NaN or +inf.
+    row sees may come out as NaN in its o and that of the others of its request and kv
+    head, while lse is NaN only for rows whose own scores hold a NaN or +inf.
 
     The requests' keys are dealt evenly to the GPU's compute units, so a batch of
-    ragged lengths costs what its keys cost. The softmax is fp32; its
-    probabilities enter the product with v as two numbers of q's format with up to 32
-    rows per kv head (Hq / Hkv * N), with more as one, as flash_attn's do. Results are deterministic; the last
-    bits of one request may depend on the lengths of the others. No gradient: tensors
-    that require grad (the slopes too) are refused outside torch.no_grad(), and duals
-    of forward mode.
+    ragged lengths costs what its keys cost. The softmax is fp32; its probabilities
+    enter the product with v as two numbers of q's format with up to 32 rows per kv head
+    (Hq / Hkv * N), with more as one, as flash_attn's do. Results are deterministic; the
+    last bits of one request may depend on the lengths of the others. No gradient:
+    tensors that require grad (the slopes too) are refused outside torch.no_grad(), and
+    duals of forward mode.
     """
     _paged_inputs("paged_attn", q, k_cache, v_cache, block_table, kv_len)
     if alibi_slopes is not None:

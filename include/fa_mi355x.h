@@ -509,32 +509,33 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
                     int N, int Hkv, int D, void* stream);
 
 /*
- * Attention of the newest N tokens of each request over its paged cache (N = 1:
- * a decoding step; a few: drafted tokens checked at once). q, o and lse as in
- * fa_fwd_ex (lse may be NULL); row n of entry b is token kv_len[b] - N + n, whose
- * own keys and values the cache holds already, and with `causal` it sees the
- * keys up to itself, else all of them. Rows without a key (kv_len[b] = 0, or
- * kv_len[b] < N: the first rows under causal masking) get o = 0, lse = +inf. What
- * lies in rows of the pool that no row of q sees reaches no output, NaN included;
- * an infinity or NaN that one row sees may come out as NaN in it and in the others
- * of its kv head (masked values are multiplied by zero). Their lse is theirs alone:
- * NaN for a row whose own scores hold a NaN or +inf, +inf for rows without a key
- * and (their weights being zero) for those whose scores are all -inf. Of `opts`, dtype, layout,
- * window (counted from the row's token), alibi_slopes and scale are taken (NULL:
- * the defaults); anything else set is refused. With a window the table entries of
- * pages wholly outside it are not read. Keys in pages whose index is outside [0,
- * pages) are hidden like masked ones. The keys of a batch are shared evenly among
- * the GPU's compute units whatever their lengths; partial results meet in
- * `workspace`, of at least fa_paged_attn_workspace_bytes() bytes (0 for invalid
- * arguments; whatever the lengths, about 2.1 MB for each of the Hq / Hkv * N rows of a kv
- * head up to 32, less at small D: 68 MB at most), which may hold anything. Calls that overlap in time need workspaces of
- * their own. q, o and the workspace are 16-byte aligned; Hq * N <= 2^24, Hq * D <
- * 2^31, and the 32-key blocks of full tables, times B, Hkv and the 32-row tiles of
- * Hq / Hkv * N, at most 2^30. Sums, maxima and scores are fp32; the
+ * Attention of the newest N tokens of each request over its paged cache (N = 1: a
+ * decoding step; a few: drafted tokens checked at once). q, o and lse as in fa_fwd_ex
+ * (lse may be NULL); row n of entry b is token kv_len[b] - N + n, whose own keys and
+ * values the cache holds already, and with `causal` it sees the keys up to itself,
+ * else all of them. Rows without a key (kv_len[b] = 0, or kv_len[b] < N: the first
+ * rows under causal masking) get o = 0, lse = +inf. What lies in rows of the pool that
+ * no row of q sees reaches no output, NaN included; an infinity or NaN that one row
+ * sees may come out as NaN in it and in the others of its kv head (masked values are
+ * multiplied by zero). Their lse is theirs alone: NaN for a row whose own scores hold
+ * a NaN or +inf, +inf for rows without a key and (their weights being zero) for those
+ * whose scores are all -inf. Of `opts`, dtype, layout, window (counted from the row's
+ * token), alibi_slopes and scale are taken (NULL: the defaults); anything else set is
+ * refused. With a window the table entries of pages wholly outside it are not read.
+ * Keys in pages whose index is outside [0, pages) are hidden like masked ones. The
+ * keys of a batch are shared evenly among the GPU's compute units whatever their
+ * lengths; partial results meet in `workspace`, of at least
+ * fa_paged_attn_workspace_bytes() bytes (0 for invalid arguments; whatever the
+ * lengths, about 2.1 MB for each of the Hq / Hkv * N rows of a kv head up to 32, less
+ * at small D: 68 MB at most), which may hold anything. Calls that overlap in time need
+ * workspaces of their own. q, o and the workspace are 16-byte aligned; Hq * N <= 2^24,
+ * Hq * D < 2^31, and the 32-key blocks of full tables, times B, Hkv and the 32-row
+ * tiles of Hq / Hkv * N, at most 2^30. Sums, maxima and scores are fp32; the
  * probabilities enter the product with v as two numbers of q's format (off by 2^-16 of
  * themselves in bf16, 2^-22 in fp16) where Hq / Hkv * N <= 32, with more rows as one,
- * as in fa_fwd (in fp16, below 2^-29 of a row's largest, as multiples of 2^-39 of it). The results are deterministic; a request's last
- * bits may depend on the lengths of the others in its batch.
+ * as in fa_fwd (in fp16, below 2^-29 of a row's largest, as multiples of 2^-39 of it).
+ * The results are deterministic; a request's last bits may depend on the lengths of
+ * the others in its batch.
  */
 size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
 int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
