@@ -571,16 +571,19 @@ static int page_shift_of(int page_size) {
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Checks a paged cache's pools and fills the kernels' description of them.
-static int paged_pool(const fa_paged_cache* c, int Hkv, int D, fa::PagedPool& p) {
-  if (!fa::valid_head_dim(D)) return FA_ERR_HEAD_DIM;
+// Checks a paged cache's pools (of K alone: k_only) and fills the kernels' description of
+// them. four: rows of 4 bits, whose strides count bytes.
+static int paged_pool(const fa_paged_cache* c, int Hkv, int D, fa::PagedPool& p, bool four = false,
+                      bool k_only = false) {
+  if (!fa::valid_head_dim(D) || (four && D % 32 != 0)) return FA_ERR_HEAD_DIM;
   if (Hkv <= 0) return FA_ERR_HEADS;
-  if (!c || !c->k || !c->v) return FA_ERR_NULL;
+  if (!c || !c->k || (!c->v && !k_only)) return FA_ERR_NULL;
   p.page_shift = page_shift_of(c->page_size);
   if (p.page_shift < 0 || c->pages <= 0 || (long long)c->pages * c->page_size > INT_MAX)
     return FA_ERR_PAGES;
-  if (!aligned16(c->k) || !aligned16(c->v) || c->stride_page < 0 || c->stride_head < 0 ||
-      c->stride_row < 0 || ((c->stride_page | c->stride_head | c->stride_row) & 7))
+  if (!aligned16(c->k) || (!k_only && !aligned16(c->v)) || c->stride_page < 0 ||
+      c->stride_head < 0 || c->stride_row < 0 ||
+      ((c->stride_page | c->stride_head | c->stride_row) & (four ? 15 : 7)))
     return FA_ERR_PAGES;
   // (pages and rows are found by products of 32 bits)
   if (c->stride_page >= 1LL << 31 || c->stride_row >= 1LL << 31) return FA_ERR_TOO_LARGE;
@@ -593,16 +596,34 @@ static int paged_pool(const fa_paged_cache* c, int Hkv, int D, fa::PagedPool& p)
   return FA_OK;
 }
 
+// The scales of a cache in 4 bits (k_only: of K).
+static int paged_scales(const fa_paged_scales* c, fa::PagedScales& s, bool k_only = false) {
+  if (!c || !c->k || (!c->v && !k_only)) return FA_ERR_NULL;
+  if (c->stride_page < 0 || c->stride_head < 0 || c->stride_row < 0) return FA_ERR_PAGES;
+  if (c->stride_page >= 1LL << 31 || c->stride_row >= 1LL << 31) return FA_ERR_TOO_LARGE;
+  s = {c->k, c->v, c->stride_page, c->stride_head, c->stride_row};
+  return FA_OK;
+}
+
+// One or two arrays over the rows of a paged pool, laid out alike: `width` units of
+// `unit` bytes per (page, kv head, row), strides in units.
+struct PoolArray {
+  const void* a;
+  const void* b;  // null: one array
+  long long page, head, row;
+  int width, unit;
+};
+
 // Whether two elements of a paged cache's pools share a place: of one pool, or of k's and
 // v's. The sizes and strides of the pool's dimensions that are walked, the innermost
 // first: each stride has to pass all that lies within it. same: k's rows are v's, and
 // both are written from the same ones.
-static bool pools_overlap(const fa::PagedPool& p, int Hkv, int page_size, int D, bool same) {
+static bool pools_overlap(const PoolArray& p, int pages, int Hkv, int page_size, bool same) {
   struct Dim {
     long long size, stride;
-  } dims[4] = {{D, 1}};
-  int n = 1;
-  for (const Dim& d : {Dim{p.pages, p.page_stride}, Dim{Hkv, p.head_stride}, Dim{page_size, p.row_stride}})
+  } dims[4];
+  int n = 0;
+  for (const Dim& d : {Dim{p.width, 1}, Dim{pages, p.page}, Dim{Hkv, p.head}, Dim{page_size, p.row}})
     if (d.size > 1) dims[n++] = d;
   std::sort(dims, dims + n, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
   long long reach[4], last = 0;  // the last element within dimension i's steps
@@ -611,10 +632,10 @@ static bool pools_overlap(const fa::PagedPool& p, int Hkv, int page_size, int D,
     reach[i] = last;
     last += (dims[i].size - 1) * dims[i].stride;
   }
-  if (same) return false;
-  // v's element x lies on k's y where their offsets differ by the pools' distance: by
+  if (same || !p.b) return false;
+  // b's element x lies on a's y where their offsets differ by the pools' distance: by
   // steps of the outermost dimension (two numbers of them leave little enough), and so on.
-  const long long bytes = (const char*)p.v - (const char*)p.k;
+  const long long bytes = (const char*)p.b - (const char*)p.a;
   auto meet = [&](auto&& self, long long apart, int i) -> bool {
     apart = apart < 0 ? -apart : apart;
     if (i < 0) return apart == 0;
@@ -625,8 +646,14 @@ static bool pools_overlap(const fa::PagedPool& p, int Hkv, int page_size, int D,
     }
     return false;
   };
-  const long long apart = (bytes < 0 ? -bytes : bytes) / 2;
+  const long long apart = (bytes < 0 ? -bytes : bytes) / p.unit;
   return apart <= last && meet(meet, apart, n - 1);
+}
+static PoolArray rows_of(const fa::PagedPool& p, int D, bool four) {
+  return {p.k, p.v, p.page_stride, p.head_stride, p.row_stride, four ? D / 2 : D, four ? 1 : 2};
+}
+static PoolArray scales_of(const fa::PagedScales& s, int D) {
+  return {s.k, s.v, s.page_stride, s.head_stride, s.row_stride, D / 32, 1};
 }
 
 int fa_paged_tables(int* table, long long table_stride, int table_width, const int* old_len,
@@ -666,7 +693,8 @@ int fa_paged_append(const void* k, const void* v, long long k_stride_b, long lon
     return FA_ERR_PAGES;
   const bool same = pool.k == pool.v && k == v && k_stride_b == v_stride_b &&
                     k_stride_n == v_stride_n && k_stride_h == v_stride_h;
-  if (pools_overlap(pool, Hkv, cache->page_size, D, same)) return FA_ERR_PAGES;
+  if (pools_overlap(rows_of(pool, D, false), pool.pages, Hkv, cache->page_size, same))
+    return FA_ERR_PAGES;
   return to_code(fa::launch_paged_append(k, v, {k_stride_b, k_stride_n, k_stride_h},
                                          {v_stride_b, v_stride_n, v_stride_h}, slots, pool, B, N,
                                          Hkv, D, stream));
@@ -688,18 +716,19 @@ size_t fa_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D) {
   return fa::paged_workspace_bytes(Hq / Hkv * N, D);
 }
 
-int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
-                  void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int N, int D,
-                  int causal, const fa_options* opts, void* stream) {
-  const fa_options& op = opts ? *opts : kDefaultOpts;
+// The checks of the calls that read a batch's newest rows over a paged cache, and their
+// arguments: all but o and the workspace.
+static int paged_rows(const void* q, const fa_paged_cache* cache, const fa_paged_scales* scales,
+                      int B, int Hq, int Hkv, int N, int D, int causal, const fa_options& op,
+                      bool k_only, void* stream, fa::PagedArgs& a) {
   int rc = check_opts(op, causal, Hq, N, D, false);
   if (rc == FA_OK) rc = check_paged_shape(B, Hq, Hkv, N, D);
   if (rc != FA_OK) return rc;
   if (op.kv_len || op.seg_start || op.mask || op.mask_t || op.drop || op.drop_t || op.bias ||
       op.kv_rows || op.block_rows)
     return FA_ERR_PAGES;
-  fa::PagedArgs a{};
-  rc = paged_pool(cache, Hkv, D, a.pool);
+  rc = paged_pool(cache, Hkv, D, a.pool, scales != nullptr, k_only);
+  if (rc == FA_OK && scales) rc = paged_scales(scales, a.scales, k_only);
   if (rc != FA_OK) return rc;
   if (cache->table_width <= 0 || cache->table_stride < cache->table_width ||
       (long long)cache->table_width * cache->page_size > (1 << 30))
@@ -710,18 +739,11 @@ int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cach
   const long long blocks = (long long)cache->table_width * cache->page_size / 32 + 4;
   if (tiles > (1 << 30) / blocks)
     return FA_ERR_TOO_LARGE;
-  const size_t need = fa::paged_workspace_bytes(Hq / Hkv * N, D);
-  if (!q || !o || !cache->table || !cache->kv_len || (need && !workspace)) return FA_ERR_NULL;
-  if (workspace_bytes < need) return FA_ERR_WORKSPACE;
-  if (!aligned16(q) || !aligned16(o) || !aligned16(workspace)) return FA_ERR_PAGES;
   a.q = q;
-  a.o = o;
-  a.lse = lse;
   a.table = cache->table;
   a.table_stride = cache->table_stride;
   a.table_width = cache->table_width;
   a.kv_len = cache->kv_len;
-  a.workspace = workspace;
   a.B = B;
   a.Hq = Hq;
   a.Hkv = Hkv;
@@ -734,7 +756,165 @@ int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cach
   a.window = op.window;
   a.alibi = op.alibi_slopes;
   a.scale = op.scale;
-  return to_code(fa::launch_paged(a));
+  return FA_OK;
+}
+
+static int paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
+                      const fa_paged_scales* scales, void* workspace, size_t workspace_bytes, int B,
+                      int Hq, int Hkv, int N, int D, int causal, const fa_options* opts, void* stream) {
+  fa::PagedArgs a{};
+  const int rc = paged_rows(q, cache, scales, B, Hq, Hkv, N, D, causal, opts ? *opts : kDefaultOpts,
+                            false, stream, a);
+  if (rc != FA_OK) return rc;
+  const size_t need = scales ? fa::paged4_workspace_bytes(Hq / Hkv * N, D)
+                             : fa::paged_workspace_bytes(Hq / Hkv * N, D);
+  if (!q || !o || !cache->table || !cache->kv_len || (need && !workspace)) return FA_ERR_NULL;
+  if (workspace_bytes < need) return FA_ERR_WORKSPACE;
+  if (!aligned16(q) || !aligned16(o) || !aligned16(workspace)) return FA_ERR_PAGES;
+  a.o = o;
+  a.lse = lse;
+  a.workspace = workspace;
+  return to_code(scales ? fa::launch_paged4(a) : fa::launch_paged(a));
+}
+
+int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
+                  void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int N, int D,
+                  int causal, const fa_options* opts, void* stream) {
+  return paged_attn(q, o, lse, cache, nullptr, workspace, workspace_bytes, B, Hq, Hkv, N, D, causal,
+                    opts, stream);
+}
+
+size_t fa_paged4_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D) {
+  if (check_paged_shape(B, Hq, Hkv, N, D) != FA_OK || D % 32 != 0) return 0;
+  return fa::paged4_workspace_bytes(Hq / Hkv * N, D);
+}
+
+int fa_paged4_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
+                   const fa_paged_scales* scales, void* workspace, size_t workspace_bytes, int B,
+                   int Hq, int Hkv, int N, int D, int causal, const fa_options* opts, void* stream) {
+  if (!scales) return FA_ERR_NULL;
+  return paged_attn(q, o, lse, cache, scales, workspace, workspace_bytes, B, Hq, Hkv, N, D, causal,
+                    opts, stream);
+}
+
+int fa_paged4_append(const void* k, const void* v, long long k_stride_b, long long k_stride_n,
+                     long long k_stride_h, long long v_stride_b, long long v_stride_n,
+                     long long v_stride_h, const int* slots, const fa_paged_cache* cache,
+                     const fa_paged_scales* scales, int B, int N, int Hkv, int D, int dtype,
+                     void* stream) {
+  if (dtype != FA_DTYPE_FP16 && dtype != FA_DTYPE_BF16) return FA_ERR_DTYPE;
+  fa::PagedPool pool{};
+  fa::PagedScales to{};
+  int rc = paged_pool(cache, Hkv, D, pool, true);
+  if (rc == FA_OK) rc = paged_scales(scales, to);
+  if (rc != FA_OK) return rc;
+  if (N <= 0) return FA_ERR_SEQLEN;
+  if (B <= 0) return FA_ERR_BATCH;
+  if ((long long)B * N > INT_MAX || (long long)Hkv * D > INT_MAX) return FA_ERR_TOO_LARGE;
+  if (!k || !v || !slots) return FA_ERR_NULL;
+  if (!aligned16(k) || !aligned16(v) ||
+      ((k_stride_b | k_stride_n | k_stride_h | v_stride_b | v_stride_n | v_stride_h) & 7))
+    return FA_ERR_PAGES;
+  const bool same = pool.k == pool.v && to.k == to.v && k == v && k_stride_b == v_stride_b &&
+                    k_stride_n == v_stride_n && k_stride_h == v_stride_h;
+  if (pools_overlap(rows_of(pool, D, true), pool.pages, Hkv, cache->page_size, same) ||
+      pools_overlap(scales_of(to, D), pool.pages, Hkv, cache->page_size, same))
+    return FA_ERR_PAGES;
+  return to_code(fa::launch_paged4_append(k, v, {k_stride_b, k_stride_n, k_stride_h},
+                                          {v_stride_b, v_stride_n, v_stride_h}, slots, pool, to, B,
+                                          N, Hkv, D, dtype, stream));
+}
+
+int fa_paged_gather(void* k, void* v, long long stride_b, long long stride_n, long long stride_h,
+                    const int* slots, const fa_paged_cache* cache, const fa_paged_scales* scales,
+                    int B, int N, int Hkv, int D, int dtype, void* stream) {
+  if (dtype != FA_DTYPE_FP16 && dtype != FA_DTYPE_BF16) return FA_ERR_DTYPE;
+  fa::PagedPool pool{};
+  fa::PagedScales from{};
+  int rc = paged_pool(cache, Hkv, D, pool, scales != nullptr);
+  if (rc == FA_OK && scales) rc = paged_scales(scales, from);
+  if (rc != FA_OK) return rc;
+  if (N <= 0) return FA_ERR_SEQLEN;
+  if (B <= 0) return FA_ERR_BATCH;
+  if ((long long)B * N > INT_MAX || (long long)Hkv * D > INT_MAX) return FA_ERR_TOO_LARGE;
+  if (!k || !v || !slots) return FA_ERR_NULL;
+  if (!aligned16(k) || !aligned16(v) || ((stride_b | stride_n | stride_h) & 7)) return FA_ERR_PAGES;
+  return to_code(fa::launch_paged_gather(k, v, {stride_b, stride_n, stride_h}, slots, pool,
+                                         scales ? &from : nullptr, B, N, Hkv, D, dtype, stream));
+}
+
+int fa_paged_weights(const void* q, const float* lse, const fa_paged_cache* cache,
+                     const fa_paged_scales* scales, float* weights, long long w_stride_page,
+                     long long w_stride_head, long long w_stride_row, int restart, int B, int Hq,
+                     int Hkv, int N, int D, int causal, const fa_options* opts, void* stream) {
+  fa::PagedArgs a{};
+  const int rc = paged_rows(q, cache, scales, B, Hq, Hkv, N, D, causal, opts ? *opts : kDefaultOpts,
+                            true, stream, a);
+  if (rc != FA_OK) return rc;
+  if (!q || !lse || !weights || !cache->table || !cache->kv_len) return FA_ERR_NULL;
+  if (!aligned16(q) || w_stride_page < 0 || w_stride_head < 0 || w_stride_row < 0 ||
+      pools_overlap({weights, nullptr, w_stride_page, w_stride_head, w_stride_row, 1, 4},
+                    a.pool.pages, Hkv, cache->page_size, false))
+    return FA_ERR_PAGES;
+  a.lse = const_cast<float*>(lse);
+  return to_code(fa::launch_paged_weights(a, {weights, w_stride_page, w_stride_head, w_stride_row},
+                                          restart != 0));
+}
+
+static bool evict_shape(int B, int Hkv, int table_width, int page_size) {
+  return B > 0 && Hkv > 0 && table_width > 0 && page_shift_of(page_size) >= 0 &&
+         (long long)table_width * page_size <= (1 << 30) && (long long)B * Hkv <= (1 << 21);
+}
+
+size_t fa_paged_evict_workspace_bytes(int B, int Hkv, int table_width, int page_size) {
+  return evict_shape(B, Hkv, table_width, page_size)
+             ? fa::evict_workspace_bytes(B, Hkv, table_width, page_size) : 0;
+}
+
+int fa_paged_evict(const fa_paged_cache* cache, const fa_paged_scales* scales, float* weights,
+                   long long w_stride_page, long long w_stride_head, long long w_stride_row,
+                   const int* max_len, int recent, int* new_len, void* workspace,
+                   size_t workspace_bytes, int B, int Hkv, int D, void* stream) {
+  const bool four = scales != nullptr;
+  fa::EvictArgs a{};
+  int rc = paged_pool(cache, Hkv, D, a.pool, four);
+  if (rc == FA_OK && four) rc = paged_scales(scales, a.scales);
+  if (rc != FA_OK) return rc;
+  if (B <= 0) return FA_ERR_BATCH;
+  if (cache->table_width <= 0 || cache->table_stride < cache->table_width ||
+      (long long)cache->table_width * cache->page_size > (1 << 30) || recent < 0)
+    return FA_ERR_PAGES;
+  if (!evict_shape(B, Hkv, cache->table_width, cache->page_size)) return FA_ERR_TOO_LARGE;
+  if (!weights || !max_len || !new_len || !workspace || !cache->table || !cache->kv_len)
+    return FA_ERR_NULL;
+  if (workspace_bytes < fa::evict_workspace_bytes(B, Hkv, cache->table_width, cache->page_size))
+    return FA_ERR_WORKSPACE;
+  const int pages = a.pool.pages, rows = cache->page_size;
+  if (w_stride_page < 0 || w_stride_head < 0 || w_stride_row < 0 ||
+      (reinterpret_cast<uintptr_t>(workspace) & 3u) ||
+      pools_overlap({weights, nullptr, w_stride_page, w_stride_head, w_stride_row, 1, 4}, pages, Hkv,
+                    rows, false) ||
+      pools_overlap(rows_of(a.pool, D, four), pages, Hkv, rows, false) ||
+      (four && pools_overlap(scales_of(a.scales, D), pages, Hkv, rows, false)))
+    return FA_ERR_PAGES;
+  const int unit = four ? 1 : 2;
+  a.pool.page_stride *= unit;
+  a.pool.head_stride *= unit;
+  a.pool.row_stride *= unit;
+  a.row_bytes = four ? D / 2 : 2 * D;
+  a.scale_bytes = four ? D / 32 : 0;
+  a.weights = {weights, w_stride_page, w_stride_head, w_stride_row};
+  a.table = cache->table;
+  a.table_stride = cache->table_stride;
+  a.table_width = cache->table_width;
+  a.kv_len = cache->kv_len;
+  a.max_len = max_len;
+  a.recent = recent;
+  a.new_len = new_len;
+  a.kept = (int*)workspace;
+  a.B = B;
+  a.Hkv = Hkv;
+  return to_code(fa::launch_paged_evict(a, stream));
 }
 
 float fa_dropout_scale(float p) {

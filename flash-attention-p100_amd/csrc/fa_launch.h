@@ -278,8 +278,16 @@ struct PagedPool {
   int pages, page_shift;  // (rows of a page: a power of two)
 };
 
+// The scales of a pool in 4 bits (fa_paged_scales): byte strides; null where rows are of
+// 16 bits. The pool's own strides then count bytes.
+struct PagedScales {
+  uint8_t* k;
+  uint8_t* v;
+  long long page_stride, head_stride, row_stride;
+};
+
 // Attention of the newest N tokens of B requests over their pages
-// (fa_paged_attn; arguments as FwdArgs).
+// (fa_paged_attn, fa_paged4_attn; arguments as FwdArgs).
 struct PagedArgs {
   const void* q;
   void* o;
@@ -298,6 +306,7 @@ struct PagedArgs {
   int window = 0;
   const float* alibi = nullptr;
   float scale = 0.f;
+  PagedScales scales = {};  // (of a pool in 4 bits)
 };
 // rows: of a kv head (Hq / Hkv * N).
 size_t paged_workspace_bytes(int rows, int D);
@@ -306,6 +315,13 @@ size_t paged_workspace_w(int rows);
 template <int W, bool BF>
 hipError_t launch_paged_w(const PagedArgs& a);
 hipError_t launch_paged(const PagedArgs& a);
+// The same over a pool in 4 bits.
+size_t paged4_workspace_bytes(int rows, int D);
+template <int W, bool BF>
+size_t paged4_workspace_w(int rows);
+template <int W, bool BF>
+hipError_t launch_paged4_w(const PagedArgs& a);
+hipError_t launch_paged4(const PagedArgs& a);
 
 // Strides (elements) of the rows that fa_paged_append writes: (b, n, head).
 struct RowStrides {
@@ -314,6 +330,45 @@ struct RowStrides {
 hipError_t launch_paged_append(const void* k, const void* v, RowStrides sk, RowStrides sv,
                                const int* slots, const PagedPool& pool, int B, int N, int Hkv,
                                int D, void* stream);
+// The same into a pool in 4 bits, and rows (of `dtype`, b, n and head apart by `strides`)
+// from a pool of either kind (scales null: 16 bits).
+hipError_t launch_paged4_append(const void* k, const void* v, RowStrides sk, RowStrides sv,
+                                const int* slots, const PagedPool& pool, const PagedScales& scales,
+                                int B, int N, int Hkv, int D, int dtype, void* stream);
+hipError_t launch_paged_gather(void* k, void* v, RowStrides strides, const int* slots,
+                               const PagedPool& pool, const PagedScales* scales, int B, int N,
+                               int Hkv, int D, int dtype, void* stream);
+
+// The weights that the newest rows give each cached key (fa_paged_weights): `a` without o, v
+// and workspace; weights at page * page_stride + head * head_stride + row * row_stride.
+struct KeyWeights {
+  float* w;
+  long long page_stride, head_stride, row_stride;
+};
+template <int W, bool BF>
+hipError_t launch_paged_weights_w(const PagedArgs& a, const KeyWeights& w, bool restart);
+hipError_t launch_paged_weights(const PagedArgs& a, const KeyWeights& w, bool restart);
+
+// Eviction (fa_paged_evict). row_bytes: of a pool's row; scale_bytes: of its scales (0: none).
+// The pool's and the scales' strides are in bytes.
+struct EvictArgs {
+  PagedPool pool;
+  PagedScales scales;
+  int row_bytes, scale_bytes;
+  KeyWeights weights;
+  const int* table;
+  long long table_stride;
+  int table_width;
+  const int* kv_len;
+  const int* max_len;
+  int recent;
+  int* new_len;
+  int* kept;  // workspace
+  int B, Hkv;
+};
+size_t evict_workspace_bytes(int B, int Hkv, int table_width, int page_size);
+hipError_t launch_paged_evict(const EvictArgs& a, void* stream);
+
 // fa_paged_tables' arguments (tokens < 0: slots of max_new per request).
 struct TablesArgs {
   int* table;

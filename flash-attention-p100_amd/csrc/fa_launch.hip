@@ -414,6 +414,30 @@ hipError_t launch_paged(const PagedArgs& a) {
   });
 }
 
+// (bf16's: its tiles hold as many rows as fp16's or more)
+size_t paged4_workspace_bytes(int rows, int D) {
+  FwdArgs a{};
+  a.D = D;
+  size_t n = 0;
+  (void)by_width(a, true, [&](auto w, auto bf, const FwdArgs&) {
+    n = paged4_workspace_w<decltype(w)::value, decltype(bf)::value>(rows);
+    return hipSuccess;
+  });
+  return n;
+}
+
+hipError_t launch_paged4(const PagedArgs& a) {
+  return by_width(a, a.dtype == kBF16, [](auto w, auto bf, const PagedArgs& a) {
+    return launch_paged4_w<decltype(w)::value, decltype(bf)::value>(a);
+  });
+}
+
+hipError_t launch_paged_weights(const PagedArgs& a, const KeyWeights& kw, bool restart) {
+  return by_width(a, a.dtype == kBF16, [&](auto w, auto bf, const PagedArgs& a) {
+    return launch_paged_weights_w<decltype(w)::value, decltype(bf)::value>(a, kw, restart);
+  });
+}
+
 unsigned long long fwd_launch_items(int B, int Hq, int N, int D) {
   const unsigned long long tiles = ((unsigned long long)N + kFwdRows - 1) / kFwdRows;
   const unsigned long long wgs = tiles * (unsigned long long)B * (unsigned long long)Hq;

@@ -706,19 +706,33 @@ static int64_t walk(const at::Tensor& t, int64_t dim) { return t.size(dim) == 1 
 // Whether 16-byte loads can take t's rows: dense, each on a 16-byte boundary.
 static bool rows_aligned(const at::Tensor& t) {
   bool ok = (t.size(-1) <= 1 || t.stride(-1) == 1) && ((uintptr_t)t.data_ptr() & 15) == 0;
-  for (int64_t i = 0; i < t.dim() - 1; ++i) ok = ok && walk(t, i) % 8 == 0;
+  for (int64_t i = 0; i < t.dim() - 1; ++i) ok = ok && walk(t, i) * t.element_size() % 16 == 0;
   return ok;
 }
 
+static bool is_16bit(const at::Tensor& t) {
+  return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16;
+}
+
+typedef c10::optional<at::Tensor> MaybeTensor;
+
 // The cache of k_cache and v_cache, (pages, Hkv, page_size, D) in any order of
-// the first three dimensions, laid out alike; the tables are left unset.
-static fa_paged_cache paged_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& like) {
+// the first three dimensions, laid out alike; the tables are left unset. four: of 4 bits,
+// (pages, Hkv, page_size, D / 2) bytes.
+static fa_paged_cache paged_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& like,
+                                  bool four = false) {
   TORCH_CHECK(k.is_cuda() && k.device() == like.device() && v.device() == like.device(),
               "k_cache and v_cache must be on ", like.device());
-  TORCH_CHECK(k.scalar_type() == like.scalar_type() && v.scalar_type() == like.scalar_type(),
-              "k_cache and v_cache must be ", like.scalar_type(), " as the tokens are");
+  if (four) {
+    TORCH_CHECK(k.scalar_type() == at::kByte && v.scalar_type() == at::kByte,
+                "with scales k_cache and v_cache must be uint8, two values of 4 bits each");
+  } else {
+    TORCH_CHECK(k.scalar_type() == like.scalar_type() && v.scalar_type() == like.scalar_type(),
+                "k_cache and v_cache must be ", like.scalar_type(), " as the tokens are");
+  }
   TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes(),
-              "k_cache and v_cache must both be (pages, Hkv, page_size, D)");
+              "k_cache and v_cache must both be (pages, Hkv, page_size, D)",
+              four ? ", D / 2 bytes a row" : "");
   const int64_t page_size = k.size(2);
   TORCH_CHECK(page_size > 0 && (page_size & (page_size - 1)) == 0 && k.size(0) > 0 &&
                   k.size(0) <= INT32_MAX / page_size,
@@ -738,6 +752,42 @@ static fa_paged_cache paged_cache(const at::Tensor& k, const at::Tensor& v, cons
   c.page_size = (int)page_size;
   return c;
 }
+
+// Whether a cache is of 4 bits: k_scale and v_scale come together.
+static bool is_four(const MaybeTensor& k_scale, const MaybeTensor& v_scale) {
+  TORCH_CHECK(k_scale.has_value() == v_scale.has_value(),
+              "k_scale and v_scale must be given together");
+  return k_scale.has_value();
+}
+
+// The scales of a cache in 4 bits, (pages, Hkv, page_size, D / 32) bytes in any order of the
+// first three dimensions, laid out alike.
+static fa_paged_scales paged_scales(const at::Tensor& k_scale, const at::Tensor& v_scale,
+                                    const at::Tensor& k_cache) {
+  fa_paged_scales s{};
+  for (const auto& tn : {std::make_pair(&k_scale, "k_scale"), std::make_pair(&v_scale, "v_scale")}) {
+    const at::Tensor& t = *tn.first;
+    TORCH_CHECK(t.device() == k_cache.device() && t.scalar_type() == at::kByte, tn.second,
+                " must be uint8 on ", k_cache.device());
+    TORCH_CHECK(t.dim() == 4 && t.size(0) == k_cache.size(0) && t.size(1) == k_cache.size(1) &&
+                    t.size(2) == k_cache.size(2) && k_cache.size(3) % 16 == 0 &&
+                    t.size(3) == k_cache.size(3) / 16,
+                tn.second, " must be (pages, Hkv, page_size, D / 32), a byte for 32 values of "
+                "k_cache and v_cache (D a multiple of 32), got ", t.sizes());
+    TORCH_CHECK(t.size(3) <= 1 || t.stride(3) == 1, tn.second, "'s rows must be dense");
+  }
+  for (int64_t i = 0; i < 3; ++i)
+    TORCH_CHECK(walk(k_scale, i) == walk(v_scale, i), "k_scale and v_scale must be laid out alike");
+  s.k = k_scale.data_ptr<uint8_t>();
+  s.v = v_scale.data_ptr<uint8_t>();
+  s.stride_page = walk(k_scale, 0);
+  s.stride_head = walk(k_scale, 1);
+  s.stride_row = walk(k_scale, 2);
+  return s;
+}
+
+// The head dim that a cache's rows hold.
+static int64_t cache_dim(const at::Tensor& cache, bool four) { return cache.size(3) * (four ? 2 : 1); }
 
 // [slots (B, max_new) or (tokens,), kv_len (B,), ring (2,)]; block_table and
 // free_pages in place (fa_paged_tables).
@@ -787,9 +837,11 @@ std::vector<at::Tensor> fa_paged_tables_t(const at::Tensor& block_table, const a
 }
 
 // k, v (T, Hkv, D) with slots (T,), or (B, Hkv, N, D) with slots (B, N), into
-// the caches (fa_paged_append).
+// the caches (fa_paged_append; with scales fa_paged4_append).
 void fa_paged_append_t(at::Tensor k, at::Tensor v, const at::Tensor& k_cache,
-                       const at::Tensor& v_cache, at::Tensor slots) {
+                       const at::Tensor& v_cache, at::Tensor slots, const MaybeTensor& k_scale,
+                       const MaybeTensor& v_scale) {
+  const bool four = is_four(k_scale, v_scale);
   check_no_grad(k, "k");
   check_no_grad(v, "v");
   check_no_grad(k_cache, "k_cache");
@@ -797,8 +849,7 @@ void fa_paged_append_t(at::Tensor k, at::Tensor v, const at::Tensor& k_cache,
   for (auto& tn : {std::make_pair(&k, "k"), std::make_pair(&v, "v")}) {
     const at::Tensor& t = *tn.first;
     TORCH_CHECK(t.is_cuda(), tn.second, " must be a CUDA tensor");
-    TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, tn.second,
-                " must be fp16 or bf16");
+    TORCH_CHECK(is_16bit(t), tn.second, " must be fp16 or bf16");
   }
   TORCH_CHECK((k.dim() == 3 || k.dim() == 4) && k.sizes() == v.sizes(),
               "k and v must both be (T, Hkv, D) or (B, Hkv, N, D)");
@@ -806,9 +857,11 @@ void fa_paged_append_t(at::Tensor k, at::Tensor v, const at::Tensor& k_cache,
   const int64_t B = k.size(0), Hkv = k.size(1), N = flat ? 1 : k.size(2), D = k.size(-1);
   TORCH_CHECK(D >= 8 && D <= 256 && D % 8 == 0, "head dim must be a multiple of 8 from 8 to 256, got ", D);
   TORCH_CHECK(v.device() == k.device(), "k and v must be on the same device");
-  const fa_paged_cache cache = paged_cache(k_cache, v_cache, k);
-  TORCH_CHECK(k_cache.size(1) == Hkv && k_cache.size(3) == D && v.scalar_type() == k.scalar_type(),
+  const fa_paged_cache cache = paged_cache(k_cache, v_cache, k, four);
+  TORCH_CHECK(k_cache.size(1) == Hkv && cache_dim(k_cache, four) == D &&
+                  v.scalar_type() == k.scalar_type(),
               "k, v, k_cache and v_cache must have the same heads, head dim and format");
+  const fa_paged_scales scales = four ? paged_scales(*k_scale, *v_scale, k_cache) : fa_paged_scales{};
   TORCH_CHECK(slots.device() == k.device() && slots.scalar_type() == at::kInt,
               "slots must be int32 on ", k.device());
   TORCH_CHECK(slots.dim() == (flat ? 1 : 2) && slots.size(0) == B && (flat || slots.size(1) == N),
@@ -817,43 +870,79 @@ void fa_paged_append_t(at::Tensor k, at::Tensor v, const at::Tensor& k_cache,
               "k and v may hold at most 2^31 - 1 tokens, of 2^31 - 1 elements");
   at::assert_no_internal_overlap(k_cache);  // (expanded ones, whose rows are several tokens')
   at::assert_no_internal_overlap(v_cache);
+  if (four) {
+    at::assert_no_internal_overlap(*k_scale);
+    at::assert_no_internal_overlap(*v_scale);
+  }
   if (B * N * Hkv == 0) return;
   c10::DeviceGuard guard(k.device());
   if (!rows_aligned(k)) k = k.clone(at::MemoryFormat::Contiguous);
   if (!rows_aligned(v)) v = v.clone(at::MemoryFormat::Contiguous);
   slots = slots.contiguous();
-  check_rc(fa_paged_append(k.data_ptr(), v.data_ptr(), walk(k, 0), flat ? 0 : walk(k, 2), walk(k, 1),
-                           walk(v, 0), flat ? 0 : walk(v, 2), walk(v, 1), slots.data_ptr<int>(),
-                           &cache, (int)B, (int)N, (int)Hkv, (int)D, current_stream(k)),
-           "fa_paged_append");
+  const int64_t kn = flat ? 0 : walk(k, 2), vn = flat ? 0 : walk(v, 2);
+  if (four) {
+    check_rc(fa_paged4_append(k.data_ptr(), v.data_ptr(), walk(k, 0), kn, walk(k, 1), walk(v, 0), vn,
+                              walk(v, 1), slots.data_ptr<int>(), &cache, &scales, (int)B, (int)N,
+                              (int)Hkv, (int)D, dtype_code(k), current_stream(k)),
+             "fa_paged4_append");
+    written(*k_scale);
+    written(*v_scale);
+  } else {
+    check_rc(fa_paged_append(k.data_ptr(), v.data_ptr(), walk(k, 0), kn, walk(k, 1), walk(v, 0), vn,
+                             walk(v, 1), slots.data_ptr<int>(), &cache, (int)B, (int)N, (int)Hkv,
+                             (int)D, current_stream(k)),
+             "fa_paged_append");
+  }
   written(k_cache);
   written(v_cache);
 }
 
-// [o] or [o, lse]: attention of the newest N tokens over the caches
-// (fa_paged_attn). q as forward_dt's, or a (B, H, N, D) view of a dense (B, N,
-// H, D) tensor, whose layout o then has too.
-std::vector<at::Tensor> fa_paged_attn_t(at::Tensor q, const at::Tensor& k_cache,
-                                        const at::Tensor& v_cache, const at::Tensor& block_table,
-                                        const at::Tensor& kv_len, bool causal, int64_t window,
-                                        c10::optional<at::Tensor> alibi_slopes, double scale,
-                                        bool want_lse) {
-  check_no_grad(q, "q");
+// [k, v]: the rows at `slots` (T,) or (B, N), (T, Hkv, D) or (B, Hkv, N, D) (fa_paged_gather).
+std::vector<at::Tensor> fa_paged_gather_t(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                          at::Tensor slots, const MaybeTensor& k_scale,
+                                          const MaybeTensor& v_scale, c10::optional<at::ScalarType> dtype) {
+  const bool four = is_four(k_scale, v_scale);
   check_no_grad(k_cache, "k_cache");
   check_no_grad(v_cache, "v_cache");
-  if (alibi_slopes) {
-    check_no_grad(*alibi_slopes, "alibi_slopes");
-    alibi_slopes = alibi_slopes->to(at::kFloat).contiguous();
-  }
-  check_in16(q, "q");
-  fa_paged_cache cache = paged_cache(k_cache, v_cache, q);
-  const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3);
-  const int64_t Hkv = k_cache.size(1);
+  const fa_paged_cache cache = paged_cache(k_cache, v_cache, k_cache, four);
+  TORCH_CHECK(four || is_16bit(k_cache), "k_cache must be fp16 or bf16, or uint8 with scales");
+  const fa_paged_scales scales = four ? paged_scales(*k_scale, *v_scale, k_cache) : fa_paged_scales{};
+  const at::ScalarType type = dtype.value_or(four ? at::kBFloat16 : k_cache.scalar_type());
+  TORCH_CHECK(four ? type == at::kHalf || type == at::kBFloat16 : type == k_cache.scalar_type(),
+              "dtype must be ", four ? "fp16 or bf16" : "the cache's", ", got ", type);
+  const int64_t Hkv = k_cache.size(1), D = cache_dim(k_cache, four);
   TORCH_CHECK(D >= 8 && D <= 256 && D % 8 == 0, "head dim must be a multiple of 8 from 8 to 256, got ", D);
+  TORCH_CHECK(slots.device() == k_cache.device() && slots.scalar_type() == at::kInt,
+              "slots must be int32 on ", k_cache.device());
+  TORCH_CHECK(slots.dim() == 1 || slots.dim() == 2, "slots must be (T,) or (B, N)");
+  const bool flat = slots.dim() == 1;
+  const int64_t B = slots.size(0), N = flat ? 1 : slots.size(1);
+  TORCH_CHECK(B <= INT32_MAX && N <= INT32_MAX && B * N <= INT32_MAX && Hkv * D <= INT32_MAX,
+              "slots may hold at most 2^31 - 1 tokens, of 2^31 - 1 elements");
+  c10::DeviceGuard guard(k_cache.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto opts = k_cache.options().dtype(type);
+  at::Tensor k = flat ? at::empty({B, Hkv, D}, opts) : at::empty({B, Hkv, N, D}, opts);
+  at::Tensor v = at::empty_like(k);
+  if (k.numel() == 0) return {k, v};
+  slots = slots.contiguous();
+  check_rc(fa_paged_gather(k.data_ptr(), v.data_ptr(), flat ? Hkv * D : Hkv * N * D, flat ? 0 : D,
+                           flat ? D : N * D, slots.data_ptr<int>(), &cache, four ? &scales : nullptr,
+                           (int)B, (int)N, (int)Hkv, (int)D, dtype_code(k), current_stream(k)),
+           "fa_paged_gather");
+  return {k, v};
+}
+
+// What the calls of a batch's newest rows over a cache have in common: checks q (B, H, N,
+// D), the table and the lengths against the cache's sizes, and fills the tables of `cache`
+// and the options. q in a layout that the kernels do not take, or not 16-byte aligned, is copied.
+static fa_options paged_rows(at::Tensor& q, fa_paged_cache& cache, int64_t Hkv,
+                             const at::Tensor& block_table, const at::Tensor& kv_len, int64_t window,
+                             const c10::optional<at::Tensor>& alibi_slopes, double scale) {
+  const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3);
   TORCH_CHECK(B > 0 && N > 0, "B and N must be positive");
   TORCH_CHECK(Hkv > 0 && H > 0 && H % Hkv == 0, "query heads (", H,
               ") must be a multiple of key/value heads (", Hkv, ")");
-  TORCH_CHECK(k_cache.size(3) == D, "k_cache must be (pages, Hkv, page_size, ", D, ") as q's head dim is");
   check_ints(block_table, q.device(), "block_table");
   TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == B && block_table.size(1) > 0 &&
                   (B == 1 || block_table.stride(0) >= block_table.size(1)),
@@ -863,8 +952,6 @@ std::vector<at::Tensor> fa_paged_attn_t(at::Tensor q, const at::Tensor& k_cache,
   check_ints(kv_len, q.device(), "kv_len");
   TORCH_CHECK(kv_len.dim() == 1 && kv_len.size(0) == B, "kv_len must be (", B, ",)");
   TORCH_CHECK(B <= INT32_MAX && H * N <= (1 << 24) && H * D <= INT32_MAX, "shape exceeds the kernels' index range");
-  c10::DeviceGuard guard(q.device());
-  at::AutoDispatchBelowADInplaceOrView below;
   fa_options op{};
   op.dtype = dtype_code(q);
   op.window = (int)std::min<int64_t>(window, INT32_MAX);
@@ -879,17 +966,164 @@ std::vector<at::Tensor> fa_paged_attn_t(at::Tensor q, const at::Tensor& k_cache,
   cache.table_stride = B == 1 ? block_table.size(1) : block_table.stride(0);
   cache.table_width = (int)block_table.size(1);
   cache.kv_len = kv_len.data_ptr<int>();
+  return op;
+}
+
+// [o] or [o, lse]: attention of the newest N tokens over the caches (fa_paged_attn, with
+// scales fa_paged4_attn). q as forward_dt's, or a (B, H, N, D) view of a dense (B, N,
+// H, D) tensor, whose layout o then has too.
+std::vector<at::Tensor> fa_paged_attn_t(at::Tensor q, const at::Tensor& k_cache,
+                                        const at::Tensor& v_cache, const at::Tensor& block_table,
+                                        const at::Tensor& kv_len, bool causal, int64_t window,
+                                        c10::optional<at::Tensor> alibi_slopes, double scale,
+                                        bool want_lse, const MaybeTensor& k_scale,
+                                        const MaybeTensor& v_scale) {
+  const bool four = is_four(k_scale, v_scale);
+  check_no_grad(q, "q");
+  check_no_grad(k_cache, "k_cache");
+  check_no_grad(v_cache, "v_cache");
+  if (alibi_slopes) {
+    check_no_grad(*alibi_slopes, "alibi_slopes");
+    alibi_slopes = alibi_slopes->to(at::kFloat).contiguous();
+  }
+  check_in16(q, "q");
+  fa_paged_cache cache = paged_cache(k_cache, v_cache, q, four);
+  const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3);
+  const int64_t Hkv = k_cache.size(1);
+  TORCH_CHECK(D >= 8 && D <= 256 && D % 8 == 0, "head dim must be a multiple of 8 from 8 to 256, got ", D);
+  TORCH_CHECK(cache_dim(k_cache, four) == D, "k_cache must be (pages, Hkv, page_size, ", D,
+              ") as q's head dim is", four ? ", two values a byte" : "");
+  const fa_paged_scales scales = four ? paged_scales(*k_scale, *v_scale, k_cache) : fa_paged_scales{};
+  c10::DeviceGuard guard(q.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const fa_options op = paged_rows(q, cache, Hkv, block_table, kv_len, window, alibi_slopes, scale);
   at::Tensor o = at::empty_like(q), lse;
   if (want_lse) lse = at::empty({B, H, N}, q.options().dtype(at::kFloat));
-  const size_t bytes = fa_paged_attn_workspace_bytes((int)B, (int)H, (int)Hkv, (int)N, (int)D);
+  const size_t bytes =
+      four ? fa_paged4_attn_workspace_bytes((int)B, (int)H, (int)Hkv, (int)N, (int)D)
+           : fa_paged_attn_workspace_bytes((int)B, (int)H, (int)Hkv, (int)N, (int)D);
   // (from torch's allocator as a tensor's memory is, without the tensor)
   const c10::DataPtr ws = c10::GetAllocator(c10::DeviceType::CUDA)->allocate(bytes);
-  check_rc(fa_paged_attn(q.data_ptr(), o.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr,
-                         &cache, ws.get(), bytes, (int)B, (int)H, (int)Hkv,
-                         (int)N, (int)D, causal ? 1 : 0, &op, current_stream(q)),
-           "fa_paged_attn");
+  float* const lse_ptr = want_lse ? lse.data_ptr<float>() : nullptr;
+  if (four)
+    check_rc(fa_paged4_attn(q.data_ptr(), o.data_ptr(), lse_ptr, &cache, &scales, ws.get(), bytes,
+                            (int)B, (int)H, (int)Hkv, (int)N, (int)D, causal ? 1 : 0, &op,
+                            current_stream(q)),
+             "fa_paged4_attn");
+  else
+    check_rc(fa_paged_attn(q.data_ptr(), o.data_ptr(), lse_ptr, &cache, ws.get(), bytes, (int)B,
+                           (int)H, (int)Hkv, (int)N, (int)D, causal ? 1 : 0, &op, current_stream(q)),
+             "fa_paged_attn");
   if (want_lse) return {o, lse};
   return {o};
+}
+
+// The weights of a cache's keys, (pages, Hkv, page_size) fp32 in any order of storage.
+static void check_weights(const at::Tensor& w, const at::Tensor& k_cache) {
+  check_no_grad(w, "weights");
+  TORCH_CHECK(w.device() == k_cache.device() && w.scalar_type() == at::kFloat,
+              "weights must be float32 on ", k_cache.device());
+  TORCH_CHECK(w.dim() == 3 && w.size(0) == k_cache.size(0) && w.size(1) == k_cache.size(1) &&
+                  w.size(2) == k_cache.size(2),
+              "weights must be (pages, Hkv, page_size) as k_cache is, got ", w.sizes());
+  at::assert_no_internal_overlap(w);
+}
+
+// Adds the newest rows' weights of the keys to `weights` (fa_paged_weights).
+void fa_paged_weights_t(at::Tensor q, const at::Tensor& k_cache, const at::Tensor& block_table,
+                        const at::Tensor& kv_len, at::Tensor lse, const at::Tensor& weights,
+                        bool causal, int64_t window, c10::optional<at::Tensor> alibi_slopes,
+                        double scale, bool restart, const MaybeTensor& k_scale) {
+  const bool four = k_scale.has_value();
+  check_no_grad(q, "q");
+  check_no_grad(k_cache, "k_cache");
+  check_no_grad(lse, "lse");
+  if (alibi_slopes) {
+    check_no_grad(*alibi_slopes, "alibi_slopes");
+    alibi_slopes = alibi_slopes->to(at::kFloat).contiguous();
+  }
+  check_in16(q, "q");
+  fa_paged_cache cache = paged_cache(k_cache, k_cache, q, four);
+  const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3);
+  TORCH_CHECK(D >= 8 && D <= 256 && D % 8 == 0, "head dim must be a multiple of 8 from 8 to 256, got ", D);
+  TORCH_CHECK(cache_dim(k_cache, four) == D, "k_cache must be (pages, Hkv, page_size, ", D,
+              ") as q's head dim is", four ? ", two values a byte" : "");
+  const fa_paged_scales scales = four ? paged_scales(*k_scale, *k_scale, k_cache) : fa_paged_scales{};
+  TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.dim() == 3 &&
+                  lse.size(0) == B && lse.size(1) == H && lse.size(2) == N,
+              "lse must be float32 (", B, ", ", H, ", ", N, ") on ", q.device());
+  check_weights(weights, k_cache);
+  c10::DeviceGuard guard(q.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  lse = lse.contiguous();
+  const fa_options op = paged_rows(q, cache, k_cache.size(1), block_table, kv_len, window, alibi_slopes, scale);
+  check_rc(fa_paged_weights(q.data_ptr(), lse.data_ptr<float>(), &cache, four ? &scales : nullptr,
+                            weights.data_ptr<float>(), walk(weights, 0), walk(weights, 1),
+                            walk(weights, 2), restart ? 1 : 0, (int)B, (int)H, (int)k_cache.size(1),
+                            (int)N, (int)D, causal ? 1 : 0, &op, current_stream(q)),
+           "fa_paged_weights");
+  written(weights);
+}
+
+// Cuts the requests to max_len tokens, in place; their new lengths (fa_paged_evict).
+at::Tensor fa_paged_evict_t(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                            const at::Tensor& weights, const at::Tensor& block_table,
+                            const at::Tensor& kv_len, const at::Tensor& max_len, int64_t recent,
+                            const MaybeTensor& k_scale, const MaybeTensor& v_scale) {
+  const bool four = is_four(k_scale, v_scale);
+  check_no_grad(k_cache, "k_cache");
+  check_no_grad(v_cache, "v_cache");
+  TORCH_CHECK(four || is_16bit(k_cache), "k_cache must be fp16 or bf16, or uint8 with scales");
+  fa_paged_cache cache = paged_cache(k_cache, v_cache, k_cache, four);
+  const int64_t Hkv = k_cache.size(1), D = cache_dim(k_cache, four);
+  TORCH_CHECK(Hkv > 0, "k_cache must have kv heads");
+  TORCH_CHECK(D >= 8 && D <= 256 && D % 8 == 0, "head dim must be a multiple of 8 from 8 to 256, got ", D);
+  const fa_paged_scales scales = four ? paged_scales(*k_scale, *v_scale, k_cache) : fa_paged_scales{};
+  check_weights(weights, k_cache);
+  const at::Device dev = k_cache.device();
+  check_ints(block_table, dev, "block_table");
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) > 0 && block_table.size(1) > 0 &&
+                  (block_table.size(0) == 1 || block_table.stride(0) >= block_table.size(1)),
+              "block_table must be (B, pages per request)");
+  const int64_t B = block_table.size(0);
+  TORCH_CHECK(block_table.size(1) <= (1 << 30) / cache.page_size,
+              "a request's pages hold at most 2^30 tokens");
+  check_ints(kv_len, dev, "kv_len");
+  check_ints(max_len, dev, "max_len");
+  TORCH_CHECK(kv_len.dim() == 1 && kv_len.size(0) == B && max_len.sizes() == kv_len.sizes(),
+              "kv_len and max_len must be (", B, ",)");
+  TORCH_CHECK(recent >= 0, "recent must not be negative");
+  TORCH_CHECK(B * Hkv <= (1 << 21), "at most 2^21 requests' kv heads");
+  at::assert_no_internal_overlap(k_cache);
+  at::assert_no_internal_overlap(v_cache);
+  if (four) {
+    at::assert_no_internal_overlap(*k_scale);
+    at::assert_no_internal_overlap(*v_scale);
+  }
+  c10::DeviceGuard guard(dev);
+  at::AutoDispatchBelowADInplaceOrView below;
+  cache.table = block_table.data_ptr<int>();
+  cache.table_stride = B == 1 ? block_table.size(1) : block_table.stride(0);
+  cache.table_width = (int)block_table.size(1);
+  cache.kv_len = kv_len.data_ptr<int>();
+  at::Tensor new_len = at::empty({B}, kv_len.options());
+  const size_t bytes =
+      fa_paged_evict_workspace_bytes((int)B, (int)Hkv, cache.table_width, cache.page_size);
+  const c10::DataPtr ws = c10::GetAllocator(c10::DeviceType::CUDA)->allocate(bytes);
+  check_rc(fa_paged_evict(&cache, four ? &scales : nullptr, weights.data_ptr<float>(),
+                          walk(weights, 0), walk(weights, 1), walk(weights, 2),
+                          max_len.data_ptr<int>(), (int)std::min<int64_t>(recent, INT32_MAX),
+                          new_len.data_ptr<int>(), ws.get(), bytes, (int)B, (int)Hkv, (int)D,
+                          current_stream(k_cache)),
+           "fa_paged_evict");
+  written(k_cache);
+  written(v_cache);
+  written(weights);
+  if (four) {
+    written(*k_scale);
+    written(*v_scale);
+  }
+  return new_len;
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -897,11 +1131,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("block_table"), py::arg("old_len"), py::arg("new_len"), py::arg("free_pages"),
         py::arg("ring"), py::arg("page_size"), py::arg("max_new"), py::arg("tokens"));
   m.def("paged_append", &fa_paged_append_t, "Writes tokens' keys and values into a paged cache",
-        py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"));
+        py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"),
+        py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none());
+  m.def("paged_gather", &fa_paged_gather_t, "Rows of a paged cache by their slots",
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"), py::arg("k_scale"),
+        py::arg("v_scale"), py::arg("dtype"));
   m.def("paged_attn", &fa_paged_attn_t, "Attention of the newest tokens over a paged cache",
         py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"),
         py::arg("kv_len"), py::arg("causal"), py::arg("window"), py::arg("alibi_slopes"),
-        py::arg("scale"), py::arg("want_lse"));
+        py::arg("scale"), py::arg("want_lse"), py::arg("k_scale") = py::none(),
+        py::arg("v_scale") = py::none());
+  m.def("paged_weights", &fa_paged_weights_t, "Adds the newest rows' attention weights of cached keys",
+        py::arg("q"), py::arg("k_cache"), py::arg("block_table"), py::arg("kv_len"), py::arg("lse"),
+        py::arg("weights"), py::arg("causal"), py::arg("window"), py::arg("alibi_slopes"),
+        py::arg("scale"), py::arg("restart"), py::arg("k_scale"));
+  m.def("paged_evict", &fa_paged_evict_t, "Cuts requests to their newest and heaviest keys",
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("weights"), py::arg("block_table"),
+        py::arg("kv_len"), py::arg("max_len"), py::arg("recent"), py::arg("k_scale"),
+        py::arg("v_scale"));
   m.def("dropout_bits", &fa_dropout_bits_t,
         "Dropout keep bits (B, H, N, ceil(N/32)) and their transpose for drop / drop_t",
         py::arg("seed"), py::arg("p"), py::arg("B"), py::arg("H"), py::arg("N"),

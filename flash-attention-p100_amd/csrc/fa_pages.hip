@@ -1,7 +1,9 @@
 // Paged key/value caches: the block tables and slots of a step from the
-// requests' lengths, and the writes of new rows into their slots. No counterpart
-// in the reference, which has no cache. (The attention over them: fa_paged.hip.)
+// requests' lengths, the writes of new rows into their slots, in 16 bits or
+// quantised to 4, and rows read back from there. No counterpart in the reference,
+// which has no cache. (The attention over them: fa_paged.hip, fa_paged4.hip.)
 #include <algorithm>
+#include <type_traits>
 
 #include "fa_device.h"
 #include "fa_launch.h"
@@ -232,7 +234,199 @@ __global__ __launch_bounds__(kAppThreads) void append_kernel(const AppendArgs a)
   }
 }
 
+// ---------------------------------------------------------------------------
+// Writes into a cache in 4 bits. With m the largest magnitude of 32 values of a row,
+// their scale is the least power of two X (from 2^-126 on) with m <= 7 X, so m keeps a
+// code next to it (up to 8 X, as the usual choice allows, the largest would be clamped
+// from 8 to 6), and a value x becomes the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 to
+// |x| / X, ties to the even code, with x's sign. x / X is exact, so the codes are those
+// that any correct rounding gives. Four lanes hold a block, a 16-byte chunk each.
+template <bool BF>
+__device__ __forceinline__ uint32_t to_codes(u32x4 x, float scale) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+  uint32_t c = 0;
+  auto two = [&](uint32_t pair, auto sel) {
+    constexpr int kByte = decltype(sel)::value;
+    if constexpr (BF) c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf2, pair), scale, kByte);
+    else c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(half2, pair), scale, kByte);
+  };
+  two(x[0], std::integral_constant<int, 0>{});
+  two(x[1], std::integral_constant<int, 1>{});
+  two(x[2], std::integral_constant<int, 2>{});
+  two(x[3], std::integral_constant<int, 3>{});
+  return c;
+}
+
+// The largest scales, of which 6 times is finite in the rows' format.
+template <bool BF>
+constexpr uint32_t kTopScale = BF ? 127 + 125 : 127 + 13;
+
+// A row's slot, or none: page < 0.
+struct Slot {
+  int page, row;
+  __device__ __forceinline__ Slot(int slot, int shift, int pages)
+      : page(slot >> shift), row(slot - (page << shift)) {
+    if (page >= pages) page = -1;
+  }
+};
+
+struct RowsArgs {
+  const half_t* from[2];  // dense rows: k and v, their strides
+  half_t* into[2];
+  RowStrides strides[2];
+  uint8_t* codes[2];  // the pools, and their scales (16-bit rows: none)
+  uint8_t* scales[2];
+  const int* slots;
+  long long page_stride, head_stride, row_stride;  // of the pools, in bytes
+  long long scale_page, scale_head, scale_row;
+  int pages, page_shift;
+  int N, row_chunks, chunks;  // 16-byte chunks of a dense row, and of a token's heads
+  long long items;            // tokens * chunks
+};
+
+template <bool BF, class Index>
+__global__ __launch_bounds__(kAppThreads) void append4_kernel(const RowsArgs a) {
+  const int v = blockIdx.x & 1;
+  const half_t* const from = v ? a.from[1] : a.from[0];
+  const RowStrides s = v ? a.strides[1] : a.strides[0];
+  uint8_t* const codes = v ? a.codes[1] : a.codes[0];
+  uint8_t* const scales = v ? a.scales[1] : a.scales[0];
+  const Index step = (Index)(gridDim.x / 2) * kAppThreads, items = (Index)a.items;
+  for (Index i = (Index)(blockIdx.x / 2) * kAppThreads + threadIdx.x; i < items; i += step) {
+    const int t = (int)(i / (Index)a.chunks), x = (int)(i - (Index)t * a.chunks);
+    const Slot at(a.slots[t], a.page_shift, a.pages);
+    if (at.page < 0) continue;  // (all four lanes of a block: one row)
+    const int h = x / a.row_chunks, c = x - h * a.row_chunks;
+    const int b = a.N == 1 ? t : t / a.N, n = t - b * a.N;
+    const u32x4 in = *reinterpret_cast<const u32x4*>(from + b * s.b + n * s.n + h * s.h + 8 * c);
+    // (magnitudes of 16 bits are in the order of their bits)
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, in[e] & 0x7fff7fffu));
+    int top = max((int)m[0], (int)m[1]);
+    top = max(top, __builtin_amdgcn_update_dpp(0, top, 0xb1, 0xf, 0xf, false));  // lane ^ 1
+    top = max(top, __builtin_amdgcn_update_dpp(0, top, 0x4e, 0xf, 0xf, false));  // lane ^ 2
+    const half_t top16 = __builtin_bit_cast(half_t, (unsigned short)top);
+    const uint32_t bits = __float_as_uint(from16<BF>(top16));
+    // (one more above 1.75 of its power of two)
+    uint32_t e = (uint32_t)min(max((int)((bits + 0x1fffffu) >> 23) - 2, 1), (int)kTopScale<BF>);
+    uint32_t out = to_codes<BF>(in, __uint_as_float(e << 23));
+    if (bits >= 0x7f800000u) {  // an infinity or a NaN: the block is NaN
+      e = 255;
+      out = 0;
+    }
+    *reinterpret_cast<uint32_t*>(codes + at.page * a.page_stride + h * a.head_stride +
+                                 at.row * a.row_stride + 4 * c) = out;
+    if ((c & 3) == 0)
+      scales[at.page * a.scale_page + h * a.scale_head + at.row * a.scale_row + (c >> 2)] = (uint8_t)e;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows back from their slots, dense: 16-bit ones as they are, 4-bit ones as the values
+// that they stand for, exact in bf16 and rounded to nearest even in fp16. Rows without a
+// slot are zeros. FOUR: the cache is in 4 bits.
+template <bool BF, bool FOUR, class Index>
+__global__ __launch_bounds__(kAppThreads) void gather_kernel(const RowsArgs a) {
+  const int v = blockIdx.x & 1;
+  half_t* const into = v ? a.into[1] : a.into[0];
+  const RowStrides s = v ? a.strides[1] : a.strides[0];
+  const uint8_t* const codes = v ? a.codes[1] : a.codes[0];
+  const uint8_t* const scales = v ? a.scales[1] : a.scales[0];
+  const Index step = (Index)(gridDim.x / 2) * kAppThreads, items = (Index)a.items;
+  for (Index i = (Index)(blockIdx.x / 2) * kAppThreads + threadIdx.x; i < items; i += step) {
+    const int t = (int)(i / (Index)a.chunks), x = (int)(i - (Index)t * a.chunks);
+    const Slot at(a.slots[t], a.page_shift, a.pages);
+    const int h = x / a.row_chunks, c = x - h * a.row_chunks;
+    const int b = a.N == 1 ? t : t / a.N, n = t - b * a.N;
+    u32x4 out = {0u, 0u, 0u, 0u};
+    if (at.page >= 0) {
+      const uint8_t* const row = codes + at.page * a.page_stride + h * a.head_stride + at.row * a.row_stride;
+      if constexpr (FOUR) {
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(row + 4 * c);
+        const float scale = __uint_as_float(
+            (uint32_t)scales[at.page * a.scale_page + h * a.scale_head + at.row * a.scale_row + (c >> 2)] << 23);
+        auto two = [&](auto sel) {
+          if constexpr (BF)
+            return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, decltype(sel)::value));
+          const auto f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, scale, decltype(sel)::value);
+          typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+          return __builtin_bit_cast(uint32_t, v2{(_Float16)f[0], (_Float16)f[1]});
+        };
+        out = u32x4{two(std::integral_constant<int, 0>{}), two(std::integral_constant<int, 1>{}),
+                    two(std::integral_constant<int, 2>{}), two(std::integral_constant<int, 3>{})};
+      } else {
+        out = *reinterpret_cast<const u32x4*>(row + 16 * c);
+      }
+    }
+    *reinterpret_cast<u32x4*>(into + b * s.b + n * s.n + h * s.h + 8 * c) = out;
+  }
+}
+
+RowsArgs rows_args(RowStrides sk, RowStrides sv, const int* slots, const PagedPool& pool,
+                   const PagedScales* scales, int B, int N, int Hkv, int D) {
+  RowsArgs a{};
+  a.strides[0] = sk;
+  a.strides[1] = sv;
+  a.codes[0] = (uint8_t*)pool.k;
+  a.codes[1] = (uint8_t*)pool.v;
+  const int unit = scales ? 1 : 2;  // (16-bit pools' strides count elements)
+  a.page_stride = unit * pool.page_stride;
+  a.head_stride = unit * pool.head_stride;
+  a.row_stride = unit * pool.row_stride;
+  if (scales) {
+    a.scales[0] = scales->k;
+    a.scales[1] = scales->v;
+    a.scale_page = scales->page_stride;
+    a.scale_head = scales->head_stride;
+    a.scale_row = scales->row_stride;
+  }
+  a.slots = slots;
+  a.pages = pool.pages;
+  a.page_shift = pool.page_shift;
+  a.N = N;
+  a.row_chunks = D / 8;
+  a.chunks = Hkv * a.row_chunks;
+  a.items = (long long)B * N * a.chunks;
+  return a;
+}
+
+unsigned rows_blocks(const RowsArgs& a) {
+  return 2 * (unsigned)std::min((a.items + kAppThreads - 1) / kAppThreads, 1LL << 20);
+}
+
 }  // namespace
+
+hipError_t launch_paged4_append(const void* k, const void* v, RowStrides sk, RowStrides sv,
+                                const int* slots, const PagedPool& pool, const PagedScales& scales,
+                                int B, int N, int Hkv, int D, int dtype, void* stream) {
+  RowsArgs a = rows_args(sk, sv, slots, pool, &scales, B, N, Hkv, D);
+  a.from[0] = (const half_t*)k;
+  a.from[1] = (const half_t*)v;
+  const bool wide = a.items > 1LL << 31;
+  const auto kernel = dtype == kBF16 ? (wide ? append4_kernel<true, uint64_t> : append4_kernel<true, uint32_t>)
+                                     : (wide ? append4_kernel<false, uint64_t> : append4_kernel<false, uint32_t>);
+  hipLaunchKernelGGL(kernel, dim3(rows_blocks(a)), dim3(kAppThreads), 0, (hipStream_t)stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_gather(void* k, void* v, RowStrides strides, const int* slots,
+                               const PagedPool& pool, const PagedScales* scales, int B, int N,
+                               int Hkv, int D, int dtype, void* stream) {
+  RowsArgs a = rows_args(strides, strides, slots, pool, scales, B, N, Hkv, D);
+  a.into[0] = (half_t*)k;
+  a.into[1] = (half_t*)v;
+  const bool wide = a.items > 1LL << 31;
+  const auto kernel =
+      !scales           ? (wide ? gather_kernel<true, false, uint64_t> : gather_kernel<true, false, uint32_t>)
+      : dtype == kBF16 ? (wide ? gather_kernel<true, true, uint64_t> : gather_kernel<true, true, uint32_t>)
+                        : (wide ? gather_kernel<false, true, uint64_t> : gather_kernel<false, true, uint32_t>);
+  hipLaunchKernelGGL(kernel, dim3(rows_blocks(a)), dim3(kAppThreads), 0, (hipStream_t)stream, a);
+  return hipGetLastError();
+}
 
 hipError_t launch_paged_tables(const TablesArgs& a, void* stream) {
   // Four slots per thread from 32768 on (6.2 us for 350000 packed ones, 7.9 one at a

@@ -530,7 +530,7 @@ def paged_tables(block_table, old_len, new_len, free_pages, ring, page_size, max
                                    max_new, tokens))
 
 
-def paged_append(k, v, k_cache, v_cache, slots):
+def paged_append(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None):
     """Writes new tokens' keys and values into a paged cache, in place.
 
     k and v (fp16 or bf16) are (T, Hkv, D) with slots (T,), or (B, Hkv, N, D) with
@@ -542,13 +542,45 @@ def paged_append(k, v, k_cache, v_cache, slots):
     (pages, 2, Hkv, page_size, D) pool), no two rows overlapping; k and v must not lie
     in rows that are written. One HIP kernel; no gradient: tensors that
     require grad are refused outside torch.no_grad(), and duals of forward mode.
+
+    With k_scale and v_scale the cache is of 4 bits, about a quarter of the size: k_cache
+    and v_cache are then uint8 (pages, Hkv, page_size, D / 2), D a multiple of 32, and
+    k_scale and v_scale uint8 (pages, Hkv, page_size, D / 32), laid out alike. Value d of a
+    row is in the low (d even) or high half of byte d // 2: a sign and one of 0, 0.5, 1,
+    1.5, 2, 3, 4, 6, times 2^(s - 127) for the scale byte s of its 32 values (255: NaN).
+    The scale of 32 values is the least power of two of which their largest magnitude is 7
+    times or less (from 2^-126 to 2^13 for fp16 rows and 2^125 for bf16); values are
+    rounded to the nearest, ties to the even code, magnitudes above 6 times the scale to
+    that. 32 values with an infinity or NaN among them all become NaN.
     """
-    _paged_inputs("paged_append", k, v, k_cache, v_cache, slots)
-    _ext.paged_append(k, v, k_cache, v_cache, slots)
+    _paged_inputs("paged_append", k, v, k_cache, v_cache, slots, *_scales(k_scale, v_scale))
+    _ext.paged_append(k, v, k_cache, v_cache, slots, k_scale, v_scale)
+
+
+def _scales(*scales):
+    return [s for s in scales if s is not None]
+
+
+def paged_gather(k_cache, v_cache, slots, k_scale=None, v_scale=None, dtype=None):
+    """(k, v) of the rows that a paged cache holds at `slots`, dense: (T, Hkv, D) for slots
+    (T,), (B, Hkv, N, D) for slots (B, N) (int32; negative ones and ones past the pool
+    give zeros, and a slot may occur several times).
+
+    The caches are as paged_append takes them. Rows of 16 bits come back as they are, rows
+    of 4 bits as the values that they stand for, in `dtype` (bf16, which holds them
+    exactly, when None; fp16 rounds to nearest even and overflows where they pass its
+    range). For a cached prefix that many new tokens attend to with flash_attn, or requests
+    that leave the GPU. Token j of request b has the slot
+    block_table[b, j // page_size] * page_size + j % page_size. One HIP kernel; no
+    gradient, as paged_append.
+    """
+    _paged_inputs("paged_gather", k_cache, v_cache, slots, *_scales(k_scale, v_scale))
+    return tuple(_ext.paged_gather(k_cache, v_cache, slots, k_scale, v_scale, dtype))
 
 
 def paged_attn(q, k_cache, v_cache, block_table, kv_len, causal=True, sliding_window=None,
-               alibi_slopes=None, softmax_scale=None, return_lse=False):
+               alibi_slopes=None, softmax_scale=None, return_lse=False, k_scale=None,
+               v_scale=None):
     """Attention of each request's newest tokens over its paged cache: o (B, Hq, N, D),
     or (o, lse) with lse (B, Hq, N) fp32 when return_lse is set.
 
@@ -577,10 +609,26 @@ def paged_attn(q, k_cache, v_cache, block_table, kv_len, causal=True, sliding_wi
     last bits of one request may depend on the lengths of the others. No gradient:
     tensors that require grad (the slopes too) are refused outside torch.no_grad(), and
     duals of forward mode.
+
+    With k_scale and v_scale the cache is of 4 bits, as paged_append writes it, and read as
+    such, for q in fp16 or bf16 whatever the rows were. The products are bf16's, which
+    holds the cache's values exactly; fp16 q enters as two bf16 numbers. With more than 32
+    rows per kv head the probabilities are rounded to bf16 once where q is bf16 and D at
+    most 128, else they are two bf16 numbers.
     """
-    _paged_inputs("paged_attn", q, k_cache, v_cache, block_table, kv_len)
+    _paged_inputs("paged_attn", q, k_cache, v_cache, block_table, kv_len,
+                  *_scales(k_scale, v_scale))
+    window, scale = _paged_options("paged_attn", q, causal, sliding_window, alibi_slopes,
+                                   softmax_scale)
+    out = _ext.paged_attn(q, k_cache, v_cache, block_table, kv_len, bool(causal), window,
+                          alibi_slopes, scale, return_lse, k_scale, v_scale)
+    return tuple(out) if return_lse else out[0]
+
+
+def _paged_options(name, q, causal, sliding_window, alibi_slopes, softmax_scale):
+    """(window, scale) of a call over a paged cache, 0 where not given."""
     if alibi_slopes is not None:
-        _paged_inputs("paged_attn", alibi_slopes)
+        _paged_inputs(name, alibi_slopes)
     window = 0
     if sliding_window is not None:
         window = int(sliding_window)
@@ -595,9 +643,58 @@ def paged_attn(q, k_cache, v_cache, block_table, kv_len, causal=True, sliding_wi
         scale = float(softmax_scale)
         if not (scale > 0.0 and math.isfinite(scale)):
             raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
-    out = _ext.paged_attn(q, k_cache, v_cache, block_table, kv_len, bool(causal), window,
-                          alibi_slopes, scale, return_lse)
-    return tuple(out) if return_lse else out[0]
+    return window, scale
+
+
+def paged_weights(q, k_cache, block_table, kv_len, lse, weights, causal=True, sliding_window=None,
+                  alibi_slopes=None, softmax_scale=None, restart=False, k_scale=None):
+    """Adds to `weights`, in place, the attention weight that each cached key gets from the
+    newest tokens of its request: what paged_evict goes by.
+
+    q, k_cache (of 4 bits with k_scale), block_table, kv_len and the options are those of
+    a paged_attn call, and lse (B, Hq, N) what it returned with return_lse. weights, float32
+    (pages, Hkv, page_size) in any order of storage, holds one number per kv head and slot:
+    the sum of exp(score - lse) over the rows of q that see the key and the query heads
+    of its kv head is added to it. The keys of the newest N tokens themselves, which no
+    earlier row saw, get that sum instead of what their slots held before; with restart
+    all of a request's keys do (a prompt judged by its last rows), those that no row sees
+    0. Rows with lse = +inf add nothing; other slots keep their values.
+
+    One HIP kernel that reads K once, after or instead of any number of calls: weights may
+    be scaled or cleared in between. Scores, weights and sums are fp32, results
+    deterministic. No gradient, as paged_append.
+    """
+    _paged_inputs("paged_weights", q, k_cache, block_table, kv_len, lse, weights, *_scales(k_scale))
+    window, scale = _paged_options("paged_weights", q, causal, sliding_window, alibi_slopes,
+                                   softmax_scale)
+    _ext.paged_weights(q, k_cache, block_table, kv_len, lse, weights, bool(causal), window,
+                       alibi_slopes, scale, bool(restart), k_scale)
+
+
+def paged_evict(k_cache, v_cache, weights, block_table, kv_len, max_len, recent=0, k_scale=None,
+                v_scale=None):
+    """Cuts requests over a paged cache to at most max_len tokens, in place; returns their
+    new lengths, int32 (B,).
+
+    Where kv_len[b] exceeds max_len[b] (int32 (B,), or one int for all), each kv head
+    keeps its newest min(recent, max_len[b]) tokens and, of the others, those of the
+    largest weights (paged_weights; of equal ones the older, NaN above all). They move to the front of the
+    request's pages, in their order, with their weights and, in a cache of 4 bits, scales;
+    the rows behind them keep what they held. The pages they no longer need go back with
+    paged_tables(block_table, kv_len, new_len, free_pages, ring, page_size, max_new=0).
+
+    Kept tokens then differ between kv heads, and a key's index no longer is its position:
+    keys are cached with their positions already applied, and sliding windows and ALiBi
+    count kept tokens. HIP kernels without a copy to the host; a page is one request's. No
+    gradient, as paged_append.
+    """
+    _paged_inputs("paged_evict", k_cache, v_cache, weights, block_table, kv_len,
+                  *_scales(k_scale, v_scale))
+    if not isinstance(max_len, torch.Tensor):
+        max_len = torch.full_like(kv_len, int(max_len))
+    _paged_inputs("paged_evict", max_len)
+    return _ext.paged_evict(k_cache, v_cache, weights, block_table, kv_len, max_len, int(recent),
+                            k_scale, v_scale)
 
 
 def _expand_kv(k, n_head):

@@ -543,6 +543,102 @@ int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cach
                   int causal, const fa_options* opts, void* stream);
 
 /*
+ * Paged caches in 4 bits. A row of D values, D a multiple of 32, is D / 2 bytes of codes
+ * (value d in the low half of byte d / 2 for even d, in the high half for odd d) and
+ * D / 32 bytes of scales: a code is a sign (bit 3) and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * (bits 2 .. 0), a scale byte x stands for 2^(x - 127), 255 for NaN, and is that of 32
+ * values in a row (the E2M1 and E8M0 of the OCP microscaling formats). The codes lie in
+ * the pools of a struct fa_paged_cache, whose strides then count bytes and are multiples
+ * of 16; the scales in two pools of their own, byte strides, the same for both, below
+ * 2^31.
+ */
+typedef struct fa_paged_scales {
+  uint8_t* k;
+  uint8_t* v;
+  long long stride_page;
+  long long stride_head;
+  long long stride_row;
+} fa_paged_scales;
+
+/*
+ * fa_paged_append into a cache in 4 bits; dtype is the rows' format (FA_DTYPE_FP16 or
+ * FA_DTYPE_BF16). With m the largest magnitude of 32 values, their scale is the least
+ * power of two X with m <= 7 X, from 2^-126 on and up to 2^13 (fp16 rows) or 2^125 (bf16),
+ * so what is read back is finite in that format; values are rounded to the nearest code
+ * times X, ties to the even code, magnitudes above 6 X to 6 X. 32 values with an infinity
+ * or a NaN among them all become NaN (scale 255, codes 0).
+ */
+int fa_paged4_append(const void* k, const void* v, long long k_stride_b, long long k_stride_n,
+                     long long k_stride_h, long long v_stride_b, long long v_stride_n,
+                     long long v_stride_h, const int* slots, const fa_paged_cache* cache,
+                     const fa_paged_scales* scales, int B, int N, int Hkv, int D, int dtype,
+                     void* stream);
+
+/*
+ * Rows of a paged cache back from their slots: what slot slots[b * N + n] holds to element
+ * (b, n, h, d) of k and v at b * stride_b + n * stride_n + h * stride_h + d (strides in
+ * elements, multiples of 8; k and v 16-byte aligned and of format dtype). Slots that are
+ * negative or past the pool give zeros; a slot may occur several times. scales NULL: the
+ * cache is of 16 bits, in that format; else of 4, whose values are exact in bf16 but where
+ * they pass its range, and rounded to nearest even in fp16.
+ */
+int fa_paged_gather(void* k, void* v, long long stride_b, long long stride_n, long long stride_h,
+                    const int* slots, const fa_paged_cache* cache, const fa_paged_scales* scales,
+                    int B, int N, int Hkv, int D, int dtype, void* stream);
+
+/*
+ * fa_paged_attn over a cache in 4 bits: the same arguments, options and rows without a
+ * key. The products are bf16's, in which the cache's values are exact; q in fp16 enters
+ * as two bf16 numbers, exactly where it is finite, so scores are sums of exact products in
+ * fp32. The probabilities are two bf16 numbers (off by 2^-16 of themselves) with up to 32
+ * rows per kv head, and for fp16 or head dims above 128 with any; else one. The workspace
+ * is at most 137 MB.
+ */
+size_t fa_paged4_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
+int fa_paged4_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,
+                   const fa_paged_scales* scales, void* workspace, size_t workspace_bytes, int B,
+                   int Hq, int Hkv, int N, int D, int causal, const fa_options* opts, void* stream);
+
+/*
+ * The attention weight that each cached key gets from the newest N tokens of its request:
+ * the sum of exp(score - lse) over those of their rows that see it and the query heads of
+ * its kv head. q, cache (of it, k alone), N and the options are fa_paged_attn's, lse (B,
+ * Hq, N) what that call wrote for them (rows with lse = +inf add nothing). scales NULL: the
+ * cache is of 16 bits, in q's format; else of 4 (of scales, k alone). weights is fp32, that
+ * of (page, kv head, row) at page * w_stride_page + head * w_stride_head + row *
+ * w_stride_row (strides in elements, not negative); no two of them share a place. The keys
+ * of the newest N tokens, which no earlier row saw, get the sum, those before it have it
+ * added to what they hold; with `restart` all of the request's keys get it, those that no
+ * row sees 0. Other weights keep their values. Each is a sum in fp32 in an order of its
+ * own: results are deterministic.
+ */
+int fa_paged_weights(const void* q, const float* lse, const fa_paged_cache* cache,
+                     const fa_paged_scales* scales, float* weights, long long w_stride_page,
+                     long long w_stride_head, long long w_stride_row, int restart, int B, int Hq,
+                     int Hkv, int N, int D, int causal, const fa_options* opts, void* stream);
+
+/*
+ * Cuts the requests that have more than max_len[b] tokens (negative: 0) to that many: each
+ * kv head keeps its newest min(recent, max_len[b]) tokens and, of the others, those of the
+ * largest weights (of equal ones the older; NaN above all, keys in pages outside the pool
+ * below all). What is kept moves to the front of the request's pages in its order, rows,
+ * scales and weights alike (places in pages outside the pool are left out); rows behind it
+ * keep what they hold. new_len[b] becomes min(kv_len[b], max_len[b]); a call of
+ * fa_paged_tables with these as new lengths gives the pages back. Tokens of different kv
+ * heads in a row of the pool then differ, and a key's row no longer says its position: what
+ * counts distances (windows, ALiBi) counts kept tokens. scales NULL: rows of 16 bits, else
+ * of 4. The pools' rows, the scales and the weights must lie apart; a page is one
+ * request's. `workspace` has fa_paged_evict_workspace_bytes() bytes, 4-byte aligned (a
+ * token list per request and kv head, for all that a table holds), may hold anything, and
+ * serves one call at a time. B * Hkv <= 2^21.
+ */
+size_t fa_paged_evict_workspace_bytes(int B, int Hkv, int table_width, int page_size);
+int fa_paged_evict(const fa_paged_cache* cache, const fa_paged_scales* scales, float* weights,
+                   long long w_stride_page, long long w_stride_head, long long w_stride_row,
+                   const int* max_len, int recent, int* new_len, void* workspace,
+                   size_t workspace_bytes, int B, int Hkv, int D, void* stream);
+
+/*
  * fa_bwd without a workspace argument and without any allocation. No
  * counterpart in the reference: it is for callers that cannot allocate device
  * memory at the call (code under HIP graph capture, tight serving loops,
