@@ -5,7 +5,7 @@
 //
 // As in fa_paged.hip the key blocks of all requests lie on one line that the waves
 // divide evenly, and the parts of an item meet in LDS and in paged_merge_kernel. A
-// wave's step is a block of 64 keys for RT tiles of 16 query rows, on
+// wave's step is a block of 32 or 64 keys for RT tiles of 16 query rows, on
 // v_mfma_f32_16x16x32_bf16: S^T = K Q^T, then O^T += V^T P^T. Every value of the cache is
 // exact in bf16 (a sign, two bits and an exponent), whatever q's format, and
 // v_cvt_scalef32_pk_bf16_fp4 makes two of them from a byte, scale included:
@@ -14,8 +14,7 @@
 //   * V: the second product runs over keys, so the values are written to LDS as bf16 and
 //     come back transposed (ds_read_b64_tr_b16).
 // q in fp16 has 11 bits: two bf16 numbers, exactly, and two products. The probabilities
-// are two bf16 numbers up to 32 rows (off by 2^-16), with more rows one, as in
-// fa_paged.hip.
+// are two bf16 numbers (off by 2^-16), two products too.
 #include "fa_paged.h"
 
 namespace fa {
@@ -25,20 +24,20 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 template <int DIM, bool OUT_BF, int RT>
 struct Paged4 {
-  static constexpr int kD = DIM, kTiles = 1, kRowTiles = RT, kRows = 16 * RT, kKeys = 64;
+  static constexpr int kD = DIM, kTiles = 1, kRowTiles = RT, kRows = 16 * RT;
+  static constexpr int kKeys = 64;
   static constexpr bool kBF = OUT_BF;
-  static constexpr int kWaves = DIM > 128 ? 4 : 8, kLine = kWaves, kThreads = 64 * kWaves;
+  static constexpr int kWaves = 8 / (DIM > 128 ? 2 : 1), kLine = kWaves;
+  static constexpr int kThreads = 64 * kWaves;
   static constexpr int kGrid = kCUs;
   static constexpr float kPUnit = 1.f, kPRescale = kRescaleLog2;
   static constexpr int kBlocks = DIM / 32;  // of a row, each with its scale
   static constexpr int kQ = OUT_BF ? 1 : 2;  // bf16 operands of q
-  static constexpr bool kTwoP = RT <= 2;
-  // LDS rows of V: eight 16-byte chunks in a row of keys, two of each, lie in 16 bank
+    // LDS rows of V: eight 16-byte chunks in a row of keys, two of each, lie in 16 bank
   // groups (the row's chunks are 2 more than a multiple of 4).
   static constexpr int kStride = 2 * DIM + 32;
   static constexpr int kTileBytes = kKeys * kStride;
-  static constexpr int kFloats = 16 * DIM;  // a row tile's partial O
-  static_assert(kFloats * 4 <= kTileBytes, "a part exceeds the wave's tile");
+  static_assert(kRows * DIM * 4 <= kTileBytes, "a part exceeds the wave's tile");
   __device__ __forceinline__ static bool joins(int stretch, int total, int items) {
     constexpr int kFrom = kLine < 4 ? kLine : 4;
     return stretch >= kFrom || (stretch >= 2 && total / 64 >= items);
@@ -49,6 +48,7 @@ struct Paged4Args : PagedKernelArgs {
   const uint8_t* k_scale;
   const uint8_t* v_scale;
   long long scale_page, scale_head, scale_row;
+  uint32_t code_bytes, scale_bytes;  // of a kv head's rows, first to last (PAGES > 0)
 };
 
 __device__ __forceinline__ floatx4 mfma_bf16(half8 a, half8 b, floatx4 c) {
@@ -65,7 +65,11 @@ __device__ __forceinline__ half8 values(uint32_t codes, float scale) {
       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
   return as_half8(u32x4{r[0], r[1], r[2], r[3]});
 }
-__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+// The scale that lies `at` bits up in a word: its bits moved to an exponent's place. (The
+// conversion takes the exponent of its scale alone, whatever the sign and mantissa are.)
+__device__ __forceinline__ float scale_of(uint32_t word, uint32_t at) {
+  return __uint_as_float(__builtin_amdgcn_alignbit(word, word, (at + 9u) & 31u));
+}
 
 // The maximum over lanes l, l ^ 16, l ^ 32 and l ^ 48, which hold the same query row.
 __device__ __forceinline__ float max_quarters(float v) {
@@ -73,13 +77,17 @@ __device__ __forceinline__ float max_quarters(float v) {
   return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
 
-// FULL: the head dim is the width (else 160, 192 or 224 of 256).
-template <class T, bool FULL>
+// FULL: the head dim is the width (else 160, 192 or 224 of 256). PAGES: those of a tile of
+// 16 keys. With 1 (pages of 16 rows or more) or 2 (of 8) a page's place is found once, in
+// scalar registers, and a lane adds an offset of its own that never changes; 0: a key at a
+// time. STREAM: one row tile reads the keys.
+template <class T, bool FULL, int PAGES, bool STREAM>
 __global__ __launch_bounds__(T::kThreads) void paged4_kernel(const Paged4Args a) {
   constexpr int D = T::kD, RT = T::kRowTiles, kWaves = T::kWaves, kLine = T::kLine;
-  constexpr int kBlocks = T::kBlocks, kDwords = D / 32;  // of a row, and of a lane's quarter of it
+  constexpr int kDwords = D / 32;  // of codes in a lane's quarter of a row
+  constexpr int kKeys = T::kKeys, kKeyTiles = kKeys / 16, kScores = 4 * kKeyTiles;
   __shared__ __align__(1024) char vt[kWaves * T::kTileBytes];
-  __shared__ float2 ml[kWaves * 64];
+  __shared__ float2 ml[RT * kWaves * 64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
   __builtin_assume(wave >= 0 && wave < kWaves);
@@ -125,224 +133,360 @@ __global__ __launch_bounds__(T::kThreads) void paged4_kernel(const Paged4Args a)
     const int j1 = some ? keys.first + max(upto - line.lead, 0) : j0;
     const int* table = a.table + b * a.table_stride;
     const int last_page = max(keys.len - 1, 0) >> a.page_shift;
-    int p0 = 0, held = 0;           // pages p0 .. p0 + 63 are in the lanes' `held`
-    unsigned long long hidden = 0;  // of those, the ones outside the pool
-    const uint8_t* base_k = (const uint8_t*)a.k + hkv * a.head_stride;
-    const uint8_t* base_v = (const uint8_t*)a.v + hkv * a.head_stride;
+    int p0 = 0, held = 0, next = 0;  // pages p0 .. p0 + 63 are in the lanes' `held`, then 64 more
+    unsigned long long hidden = 0;   // of those held, the ones outside the pool
+    const uint8_t* const base_k = (const uint8_t*)a.k + hkv * a.head_stride;
+    const uint8_t* const base_v = (const uint8_t*)a.v + hkv * a.head_stride;
+    // (the scales of a kv head begin anywhere in a word: with PAGES from the word on)
     const uint8_t* base_ks = a.k_scale + hkv * a.scale_head;
     const uint8_t* base_vs = a.v_scale + hkv * a.scale_head;
-    auto fetch = [&](int j) {  // pages for block j
-      p0 = max(j * 64, keys.lo) >> a.page_shift;
-      const int page = table[min(p0 + lane, last_page)];
+    const uint32_t sub_k = PAGES ? (uint32_t)((uintptr_t)base_ks & 3) : 0u;
+    const uint32_t sub_v = PAGES ? (uint32_t)((uintptr_t)base_vs & 3) : 0u;
+    base_ks -= sub_k;
+    base_vs -= sub_v;
+    const rsrc_t codes_k = make_rsrc(base_k, a.code_bytes), codes_v = make_rsrc(base_v, a.code_bytes);
+    const rsrc_t scales_k = make_rsrc(base_ks, a.scale_bytes), scales_v = make_rsrc(base_vs, a.scale_bytes);
+    auto hold = [&](int page) {
       const bool ok = page >= 0 && page < a.pages;
       hidden = __ballot(!ok);
       held = ok ? page : 0;
+      next = table[min(p0 + 64 + lane, last_page)];
+    };
+    auto fetch = [&](int j) {  // pages for block j
+      p0 = max(j * kKeys, keys.lo) >> a.page_shift;
+      hold(table[min(p0 + lane, last_page)]);
     };
     auto place = [&](int j) {
-      if ((min(j * 64 + 64, keys.len) - 1) >> a.page_shift > p0 + 63) fetch(j);
+      if ((min(j * kKeys + kKeys, keys.len) - 1) >> a.page_shift <= p0 + 63) return;
+      if (PAGES > 0 && (j * kKeys) >> a.page_shift == p0 + 64) {  // (in order: they have been asked for)
+        p0 += 64;
+        hold(next);
+      } else {
+        fetch(j);
+      }
     };
-    // Where key `x` of a block lies (rows outside the request's keys: one of its own).
-    auto page_of = [&](int x, int& row) {
-      const int key = min(max(x, keys.lo), keys.len - 1);
-      row = key & page_mask;
-      return (uint32_t)__shfl(held, (key >> a.page_shift) - p0);
+    // A block in registers: a quarter of a row in each of its tiles of 16 keys, K's of key
+    // lane % 16 (as the product takes it), V's of key lane / 4 (as it lies in memory). Scales
+    // come as the words that hold them: a byte would be widened, and waited for, at once.
+    constexpr int kScales = D == 96 || (D == 256 && !FULL) ? 2 : 1;
+    constexpr int kBits = PAGES == 0 ? kScales : 0;  // (rows anywhere: their scales' bits too)
+    struct Codes {
+      uint32_t c[kDwords], s[kScales], bit[kBits + 1];
     };
-    // A block in registers: K's codes (key 16 t + lane % 16, a quarter of its row), V's
-    // (unit u = lane + 64 i: block u % kBlocks of key u / kBlocks), and their scales.
-    constexpr int kScales = D == 96 ? 3 : D == 256 ? 2 : 1;
-    uint32_t kc[4][kDwords], ks[4][kScales], vs[kBlocks];
-    u32x4 vc[kBlocks];
-    auto load_k = [&](int j, bool live) {
+    // Where a lane's quarter `part` of key `key` of a tile lies, and its scales: the words
+    // that hold them and the bits that they begin at.
+    struct Place {
+      uint32_t code, scale[kScales], bit[kScales];
+      int second;        // the page of a tile that the key is in
+      bool there, both;  // whether the quarter begins, and ends, within the head dim
+      __device__ __forceinline__ Place(int key, int part, uint32_t row_bytes, uint32_t scale_row, int dr,
+                                       uint32_t sub) : second(0) {
+        if (PAGES == 2) {
+          second = key >> 3;
+          key &= 7;
+        }
+        if (PAGES == 0) key = 0;  // (rows are found one by one)
+        there = FULL || 64 * part < dr;
+        both = FULL || 64 * part + 32 < dr;
+        code = (uint32_t)key * row_bytes + 4u * kDwords * (there ? part : 0);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        int row;
-        const uint32_t page = page_of(j * 64 + 16 * t + l16, row);
-        const unsigned long long at = live ? (unsigned long long)page * page_bytes +
-                                                 (unsigned long long)(uint32_t)row * row_bytes : 0;
-        const unsigned long long sat = live ? (unsigned long long)page * scale_page +
-                                                  (unsigned long long)(uint32_t)row * scale_row : 0;
-        if constexpr (D == 256) {
+        for (int i = 0; i < kScales; ++i) {
+          const int block = !there ? 0 : D == 256 ? 2 * part + (both ? i : 0) : (kDwords * part + 2 * i) / 4;
+          const uint32_t at = (uint32_t)key * scale_row + (uint32_t)block + sub;
+          scale[i] = PAGES == 0 ? at : at & ~3u;
+          bit[i] = 8 * (at & 3u);
+        }
+      }
+      // The scales of a quarter's eighths, of 8 values each. (Values past the head dim meet
+      // zeros of q: a finite scale.)
+      __device__ __forceinline__ void sizes(const Codes& x, int part, float (&size)[kDwords]) const {
+        float two[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int blk = FULL || 64 * g + 32 * h < dr ? 2 * g + h : 0;
-            const u32x4 x = *reinterpret_cast<const u32x4*>(base_k + at + 16 * blk);
-            for (int i = 0; i < 4; ++i) kc[t][(4 * h + i) % kDwords] = x[i];
-            ks[t][h % kScales] = FULL || 64 * g + 32 * h < dr ? base_ks[sat + blk] : 127u;
-          }
-        } else {
-          __builtin_memcpy(kc[t], __builtin_assume_aligned(base_k + at + 4 * kDwords * g, kDwords == 3 ? 4 : 4 * kDwords),
-                           4 * kDwords);
+        for (int i = 0; i < kScales; ++i) two[i] = scale_of(x.s[i], PAGES == 0 ? x.bit[i % (kBits + 1)] : bit[i]);
+        if constexpr (kScales == 1) two[1] = D == 256 ? scale_of(x.s[0], (PAGES == 0 ? x.bit[0] : bit[0]) + 8) : two[0];
+        if constexpr (!FULL) {
+          two[0] = there ? two[0] : 1.f;
+          two[1] = both ? two[1] : 1.f;
+        }
 #pragma unroll
-          for (int i = 0; i < kScales; ++i) ks[t][i] = base_ks[sat + (kDwords * g + i) / 4];
+        for (int i = 0; i < kDwords; ++i) {
+          if constexpr (D == 96) size[i] = i == 0 || (i == 1 && part != 1) ? two[0] : two[1];
+          else size[i] = two[D == 256 ? i / 4 : 0];
         }
       }
     };
-    auto load_v = [&](int j, bool live) {
+    const Place place_k(l16, g, row_bytes, scale_row, dr, sub_k);
+    const Place place_v(lane >> 2, lane & 3, row_bytes, scale_row, dr, sub_v);
+    // Where a quarter comes from: with PAGES a buffer of the kv head's rows, the tile's place
+    // in it (uniform) and the lane's in the tile; else the row's own addresses.
+    auto fill = [&](Codes& x, const Place& at, auto&& code16, auto&& scale_word) {
+      if constexpr (D == 256) {
 #pragma unroll
-      for (int i = 0; i < kBlocks; ++i) {
-        const int u = lane + 64 * i, key = u / kBlocks, blk = FULL || 32 * (u % kBlocks) < dr ? u % kBlocks : 0;
-        int row;
-        const uint32_t page = page_of(j * 64 + key, row);
-        const unsigned long long at = live ? (unsigned long long)page * page_bytes +
-                                                 (unsigned long long)(uint32_t)row * row_bytes : 0;
-        const unsigned long long sat = live ? (unsigned long long)page * scale_page +
-                                                  (unsigned long long)(uint32_t)row * scale_row : 0;
-        vc[i] = *reinterpret_cast<const u32x4*>(base_v + at + 16 * blk);
-        vs[i] = base_vs[sat + blk];
+        for (int h = 0; h < 2; ++h) {
+          const u32x4 v = code16(FULL || at.both ? 16 * h : 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x.c[(4 * h + i) % kDwords] = v[i];
+        }
+      } else {
+        const u32x4 v = code16(0);  // (of less where a quarter is less)
+#pragma unroll
+        for (int i = 0; i < kDwords; ++i) x.c[i] = v[i % 4];
+      }
+#pragma unroll
+      for (int i = 0; i < kScales; ++i) x.s[i] = scale_word(i, x);
+    };
+    auto load_tile = [&](Codes& x, rsrc_t codes, rsrc_t scales, const Place& at, uint32_t to, uint32_t sto,
+                         uint32_t lane_to, uint32_t lane_sto) {
+      constexpr int kAux = STREAM ? 2 : 0;  // (the nontemporal hint)
+      fill(x, at,
+           [&](int off) {
+             const uint32_t v = at.code + lane_to;
+             if constexpr (kDwords == 1) return u32x4{__builtin_amdgcn_raw_buffer_load_b32(codes, v, to, kAux), 0, 0, 0};
+             if constexpr (kDwords == 2) {
+               const auto r = __builtin_amdgcn_raw_buffer_load_b64(codes, v, to, kAux);
+               return u32x4{r[0], r[1], 0, 0};
+             }
+             if constexpr (kDwords == 3) {
+               const auto r = __builtin_amdgcn_raw_buffer_load_b96(codes, v, to, kAux);
+               return u32x4{r[0], r[1], r[2], 0};
+             }
+             return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(codes, v + off, to, kAux));
+           },
+           [&](int i, Codes&) { return __builtin_amdgcn_raw_buffer_load_b32(scales, at.scale[i] + lane_sto, sto, 0); });
+    };
+    auto load_row = [&](Codes& x, const uint8_t* row, const uint8_t* scales, const Place& at) {
+      const uint8_t* const from = row + at.code;
+      fill(x, at,
+           [&](int off) {
+             u32x4 v = {0u, 0u, 0u, 0u};
+             if constexpr (kDwords < 4) __builtin_memcpy(&v, __builtin_assume_aligned(from, 4), 4 * kDwords);
+             else v = *reinterpret_cast<const u32x4*>(from + off);
+             return v;
+           },
+           [&](int i, Codes& x) {
+             const uint8_t* word = scales + at.scale[i];
+             x.bit[i % (kBits + 1)] = 8u * (uint32_t)((uintptr_t)word & 3u);
+             return *reinterpret_cast<const uint32_t*>(word - ((uintptr_t)word & 3u));
+           });
+    };
+    // Block j's K or V, or, where it is not live, a row of its memory, not used: a branch
+    // around the loads would leave their number unknown, and every wait full.
+    auto load_tiles = [&](Codes (&k)[kKeyTiles], Codes (&v)[kKeyTiles], int j, bool live) {
+      // (a tile behind the last key: some of its rows' memory, masked)
+      auto place_of = [&](int key, uint32_t& to, uint32_t& sto) {
+        const int i = max((min(key, keys.len - 1) >> a.page_shift) - p0, 0);
+        const uint32_t page = live ? (uint32_t)__builtin_amdgcn_readlane(held, i) : 0u;
+        const uint32_t row = live && PAGES == 1 ? (uint32_t)(key & page_mask) : 0u;
+        to = page * page_bytes + row * row_bytes;
+        sto = page * scale_page + row * scale_row;
+      };
+      uint32_t to[kKeyTiles], sto[kKeyTiles], to2[kKeyTiles], sto2[kKeyTiles];
+#pragma unroll
+      for (int t = 0; t < kKeyTiles; ++t) {
+        place_of(j * kKeys + 16 * t, to[t], sto[t]);
+        if constexpr (PAGES == 2) place_of(j * kKeys + 16 * t + 8, to2[t], sto2[t]);
+        else to2[t] = to[t], sto2[t] = sto[t];
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int t = 0; t < kKeyTiles; ++t) {
+          const Place& at = half ? place_v : place_k;
+          const uint32_t lane_to = at.second ? to2[t] : to[t], lane_sto = at.second ? sto2[t] : sto[t];
+          load_tile(half ? v[t] : k[t], half ? codes_v : codes_k, half ? scales_v : scales_k, at,
+                    PAGES == 1 ? to[t] : 0u, PAGES == 1 ? sto[t] : 0u, PAGES == 1 ? 0u : lane_to,
+                    PAGES == 1 ? 0u : lane_sto);
+        }
+    };
+    auto load_rows = [&](Codes (&x)[kKeyTiles], const uint8_t* base, const uint8_t* scales, int key, const Place& at,
+                         int j, bool live) {
+#pragma unroll
+      for (int t = 0; t < kKeyTiles; ++t) {
+        const int k = min(max(j * kKeys + 16 * t + key, keys.lo), keys.len - 1);
+        const uint32_t page = live ? (uint32_t)__shfl(held, (k >> a.page_shift) - p0) : 0u;
+        const uint32_t row = live ? (uint32_t)(k & page_mask) : 0u;
+        load_row(x[t], base + (unsigned long long)page * page_bytes + (unsigned long long)row * row_bytes,
+                 scales + (unsigned long long)page * scale_page + (unsigned long long)row * scale_row, at);
+      }
+    };
+    Codes kc[kKeyTiles], vc[kKeyTiles];
+    auto load_both = [&](int j, bool live) {
+      if (live) place(j);
+      if constexpr (PAGES > 0) {
+        load_tiles(kc, vc, j, live);
+      } else {
+        load_rows(kc, base_k, base_ks, l16, place_k, j, live);
+        load_rows(vc, base_v, base_vs, lane >> 2, place_v, j, live);
       }
     };
 
-    if (j0 < j1) {
-      fetch(j0);
-      load_k(j0, true);
-      load_v(j0, true);
-    }
-    LateArgs& qa = late_args();
-    half8 q[RT][T::kQ][kDwords];
-    float slope[RT], m_raw[RT], l[RT];
-    int row_n[RT];
+    float m_raw[RT], l[RT];
     floatx4 oacc[RT][D / 16];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const Row<T::kRows> row(qa, hkv, tile, 16 * rt + l16);
-      const half_t* qrow = qa.q + b * qa.stq.b + row.hq * qa.stq.h + (size_t)row.n * qa.stq.n;
-      row_n[rt] = row.n;
-      slope[rt] = qa.alibi ? qa.alibi[row.hq] * qa.alibi_unit : 0.f;
       m_raw[rt] = -INFINITY;
       l[rt] = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) oacc[rt][c] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < kDwords; ++i) {
-        const int d = D / 4 * g + 8 * i;
-        const half8 x = as_half8(load16(qrow + d, FULL || d < dr));
-        if constexpr (T::kBF) {
-          q[rt][0][i] = x;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float f = (float)x[e];
-            q[rt][0][i][e] = to16<true>(f);
-            const float rest = f - from16<true>(q[rt][0][i][e]);
-            q[rt][T::kQ - 1][i][e] = to16<true>(__builtin_isfinite(f) ? rest : 0.f);
-          }
-        }
-      }
     }
-    const int at0 = keys.len - qa.N, window = qa.window;
-    const int all_lo = window > 0 ? max(0, keys.len - window) : 0;
-    const int all_hi = qa.causal ? at0 + 1 : keys.len;
-    const bool causal = qa.causal, biased = qa.alibi != nullptr;
-    const float c = qa.scale_log2, thr_raw = qa.rescale;
-    for (int j = j0; j < j1; ++j) {
-      const unsigned long long hide = hidden;  // (of block j's pages, from page hide0 on)
-      const int hide0 = p0;
-      floatx4 s[RT][4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < kDwords; ++i) {
-          // (a lane's quarter begins in block g kDwords / 4 and may end in another)
-          const half8 k = values(kc[t][i], scale_of(ks[t][D == 256 ? i / 4 % kScales : i % kScales]));
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int x = 0; x < T::kQ; ++x) s[rt][t] = mfma_bf16(k, q[rt][x][i], s[rt][t]);
-        }
-      }
-      const bool more = j + 1 < j1;
-      if (more) place(j + 1);
-      load_k(more ? j + 1 : j, more);
-      const int base = j * 64 + 4 * g;  // key of s[.][t][r]: base + 16 t + r
-      const bool edge = j * 64 < all_lo || j * 64 + 64 > all_hi;
-      half8 pb[RT][2], rest[RT][2];
+    const float c = late_args().scale_log2;
+    if (j0 < j1) {
+      fetch(j0);
+      LateArgs& qa = late_args();
+      half8 q[RT][T::kQ][kDwords];
+      float slope[RT];
+      int row_n[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const int at = at0 + row_n[rt];
-        if (biased) {
-          const float d0 = (float)(at - base);
+        const Row<T::kRows> row(qa, hkv, tile, 16 * rt + l16);
+        const half_t* qrow = qa.q + b * qa.stq.b + row.hq * qa.stq.h + (size_t)row.n * qa.stq.n;
+        row_n[rt] = row.n;
+        slope[rt] = qa.alibi ? qa.alibi[row.hq] * qa.alibi_unit : 0.f;
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            s[rt][e >> 2][e & 3] =
-                fmaf(-slope[rt], fabsf(d0 - (float)(16 * (e >> 2) + (e & 3))), s[rt][e >> 2][e & 3]);
+        for (int i = 0; i < kDwords; ++i) {
+          const int d = D / 4 * g + 8 * i;
+          q[rt][0][i] = as_half8(load16(qrow + d, FULL || d < dr));
         }
-        if (edge) {
-          const int lo = window > 0 ? max(0, at - window + 1) : 0;
-          const int hi = causal ? min(keys.len, at + 1) : keys.len;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = base + 16 * (e >> 2) + (e & 3);
-            if (key < lo || key >= hi) s[rt][e >> 2][e & 3] = -INFINITY;
-          }
-        }
-        if (hide) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = min(max(base + 16 * (e >> 2) + (e & 3), keys.lo), keys.len - 1);
-            if ((hide >> ((key >> a.page_shift) - hide0)) & 1) s[rt][e >> 2][e & 3] = -INFINITY;
-          }
-        }
-        float mloc = s[rt][0][0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) mloc = fmaxf(mloc, s[rt][e >> 2][e & 3]);
-        mloc = max_quarters(mloc);
-        if (__any(mloc > m_raw[rt] + thr_raw)) {
-          const float m_new = fmaxf(m_raw[rt], mloc);
-          const float corr = m_raw[rt] == -INFINITY ? 0.f : fast_exp2((m_raw[rt] - m_new) * c);
-          l[rt] *= corr;
-#pragma unroll
-          for (int cb = 0; cb < D / 16; ++cb) oacc[rt][cb] *= corr;
-          m_raw[rt] = m_new;
-        }
-        const float m_use = m_raw[rt] == -INFINITY ? 0.f : m_raw[rt];
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = fast_exp2((s[rt][e >> 2][e & 3] - m_use) * c);
-          ls[e & 3] += p;
-          const half_t p16 = to16<true>(p);
-          pb[rt][e >> 3][e & 7] = p16;
-          if constexpr (T::kTwoP) rest[rt][e >> 3][e & 7] = to16<true>(p - from16<true>(p16));
-        }
-        l[rt] += (ls[0] + ls[1]) + (ls[2] + ls[3]);
       }
-      // V's block as bf16 to LDS; values of keys that no row sees become zero.
-      const bool part = j * 64 < keys.lo || j * 64 + 64 > keys.len || hide;
+      load_both(j0, true);
+      {
+        // (q is waited for here, behind the loads of K and V: left to its first use, in the loop,
+        // it would be waited for there, and with it all loads of every block)
 #pragma unroll
-      for (int i = 0; i < kBlocks; ++i) {
-        const int u = lane + 64 * i, key = u / kBlocks, blk = u % kBlocks;
-        u32x4 codes = vc[i];
-        float scale = scale_of(vs[i]);
-        if (part) {
-          const int x = j * 64 + key, y = min(max(x, keys.lo), keys.len - 1);
-          if (x != y || ((hide >> ((y >> a.page_shift) - hide0)) & 1)) {
-            codes = u32x4{0u, 0u, 0u, 0u};
-            scale = 1.f;
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < kDwords; ++i) {
+            asm volatile("" : "+v"(q[rt][0][i]));
+            if constexpr (!T::kBF) {
+              const half8 x = q[rt][0][i];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float f = (float)x[e];
+                q[rt][0][i][e] = to16<true>(f);
+                const float rest = f - from16<true>(q[rt][0][i][e]);
+                q[rt][T::kQ - 1][i][e] = to16<true>(__builtin_isfinite(f) ? rest : 0.f);
+              }
+            }
           }
-        }
-        char* to = my_v + key * T::kStride + 64 * blk;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) *reinterpret_cast<half8*>(to + 16 * e) = values(codes[e], scale);
       }
-      load_v(more ? j + 1 : j, more);
-      // (row 4 g + t of 16 keys at columns 4 a .. 4 a + 3 of 16, lane = 16 g + 4 t + a)
-      const half_t* from_v =
-          reinterpret_cast<const half_t*>(my_v + (4 * g + (l16 >> 2)) * T::kStride + 8 * (l16 & 3));
+      const int at0 = keys.len - qa.N, window = qa.window;
+      const int all_lo = window > 0 ? max(0, keys.len - window) : 0;
+      const int all_hi = qa.causal ? at0 + 1 : keys.len;
+      const bool causal = qa.causal, biased = qa.alibi != nullptr;
+      const float thr_raw = qa.rescale;
+      for (int j = j0; j < j1; ++j) {
+        const unsigned long long hide = hidden;  // (of block j's pages, from page hide0 on)
+        const int hide0 = p0;
+        floatx4 s[RT][kKeyTiles];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+        for (int t = 0; t < kKeyTiles; ++t) {
 #pragma unroll
-        for (int cb = 0; cb < D / 16; ++cb) {
-          const half4 lo = lds_read_tr(from_v + 32 * u * (T::kStride / 2) + 16 * cb);
-          const half4 hi = lds_read_tr(from_v + (32 * u + 16) * (T::kStride / 2) + 16 * cb);
-          const half8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          for (int rt = 0; rt < RT; ++rt) s[rt][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+          float size[kDwords];
+          place_k.sizes(kc[t], g, size);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            oacc[rt][cb] = mfma_bf16(v, pb[rt][u], oacc[rt][cb]);
-            if constexpr (T::kTwoP) oacc[rt][cb] = mfma_bf16(v, rest[rt][u], oacc[rt][cb]);
+          for (int i = 0; i < kDwords; ++i) {
+            const half8 k = values(kc[t].c[i], size[i]);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int x = 0; x < T::kQ; ++x) s[rt][t] = mfma_bf16(k, q[rt][x][i], s[rt][t]);
           }
         }
+        // V's block as bf16 to LDS; values of keys that no row sees become zero.
+        const bool part = j * kKeys < keys.lo || j * kKeys + kKeys > keys.len || hide;
+#pragma unroll
+        for (int t = 0; t < kKeyTiles; ++t) {
+          const int key = 16 * t + (lane >> 2);
+          if (part) {
+            const int x = j * kKeys + key, y = min(max(x, keys.lo), keys.len - 1);
+            if (x != y || ((hide >> ((y >> a.page_shift) - hide0)) & 1)) {
+#pragma unroll
+              for (int i = 0; i < kDwords; ++i) vc[t].c[i] = 0u;
+#pragma unroll
+              for (int i = 0; i < kScales; ++i) vc[t].s[i] = 0u;
+            }
+          }
+          float size[kDwords];
+          place_v.sizes(vc[t], lane & 3, size);
+          char* to = my_v + key * T::kStride + 16 * kDwords * (lane & 3);
+#pragma unroll
+          for (int i = 0; i < kDwords; ++i)
+            *reinterpret_cast<half8*>(to + 16 * i) =
+                values(vc[t].c[i], size[i]);
+        }
+        const bool more = j + 1 < j1;
+        load_both(more ? j + 1 : j, more);
+        const int base = j * kKeys + 4 * g;  // key of s[.][t][r]: base + 16 t + r
+        const bool edge = j * kKeys < all_lo || j * kKeys + kKeys > all_hi;
+        half8 pb[RT][kKeyTiles / 2], rest[RT][kKeyTiles / 2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const int at = at0 + row_n[rt];
+          if (biased) {
+            const float d0 = (float)(at - base);
+#pragma unroll
+            for (int e = 0; e < kScores; ++e)
+              s[rt][e >> 2][e & 3] =
+                  fmaf(-slope[rt], fabsf(d0 - (float)(16 * (e >> 2) + (e & 3))), s[rt][e >> 2][e & 3]);
+          }
+          if (edge) {
+            const int lo = window > 0 ? max(0, at - window + 1) : 0;
+            const int hi = causal ? min(keys.len, at + 1) : keys.len;
+#pragma unroll
+            for (int e = 0; e < kScores; ++e) {
+              const int key = base + 16 * (e >> 2) + (e & 3);
+              if (key < lo || key >= hi) s[rt][e >> 2][e & 3] = -INFINITY;
+            }
+          }
+          if (hide) {
+#pragma unroll
+            for (int e = 0; e < kScores; ++e) {
+              const int key = min(max(base + 16 * (e >> 2) + (e & 3), keys.lo), keys.len - 1);
+              if ((hide >> ((key >> a.page_shift) - hide0)) & 1) s[rt][e >> 2][e & 3] = -INFINITY;
+            }
+          }
+          float mloc = s[rt][0][0];
+#pragma unroll
+          for (int e = 1; e < kScores; ++e) mloc = fmaxf(mloc, s[rt][e >> 2][e & 3]);
+          mloc = max_quarters(mloc);
+          if (__any(mloc > m_raw[rt] + thr_raw)) {
+            const float m_new = fmaxf(m_raw[rt], mloc);
+            const float corr = m_raw[rt] == -INFINITY ? 0.f : fast_exp2((m_raw[rt] - m_new) * c);
+            l[rt] *= corr;
+#pragma unroll
+            for (int cb = 0; cb < D / 16; ++cb) oacc[rt][cb] *= corr;
+            m_raw[rt] = m_new;
+          }
+          float ls[4] = {0.f, 0.f, 0.f, 0.f};
+          const float m_c = m_raw[rt] == -INFINITY ? 0.f : m_raw[rt] * c;
+#pragma unroll
+          for (int e = 0; e < kScores; ++e) {
+            const float p = fast_exp2(fmaf(s[rt][e >> 2][e & 3], c, -m_c));
+            ls[e & 3] += p;
+            const half_t p16 = to16<true>(p);
+            pb[rt][e >> 3][e & 7] = p16;
+            rest[rt][e >> 3][e & 7] = to16<true>(p - from16<true>(p16));
+          }
+          l[rt] += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        }
+        // (row 4 g + t of 16 keys at columns 4 a .. 4 a + 3 of 16, lane = 16 g + 4 t + a)
+        const half_t* from_v =
+            reinterpret_cast<const half_t*>(my_v + (4 * g + (l16 >> 2)) * T::kStride + 8 * (l16 & 3));
+#pragma unroll
+        for (int u = 0; u < kKeyTiles / 2; ++u)
+#pragma unroll
+          for (int cb = 0; cb < D / 16; ++cb) {
+            const half4 lo = lds_read_tr(from_v + 32 * u * (T::kStride / 2) + 16 * cb);
+            const half4 hi = lds_read_tr(from_v + (32 * u + 16) * (T::kStride / 2) + 16 * cb);
+            const half8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              oacc[rt][cb] = mfma_bf16(v, pb[rt][u], oacc[rt][cb]);
+              oacc[rt][cb] = mfma_bf16(v, rest[rt][u], oacc[rt][cb]);
+            }
+          }
+      }
     }
 
     // The rows' results, or the part's (slots as in fa_paged.hip).
@@ -391,59 +535,53 @@ __global__ __launch_bounds__(T::kThreads) void paged4_kernel(const Paged4Args a)
       }
       continue;
     }
-    // One item: the waves' parts meet in LDS, a row tile at a time, in the accumulator's
-    // order: float4 cb * 64 + lane.
+    // One item: the waves' parts meet in LDS, in the accumulator's order: float4 (rt * D / 16
+    // + cb) * 64 + lane.
     const bool whole = wg1 - wg0 == units;
     if (whole) owned.w = 0;
     if (lane == 0) ra.owned[wg * kLine + wave] = owned;
     slot = 2 * (size_t)(wg * kLine);
+    constexpr int kRuns = D / 16;
+    __syncthreads();
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      __syncthreads();
-      float* const mine = reinterpret_cast<float*>(my_v);
 #pragma unroll
-      for (int cb = 0; cb < D / 16; ++cb)
-        *reinterpret_cast<floatx4*>(mine + (cb * 64 + lane) * 4) = oacc[rt][cb];
-      ml[wave * 64 + lane] = make_float2(m_raw[rt], l[rt]);
-      __syncthreads();
-      float m_star = -INFINITY, l_star = 0.f, wk[kLine];
+      for (int cb = 0; cb < kRuns; ++cb)
+        *reinterpret_cast<floatx4*>(my_v + ((rt * kRuns + cb) * 64 + lane) * 16) = oacc[rt][cb];
+      ml[(rt * kWaves + wave) * 64 + lane] = make_float2(m_raw[rt], l[rt]);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int task = wave; task < RT * kRuns; task += kLine) {
+      const int rt = task / kRuns, cb = task % kRuns;
+      const float2* const mine = ml + rt * kWaves * 64;
+      float m_star = -INFINITY, l_star = 0.f;
 #pragma unroll
-      for (int k = 0; k < kLine; ++k) m_star = fmaxf(m_star, ml[k * 64 + lane].x);
+      for (int k = 0; k < kLine; ++k) m_star = fmaxf(m_star, mine[k * 64 + lane].x);
+      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < kLine; ++k) {
-        const float m = ml[k * 64 + lane].x;
-        wk[k] = m == -INFINITY ? 0.f : fast_exp2((m - m_star) * c);
-        l_star += wk[k] * ((ml[k * 64 + l16].y + ml[k * 64 + l16 + 16].y) +
-                           (ml[k * 64 + l16 + 32].y + ml[k * 64 + l16 + 48].y));
+        const float2* const x = mine + k * 64 + l16;
+        const float wk = x->x == -INFINITY ? 0.f : fast_exp2((x->x - m_star) * c);
+        l_star += wk * ((x[0].y + x[16].y) + (x[32].y + x[48].y));
+        acc += *reinterpret_cast<const floatx4*>(vt + k * T::kTileBytes + (task * 64 + lane) * 16) * wk;
       }
       const int lr = 16 * rt + l16;
       const Row<T::kRows> row(ra, hkv, tile, lr);
-      if (!row.ok) continue;
-      const float inv = l_star > 0.f ? 1.f / l_star : 0.f;
-      for (int cb = wave; cb < D / 16; cb += kLine) {
-        floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < kLine; ++k)
-          acc += *reinterpret_cast<const floatx4*>(
-                     reinterpret_cast<const float*>(vt + k * T::kTileBytes) + (cb * 64 + lane) * 4) * wk[k];
-        put(row, whole, lr, inv, 16 * cb + 4 * g, acc);
+      if (row.ok) {
+        put(row, whole, lr, l_star > 0.f ? 1.f / l_star : 0.f, 16 * cb + 4 * g, acc);
+        if (cb == 0 && g == 0) finish(row, whole, lr, m_star, l_star);
       }
-      if (wave == 0 && g == 0) finish(row, whole, lr, m_star, l_star);
     }
     return;
   } while (pos < end);
   if (lane == 0) late_args().owned[wg * kLine + wave] = owned;
 }
 
-// Row tiles that a wave takes: all of a kv head's up to four, of bf16 rows at most 128
-// wide, else two (fp16 rows take twice the registers, wide ones too).
-template <int D, bool BF>
-constexpr int kMostTiles = BF && D <= 128 ? 4 : 2;
+// Row tiles that a wave takes: one or two.
 template <int D, bool BF, class F>
 auto by_row_tiles(int rows, const F& f) {
   if (rows <= 16) return f(Paged4<D, BF, 1>{});
-  if constexpr (kMostTiles<D, BF> == 4)
-    if (rows > 32) return f(Paged4<D, BF, 4>{});
   return f(Paged4<D, BF, 2>{});
 }
 
@@ -465,10 +603,28 @@ hipError_t launch_paged4_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
     d.scale_page = a.scales.page_stride;
     d.scale_head = a.scales.head_stride;
     d.scale_row = a.scales.row_stride;
+    // Tiles go by 32-bit places in a kv head's rows, and by words of scales that begin at the
+    // same bits in every tile (a lane of width 256 takes two scales, of one word).
+    const auto& sc = a.scales;
+    const long long code_bytes = (a.pool.pages - 1LL) * a.pool.page_stride +
+                                 ((1LL << a.pool.page_shift) - 1) * a.pool.row_stride + a.D / 2;
+    const long long scale_bytes = (a.pool.pages - 1LL) * sc.page_stride +
+                                  ((1LL << a.pool.page_shift) - 1) * sc.row_stride + a.D / 32;
+    const uintptr_t odd = (uintptr_t)sc.k | (uintptr_t)sc.v | (uintptr_t)sc.head_stride | (uintptr_t)sc.row_stride;
+    const bool words = sc.page_stride % 4 == 0 && (a.D != 256 || odd % 2 == 0);
+    const bool near = code_bytes < 1LL << 32 && scale_bytes < (1LL << 32) - 8;
+    const int pages = !words || !near ? 0 : a.pool.page_shift >= 4 ? 1 : a.pool.page_shift == 3 ? 2 : 0;
+    if (pages > 0) {
+      d.code_bytes = (uint32_t)code_bytes;
+      d.scale_bytes = (uint32_t)(scale_bytes + 6) & ~3u;  // (of whole words, from the first's)
+    }
     auto launch = [&](auto full) {
       constexpr bool kFull = decltype(full)::value;
-      hipLaunchKernelGGL((paged4_kernel<T, kFull>), dim3(T::kGrid), dim3(T::kThreads), 0,
-                         (hipStream_t)a.stream, d);
+      constexpr bool kStream = T::kRowTiles == 1;
+      const auto kernel = pages == 1   ? paged4_kernel<T, kFull, 1, kStream>
+                          : pages == 2 ? paged4_kernel<T, kFull, 2, kStream>
+                                       : paged4_kernel<T, kFull, 0, kStream>;
+      hipLaunchKernelGGL(kernel, dim3(T::kGrid), dim3(T::kThreads), 0, (hipStream_t)a.stream, d);
       const hipError_t e = hipGetLastError();
       return e != hipSuccess ? e : launch_paged_join<T, kFull>(d, (hipStream_t)a.stream);
     };

@@ -612,9 +612,7 @@ def paged_attn(q, k_cache, v_cache, block_table, kv_len, causal=True, sliding_wi
 
     With k_scale and v_scale the cache is of 4 bits, as paged_append writes it, and read as
     such, for q in fp16 or bf16 whatever the rows were. The products are bf16's, which
-    holds the cache's values exactly; fp16 q enters as two bf16 numbers. With more than 32
-    rows per kv head the probabilities are rounded to bf16 once where q is bf16 and D at
-    most 128, else they are two bf16 numbers.
+    holds the cache's values exactly; fp16 q and the probabilities enter as two bf16 numbers.
     """
     _paged_inputs("paged_attn", q, k_cache, v_cache, block_table, kv_len,
                   *_scales(k_scale, v_scale))

@@ -590,9 +590,8 @@ int fa_paged_gather(void* k, void* v, long long stride_b, long long stride_n, lo
  * fa_paged_attn over a cache in 4 bits: the same arguments, options and rows without a
  * key. The products are bf16's, in which the cache's values are exact; q in fp16 enters
  * as two bf16 numbers, exactly where it is finite, so scores are sums of exact products in
- * fp32. The probabilities are two bf16 numbers (off by 2^-16 of themselves) with up to 32
- * rows per kv head, and for fp16 or head dims above 128 with any; else one. The workspace
- * is at most 137 MB.
+ * fp32. The probabilities are two bf16 numbers (off by 2^-16 of themselves). The workspace
+ * is about 68 MB at most.
  */
 size_t fa_paged4_attn_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
 int fa_paged4_attn(const void* q, void* o, float* lse, const fa_paged_cache* cache,

@@ -49,8 +49,7 @@ def attention(q, k, v, table, kv_len, **kw):
     paged4's own rounding:
       * o is rounded once, to q's format (u |o|);
       * the probabilities are two bf16 numbers, each half a step (2^-8) off at most, so off
-        by 2^-16 of themselves, or one (2^-8) where q is bf16, D at most 128 and the rows of
-        a kv head more than 32;
+        by 2^-16 of themselves;
       * a score is a sum of D exact products in fp32 (2 D with fp16 q as two numbers),
         whose rounding is at most (2 D + 4) 2^-24 sum |q k| scale, plus 2^-22 of the
         score's and the bias's magnitude;
@@ -59,16 +58,13 @@ def attention(q, k, v, table, kv_len, **kw):
         2^-126 |v| for each key (a code of 0 is exact, so o can be as small as that where
         the heavy keys' values are 0).
     paged_ref's score bound counts D products: twice it covers 2 D."""
-    D, rows = q.size(3), q.size(1) // k.size(1) * q.size(2)
     o, lse, o_tol, lse_tol = paged_ref.attention(q, k, v, table, kv_len, **kw)
     a, _, a_tol, _ = paged_ref.attention(q, k, v.abs(), table, kv_len, **kw)
     u = torch.finfo(q.dtype).eps / 2
-    one = q.dtype == torch.bfloat16 and D <= 128 and rows > 32
     # paged_ref: o_tol = u (|o| + A) + (2 E + 2^-18) A, and for |v|, o = A itself.
     scores = a_tol - 2 * u * a
-    p_off = 2.0 ** -8 if one else 2.0 ** -16
     dropped = 2.0 ** -126 * table.size(1) * k.size(2) * v.abs().nan_to_num(nan=0.0).max()
-    return o, lse, u * o.abs() + p_off * a + 2 * scores + dropped, 2 * lse_tol
+    return o, lse, u * o.abs() + 2.0 ** -16 * a + 2 * scores + dropped, 2 * lse_tol
 
 
 def weights(q, k, table, kv_len, lse, before, causal=True, window=None, alibi=None, scale=None,
