@@ -158,7 +158,7 @@ def test_evict_refusals():
     assert call(D=72) == 10001 and call(Hkv=0) == 10003 and call(B=0) == 10004
     assert call(B=1 << 20, Hkv=4) == 10007
     need = lib.fa_paged_evict_workspace_bytes(1, 2, 3, 16)
-    assert need == 2 * (3 * 16 + 1) * 4 and call(nbytes=need - 1) == 10006
+    assert need == 2 * (3 * 16 + 2) * 4 and call(nbytes=need - 1) == 10006
     for bad in ((0, 2, 3, 16), (1, 0, 3, 16), (1, 2, 0, 16), (1, 2, 3, 24), (1 << 21, 2, 3, 16)):
         assert lib.fa_paged_evict_workspace_bytes(*bad) == 0, bad
 
