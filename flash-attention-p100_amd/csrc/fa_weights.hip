@@ -15,12 +15,13 @@
 namespace fa {
 namespace {
 
-template <int DIM, bool BF>
+// PER: workgroups of a CU.
+template <int DIM, bool BF, int PER>
 struct Weigh {
   static constexpr int kD = DIM, kTiles = 1, kRows = 16, kKeys = 64;
   static constexpr bool kBF = BF;
   static constexpr int kWaves = 4, kLine = kWaves, kThreads = 64 * kWaves;
-  static constexpr int kGrid = kCUs * (DIM > 128 ? 2 : 4);
+  static constexpr int kGrid = kCUs * PER;
   static constexpr float kPUnit = 1.f, kPRescale = 0.f;
 };
 
@@ -45,10 +46,14 @@ __device__ __forceinline__ floatx4 mfma4(half8 a, half8 b, floatx4 c) {
 }
 
 // FOUR: K is in 4 bits (its values are bf16, and q two bf16 numbers where it is fp16).
-// FULL: the head dim is the width.
-template <int D, bool BF, bool FOUR, bool FULL>
-__global__ __launch_bounds__(256) void weights_kernel(const WeighArgs a) {
-  using T = Weigh<D, BF>;
+// FULL: the head dim is the width. ONE: all rows of a kv head are one tile: it stays in
+// registers while the blocks go by, each loaded while the one before is multiplied. Else a
+// block stays, as operands, and the tiles go by the same way.
+template <int D, bool FOUR, bool ONE>
+constexpr int kPerCu = D <= 64 ? 3 : D <= 128 ? (ONE && FOUR ? 3 : 2) : ONE && FOUR ? 2 : 1;
+template <int D, bool BF, bool FOUR, bool FULL, bool ONE>
+__global__ __launch_bounds__(256, (kPerCu<D, FOUR, ONE>)) void weights_kernel(const WeighArgs a) {
+  using T = Weigh<D, BF, kPerCu<D, FOUR, ONE>>;
   constexpr int kWaves = T::kWaves, kChunks = D / 32, kQ = FOUR && !BF ? 2 : 1;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
@@ -67,9 +72,22 @@ __global__ __launch_bounds__(256) void weights_kernel(const WeighArgs a) {
   Keys<T> keys = line.keys(b);
   int item = (pos - start) / line.units(keys);
   start += item * line.units(keys);
-  const int unit = FOUR ? 1 : 2;
+  constexpr int kUnit = FOUR ? 1 : 2;
   const int page_mask = (1 << a.page_shift) - 1, dr = FULL ? D : a.dr;
   const int rows = a.group * a.N, row_tiles = (rows + 15) / 16;
+  const float over_n = __builtin_amdgcn_rcpf((float)a.N);
+  // Row r of a kv head as query head and row of it. (r < 2^24: off by one at most.)
+  auto split = [&](int r, int& head, int& n) {
+    head = (int)(((float)r + 0.5f) * over_n);
+    n = r - head * a.N;
+    if (n < 0) {
+      --head;
+      n += a.N;
+    } else if (n >= a.N) {
+      ++head;
+      n -= a.N;
+    }
+  };
 
   while (pos < end) {
     const int units = line.units(keys), from = pos - start, upto = min(from + end - pos, units);
@@ -77,104 +95,224 @@ __global__ __launch_bounds__(256) void weights_kernel(const WeighArgs a) {
     const int j0 = keys.first + max(from - line.lead, 0);
     const int j1 = keys.len > keys.lo ? keys.first + max(upto - line.lead, 0) : j0;
     const int* table = a.table + b * a.table_stride;
-    const uint8_t* base_k = (const uint8_t*)a.k + unit * hkv * a.head_stride;
+    const int last_page = max(keys.len - 1, 0) >> a.page_shift;
+    const uint8_t* base_k = (const uint8_t*)a.k + kUnit * hkv * a.head_stride;
     const uint8_t* base_s = FOUR ? a.k_scale + hkv * a.scale_head : nullptr;
     float* base_w = a.weights + hkv * a.weight_head;
-    for (int j = j0; j < j1; ++j) {
-      // A lane's own key (its page, its weight), and those of the tiles.
-      const int my_key = min(max(j * 64 + lane, keys.lo), keys.len - 1);
-      int my_page = table[my_key >> a.page_shift];
-      const bool ok = my_page >= 0 && my_page < a.pages;
-      my_page = ok ? my_page : 0;
-      float* const my_w = base_w + my_page * a.weight_page + (my_key & page_mask) * a.weight_row;
-      const bool mine = ok && j * 64 + lane == my_key;
-      const bool fresh = a.restart || my_key >= keys.len - a.N;
-      const float before = mine && !fresh ? *my_w : 0.f;
-      half8 k[4][kChunks];
+    const float* lse_rows = a.lse + ((size_t)b * a.Hq + hkv * a.group) * a.N;
+    int p0 = 0, held = 0;  // pages p0 .. p0 + 63 of the request are in the lanes
+    auto fetch = [&](int j) {
+      p0 = max(j * 64, keys.lo) >> a.page_shift;
+      held = table[min(p0 + lane, last_page)];
+    };
+
+    // A block as it is loaded: K's rows (of key 16 t + lane % 16 in 16 bits the chunks 4 i + g,
+    // in 4 a quarter of the row and the words of its scales), and the weight of key `lane`.
+    constexpr int kScales = D == 96 || D == 256 ? 2 : 1;
+    struct Block {
+      u32x4 rows[FOUR ? 1 : 4][FOUR ? 1 : kChunks];
+      uint32_t codes[FOUR ? 4 : 1][kChunks], scale[4][kScales], bit[4][kScales];
+      float before;
+      float* at;  // null where the lane has no key of the request
+      bool fresh;
+    };
+    auto load = [&](Block& x, int j) {
+      if ((min(j * 64 + 64, keys.len) - 1) >> a.page_shift > p0 + 63) fetch(j);
+      const int key = min(max(j * 64 + lane, keys.lo), keys.len - 1);
+      const int page = __shfl(held, (key >> a.page_shift) - p0);
+      const bool there = page >= 0 && page < a.pages;
+      const int row = key & page_mask;
+      x.at = there && key == j * 64 + lane ? base_w + (there ? page : 0) * a.weight_page + row * a.weight_row : nullptr;
+      x.fresh = a.restart || key >= keys.len - a.N;
+      x.before = x.at && !x.fresh ? *x.at : 0.f;
+      const int my_page = there ? page : 0;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int page = __shfl(my_page, 16 * t + l16), key = __shfl(my_key, 16 * t + l16);
-        const uint8_t* row = base_k + unit * (page * a.page_stride + (key & page_mask) * a.row_stride);
+        const int p = __shfl(my_page, 16 * t + l16), r = __shfl(row, 16 * t + l16);
+        const uint8_t* k = base_k + kUnit * (p * a.page_stride + r * a.row_stride);
         if constexpr (FOUR) {
-          const uint8_t* scales = base_s + page * a.scale_page + (key & page_mask) * a.scale_row;
+          const uint8_t* scales = base_s + p * a.scale_page + r * a.scale_row;
+          const bool begins = FULL || 64 * g < dr, both = FULL || 64 * g + 32 < dr;
+          const uint8_t* q = k + 4 * kChunks * (begins ? g : 0);
+          if constexpr (kChunks < 4) {
+            __builtin_memcpy(x.codes[t], __builtin_assume_aligned(q, 4), 4 * kChunks);
+          } else {
 #pragma unroll
-          for (int i = 0; i < kChunks; ++i) {
-            const int d = D / 4 * g + 8 * i;  // (of a quarter of the row)
-            const bool there = FULL || d < dr;
-            const uint32_t codes = there ? *reinterpret_cast<const uint32_t*>(row + d / 2) : 0u;
-            const float scale = __uint_as_float((there ? (uint32_t)scales[d / 32] : 127u) << 23);
-            auto two = [&](auto sel) {
-              return __builtin_bit_cast(
-                  uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, decltype(sel)::value));
-            };
-            k[t][i] = as_half8(u32x4{two(std::integral_constant<int, 0>{}), two(std::integral_constant<int, 1>{}),
-                                     two(std::integral_constant<int, 2>{}), two(std::integral_constant<int, 3>{})});
+            for (int h = 0; h < kChunks / 4; ++h) {
+              const u32x4 v = *reinterpret_cast<const u32x4*>(q + (both ? 16 * h : 0));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x.codes[t][4 * h + i] = v[i];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kScales; ++i) {
+            const int block = !begins ? 0 : D == 256 ? 2 * g + (both ? i : 0) : (kChunks * g + 2 * i) / 4;
+            const uint8_t* s = scales + block;
+            const uint32_t sub = (uint32_t)((uintptr_t)s & 3);
+            x.bit[t][i] = 8 * sub;
+            x.scale[t][i] = *reinterpret_cast<const uint32_t*>(s - sub);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < kChunks; ++i)
-            k[t][i] = as_half8(load16(reinterpret_cast<const half_t*>(row) + 32 * i + 8 * g,
-                                      FULL || 32 * i + 8 * g < dr));
+            x.rows[t][i] = load16(reinterpret_cast<const half_t*>(k) + 32 * i + 8 * g, FULL || 32 * i + 8 * g < dr);
         }
       }
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int rt = 0; rt < row_tiles; ++rt) {
-        half8 q[kQ][kChunks];
-        const Row<16> mine(a, hkv, rt, l16);
-        const half_t* qrow = a.q + b * a.stq.b + mine.hq * a.stq.h + (size_t)mine.n * a.stq.n;
+    };
+    // Its operands, a tile at a time (values past the head dim meet zeros of q: finite ones).
+    auto operands = [&](const Block& x, int t, half8 (&k)[kChunks]) {
+      if constexpr (FOUR) {
+        float two[2];
+#pragma unroll
+        for (int i = 0; i < kScales; ++i)
+          two[i] = __uint_as_float(__builtin_amdgcn_alignbit(x.scale[t][i], x.scale[t][i], (x.bit[t][i] + 9u) & 31u));
+        if constexpr (kScales == 1) two[1] = two[0];
+        if constexpr (!FULL) {
+          two[0] = 64 * g < dr ? two[0] : 1.f;
+          two[1] = 64 * g + 32 < dr ? two[1] : 1.f;
+        }
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
-          const int d = FOUR ? D / 4 * g + 8 * i : 32 * i + 8 * g;
-          const half8 x = as_half8(load16(qrow + d, FULL || d < dr));
-          if constexpr (kQ == 1) {
-            q[0][i] = x;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float f = (float)x[e];
-              q[0][i][e] = to16<true>(f);
-              const float rest = f - from16<true>(q[0][i][e]);
-              q[kQ - 1][i][e] = to16<true>(__builtin_isfinite(f) ? rest : 0.f);
-            }
-          }
+          const float scale = D == 96 ? (i == 0 || (i == 1 && g != 1) ? two[0] : two[1]) : two[D == 256 ? i / 4 : 0];
+          const uint32_t c = x.codes[t][i];
+          k[i] = as_half8(u32x4{
+              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0)),
+              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1)),
+              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2)),
+              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3))});
         }
-        // The four rows of this lane's scores.
-        float lse[4], slope[4];
-        int lo[4], hi[4], at[4];
+      } else {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) k[i] = as_half8(x.rows[t][i]);
+      }
+    };
+    // A tile of rows: q of row lane % 16, lse of rows 4 g .. 4 g + 3 (+inf, a weight of 0,
+    // where there is none).
+    struct Rows {
+      half8 q[kChunks];
+      float lse[4];
+    };
+    auto load_rows = [&](Rows& x, int rt) {
+      int head, n;
+      split(min(16 * rt + l16, rows - 1), head, n);
+      const half_t* q = a.q + b * a.stq.b + (hkv * a.group + head) * a.stq.h + (size_t)n * a.stq.n;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int d = FOUR ? D / 4 * g + 8 * i : 32 * i + 8 * g;
+        x.q[i] = as_half8(load16(q + d, FULL || d < dr));
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x.lse[r] = lse_rows[min(16 * rt + 4 * g + r, rows - 1)];
+    };
+    const int all_lo = a.hide_window > 0 ? max(0, keys.len - a.hide_window) : 0;
+    const int all_hi = a.causal ? keys.len - a.N + 1 : keys.len;
+    // Adds to acc the weights that rows of tile rt give the keys of tile t.
+    auto weigh = [&](const Rows& x, const half8 (&q)[kQ][kChunks], const half8 (&k)[kChunks], int rt, int j, int t,
+                     float& acc) {
+      floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int y = 0; y < kQ; ++y)
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) s = mfma4<BF || FOUR>(q[y][i], k[i], s);
+      const int key = j * 64 + 16 * t + l16;
+      const bool edge = j * 64 < all_lo || j * 64 + 64 > all_hi || 16 * rt + 16 > rows;
+      // (score - lse first: exact near 0, where the weights are large)
+      float z[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) z[r] = fmaf(s[r], a.scale, -x.lse[r]);
+      if (edge || a.alibi) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const Row<16> row(a, hkv, rt, 4 * g + r);
-          lse[r] = a.lse[((size_t)b * a.Hq + row.hq) * a.N + row.n];
-          slope[r] = a.alibi ? a.alibi[row.hq] : 0.f;
-          at[r] = keys.len - a.N + row.n;
-          lo[r] = a.hide_window > 0 ? max(0, at[r] - a.hide_window + 1) : 0;
-          hi[r] = !row.ok ? 0 : a.causal ? min(keys.len, at[r] + 1) : keys.len;
+          const int row = 16 * rt + 4 * g + r;
+          int head, n;
+          split(min(row, rows - 1), head, n);
+          const int at = keys.len - a.N + n;
+          if (a.alibi) z[r] = fmaf(-a.alibi[hkv * a.group + head], (float)abs(at - key), z[r]);
+          const int lo = a.hide_window > 0 ? max(0, at - a.hide_window + 1) : 0;
+          const int hi = row >= rows ? 0 : a.causal ? min(keys.len, at + 1) : keys.len;
+          if (key < lo || key >= hi) z[r] = -INFINITY;
         }
+      }
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          floatx4 s = {0.f, 0.f, 0.f, 0.f};
+      for (int r = 0; r < 4; ++r) acc += fast_exp2(z[r] * kLog2e);
+    };
+    auto split_q = [&](const Rows& x, half8 (&q)[kQ][kChunks]) {
 #pragma unroll
-          for (int x = 0; x < kQ; ++x)
+      for (int i = 0; i < kChunks; ++i) {
+        q[0][i] = x.q[i];
+        if constexpr (kQ == 2) {
 #pragma unroll
-            for (int i = 0; i < kChunks; ++i) s = mfma4<BF || FOUR>(q[x][i], k[t][i], s);
-          const int key = j * 64 + 16 * t + l16;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            // (score - lse first: exact near 0, where the weights are large)
-            float z = fmaf(s[r], a.scale, -lse[r]);
-            if (a.alibi) z = fmaf(-slope[r], (float)abs(at[r] - key), z);
-            acc[t] += key >= lo[r] && key < hi[r] ? fast_exp2(z * kLog2e) : 0.f;
+          for (int e = 0; e < 8; ++e) {
+            const float f = (float)x.q[i][e];
+            q[0][i][e] = to16<true>(f);
+            const float rest = f - from16<true>(q[0][i][e]);
+            q[kQ - 1][i][e] = to16<true>(__builtin_isfinite(f) ? rest : 0.f);
           }
         }
       }
+    };
+    auto store = [&](const Block& x, const float (&acc)[4]) {
       float sum = 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        float x = acc[t] + __shfl_xor(acc[t], 16);
-        x += xor32(x);
-        sum = g == t ? x : sum;
+        float y = acc[t] + __shfl_xor(acc[t], 16);
+        y += xor32(y);
+        sum = g == t ? y : sum;
       }
-      if (mine) *my_w = before + sum;
+      if (x.at) *x.at = x.before + sum;
+    };
+
+    if (j0 < j1) {
+      fetch(j0);
+      if constexpr (ONE) {
+        Rows now;
+        load_rows(now, 0);
+        half8 q[kQ][kChunks];
+        Block x;
+        load(x, j0);
+        split_q(now, q);
+        for (int j = j0; j < j1; ++j) {
+          // (behind the last block that block again: a branch around the loads would have all
+          // of them waited for)
+          Block next;
+          if constexpr (FOUR) load(next, min(j + 1, j1 - 1));
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            half8 k[kChunks];
+            operands(x, t, k);
+            weigh(now, q, k, 0, j, t, acc[t]);
+          }
+          if constexpr (FOUR) {
+            store(x, acc);
+            x = next;
+          } else {
+            const Block old = x;
+            if (j + 1 < j1) load(x, j + 1);
+            store(old, acc);
+          }
+        }
+      } else {
+        for (int j = j0; j < j1; ++j) {
+          Block x;
+          Rows now, next;
+          load(x, j);
+          load_rows(now, 0);
+          half8 k[4][kChunks];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) operands(x, t, k[t]);
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int rt = 0; rt < row_tiles; ++rt) {
+            load_rows(next, min(rt + 1, row_tiles - 1));
+            half8 q[kQ][kChunks];
+            split_q(now, q);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) weigh(now, q, k[t], rt, j, t, acc[t]);
+            now = next;
+          }
+          store(x, acc);
+        }
+      }
     }
     pos += upto - from;
     start += units;
@@ -190,9 +328,8 @@ __global__ __launch_bounds__(256) void weights_kernel(const WeighArgs a) {
 
 template <>
 hipError_t launch_paged_weights_w<FA_WIDTH, FA_BF>(const PagedArgs& a, const KeyWeights& w, bool restart) {
-  using T = Weigh<FA_WIDTH, FA_BF>;
   WeighArgs d{};
-  paged_args<T>(d, a);
+  paged_args<Weigh<FA_WIDTH, FA_BF, 1>>(d, a);
   d.n_groups = 1;
   d.items = a.Hkv;
   d.k_scale = a.scales.k;
@@ -207,15 +344,22 @@ hipError_t launch_paged_weights_w<FA_WIDTH, FA_BF>(const PagedArgs& a, const Key
   d.hide_window = d.window;
   if (restart) d.window = 0;
   d.restart = restart;
+  auto launch = [&](auto four, auto full, auto one) {
+    constexpr bool kFour = decltype(four)::value, kFull = decltype(full)::value, kOne = decltype(one)::value;
+    using T = Weigh<FA_WIDTH, FA_BF, kPerCu<FA_WIDTH, kFour, kOne>>;
+    hipLaunchKernelGGL((weights_kernel<FA_WIDTH, FA_BF, kFour, kFull, kOne>), dim3(T::kGrid), dim3(T::kThreads), 0,
+                       (hipStream_t)a.stream, d);
+    return hipGetLastError();
+  };
+  using std::false_type, std::true_type;
+  auto by_rows = [&](auto four, auto full) {
+    return d.group * d.N <= 16 ? launch(four, full, true_type{}) : launch(four, full, false_type{});
+  };
   // (4-bit rows are whole blocks of 32: of the widths, 256 alone serves narrower ones)
-  constexpr bool kFull4 = FA_WIDTH != 256;
   const bool full = a.D == FA_WIDTH;
-  const auto kernel = a.scales.k ? (full ? weights_kernel<FA_WIDTH, FA_BF, true, true>
-                                         : weights_kernel<FA_WIDTH, FA_BF, true, kFull4>)
-                                 : (full ? weights_kernel<FA_WIDTH, FA_BF, false, true>
-                                         : weights_kernel<FA_WIDTH, FA_BF, false, false>);
-  hipLaunchKernelGGL(kernel, dim3(T::kGrid), dim3(T::kThreads), 0, (hipStream_t)a.stream, d);
-  return hipGetLastError();
+  using Narrow4 = std::integral_constant<bool, FA_WIDTH != 256>;
+  if (a.scales.k) return full ? by_rows(true_type{}, true_type{}) : by_rows(true_type{}, Narrow4{});
+  return full ? by_rows(false_type{}, true_type{}) : by_rows(false_type{}, false_type{});
 }
 
 }  // namespace fa
