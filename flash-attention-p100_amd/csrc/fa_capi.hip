@@ -856,6 +856,7 @@ int fa_paged_weights(const void* q, const float* lse, const fa_paged_cache* cach
       pools_overlap({weights, nullptr, w_stride_page, w_stride_head, w_stride_row, 1, 4},
                     a.pool.pages, Hkv, cache->page_size, false))
     return FA_ERR_PAGES;
+  if (w_stride_page >= 1LL << 31 || w_stride_row >= 1LL << 31) return FA_ERR_TOO_LARGE;
   a.lse = const_cast<float*>(lse);
   return to_code(fa::launch_paged_weights(a, {weights, w_stride_page, w_stride_head, w_stride_row},
                                           restart != 0));

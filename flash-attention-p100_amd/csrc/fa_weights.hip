@@ -3,13 +3,19 @@
 // query heads of the group of exp(score - lse). (What eviction by accumulated attention
 // goes by: fa_evict.hip.) No counterpart in the reference, which has no cache.
 //
-// Bound: HBM, K is read once, a quarter or less of the bytes that attention needs in
-// 16 bits where few rows share a key. The lse is known, so keys do not depend on each
-// other: the blocks of 64 keys of all requests and kv heads lie on one line that the
-// waves divide evenly (as in fa_paged.hip), a wave holds a block of K as operands and
-// goes over all rows of the kv head, 16 at a time, on v_mfma_f32_16x16x32, S = Q K^T: a
-// lane has one key of a tile, so the rows' weights add up in it. Scores, weights and
-// sums are fp32, each key's sum in one order.
+// The lse is known, so keys do not depend on each other: the blocks of 64 keys of all
+// requests and kv heads lie on one line that the waves divide evenly (as in fa_paged.hip), a
+// wave holds a block of K as operands and goes over all rows of the kv head, 16 at a time, on
+// v_mfma_f32_16x16x32, S = Q K^T: a lane has one key of a tile, so the rows' weights add up in
+// it. Scores, weights and sums are fp32, each key's sum in one order.
+//
+// Bound: HBM, K is read once; near it the instructions (an exponential per score and, in 4
+// bits, a conversion per two values). Single tokens, B=16 H=32/8 D=128, up to 8192 keys of 4
+// bits (43 MB): 12 us, of which 3.5 pass before a wave has its first keys. B=2 H=32/8 N=32,
+// 16384 keys of 16 bits (69 MB): 27 us, two blocks to a wave, each loaded in 4 us and
+// multiplied in 8.
+#include <climits>
+
 #include "fa_paged.h"
 
 namespace fa {
@@ -20,7 +26,8 @@ template <int DIM, bool BF, int PER>
 struct Weigh {
   static constexpr int kD = DIM, kTiles = 1, kRows = 16, kKeys = 64;
   static constexpr bool kBF = BF;
-  static constexpr int kWaves = 4, kLine = kWaves, kThreads = 64 * kWaves;
+  static constexpr int kWaves = 4, kThreads = 64 * kWaves;
+  static constexpr int kLine = INT_MAX;  // (an item's begin costs no more than a block's: no lead)
   static constexpr int kGrid = kCUs * PER;
   static constexpr float kPUnit = 1.f, kPRescale = 0.f;
 };
@@ -48,16 +55,29 @@ __device__ __forceinline__ floatx4 mfma4(half8 a, half8 b, floatx4 c) {
 // FOUR: K is in 4 bits (its values are bf16, and q two bf16 numbers where it is fp16).
 // FULL: the head dim is the width. ONE: all rows of a kv head are one tile: it stays in
 // registers while the blocks go by, each loaded while the one before is multiplied. Else a
-// block stays, as operands, and the tiles go by the same way.
-template <int D, bool FOUR, bool ONE>
-constexpr int kPerCu = D <= 64 ? 3 : D <= 128 ? (ONE && FOUR ? 3 : 2) : ONE && FOUR ? 2 : 1;
-template <int D, bool BF, bool FOUR, bool FULL, bool ONE>
-__global__ __launch_bounds__(256, (kPerCu<D, FOUR, ONE>)) void weights_kernel(const WeighArgs a) {
-  using T = Weigh<D, BF, kPerCu<D, FOUR, ONE>>;
+// block stays, as operands, and the tiles go by the same way. FEW: the rows of ONE are four
+// at most, and stand in the tile four times, so that each quarter of the wave has a key
+// tile's scores for itself (B=16 H=32/8 N=1, up to 8192 keys of 4 bits: 12 us instead of 15).
+template <int D, bool FOUR, bool ONE, bool FEW>
+constexpr int kPerCu = D <= 64 ? 3 + FEW : D <= 128 ? 2 + (ONE && FOUR) : 1 + (ONE && FOUR);
+template <int D, bool BF, bool FOUR, bool FULL, bool ONE, bool FEW>
+__global__ __launch_bounds__(256, (kPerCu<D, FOUR, ONE, FEW>)) void weights_kernel(const WeighArgs a) {
+  static_assert(ONE || !FEW, "");
+  using T = Weigh<D, BF, kPerCu<D, FOUR, ONE, FEW>>;
   constexpr int kWaves = T::kWaves, kChunks = D / 32, kQ = FOUR && !BF ? 2 : 1;
+  // Operands' rows lie a row to a lane, whose loads would not join: they are loaded by
+  // kLanes neighbouring lanes to a row, 16 bytes each, and go through LDS, where a row is
+  // an odd number of 16 bytes (their banks differ). At B=2 H=32/8 N=32 D=128, 16384 keys in
+  // 16 bits: 27 us instead of 32, and 3.9 M of L1's accesses instead of 13.7 M.
+  constexpr int kUnits = FOUR ? D / 32 : D / 8, kLoads = (kUnits + 3) / 4;  // of a row
+  constexpr int kLanes = kUnits < 3 ? kUnits : 4, kRowsAtOnce = 64 / kLanes;
+  constexpr int kStride = kUnits | 1, kQStride = (D / 8) | 1;
+  constexpr int kStage = (FOUR ? 64 : 16) * kStride;
+  __shared__ u32x4 lds[kWaves][kStage + (ONE ? 0 : 16 * kQStride)];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
   __builtin_assume(wave >= 0 && wave < kWaves);
+  u32x4 *const stage = lds[wave], *const q_stage = lds[wave] + kStage;
   const int wg = xcd_work_index(T::kGrid);
   const int l16 = lane & 15, g = lane >> 4;
   Line<T> line(a, lane);
@@ -89,6 +109,13 @@ __global__ __launch_bounds__(256, (kPerCu<D, FOUR, ONE>)) void weights_kernel(co
     }
   };
 
+  // Where a lane's operand i of q begins.
+  auto q_dim = [&](int i) { return FOUR ? D / 4 * g + 8 * i : 32 * i + 8 * g; };
+  // (16 rows on: hop_n of them in a head, or into the next.)
+  const int hop_n = 16 % a.N;
+  const long long hop = 16 / a.N * (long long)a.stq.h + hop_n * (long long)a.stq.n;
+  const long long hop_next = hop + a.stq.h - a.N * (long long)a.stq.n;
+
   while (pos < end) {
     const int units = line.units(keys), from = pos - start, upto = min(from + end - pos, units);
     const int hkv = item;
@@ -104,77 +131,103 @@ __global__ __launch_bounds__(256, (kPerCu<D, FOUR, ONE>)) void weights_kernel(co
     auto fetch = [&](int j) {
       p0 = max(j * 64, keys.lo) >> a.page_shift;
       held = table[min(p0 + lane, last_page)];
+      asm volatile("" : "+v"(held));  // (waited for here: behind a branch all loads would be)
     };
 
-    // A block as it is loaded: K's rows (of key 16 t + lane % 16 in 16 bits the chunks 4 i + g,
-    // in 4 a quarter of the row and the words of its scales), and the weight of key `lane`.
-    constexpr int kScales = D == 96 || D == 256 ? 2 : 1;
+    // A block as it is loaded: K's rows, the words that hold the scales of key `lane`, from
+    // byte `sub` of the first on, and the weight of that key.
+    constexpr int kWords = D > 128 ? 3 : 2;
     struct Block {
-      u32x4 rows[FOUR ? 1 : 4][FOUR ? 1 : kChunks];
-      uint32_t codes[FOUR ? 4 : 1][kChunks], scale[4][kScales], bit[4][kScales];
+      u32x4 rows[64 / kRowsAtOnce][kLoads];
+      uint32_t words[FOUR ? kWords : 1], sub;
       float before;
       float* at;  // null where the lane has no key of the request
       bool fresh;
     };
+    // (strides are below 2^31)
+    auto place = [](int page, long long page_stride, int row, long long row_stride) {
+      return (uint64_t)(uint32_t)page * (uint32_t)page_stride +
+             (uint64_t)(uint32_t)row * (uint32_t)row_stride;
+    };
+    typedef __attribute__((address_space(1))) const uint32_t Word;
     auto load = [&](Block& x, int j) {
       if ((min(j * 64 + 64, keys.len) - 1) >> a.page_shift > p0 + 63) fetch(j);
       const int key = min(max(j * 64 + lane, keys.lo), keys.len - 1);
       const int page = __shfl(held, (key >> a.page_shift) - p0);
       const bool there = page >= 0 && page < a.pages;
-      const int row = key & page_mask;
-      x.at = there && key == j * 64 + lane ? base_w + (there ? page : 0) * a.weight_page + row * a.weight_row : nullptr;
+      const int row = key & page_mask, my_page = there ? page : 0;
+      x.at = there && key == j * 64 + lane ? base_w + place(page, a.weight_page, row, a.weight_row)
+                                           : nullptr;
       x.fresh = a.restart || key >= keys.len - a.N;
       x.before = x.at && !x.fresh ? *x.at : 0.f;
-      const int my_page = there ? page : 0;
+      if constexpr (FOUR) {
+        // (words that hold a scale of the row: none lies behind the pool)
+        const uint64_t first = (uint64_t)base_s + place(my_page, a.scale_page, row, a.scale_row);
+        const uint64_t from = first & ~3ull, upto = (first + dr / 32 - 1) & ~3ull;
+        x.sub = (uint32_t)first & 3;
+        x.words[0] = *(Word*)from;
+        if constexpr (kWords == 3) x.words[1] = *(Word*)(from + 4 < upto ? from + 4 : upto);
+        x.words[kWords - 1] = *(Word*)upto;
+      }
+      const uint64_t k_at = kUnit * place(my_page, a.page_stride, row, a.row_stride);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int p = __shfl(my_page, 16 * t + l16), r = __shfl(row, 16 * t + l16);
-        const uint8_t* k = base_k + kUnit * (p * a.page_stride + r * a.row_stride);
-        if constexpr (FOUR) {
-          const uint8_t* scales = base_s + p * a.scale_page + r * a.scale_row;
-          const bool begins = FULL || 64 * g < dr, both = FULL || 64 * g + 32 < dr;
-          const uint8_t* q = k + 4 * kChunks * (begins ? g : 0);
-          if constexpr (kChunks < 4) {
-            __builtin_memcpy(x.codes[t], __builtin_assume_aligned(q, 4), 4 * kChunks);
-          } else {
+      for (int t = 0; t < 64 / kRowsAtOnce; ++t) {
+        const int i = t * kRowsAtOnce + lane / kLanes;
+        const uint32_t low = __shfl((uint32_t)k_at, i), high = __shfl((uint32_t)(k_at >> 32), i);
+        const uint8_t* k = base_k + ((uint64_t)high << 32 | low);
 #pragma unroll
-            for (int h = 0; h < kChunks / 4; ++h) {
-              const u32x4 v = *reinterpret_cast<const u32x4*>(q + (both ? 16 * h : 0));
-#pragma unroll
-              for (int i = 0; i < 4; ++i) x.codes[t][4 * h + i] = v[i];
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < kScales; ++i) {
-            const int block = !begins ? 0 : D == 256 ? 2 * g + (both ? i : 0) : (kChunks * g + 2 * i) / 4;
-            const uint8_t* s = scales + block;
-            const uint32_t sub = (uint32_t)((uintptr_t)s & 3);
-            x.bit[t][i] = 8 * sub;
-            x.scale[t][i] = *reinterpret_cast<const uint32_t*>(s - sub);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < kChunks; ++i)
-            x.rows[t][i] = load16(reinterpret_cast<const half_t*>(k) + 32 * i + 8 * g, FULL || 32 * i + 8 * g < dr);
+        for (int e = 0; e < kLoads; ++e) {
+          const int unit = min(4 * e + lane % kLanes, kUnits - 1);
+          const bool is = FULL || (FOUR ? 32 : 8) * unit < dr;
+          // (behind the head dim the first unit again: finite values that meet zeros of q)
+          if constexpr (FOUR)
+            x.rows[t][e] = *reinterpret_cast<const u32x4*>(k + 16 * (is ? unit : 0));
+          else
+            x.rows[t][e] = load16(reinterpret_cast<const half_t*>(k) + 8 * unit, is);
         }
       }
     };
-    // Its operands, a tile at a time (values past the head dim meet zeros of q: finite ones).
+    auto put = [&](u32x4* to, int stride, int row, int e, u32x4 x) {
+      const int unit = 4 * e + lane % kLanes;
+      if (kUnits % kLanes == 0 || unit < kUnits) to[row * stride + unit] = x;
+    };
+    // Its operands: first all of it (in 4 bits), then a tile at a time.
+    auto begin_operands = [&](const Block& x) {
+      if constexpr (FOUR)
+#pragma unroll
+        for (int t = 0; t < 64 / kRowsAtOnce; ++t)
+#pragma unroll
+          for (int e = 0; e < kLoads; ++e)
+            put(stage, kStride, t * kRowsAtOnce + lane / kLanes, e, x.rows[t][e]);
+    };
     auto operands = [&](const Block& x, int t, half8 (&k)[kChunks]) {
       if constexpr (FOUR) {
+        // The scales of the row, then of the lane's quarter of it (of either half where it is
+        // 64 values; in 96 a quarter ends in the next scale's).
+        uint32_t word = __builtin_amdgcn_alignbit(x.words[1], x.words[0], 8 * x.sub);
+        word = __shfl(word, 16 * t + l16);
+        if constexpr (kWords == 3) {
+          const uint32_t high = __builtin_amdgcn_alignbit(x.words[2], x.words[1], 8 * x.sub);
+          const uint32_t second = __shfl(high, 16 * t + l16);
+          word = g < 2 ? word : second;
+        }
         float two[2];
 #pragma unroll
-        for (int i = 0; i < kScales; ++i)
-          two[i] = __uint_as_float(__builtin_amdgcn_alignbit(x.scale[t][i], x.scale[t][i], (x.bit[t][i] + 9u) & 31u));
-        if constexpr (kScales == 1) two[1] = two[0];
-        if constexpr (!FULL) {
-          two[0] = 64 * g < dr ? two[0] : 1.f;
-          two[1] = 64 * g + 32 < dr ? two[1] : 1.f;
+        for (int i = 0; i < 2; ++i) {
+          const int block = D == 256  ? 2 * (g & 1) + i
+                            : D == 96 ? (3 * g + 2 * i) / 4
+                                      : kChunks * g / 4;
+          two[i] = __uint_as_float(__builtin_amdgcn_alignbit(word, word, (8 * block + 9u) & 31u));
+          if constexpr (!FULL) two[i] = 64 * g + 32 * i < dr ? two[i] : 1.f;
         }
+        uint32_t codes[kChunks];
+        const char* const quarter = (const char*)(stage + (16 * t + l16) * kStride) + 4 * kChunks * g;
+        __builtin_memcpy(codes, __builtin_assume_aligned(quarter, 4), 4 * kChunks);
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
-          const float scale = D == 96 ? (i == 0 || (i == 1 && g != 1) ? two[0] : two[1]) : two[D == 256 ? i / 4 : 0];
-          const uint32_t c = x.codes[t][i];
+          const float scale = D == 96 ? (i == 0 || (i == 1 && g != 1) ? two[0] : two[1])
+                                      : two[D == 256 ? i / 4 : 0];
+          const uint32_t c = codes[i];
           k[i] = as_half8(u32x4{
               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0)),
               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1)),
@@ -183,67 +236,61 @@ __global__ __launch_bounds__(256, (kPerCu<D, FOUR, ONE>)) void weights_kernel(co
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) k[i] = as_half8(x.rows[t][i]);
+        for (int e = 0; e < kLoads; ++e) put(stage, kStride, lane / kLanes, e, x.rows[t][e]);
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) k[i] = as_half8(stage[l16 * kStride + 4 * i + g]);
       }
     };
-    // A tile of rows: q of row lane % 16, lse of rows 4 g .. 4 g + 3 (+inf, a weight of 0,
-    // where there is none).
+    // A tile of rows: q, of row lane % 16 (ONE) or as it goes to LDS, and lse of the rows that
+    // the lane has scores of, 4 row_group .. 4 row_group + 3. They go by from the first tile
+    // to the last, and again; lanes behind the last row keep the row they had.
     struct Rows {
-      half8 q[kChunks];
+      u32x4 q[kChunks];
       float lse[4];
     };
+    const int row_group = FEW ? 0 : g;
+    const auto lse_rsrc = make_rsrc(lse_rows, 4u * rows);
+    const int my_row = FEW ? lane % 4 : ONE ? l16 : lane / 4;
+    const half_t* q0;
+    int n0;
+    {
+      int head;
+      split(min(my_row, rows - 1), head, n0);
+      q0 = a.q + b * a.stq.b + (hkv * a.group + head) * a.stq.h + n0 * (long long)a.stq.n;
+    }
+    const half_t* q_at = q0;
+    int n_at = n0;
     auto load_rows = [&](Rows& x, int rt) {
-      int head, n;
-      split(min(16 * rt + l16, rows - 1), head, n);
-      const half_t* q = a.q + b * a.stq.b + (hkv * a.group + head) * a.stq.h + (size_t)n * a.stq.n;
+      if (rt == 0) {
+        q_at = q0;
+        n_at = n0;
+      } else if (16 * rt + my_row < rows) {
+        n_at += hop_n;
+        q_at += n_at >= a.N ? hop_next : hop;
+        n_at -= n_at >= a.N ? a.N : 0;
+      }
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        const int d = FOUR ? D / 4 * g + 8 * i : 32 * i + 8 * g;
-        x.q[i] = as_half8(load16(q + d, FULL || d < dr));
+        const int d = ONE ? q_dim(i) : 32 * i + 8 * (lane % 4);
+        x.q[i] = load16(q_at + d, FULL || d < dr);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x.lse[r] = lse_rows[min(16 * rt + 4 * g + r, rows - 1)];
+      for (int r = 0; r < 4; ++r)
+        x.lse[r] = buf_load_f32(lse_rsrc, 64 * rt + 16 * row_group + 4 * r, 0);
     };
-    const int all_lo = a.hide_window > 0 ? max(0, keys.len - a.hide_window) : 0;
-    const int all_hi = a.causal ? keys.len - a.N + 1 : keys.len;
-    // Adds to acc the weights that rows of tile rt give the keys of tile t.
-    auto weigh = [&](const Rows& x, const half8 (&q)[kQ][kChunks], const half8 (&k)[kChunks], int rt, int j, int t,
-                     float& acc) {
-      floatx4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int y = 0; y < kQ; ++y)
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) s = mfma4<BF || FOUR>(q[y][i], k[i], s);
-      const int key = j * 64 + 16 * t + l16;
-      const bool edge = j * 64 < all_lo || j * 64 + 64 > all_hi || 16 * rt + 16 > rows;
-      // (score - lse first: exact near 0, where the weights are large)
-      float z[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) z[r] = fmaf(s[r], a.scale, -x.lse[r]);
-      if (edge || a.alibi) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * rt + 4 * g + r;
-          int head, n;
-          split(min(row, rows - 1), head, n);
-          const int at = keys.len - a.N + n;
-          if (a.alibi) z[r] = fmaf(-a.alibi[hkv * a.group + head], (float)abs(at - key), z[r]);
-          const int lo = a.hide_window > 0 ? max(0, at - a.hide_window + 1) : 0;
-          const int hi = row >= rows ? 0 : a.causal ? min(keys.len, at + 1) : keys.len;
-          if (key < lo || key >= hi) z[r] = -INFINITY;
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc += fast_exp2(z[r] * kLog2e);
-    };
+    // Its operands.
     auto split_q = [&](const Rows& x, half8 (&q)[kQ][kChunks]) {
+      if constexpr (!ONE)
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) q_stage[lane / 4 * kQStride + 4 * i + lane % 4] = x.q[i];
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        q[0][i] = x.q[i];
+        const half8 both = as_half8(ONE ? x.q[i] : q_stage[l16 * kQStride + q_dim(i) / 8]);
+        q[0][i] = both;
         if constexpr (kQ == 2) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float f = (float)x.q[i][e];
+            const float f = (float)both[e];
             q[0][i][e] = to16<true>(f);
             const float rest = f - from16<true>(q[0][i][e]);
             q[kQ - 1][i][e] = to16<true>(__builtin_isfinite(f) ? rest : 0.f);
@@ -251,15 +298,72 @@ __global__ __launch_bounds__(256, (kPerCu<D, FOUR, ONE>)) void weights_kernel(co
         }
       }
     };
-    auto store = [&](const Block& x, const float (&acc)[4]) {
-      float sum = 0.f;
+    const int all_lo = a.hide_window > 0 ? max(0, keys.len - a.hide_window) : 0;
+    const int all_hi = a.causal ? keys.len - a.N + 1 : keys.len;
+    // What rows score above their lse with the block's keys (tile t, or the lane's own); operands(t,
+    // k): those of key tile t.
+    constexpr int kOwn = FEW ? 1 : 4;
+    auto scores = [&](const Rows& x, const half8 (&q)[kQ][kChunks], floatx4 (&z)[kOwn],
+                      auto&& operands) {
+      floatx4 s[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        float y = acc[t] + __shfl_xor(acc[t], 16);
-        y += xor32(y);
-        sum = g == t ? y : sum;
+        half8 k[kChunks];
+        operands(t, k);
+        s[t] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int y = 0; y < kQ; ++y)
+#pragma unroll
+          for (int i = 0; i < kChunks; ++i) s[t] = mfma4<BF || FOUR>(q[y][i], k[i], s[t]);
       }
-      if (x.at) *x.at = x.before + sum;
+      // (score - lse first: exact near 0, where the weights are large)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (FEW) s[0][r] = g < 2 ? (g == 0 ? s[0][r] : s[1][r]) : g == 2 ? s[2][r] : s[3][r];
+#pragma unroll
+        for (int t = 0; t < kOwn; ++t) z[t][r] = fmaf(s[t][r], a.scale, -x.lse[r]);
+      }
+    };
+    // Adds to acc the weights that they, of tile rt, give the keys.
+    auto weigh = [&](floatx4 (&z)[kOwn], int rt, int j, float (&acc)[kOwn]) {
+      if (j * 64 < all_lo || j * 64 + 64 > all_hi || a.alibi) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          int head, n;
+          split(min(16 * rt + 4 * row_group + r, rows - 1), head, n);
+          const int at = keys.len - a.N + n;
+          const float slope = a.alibi ? a.alibi[hkv * a.group + head] : 0.f;
+          const int lo = a.hide_window > 0 ? max(0, at - a.hide_window + 1) : 0;
+          const int hi = a.causal ? min(keys.len, at + 1) : keys.len;
+#pragma unroll
+          for (int t = 0; t < kOwn; ++t) {
+            const int key = j * 64 + (FEW ? lane : 16 * t + l16);
+            const float biased = fmaf(-slope, (float)abs(at - key), z[t][r]);
+            z[t][r] = key < lo || key >= hi ? -INFINITY : a.alibi ? biased : z[t][r];
+          }
+        }
+      }
+      if (16 * rt + (FEW ? 4 : 16) > rows)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int t = 0; t < kOwn; ++t)
+            z[t][r] = 16 * rt + 4 * row_group + r < rows ? z[t][r] : -INFINITY;
+#pragma unroll
+      for (int t = 0; t < kOwn; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[t] += fast_exp2(z[t][r] * kLog2e);
+    };
+    auto store = [&](float* at, float before, const float (&acc)[kOwn]) {
+      float sum = acc[0];
+      if constexpr (!FEW)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          float y = acc[t] + __shfl_xor(acc[t], 16);
+          y += xor32(y);
+          sum = g == t ? y : sum;
+        }
+      if (at) *at = before + sum;
     };
 
     if (j0 < j1) {
@@ -276,41 +380,51 @@ __global__ __launch_bounds__(256, (kPerCu<D, FOUR, ONE>)) void weights_kernel(co
           // of them waited for)
           Block next;
           if constexpr (FOUR) load(next, min(j + 1, j1 - 1));
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            half8 k[kChunks];
-            operands(x, t, k);
-            weigh(now, q, k, 0, j, t, acc[t]);
-          }
-          if constexpr (FOUR) {
-            store(x, acc);
+          float acc[kOwn] = {};
+          floatx4 z[kOwn];
+          begin_operands(x);
+          scores(now, q, z, [&](int t, half8 (&k)[kChunks]) { operands(x, t, k); });
+          weigh(z, 0, j, acc);
+          float* const at = x.at;
+          const float before = x.before;
+          // (the next block is waited for ahead of the store, which it would wait for too)
+          if constexpr (FOUR)
             x = next;
-          } else {
-            const Block old = x;
-            if (j + 1 < j1) load(x, j + 1);
-            store(old, acc);
-          }
+          else if (j + 1 < j1)
+            load(x, j + 1);
+          store(at, before, acc);
         }
       } else {
+        // Two tiles of rows by turns: one is loaded while the other is multiplied, the first
+        // again for the next block. (The next block's keys are not: what the rows wait for
+        // would wait for those too, 31 us instead of 27.)
+        Rows even, odd;
+        load_rows(even, 0);
         for (int j = j0; j < j1; ++j) {
           Block x;
-          Rows now, next;
           load(x, j);
-          load_rows(now, 0);
+          begin_operands(x);
           half8 k[4][kChunks];
 #pragma unroll
           for (int t = 0; t < 4; ++t) operands(x, t, k[t]);
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int rt = 0; rt < row_tiles; ++rt) {
-            load_rows(next, min(rt + 1, row_tiles - 1));
+          float acc[kOwn] = {};
+          auto tile = [&](const Rows& rows, int rt) {
             half8 q[kQ][kChunks];
-            split_q(now, q);
+            split_q(rows, q);
+            floatx4 z[kOwn];
+            scores(rows, q, z, [&](int t, half8 (&tile)[kChunks]) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) weigh(now, q, k[t], rt, j, t, acc[t]);
-            now = next;
+              for (int i = 0; i < kChunks; ++i) tile[i] = k[t][i];
+            });
+            weigh(z, rt, j, acc);
+          };
+          for (int rt = 0; rt < row_tiles; rt += 2) {
+            load_rows(odd, rt + 1);
+            tile(even, rt);
+            load_rows(even, rt + 2 < row_tiles ? rt + 2 : 0);
+            if (rt + 1 < row_tiles) tile(odd, rt + 1);
           }
-          store(x, acc);
+          store(x.at, x.before, acc);
         }
       }
     }
@@ -327,7 +441,8 @@ __global__ __launch_bounds__(256, (kPerCu<D, FOUR, ONE>)) void weights_kernel(co
 }  // namespace
 
 template <>
-hipError_t launch_paged_weights_w<FA_WIDTH, FA_BF>(const PagedArgs& a, const KeyWeights& w, bool restart) {
+hipError_t launch_paged_weights_w<FA_WIDTH, FA_BF>(const PagedArgs& a, const KeyWeights& w,
+                                                   bool restart) {
   WeighArgs d{};
   paged_args<Weigh<FA_WIDTH, FA_BF, 1>>(d, a);
   d.n_groups = 1;
@@ -344,16 +459,19 @@ hipError_t launch_paged_weights_w<FA_WIDTH, FA_BF>(const PagedArgs& a, const Key
   d.hide_window = d.window;
   if (restart) d.window = 0;
   d.restart = restart;
-  auto launch = [&](auto four, auto full, auto one) {
-    constexpr bool kFour = decltype(four)::value, kFull = decltype(full)::value, kOne = decltype(one)::value;
-    using T = Weigh<FA_WIDTH, FA_BF, kPerCu<FA_WIDTH, kFour, kOne>>;
-    hipLaunchKernelGGL((weights_kernel<FA_WIDTH, FA_BF, kFour, kFull, kOne>), dim3(T::kGrid), dim3(T::kThreads), 0,
-                       (hipStream_t)a.stream, d);
+  auto launch = [&](auto four, auto full, auto one, auto few) {
+    constexpr bool kFour = decltype(four)::value, kFull = decltype(full)::value;
+    constexpr bool kOne = decltype(one)::value, kFew = decltype(few)::value;
+    using T = Weigh<FA_WIDTH, FA_BF, kPerCu<FA_WIDTH, kFour, kOne, kFew>>;
+    hipLaunchKernelGGL((weights_kernel<FA_WIDTH, FA_BF, kFour, kFull, kOne, kFew>), dim3(T::kGrid),
+                       dim3(T::kThreads), 0, (hipStream_t)a.stream, d);
     return hipGetLastError();
   };
   using std::false_type, std::true_type;
   auto by_rows = [&](auto four, auto full) {
-    return d.group * d.N <= 16 ? launch(four, full, true_type{}) : launch(four, full, false_type{});
+    if (d.group * d.N <= 4) return launch(four, full, true_type{}, true_type{});
+    return d.group * d.N <= 16 ? launch(four, full, true_type{}, false_type{})
+                               : launch(four, full, false_type{}, false_type{});
   };
   // (4-bit rows are whole blocks of 32: of the widths, 256 alone serves narrower ones)
   const bool full = a.D == FA_WIDTH;
