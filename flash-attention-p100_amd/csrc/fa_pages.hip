@@ -262,15 +262,6 @@ __device__ __forceinline__ uint32_t to_codes(u32x4 x, float scale) {
 template <bool BF>
 constexpr uint32_t kTopScale = BF ? 127 + 125 : 127 + 13;
 
-// A row's slot, or none: page < 0.
-struct Slot {
-  int page, row;
-  __device__ __forceinline__ Slot(int slot, int shift, int pages)
-      : page(slot >> shift), row(slot - (page << shift)) {
-    if (page >= pages) page = -1;
-  }
-};
-
 struct RowsArgs {
   const half_t* from[2];  // dense rows: k and v, their strides
   half_t* into[2];
@@ -278,28 +269,90 @@ struct RowsArgs {
   uint8_t* codes[2];  // the pools, and their scales (16-bit rows: none)
   uint8_t* scales[2];
   const int* slots;
-  long long page_stride, head_stride, row_stride;  // of the pools, in bytes
-  long long scale_page, scale_head, scale_row;
+  uint32_t page_stride, row_stride, scale_page, scale_row;  // in bytes
+  long long head_stride, scale_head;
   int pages, page_shift;
+  uint32_t tokens;
   int N, row_chunks, chunks;  // 16-byte chunks of a dense row, and of a token's heads
-  long long items;            // tokens * chunks
+  int width, per;             // chunks of a token, and tokens, that a workgroup takes at once
+  int step, step_n;           // a thread's next token, and by how many rows in its request
+  long long hop[2], hop_next[2];  // as far in the dense rows: within a request, to the next
 };
 
-template <bool BF, class Index>
-__global__ __launch_bounds__(kAppThreads) void append4_kernel(const RowsArgs a) {
-  const int v = blockIdx.x & 1;
-  const half_t* const from = v ? a.from[1] : a.from[0];
+// The chunk of a token that a thread moves.
+struct Chunk {
+  int v, h, c;
+};
+// A token's place in the pools, or none: page < 0.
+struct Place {
+  int page, row;
+  __device__ __forceinline__ Place() {}
+  __device__ __forceinline__ Place(const RowsArgs& a, uint32_t t) {
+    const int slot = a.slots[min(t, a.tokens - 1)];
+    page = slot >> a.page_shift;
+    row = slot - (page << a.page_shift);
+    if (t >= a.tokens || page >= a.pages) page = -1;
+  }
+  __device__ __forceinline__ uint64_t in_pool(const RowsArgs& a) const {
+    return (uint64_t)(uint32_t)page * a.page_stride + (uint64_t)(uint32_t)row * a.row_stride;
+  }
+  __device__ __forceinline__ uint64_t in_scales(const RowsArgs& a) const {
+    return (uint64_t)(uint32_t)page * a.scale_page + (uint64_t)(uint32_t)row * a.scale_row;
+  }
+};
+
+// Goes over the chunks: a thread keeps its place within the tokens and goes from token to
+// token, COUNT at a time, so that it divides once. load(chunk, place, dense offset) for all
+// of them (any token's where theirs is missing), then done(chunk, place, dense offset, what
+// was loaded). Both directions are bound by HBM: 65536 tokens of 8 heads of 128 are written
+// in 65 us and read back in 56 (340 MB each), with a chunk to a thread, found by division
+// (150 instructions each, and bound by them), 94 each, and without the streaming hint for
+// the dense rows 77 and 70.
+template <int COUNT, class Load, class Done>
+__device__ __forceinline__ void each_chunk(const RowsArgs& a, Load&& load, Done&& done) {
+  const int v = blockIdx.x & 1, sub = threadIdx.x / a.width;
+  const int x = blockIdx.y * kAppThreads + (int)threadIdx.x - sub * a.width;
+  if (sub >= a.per || x >= a.chunks) return;
+  const int h = x / a.row_chunks;
+  const Chunk chunk{v, h, x - h * a.row_chunks};
   const RowStrides s = v ? a.strides[1] : a.strides[0];
-  uint8_t* const codes = v ? a.codes[1] : a.codes[0];
-  uint8_t* const scales = v ? a.scales[1] : a.scales[0];
-  const Index step = (Index)(gridDim.x / 2) * kAppThreads, items = (Index)a.items;
-  for (Index i = (Index)(blockIdx.x / 2) * kAppThreads + threadIdx.x; i < items; i += step) {
-    const int t = (int)(i / (Index)a.chunks), x = (int)(i - (Index)t * a.chunks);
-    const Slot at(a.slots[t], a.page_shift, a.pages);
-    if (at.page < 0) continue;  // (all four lanes of a block: one row)
-    const int h = x / a.row_chunks, c = x - h * a.row_chunks;
-    const int b = a.N == 1 ? t : t / a.N, n = t - b * a.N;
-    const u32x4 in = *reinterpret_cast<const u32x4*>(from + b * s.b + n * s.n + h * s.h + 8 * c);
+  const long long hop = v ? a.hop[1] : a.hop[0], hop_next = v ? a.hop_next[1] : a.hop_next[0];
+  uint32_t t = (blockIdx.x >> 1) * a.per + sub;
+  if (t >= a.tokens) return;
+  const int b = t / a.N;
+  int n = t - b * a.N;
+  long long at = b * s.b + n * s.n + h * s.h + 8 * chunk.c;
+  for (; t < a.tokens; t += COUNT * a.step) {
+    Place places[COUNT];
+    long long dense[COUNT];
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) {
+      places[e] = Place(a, t + e * a.step);
+      dense[e] = t + e * a.step < a.tokens ? at : dense[0];
+      n += a.step_n;
+      at += n >= a.N ? hop_next : hop;
+      n -= n >= a.N ? a.N : 0;
+    }
+    decltype(load(chunk, places[0], at)) x[COUNT];
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) x[e] = load(chunk, places[e], dense[e]);
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e)
+      if (t + e * a.step < a.tokens) done(chunk, places[e], dense[e], x[e]);
+  }
+}
+
+template <bool BF, int COUNT>
+__global__ __launch_bounds__(kAppThreads) void append4_kernel(const RowsArgs a) {
+  const half_t* const from = blockIdx.x & 1 ? a.from[1] : a.from[0];
+  uint8_t* const codes = blockIdx.x & 1 ? a.codes[1] : a.codes[0];
+  uint8_t* const scales = blockIdx.x & 1 ? a.scales[1] : a.scales[0];
+  auto load = [&](const Chunk&, const Place&, long long dense) {
+    const u32x4* const at = reinterpret_cast<const u32x4*>(from + dense);
+    return COUNT > 1 ? __builtin_nontemporal_load(at) : *at;
+  };
+  auto done = [&](const Chunk& x, const Place& at, long long, u32x4 in) {
+    if (at.page < 0) return;  // (all four lanes of a block: one row)
     // (magnitudes of 16 bits are in the order of their bits)
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     u16x2 m = {0, 0};
@@ -318,52 +371,57 @@ __global__ __launch_bounds__(kAppThreads) void append4_kernel(const RowsArgs a) 
       e = 255;
       out = 0;
     }
-    *reinterpret_cast<uint32_t*>(codes + at.page * a.page_stride + h * a.head_stride +
-                                 at.row * a.row_stride + 4 * c) = out;
-    if ((c & 3) == 0)
-      scales[at.page * a.scale_page + h * a.scale_head + at.row * a.scale_row + (c >> 2)] = (uint8_t)e;
-  }
+    *reinterpret_cast<uint32_t*>(codes + at.in_pool(a) + x.h * a.head_stride + 4 * x.c) = out;
+    if ((x.c & 3) == 0) scales[at.in_scales(a) + x.h * a.scale_head + (x.c >> 2)] = (uint8_t)e;
+  };
+  each_chunk<COUNT>(a, load, done);
 }
 
 // ---------------------------------------------------------------------------
 // Rows back from their slots, dense: 16-bit ones as they are, 4-bit ones as the values
 // that they stand for, exact in bf16 and rounded to nearest even in fp16. Rows without a
 // slot are zeros. FOUR: the cache is in 4 bits.
-template <bool BF, bool FOUR, class Index>
+template <bool BF, bool FOUR, int COUNT>
 __global__ __launch_bounds__(kAppThreads) void gather_kernel(const RowsArgs a) {
-  const int v = blockIdx.x & 1;
-  half_t* const into = v ? a.into[1] : a.into[0];
-  const RowStrides s = v ? a.strides[1] : a.strides[0];
-  const uint8_t* const codes = v ? a.codes[1] : a.codes[0];
-  const uint8_t* const scales = v ? a.scales[1] : a.scales[0];
-  const Index step = (Index)(gridDim.x / 2) * kAppThreads, items = (Index)a.items;
-  for (Index i = (Index)(blockIdx.x / 2) * kAppThreads + threadIdx.x; i < items; i += step) {
-    const int t = (int)(i / (Index)a.chunks), x = (int)(i - (Index)t * a.chunks);
-    const Slot at(a.slots[t], a.page_shift, a.pages);
-    const int h = x / a.row_chunks, c = x - h * a.row_chunks;
-    const int b = a.N == 1 ? t : t / a.N, n = t - b * a.N;
-    u32x4 out = {0u, 0u, 0u, 0u};
-    if (at.page >= 0) {
-      const uint8_t* const row = codes + at.page * a.page_stride + h * a.head_stride + at.row * a.row_stride;
-      if constexpr (FOUR) {
-        const uint32_t x = *reinterpret_cast<const uint32_t*>(row + 4 * c);
-        const float scale = __uint_as_float(
-            (uint32_t)scales[at.page * a.scale_page + h * a.scale_head + at.row * a.scale_row + (c >> 2)] << 23);
-        auto two = [&](auto sel) {
-          if constexpr (BF)
-            return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, decltype(sel)::value));
-          const auto f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, scale, decltype(sel)::value);
-          typedef _Float16 v2 __attribute__((ext_vector_type(2)));
-          return __builtin_bit_cast(uint32_t, v2{(_Float16)f[0], (_Float16)f[1]});
-        };
-        out = u32x4{two(std::integral_constant<int, 0>{}), two(std::integral_constant<int, 1>{}),
-                    two(std::integral_constant<int, 2>{}), two(std::integral_constant<int, 3>{})};
-      } else {
-        out = *reinterpret_cast<const u32x4*>(row + 16 * c);
-      }
+  half_t* const into = blockIdx.x & 1 ? a.into[1] : a.into[0];
+  const uint8_t* const codes = blockIdx.x & 1 ? a.codes[1] : a.codes[0];
+  const uint8_t* const scales = blockIdx.x & 1 ? a.scales[1] : a.scales[0];
+  struct Cached {
+    u32x4 x;
+    uint32_t scale;
+  };
+  auto load = [&](const Chunk& x, Place at, long long) {
+    if (at.page < 0) at.page = at.row = 0;
+    const uint8_t* const row = codes + at.in_pool(a) + x.h * a.head_stride;
+    if constexpr (FOUR)
+      return Cached{{*reinterpret_cast<const uint32_t*>(row + 4 * x.c), 0u, 0u, 0u},
+                    scales[at.in_scales(a) + x.h * a.scale_head + (x.c >> 2)]};
+    else
+      return Cached{*reinterpret_cast<const u32x4*>(row + 16 * x.c), 0u};
+  };
+  auto done = [&](const Chunk&, const Place& at, long long dense, const Cached& in) {
+    u32x4 out = in.x;
+    if constexpr (FOUR) {
+      const uint32_t x = in.x[0];
+      const float scale = __uint_as_float(in.scale << 23);
+      auto two = [&](auto sel) {
+        if constexpr (BF)
+          return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, decltype(sel)::value));
+        const auto f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, scale, decltype(sel)::value);
+        typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, v2{(_Float16)f[0], (_Float16)f[1]});
+      };
+      out = u32x4{two(std::integral_constant<int, 0>{}), two(std::integral_constant<int, 1>{}),
+                  two(std::integral_constant<int, 2>{}), two(std::integral_constant<int, 3>{})};
     }
-    *reinterpret_cast<u32x4*>(into + b * s.b + n * s.n + h * s.h + 8 * c) = out;
-  }
+    if (at.page < 0) out = u32x4{0u, 0u, 0u, 0u};
+    u32x4* const to = reinterpret_cast<u32x4*>(into + dense);
+    if constexpr (COUNT > 1)
+      __builtin_nontemporal_store(out, to);
+    else
+      *to = out;
+  };
+  each_chunk<COUNT>(a, load, done);
 }
 
 RowsArgs rows_args(RowStrides sk, RowStrides sv, const int* slots, const PagedPool& pool,
@@ -374,28 +432,48 @@ RowsArgs rows_args(RowStrides sk, RowStrides sv, const int* slots, const PagedPo
   a.codes[0] = (uint8_t*)pool.k;
   a.codes[1] = (uint8_t*)pool.v;
   const int unit = scales ? 1 : 2;  // (16-bit pools' strides count elements)
-  a.page_stride = unit * pool.page_stride;
+  a.page_stride = (uint32_t)(unit * pool.page_stride);
   a.head_stride = unit * pool.head_stride;
-  a.row_stride = unit * pool.row_stride;
+  a.row_stride = (uint32_t)(unit * pool.row_stride);
   if (scales) {
     a.scales[0] = scales->k;
     a.scales[1] = scales->v;
-    a.scale_page = scales->page_stride;
+    a.scale_page = (uint32_t)scales->page_stride;
     a.scale_head = scales->head_stride;
-    a.scale_row = scales->row_stride;
+    a.scale_row = (uint32_t)scales->row_stride;
   }
   a.slots = slots;
   a.pages = pool.pages;
   a.page_shift = pool.page_shift;
+  a.tokens = (uint32_t)B * N;
   a.N = N;
   a.row_chunks = D / 8;
   a.chunks = Hkv * a.row_chunks;
-  a.items = (long long)B * N * a.chunks;
+  a.width = std::min(a.chunks, kAppThreads);
+  a.per = kAppThreads / a.width;
   return a;
 }
 
-unsigned rows_blocks(const RowsArgs& a) {
-  return 2 * (unsigned)std::min((a.items + kAppThreads - 1) / kAppThreads, 1LL << 20);
+// Launches kernel_of(COUNT): several chunks to a thread where the card is full (kRowsPerCu
+// workgroups to a CU; with 8 the calls above take 67 and 59 us, with 64 74 and 53).
+constexpr int kRowsPerCu = 16;
+template <class KernelOf>
+hipError_t launch_rows(RowsArgs& a, const KernelOf& kernel_of, void* stream) {
+  const unsigned slices = (unsigned)((a.chunks + kAppThreads - 1) / kAppThreads);
+  const unsigned all = (a.tokens + a.per - 1) / a.per;
+  const unsigned most = std::max(1u, (unsigned)(kRowsPerCu * kCUs) / (2 * slices));
+  const unsigned blocks = std::min(all, most);
+  a.step = (int)blocks * a.per;
+  const long long step_b = a.step / a.N;
+  a.step_n = a.step % a.N;
+  for (int v = 0; v < 2; ++v) {
+    a.hop[v] = step_b * a.strides[v].b + a.step_n * a.strides[v].n;
+    a.hop_next[v] = a.hop[v] + a.strides[v].b - a.N * a.strides[v].n;
+  }
+  const auto kernel = all > most ? kernel_of(std::integral_constant<int, 4>{})
+                                 : kernel_of(std::integral_constant<int, 1>{});
+  hipLaunchKernelGGL(kernel, dim3(2 * blocks, slices), dim3(kAppThreads), 0, (hipStream_t)stream, a);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -406,11 +484,8 @@ hipError_t launch_paged4_append(const void* k, const void* v, RowStrides sk, Row
   RowsArgs a = rows_args(sk, sv, slots, pool, &scales, B, N, Hkv, D);
   a.from[0] = (const half_t*)k;
   a.from[1] = (const half_t*)v;
-  const bool wide = a.items > 1LL << 31;
-  const auto kernel = dtype == kBF16 ? (wide ? append4_kernel<true, uint64_t> : append4_kernel<true, uint32_t>)
-                                     : (wide ? append4_kernel<false, uint64_t> : append4_kernel<false, uint32_t>);
-  hipLaunchKernelGGL(kernel, dim3(rows_blocks(a)), dim3(kAppThreads), 0, (hipStream_t)stream, a);
-  return hipGetLastError();
+  return launch_rows(
+      a, [&](auto n) { return dtype == kBF16 ? append4_kernel<true, n()> : append4_kernel<false, n()>; }, stream);
 }
 
 hipError_t launch_paged_gather(void* k, void* v, RowStrides strides, const int* slots,
@@ -419,13 +494,14 @@ hipError_t launch_paged_gather(void* k, void* v, RowStrides strides, const int* 
   RowsArgs a = rows_args(strides, strides, slots, pool, scales, B, N, Hkv, D);
   a.into[0] = (half_t*)k;
   a.into[1] = (half_t*)v;
-  const bool wide = a.items > 1LL << 31;
-  const auto kernel =
-      !scales           ? (wide ? gather_kernel<true, false, uint64_t> : gather_kernel<true, false, uint32_t>)
-      : dtype == kBF16 ? (wide ? gather_kernel<true, true, uint64_t> : gather_kernel<true, true, uint32_t>)
-                        : (wide ? gather_kernel<false, true, uint64_t> : gather_kernel<false, true, uint32_t>);
-  hipLaunchKernelGGL(kernel, dim3(rows_blocks(a)), dim3(kAppThreads), 0, (hipStream_t)stream, a);
-  return hipGetLastError();
+  return launch_rows(
+      a,
+      [&](auto n) {
+        return !scales          ? gather_kernel<true, false, n()>
+               : dtype == kBF16 ? gather_kernel<true, true, n()>
+                                : gather_kernel<false, true, n()>;
+      },
+      stream);
 }
 
 hipError_t launch_paged_tables(const TablesArgs& a, void* stream) {
