@@ -5,7 +5,7 @@
 //
 // As in fa_paged.hip the key blocks of all requests lie on one line that the waves
 // divide evenly, and the parts of an item meet in LDS and in paged_merge_kernel. A
-// wave's step is a block of 32 or 64 keys for RT tiles of 16 query rows, on
+// wave's step is a block of 64 keys for RT tiles of 16 query rows, on
 // v_mfma_f32_16x16x32_bf16: S^T = K Q^T, then O^T += V^T P^T. Every value of the cache is
 // exact in bf16 (a sign, two bits and an exponent), whatever q's format, and
 // v_cvt_scalef32_pk_bf16_fp4 makes two of them from a byte, scale included:
@@ -14,7 +14,18 @@
 //   * V: the second product runs over keys, so the values are written to LDS as bf16 and
 //     come back transposed (ds_read_b64_tr_b16).
 // q in fp16 has 11 bits: two bf16 numbers, exactly, and two products. The probabilities
-// are two bf16 numbers (off by 2^-16), two products too.
+// are two bf16 numbers (off by 2^-16), two products too. Sums of the rows are taken of the
+// fp32 weights (by the matrix unit, of the rounded ones, the lse was off by 2^-9).
+//
+// Bound: HBM. 64 requests of 3300 to 16384 tokens, H=32/8 D=128 N=1 (684 MB): 116 us, 5.9
+// TB/s, where the loads alone take 110, and 5 to join the parts. That took blocks loaded
+// ahead of the one that is multiplied, at places held in scalar registers, with scales as
+// whole words (145 us before: bytes are widened, and so waited for, at once); 16 waves of 32
+// keys, with half the LDS each, took 124. Short lines are bound by latency: 3.5 us until a
+// wave's first keys are there, then a block in 2.5 us (16 requests of 800 to 8192: 23 us,
+// five blocks at most to a wave, 12 for their 77 MB alone; one of 1021: 6.6, and 3.4 to
+// join). One conversion of a block serves two row tiles; four, with their sums, do not fit
+// into registers (N=16 H=32/8: 186 us against 59).
 #include "fa_paged.h"
 
 namespace fa {
@@ -33,7 +44,7 @@ struct Paged4 {
   static constexpr float kPUnit = 1.f, kPRescale = kRescaleLog2;
   static constexpr int kBlocks = DIM / 32;  // of a row, each with its scale
   static constexpr int kQ = OUT_BF ? 1 : 2;  // bf16 operands of q
-    // LDS rows of V: eight 16-byte chunks in a row of keys, two of each, lie in 16 bank
+  // LDS rows of V: eight 16-byte chunks in a row of keys, two of each, lie in 16 bank
   // groups (the row's chunks are 2 more than a multiple of 4).
   static constexpr int kStride = 2 * DIM + 32;
   static constexpr int kTileBytes = kKeys * kStride;
@@ -349,26 +360,24 @@ __global__ __launch_bounds__(T::kThreads) void paged4_kernel(const Paged4Args a)
         }
       }
       load_both(j0, true);
-      {
-        // (q is waited for here, behind the loads of K and V: left to its first use, in the loop,
-        // it would be waited for there, and with it all loads of every block)
+      // (q is waited for here, behind the loads of K and V: left to its first use, in the loop,
+      // it would be waited for there, and with it all loads of every block)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int i = 0; i < kDwords; ++i) {
-            asm volatile("" : "+v"(q[rt][0][i]));
-            if constexpr (!T::kBF) {
-              const half8 x = q[rt][0][i];
+        for (int i = 0; i < kDwords; ++i) {
+          asm volatile("" : "+v"(q[rt][0][i]));
+          if constexpr (!T::kBF) {
+            const half8 x = q[rt][0][i];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float f = (float)x[e];
-                q[rt][0][i][e] = to16<true>(f);
-                const float rest = f - from16<true>(q[rt][0][i][e]);
-                q[rt][T::kQ - 1][i][e] = to16<true>(__builtin_isfinite(f) ? rest : 0.f);
-              }
+            for (int e = 0; e < 8; ++e) {
+              const float f = (float)x[e];
+              q[rt][0][i][e] = to16<true>(f);
+              const float rest = f - from16<true>(q[rt][0][i][e]);
+              q[rt][T::kQ - 1][i][e] = to16<true>(__builtin_isfinite(f) ? rest : 0.f);
             }
           }
-      }
+        }
       const int at0 = keys.len - qa.N, window = qa.window;
       const int all_lo = window > 0 ? max(0, keys.len - window) : 0;
       const int all_hi = qa.causal ? at0 + 1 : keys.len;
