@@ -146,8 +146,8 @@ __device__ __forceinline__ void select(const EvictArgs& a, const Budget& q, int 
   }
 
   // The kept-th largest key: its high bits so far, and how many of the keys that agree with
-  // them stay.
-  uint32_t high = 0;
+  // them stay. (None does where nothing is kept.)
+  uint32_t high = q.kept > 0 ? 0u : kNewest;
   int left = q.kept;
   const u32x4 zeros = {0u, 0u, 0u, 0u};
   if (left > 0) {

@@ -320,7 +320,8 @@ __device__ __forceinline__ void each_chunk(const RowsArgs& a, Load&& load, Done&
   uint32_t t = (blockIdx.x >> 1) * a.per + sub;
   if (t >= a.tokens) return;
   const int b = t / a.N;
-  int n = t - b * a.N;
+  const uint32_t N = (uint32_t)a.N;
+  uint32_t n = t - (uint32_t)b * N;
   long long at = b * s.b + n * s.n + h * s.h + 8 * chunk.c;
   for (; t < a.tokens; t += COUNT * a.step) {
     Place places[COUNT];
@@ -330,8 +331,8 @@ __device__ __forceinline__ void each_chunk(const RowsArgs& a, Load&& load, Done&
       places[e] = Place(a, t + e * a.step);
       dense[e] = t + e * a.step < a.tokens ? at : dense[0];
       n += a.step_n;
-      at += n >= a.N ? hop_next : hop;
-      n -= n >= a.N ? a.N : 0;
+      at += n >= N ? hop_next : hop;
+      n -= n >= N ? N : 0;
     }
     decltype(load(chunk, places[0], at)) x[COUNT];
 #pragma unroll

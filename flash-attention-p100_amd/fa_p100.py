@@ -656,7 +656,8 @@ def paged_weights(q, k_cache, block_table, kv_len, lse, weights, causal=True, sl
     of its kv head is added to it. The keys of the newest N tokens themselves, which no
     earlier row saw, get that sum instead of what their slots held before; with restart
     all of a request's keys do (a prompt judged by its last rows), those that no row sees
-    0. Rows with lse = +inf add nothing; other slots keep their values.
+    0. Rows with lse = +inf add nothing; other slots keep their values. A page is one
+    request's: requests that share one would add to its weights at the same time.
 
     One HIP kernel that reads K once, after or instead of any number of calls: weights may
     be scaled or cleared in between. Scores, weights and sums are fp32, results
@@ -676,9 +677,9 @@ def paged_evict(k_cache, v_cache, weights, block_table, kv_len, max_len, recent=
 
     Where kv_len[b] exceeds max_len[b] (int32 (B,), or one int for all), each kv head
     keeps its newest min(recent, max_len[b]) tokens and, of the others, those of the
-    largest weights (paged_weights; of equal ones the older, NaN above all). They move to the front of the
-    request's pages, in their order, with their weights and, in a cache of 4 bits, scales;
-    the rows behind them keep what they held. The pages they no longer need go back with
+    largest weights (paged_weights; of equal ones the older, NaN above all). They move to
+    the front of the request's pages, in their order, with their weights and, in a cache of
+    4 bits, scales; the rows behind them keep what they held. The pages they no longer need go back with
     paged_tables(block_table, kv_len, new_len, free_pages, ring, page_size, max_new=0).
 
     Kept tokens then differ between kv heads, and a key's index no longer is its position:

@@ -605,7 +605,8 @@ int fa_paged4_attn(const void* q, void* o, float* lse, const fa_paged_cache* cac
  * Hq, N) what that call wrote for them (rows with lse = +inf add nothing). scales NULL: the
  * cache is of 16 bits, in q's format; else of 4 (of scales, k alone). weights is fp32, that
  * of (page, kv head, row) at page * w_stride_page + head * w_stride_head + row *
- * w_stride_row (strides in elements, not negative); no two of them share a place. The keys
+ * w_stride_row (strides in elements, not negative, those of pages and rows below 2^31); no
+ * two of them share a place, and a page is one request's. The keys
  * of the newest N tokens, which no earlier row saw, get the sum, those before it have it
  * added to what they hold; with `restart` all of the request's keys get it, those that no
  * row sees 0. Other weights keep their values. Each is a sum in fp32 in an order of its
@@ -622,7 +623,8 @@ int fa_paged_weights(const void* q, const float* lse, const fa_paged_cache* cach
  * largest weights (of equal ones the older; NaN above all, keys in pages outside the pool
  * below all). What is kept moves to the front of the request's pages in its order, rows,
  * scales and weights alike (places in pages outside the pool are left out); rows behind it
- * keep what they hold. new_len[b] becomes min(kv_len[b], max_len[b]); a call of
+ * keep what they hold. new_len[b], not in kv_len's place, becomes min(kv_len[b],
+ * max_len[b]); a call of
  * fa_paged_tables with these as new lengths gives the pages back. Tokens of different kv
  * heads in a row of the pool then differ, and a key's row no longer says its position: what
  * counts distances (windows, ALiBi) counts kept tokens. scales NULL: rows of 16 bits, else

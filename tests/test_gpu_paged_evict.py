@@ -224,6 +224,17 @@ def test_evict_orders_every_kind_of_weight():
     check_evict(arrays, w, table, lens, 100, 10)
 
 
+@pytest.mark.parametrize("four", [True, False])
+def test_evict_of_all_with_any_workspace(four):
+    """Nothing is kept, and what the workspace held does not matter."""
+    lens = [300, 40000, 1]
+    case = evict_case(four, 3, 2, 64, 16, lens, 4)
+    size = 3 * 2 * (case[2].size(1) * 16 + 2)
+    for junk in (0, 2 ** 20, -2 ** 20):
+        torch.full((size,), junk, dtype=torch.int32, device=DEV)  # (freed, and allocated again)
+        check_evict(*case, lens, 0, 5)
+
+
 def test_evict_with_pages_outside_the_pool():
     """Their tokens are the lightest, and nothing is read or written there."""
     lens = [200, 64]

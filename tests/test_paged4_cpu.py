@@ -136,6 +136,7 @@ def test_weights_refusals():
         assert call(**bad) == 10019, bad
     assert call(D=80) == 10001 and call(Hkv=3) == 10003 and call(B=0) == 10004 and call(N=0) == 10002
     assert call(four=False, D=60) == 10001 and call(four=False, strides=(32, 16, 0)) == 10019
+    assert call(strides=(1 << 31, 16, 1)) == 10007 and call(strides=(1, 1 << 20, 1 << 31)) == 10007
 
 
 def test_evict_refusals():
@@ -152,7 +153,8 @@ def test_evict_refusals():
         assert call(**bad) == 10005, bad
     for bad in (dict(strides=(32, 16, 0)), dict(recent=-1), dict(ws=18), dict(c=cache4(table_width=0)),
                 dict(c=cache4(stride_row=16)), dict(s=scales(stride_row=1)),
-                dict(c=cache4(v=(1 << 24) + 32))):
+                dict(c=cache4(v=(1 << 24) + 32)), dict(c=cache4(kv_len=1 << 26), new=1 << 26),
+                dict(c=cache4(kv_len=1 << 26), new=(1 << 26) + 4, B=2)):
         assert call(**bad) == 10019, bad
     assert call(four=False, c=cache(v=1 << 25, stride_row=32)) == 10019
     assert call(D=72) == 10001 and call(Hkv=0) == 10003 and call(B=0) == 10004
