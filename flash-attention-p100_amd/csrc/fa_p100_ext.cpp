@@ -17,7 +17,9 @@
 // sequences' bounds, and flash_attn is the autograd Function over these entries
 // for the calls that need no packed mask, dropout, bias or block lists.
 // paged_tables, paged_append and paged_attn are a serving step over a paged
-// key/value cache, without gradients.
+// key/value cache of 16 or 4 bits, paged_gather reads rows of it back, and
+// paged_weights and paged_evict cut it to its newest and heaviest keys; all
+// without gradients.
 //
 // Plain C++ (no device code): every launch goes through the C ABI of
 // libfa_mi355x.so (include/fa_mi355x.h). Unlike the reference, which uses the

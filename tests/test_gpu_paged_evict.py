@@ -67,7 +67,8 @@ LENGTHS = [1, 63, 64, 65, 0, 700, 129, 17]
 
 @pytest.mark.parametrize("restart", [False, True])
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
-@pytest.mark.parametrize("Hq,Hkv,N", [(4, 4, 1), (8, 1, 1), (6, 2, 5), (12, 1, 7)])
+@pytest.mark.parametrize("Hq,Hkv,N", [(4, 4, 1), (8, 1, 1), (6, 2, 5), (12, 1, 7), (6, 2, 1), (4, 2, 2),
+                                      (32, 2, 1), (34, 2, 1)])
 @pytest.mark.parametrize("four,D", [(True, 32), (True, 64), (True, 96), (True, 128), (True, 160), (True, 256),
                                     (False, 8), (False, 40), (False, 64), (False, 80), (False, 128), (False, 256)])
 def test_weights_match_float64(four, D, Hq, Hkv, N, dtype, restart):
