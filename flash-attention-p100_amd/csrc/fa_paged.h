@@ -36,7 +36,7 @@ struct PagedKernelArgs {
   int part_rows;    // of a tile: kRows, or all of a kv head's
   // items: of a request, groups of row tiles of each kv head
   int B, Hq, group, N, n_groups, items, causal, window, dr;
-  bool by_item;  // the join's workgroups take an item each
+  bool by_item;  // the kernel's, or the join's, workgroups take an item each
   int runs;  // of 64 or 16 float4 columns in a tile's rows, slice (1 or 2) a join's workgroup
   int slice;
   float scale_log2, rescale, alibi_unit;  // (the last two in units of q . k)
@@ -78,6 +78,9 @@ struct Line {
   int lead;            // units of an item beside its blocks
   int total, stretch;  // all units, and those of a workgroup
 
+  // A line of one item's `units`.
+  __device__ __forceinline__ Line(const PagedKernelArgs& a, int lane, int units)
+      : a(a), lane(lane), lens(0), c0(0), per(1), through(units), lead(0), total(units), stretch(units) {}
   __device__ __forceinline__ Line(const PagedKernelArgs& a, int lane)
       : a(a), lane(lane), lens(0), c0(a.B > 64 ? -64 : 0), per((a.B + 63) / 64) {
     int mine = 0;

@@ -4,7 +4,8 @@
 // reference, which has no cache.
 //
 // As in fa_paged.hip the key blocks of all requests lie on one line that the waves
-// divide evenly, and the parts of an item meet in LDS and in paged_merge_kernel. A
+// divide evenly, and the parts of an item meet in LDS and in paged_merge_kernel (few short
+// items take a workgroup each, and meet in LDS alone). A
 // wave's step is a block of 64 keys for RT tiles of 16 query rows, on
 // v_mfma_f32_16x16x32_bf16: S^T = K Q^T, then O^T += V^T P^T. Every value of the cache is
 // exact in bf16 (a sign, two bits and an exponent), whatever q's format, and
@@ -102,14 +103,17 @@ __global__ __launch_bounds__(T::kThreads) void paged4_kernel(const Paged4Args a)
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
   __builtin_assume(wave >= 0 && wave < kWaves);
-  const int wg = xcd_work_index(T::kGrid);
+  const int wg = a.by_item ? (int)blockIdx.x : xcd_work_index(T::kGrid);
   const int l16 = lane & 15, g = lane >> 4;
-  Line<T> line(a, lane);
-  if (wg == 0 && tid == 0) {
+  // by_item: an item to a workgroup, whose waves meet in LDS. Else the line.
+  int b = a.by_item ? wg / a.items : 0, item = wg - b * a.items, start = 0;
+  Keys<T> keys(a, a.by_item ? a.kv_len[b] : 0);
+  Line<T> line = a.by_item ? Line<T>(a, lane, keys.blocks) : Line<T>(a, lane);
+  if (!a.by_item && wg == 0 && tid == 0) {
     a.sizes[0] = line.stretch;
     a.sizes[1] = line.total;
   }
-  const int wg0 = wg * line.stretch, wg1 = min(wg0 + line.stretch, line.total);
+  const int wg0 = a.by_item ? 0 : wg * line.stretch, wg1 = min(wg0 + line.stretch, line.total);
   int4 owned = make_int4(0, 0, 0, 0);  // request, item, its start and units (none: 0)
   if (wg0 >= wg1) {
     if (lane == 0) a.owned[wg * kLine + wave] = owned;
@@ -118,12 +122,13 @@ __global__ __launch_bounds__(T::kThreads) void paged4_kernel(const Paged4Args a)
   const bool single = line.stretch < kLine;
   int pos = min(wg0 + (single ? wave : wave * line.stretch / kLine), wg1);
   const int end = min(wg0 + (single ? wave + 1 : (wave + 1) * line.stretch / kLine), wg1);
-  int b, start;
-  line.locate(min(pos, wg1 - 1), b, start);
-  Keys<T> keys = line.keys(b);
-  int item = (min(pos, wg1 - 1) - start) / line.units(keys);
-  start += item * line.units(keys);  // of the item, from here on
-  const bool joins = T::joins(line.stretch, line.total, a.B * a.items);
+  if (!a.by_item) {
+    line.locate(min(pos, wg1 - 1), b, start);
+    keys = line.keys(b);
+    item = (min(pos, wg1 - 1) - start) / line.units(keys);
+    start += item * line.units(keys);  // of the item, from here on
+  }
+  const bool joins = a.by_item || T::joins(line.stretch, line.total, a.B * a.items);
   const bool join = joins && start <= wg0 && wg1 <= start + line.units(keys);
   if (!join && pos == end) {
     if (lane == 0) a.owned[wg * kLine + wave] = owned;
@@ -548,7 +553,7 @@ __global__ __launch_bounds__(T::kThreads) void paged4_kernel(const Paged4Args a)
     // + cb) * 64 + lane.
     const bool whole = wg1 - wg0 == units;
     if (whole) owned.w = 0;
-    if (lane == 0) ra.owned[wg * kLine + wave] = owned;
+    if (lane == 0 && !ra.by_item) ra.owned[wg * kLine + wave] = owned;
     slot = 2 * (size_t)(wg * kLine);
     constexpr int kRuns = D / 16;
     __syncthreads();
@@ -627,15 +632,24 @@ hipError_t launch_paged4_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
       d.code_bytes = (uint32_t)code_bytes;
       d.scale_bytes = (uint32_t)(scale_bytes + 6) & ~3u;  // (of whole words, from the first's)
     }
+    // Where a table holds two blocks of a request for each of a workgroup's waves at most, and
+    // the card has a CU for every item: an item to a workgroup, and no parts to join. (H=16/8
+    // D=128, us with the call's host, against the line: one request of 200 keys 7.9 and 10.6, of
+    // 1021 10.8 and 11.6, of 1500 13.3 and 10.9; 32 of 1000 13.2 and 17.8, 128 of 500 34.7
+    // and 26.0.)
+    const long long items = (long long)a.B * d.items;
+    const int most = d.window > 0 ? min(d.cap, d.window + a.N + T::kKeys) : d.cap;
+    d.by_item = items <= kCUs && most <= 2 * T::kLine * T::kKeys;
     auto launch = [&](auto full) {
       constexpr bool kFull = decltype(full)::value;
       constexpr bool kStream = T::kRowTiles == 1;
       const auto kernel = pages == 1   ? paged4_kernel<T, kFull, 1, kStream>
                           : pages == 2 ? paged4_kernel<T, kFull, 2, kStream>
                                        : paged4_kernel<T, kFull, 0, kStream>;
-      hipLaunchKernelGGL(kernel, dim3(T::kGrid), dim3(T::kThreads), 0, (hipStream_t)a.stream, d);
+      hipLaunchKernelGGL(kernel, dim3(d.by_item ? (unsigned)items : T::kGrid), dim3(T::kThreads), 0,
+                         (hipStream_t)a.stream, d);
       const hipError_t e = hipGetLastError();
-      return e != hipSuccess ? e : launch_paged_join<T, kFull>(d, (hipStream_t)a.stream);
+      return e != hipSuccess || d.by_item ? e : launch_paged_join<T, kFull>(d, (hipStream_t)a.stream);
     };
     if constexpr (T::kD == 256)
       if (a.D != T::kD) return launch(std::false_type{});

@@ -216,6 +216,11 @@ def run(q, caches, table, lens, **kw):
                            return_lse=True, k_scale=ks, v_scale=vs, **kw)
 
 
+def long_table(table, page):
+    """One for requests so long that several workgroups would share an item."""
+    return torch.nn.functional.pad(table, (0, 20000 // page), value=2 ** 30)
+
+
 LENGTHS = [1, 63, 64, 65, 0, 700, 129, 17]
 
 
@@ -224,13 +229,15 @@ LENGTHS = [1, 63, 64, 65, 0, 700, 129, 17]
                                       (8, 2, 9), (64, 1, 1), (12, 1, 7), (32, 1, 5)])
 @pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
 def test_attention_matches_float64(D, Hq, Hkv, N, dtype):
-    """Each row tiling (1, 2, 4 tiles of 16, several groups of them) at each width."""
+    """Each row tiling (1, 2, several groups of 2 tiles of 16) at each width, items of a workgroup
+    and on the line."""
     page = {32: 1, 64: 16, 96: 8, 128: 32, 160: 2, 192: 4, 224: 64, 256: 16}[D]
     caches, k, v, table = cache_of(len(LENGTHS), Hkv, D, page, LENGTHS, seed=D + N)
     hide_rest(caches, table, LENGTHS, page)
     q = rows((len(LENGTHS), Hq, N, D), DTYPES[dtype], 9)
-    o, lse = run(q, caches, table, LENGTHS)
-    paged_ref.check(o, lse, paged4_ref.attention(q, k, v, table, LENGTHS))
+    want = paged4_ref.attention(q, k, v, table, LENGTHS)
+    for t in (table, long_table(table, page)):
+        paged_ref.check(*run(q, caches, t, LENGTHS), want)
 
 
 @pytest.mark.parametrize("layout", ["bhnd", "bnhd", "inner"])
@@ -244,11 +251,13 @@ def test_options(D, dtype, causal, window, alibi, scale, layout):
     hide_rest(caches, table, lens, 16)
     q = rows((6, 3, 10, D), DTYPES[dtype], 9).transpose(1, 2)  # (B, 10 heads, 3 rows)
     slopes = torch.linspace(-0.1, 0.5, 10, device=DEV) if alibi else None
-    o, lse = run(q, caches, table, lens, causal=causal, sliding_window=window, alibi_slopes=slopes,
-                 softmax_scale=scale)
-    assert o.shape == q.shape and o.stride() == q.stride()
-    paged_ref.check(o, lse, paged4_ref.attention(q, k, v, table, lens, causal=causal, window=window,
-                                                 alibi=slopes, scale=scale))
+    want = paged4_ref.attention(q, k, v, table, lens, causal=causal, window=window, alibi=slopes,
+                                scale=scale)
+    for t in (table, long_table(table, 16)):
+        o, lse = run(q, caches, t, lens, causal=causal, sliding_window=window, alibi_slopes=slopes,
+                     softmax_scale=scale)
+        assert o.shape == q.shape and o.stride() == q.stride()
+        paged_ref.check(o, lse, want)
 
 
 @pytest.mark.parametrize("B,Hq,Hkv,N,D,top,page", [(1, 8, 1, 1, 128, 20000, 16), (1, 16, 2, 2, 256, 8000, 8),
