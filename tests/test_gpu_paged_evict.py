@@ -245,6 +245,36 @@ def test_evict_with_pages_outside_the_pool():
         check_evict(arrays, w, table, lens, keep, 30)
 
 
+@pytest.mark.parametrize("four", [True, False])
+def test_pages_past_32_bits(four):
+    """Pools of more than 2^32 bytes: as in a small one, with the same pages near the end."""
+    Hkv, page, D, n = 8, 256, 256, 700
+    row = [D // 2, D // 2, D // 32, D // 32] if four else [D, D]
+    dtype = torch.uint8 if four else torch.bfloat16
+    P = (1 << 32) // (Hkv * page * D // (2 if four else 1)) + 9
+    ends = torch.tensor([P - 1, P - 4, P - 2], device=DEV)
+    if four:
+        small = [torch.randint(1, 120, (3, Hkv, page, w), dtype=dtype, device=DEV) for w in row]
+    else:
+        small = [rows((3, Hkv, page, w), dtype, w) for w in row]
+    w = rows((3, Hkv, page), torch.float32, 7).abs()
+    q, lens = rows((1, 16, 3, D), torch.bfloat16, 5), torch.tensor([n], dtype=torch.int32, device=DEV)
+    lse = torch.full((1, 16, 3), 6.0, device=DEV)
+
+    def step(arrays, w, table):
+        four_args = dict(k_scale=arrays[2], v_scale=arrays[3]) if four else {}
+        fa().paged_weights(q, arrays[0], table, lens, lse, w, k_scale=arrays[2] if four else None)
+        fa().paged_evict(arrays[0], arrays[1], w, table, lens, 300, recent=9, **four_args)
+
+    large = [torch.empty(P, *x.shape[1:], dtype=x.dtype, device=DEV) for x in (*small, w)]
+    for x, y in zip(large, (*small, w)):
+        x[ends] = y
+    step(large[:-1], large[-1], ends[None].to(torch.int32))
+    step(small, w, torch.arange(3, dtype=torch.int32, device=DEV)[None])
+    for x, y in zip(large, (*small, w)):
+        assert torch.equal(x[ends].contiguous().view(torch.uint8), y.view(torch.uint8))
+
+
 def test_evict_captured_and_on_another_stream():
     lens = [500, 80, 333]
     case = evict_case(True, 3, 2, 128, 16, lens, 5)
