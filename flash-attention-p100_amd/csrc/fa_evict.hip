@@ -3,21 +3,21 @@
 // (fa_weights.hip), in their order at the front of its pages. No counterpart in the
 // reference, which has no cache.
 //
-// Three launches. evict_select_kernel, a workgroup per request and kv head, finds the
-// least weight that is kept by its bits, eight at a time from the highest (a histogram
-// of the weights that agree with it so far), then lists the kept tokens in order. Their
-// rows, scales and weights then move by that list in two:
-//   * tokens from within the kept length L move in place, by a workgroup per request, kv
-//     head, pool and slice of a row. Kept token number r comes from a token i >= r, so
-//     tiles of rows in order are safe: a tile's rows are all read before they are
-//     written, and what it writes lies at or before what it read, below all that the
-//     tiles behind it read;
+// evict_select_kernel, a workgroup per request and kv head, finds the least weight that is
+// kept by its bits, eight at a time from the highest (a histogram of the weights that agree
+// with it so far), then lists the kept tokens in order. Their rows, scales and weights then
+// move by that list. Kept token number r comes from a token i >= r, so tiles of rows in
+// order are safe: a tile's rows are all read before they are written, and what it writes
+// lies at or before what it read, below all that the tiles behind it read. Where there is a
+// kv head for every CU, or little to move, the same workgroup goes over the tiles; else two
+// more launches take what workgroups can share:
+//   * tokens from within the kept length L, by a workgroup per pool and slice of a row;
 //   * tokens from behind L: nothing writes there, and what their places held has moved,
 //     so all of them move at once.
 // Bound by HBM where many rows move: 32 requests of 8 kv heads of about 1024 rows of 256
-// bytes, 270 MB read and written, take 55 us (5 TB/s) after 10 us of selecting; 4 requests
-// of 16384 to 32768 tokens of which 4096 stay, 26 us of selecting (half of that reading
-// 2 MB of weights and counting: one CU to a kv head) and 45 us of moving 134 MB.
+// bytes, 270 MB read and written, take 50 to 80 us, 10 of them selecting; 4 requests of
+// 16384 to 32768 tokens of which 4096 stay, 26 us of selecting (half of that reading 2 MB
+// of weights and counting: one CU to a kv head) and 45 us of moving 134 MB.
 #include <algorithm>
 
 #include "fa_device.h"
@@ -252,24 +252,6 @@ __device__ __forceinline__ void select(const EvictArgs& a, const Budget& q, int 
   }
 }
 
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictArgs a) {
-  __shared__ SelectLds lds;
-  const int b = blockIdx.x / a.Hkv, h = blockIdx.x - b * a.Hkv;
-  const Budget q(a, b);
-  if (h == 0 && threadIdx.x == 0) a.new_len[b] = q.kept;
-  if (!q.over()) return;
-  if (q.len <= kHeld)
-    select<true>(a, q, b, h, lds);
-  else
-    select<false>(a, q, b, h, lds);
-}
-
-// ---------------------------------------------------------------------------
-constexpr int kMoveThreads = 1024, kMoveRows = 8;  // rows of a tile that a thread moves
-// Bytes of a row that a workgroup moves. (4 requests of 8 kv heads that keep 4096 rows of
-// 256 bytes, 128 -> 64 -> 32: 53 -> 29 -> 36 us; 32 requests of 1024 rows: 55, 58, 85.)
-constexpr int kSlice = 64;
-
 // Where a kv head's tokens have something; null where a token has no page.
 template <typename T>
 struct Places {
@@ -293,6 +275,74 @@ __device__ __forceinline__ Places<uint8_t> scales_of(const EvictArgs& a, int b, 
 __device__ __forceinline__ Places<float> weights_of(const EvictArgs& a, int b, int h) {
   return {a.weights.w + h * a.weights.head_stride, a.weights.page_stride, a.weights.row_stride, Table(a, b)};
 }
+
+// Moves a kv head's kept tokens, rows, scales and weights together, tile by tile in order.
+// An item is 16 bytes of a row and the scale of its 32 values (both are `lanes` to a row).
+constexpr int kItems = 8;  // of a tile that a thread moves
+__device__ __forceinline__ void move_all(const EvictArgs& a, int b, int h, int kept_count, const int* kept,
+                                         int lanes_log2) {
+  const int tid = threadIdx.x, c = tid & ((1 << lanes_log2) - 1), v = tid >> lanes_log2 & 1;
+  const int at_once = kSelThreads >> (lanes_log2 + 1), row0 = tid >> (lanes_log2 + 1);
+  const auto rows = rows_of(a, b, h, v, 16 * c);
+  const auto scales = scales_of(a, b, h, v);
+  const auto weights = weights_of(a, b, h);
+  const bool live = 16 * c < a.row_bytes, scaled = live && a.scale_bytes > 0, weighed = c == 0 && v == 0;
+  for (int r0 = kept[0]; r0 < kept_count; r0 += kItems * at_once) {
+    u32x4 x[kItems];
+    uint8_t scale[kItems];
+    float weight[kItems];
+    uint32_t there = 0;
+#pragma unroll
+    for (int e = 0; e < kItems; ++e) {
+      const int r = r0 + e * at_once + row0;
+      if (r < kept_count && live) {
+        const int i = kept[kHead + r];
+        const uint8_t* const from = rows.at(i);
+        if (from) {
+          there |= 1u << e;
+          x[e] = *reinterpret_cast<const u32x4*>(from);
+          if (scaled) scale[e] = scales.at(i)[c];
+          if (weighed) weight[e] = *weights.at(i);
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kItems; ++e) {
+      const int r = r0 + e * at_once + row0;
+      uint8_t* const to = there >> e & 1 ? rows.at(r) : nullptr;
+      if (to) {
+        *reinterpret_cast<u32x4*>(to) = x[e];
+        if (scaled) scales.at(r)[c] = scale[e];
+        if (weighed) *weights.at(r) = weight[e];
+      }
+    }
+  }
+}
+
+// ALL: moves them as well.
+template <bool ALL>
+__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictArgs a, int lanes_log2) {
+  __shared__ SelectLds lds;
+  const int b = blockIdx.x / a.Hkv, h = blockIdx.x - b * a.Hkv;
+  const Budget q(a, b);
+  if (h == 0 && threadIdx.x == 0) a.new_len[b] = q.kept;
+  if (!q.over()) return;
+  if (q.len <= kHeld)
+    select<true>(a, q, b, h, lds);
+  else
+    select<false>(a, q, b, h, lds);
+  if constexpr (ALL) {
+    __syncthreads();
+    move_all(a, b, h, q.kept, kept_of(a, blockIdx.x), lanes_log2);
+  }
+}
+
+// ---------------------------------------------------------------------------
+constexpr int kMoveThreads = 1024, kMoveRows = 8;  // rows of a tile that a thread moves
+// Bytes of a row that a workgroup moves. (4 requests of 8 kv heads that keep 4096 rows of
+// 256 bytes, 128 -> 64 -> 32: 53 -> 29 -> 36 us; 32 requests of 1024 rows: 55, 58, 85.)
+constexpr int kSlice = 64;
 
 __global__ __launch_bounds__(kMoveThreads) void evict_inner_kernel(const EvictArgs a, int slices) {
   const int head = blockIdx.x, b = head / a.Hkv, h = head - b * a.Hkv;
@@ -426,16 +476,21 @@ size_t evict_workspace_bytes(int B, int Hkv, int table_width, int page_size) {
 hipError_t launch_paged_evict(const EvictArgs& a, void* stream) {
   const unsigned heads = (unsigned)(a.B * a.Hkv);
   const long long cap = (long long)a.table_width << a.pool.page_shift;
-  hipLaunchKernelGGL(evict_select_kernel, dim3(heads), dim3(kSelThreads), 0, (hipStream_t)stream, a);
+  int lanes_log2 = 0;
+  while (16 << lanes_log2 < a.row_bytes) ++lanes_log2;
+  // A launch for all where every CU has a kv head, or these are small. (Rows of 256 bytes, us
+  // for one launch and for three: 32 requests of 8 heads of up to 1100 tokens 73 and 73, 64 of
+  // 2000 151 and 179, 4 of 300 14.6 and 17.4; 16 of 2200 113 and 73, 1 of 2000 22 and 16.)
+  const bool all = heads >= (unsigned)kCUs || cap * 2 * a.row_bytes <= 1 << 18;
+  const auto select = all ? evict_select_kernel<true> : evict_select_kernel<false>;
+  hipLaunchKernelGGL(select, dim3(heads), dim3(kSelThreads), 0, (hipStream_t)stream, a, lanes_log2);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || all) return e;
   const int slices = (a.row_bytes + kSlice - 1) / kSlice;
   hipLaunchKernelGGL(evict_inner_kernel, dim3(heads, (unsigned)(2 * slices + 1 + (a.scales.k ? 2 : 0))),
                      dim3(kMoveThreads), 0, (hipStream_t)stream, a, slices);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  int lanes_log2 = 0;
-  while (16 << lanes_log2 < a.row_bytes) ++lanes_log2;
   // (no more workgroups than there can be units for)
   const long long most = ((2 * cap << lanes_log2) + 1023) / 1024;
   const long long fill = ((long long)kOuter * kCUs + heads - 1) / heads;

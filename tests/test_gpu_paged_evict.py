@@ -195,13 +195,20 @@ def check_evict(arrays, w, table, lens, max_len, recent):
                                              (False, 72, 16, 3), (False, 128, 16, 8), (False, 256, 128, 1)])
 def test_evict_keeps_the_newest_and_heaviest(four, D, page, Hkv, layout, ties):
     lens = [1, 2, 0, 65, 700, 129, 300, 17]
-    case = evict_case(four, len(lens), Hkv, D, page, lens, D, layout=layout, ties=ties)
-    for max_len, recent in ((299, 16), ([0, 1, 5, 64, 100, 129, -4, 3], 2), (40, 1000), (7, 0)):
-        check_evict(*case, lens, max_len, recent)
+    arrays, w, table = evict_case(four, len(lens), Hkv, D, page, lens, D, layout=layout, ties=ties)
+    # (of a longer table: in several launches)
+    long_table = torch.nn.functional.pad(table, (0, 20000 // page), value=2 ** 30)
+    kept = [t.clone() for t in (*arrays, w)]
+    for t in (table, long_table):
+        for x, y in zip((*arrays, w), kept):
+            x.copy_(y)
+        for max_len, recent in ((299, 16), ([0, 1, 5, 64, 100, 129, -4, 3], 2), (40, 1000), (7, 0)):
+            check_evict(arrays, w, t, lens, max_len, recent)
 
 
 @pytest.mark.parametrize("B,Hkv,top,keep,recent", [(1, 2, 60000, 5000, 64), (1, 1, 9000, 8999, 0), (1, 8, 4097, 4096, 4095),
-                                                   (40, 2, 1500, 200, 100), (130, 1, 90, 30, 8), (2, 1, 20000, 17000, 7)])
+                                                   (40, 2, 1500, 200, 100), (130, 1, 90, 30, 8), (2, 1, 20000, 17000, 7),
+                                                   (140, 2, 2500, 900, 50)])
 @pytest.mark.parametrize("four", [True, False])
 def test_evict_long_and_many(B, Hkv, top, keep, recent, four):
     lens = [max(1, int(top * ((0.5 + 0.618034 * i) % 1.0))) for i in range(B)]
