@@ -276,6 +276,13 @@ __device__ __forceinline__ Places<float> weights_of(const EvictArgs& a, int b, i
   return {a.weights.w + h * a.weights.head_stride, a.weights.page_stride, a.weights.row_stride, Table(a, b)};
 }
 
+// What the workgroup's waves have loaded and stored is done: what was read may be written, and
+// what was written read. (A barrier alone orders what is issued, and waits for neither.)
+__device__ __forceinline__ void all_done() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
 // Moves a kv head's kept tokens, rows, scales and weights together, tile by tile in order.
 // An item is 16 bytes of a row and the scale of its 32 values (both are `lanes` to a row).
 constexpr int kItems = 8;  // of a tile that a thread moves
@@ -306,7 +313,7 @@ __device__ __forceinline__ void move_all(const EvictArgs& a, int b, int h, int k
         }
       }
     }
-    __syncthreads();
+    all_done();
 #pragma unroll
     for (int e = 0; e < kItems; ++e) {
       const int r = r0 + e * at_once + row0;
@@ -333,7 +340,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictAr
   else
     select<false>(a, q, b, h, lds);
   if constexpr (ALL) {
-    __syncthreads();
+    all_done();
     move_all(a, b, h, q.kept, kept_of(a, blockIdx.x), lanes_log2);
   }
 }
@@ -366,7 +373,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_inner_kernel(const EvictAr
         x[e] = from ? *reinterpret_cast<const u32x4*>(from) : u32x4{0u, 0u, 0u, 0u};
         there |= (from ? 1u : 0u) << e;
       }
-      __syncthreads();
+      all_done();
 #pragma unroll
       for (int e = 0; e < kMoveRows; ++e) {
         uint8_t* to = there >> e & 1 ? rows.at(r0 + e * kAtOnce + tid / kLanes) : nullptr;
@@ -387,7 +394,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_inner_kernel(const EvictAr
         x[e] = from ? *from : 0.f;
         there |= (from ? 1u : 0u) << e;
       }
-      __syncthreads();
+      all_done();
 #pragma unroll
       for (int e = 0; e < kMoveRows; ++e) {
         float* to = there >> e & 1 ? weights.at(r0 + e * kMoveThreads + tid) : nullptr;
@@ -404,7 +411,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_inner_kernel(const EvictAr
     uint8_t x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = from && e < a.scale_bytes ? from[e] : 0;
-    __syncthreads();
+    all_done();
     uint8_t* to = from ? scales.at(r) : nullptr;
     if (to)
 #pragma unroll
