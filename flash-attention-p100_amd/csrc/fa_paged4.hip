@@ -194,9 +194,11 @@ __global__ __launch_bounds__(T::kThreads) void paged4_kernel(const Paged4Args a)
     struct Place {
       uint32_t code, scale[kScales], bit[kScales];
       int second;        // the page of a tile that the key is in
+      uint32_t back;     // how far before its first scale the row begins, or 2 bytes
       bool there, both;  // whether the quarter begins, and ends, within the head dim
       __device__ __forceinline__ Place(int key, int part, uint32_t row_bytes, uint32_t scale_row, int dr,
-                                       uint32_t sub) : second(0) {
+                                       uint32_t sub)
+          : second(0), back(part ? 2u : 0u) {
         if (PAGES == 2) {
           second = key >> 3;
           key &= 7;
@@ -281,8 +283,16 @@ __global__ __launch_bounds__(T::kThreads) void paged4_kernel(const Paged4Args a)
            },
            [&](int i, Codes& x) {
              const uint8_t* word = scales + at.scale[i];
-             x.bit[i % (kBits + 1)] = 8u * (uint32_t)((uintptr_t)word & 3u);
-             return *reinterpret_cast<const uint32_t*>(word - ((uintptr_t)word & 3u));
+             uint32_t before = (uint32_t)((uintptr_t)word & 3u);
+             // (Two scales of which the second lies behind the word: a word from an odd byte
+             // on, within the row. Such words alone take longer, 53.7 us for 51 at B=16 H=32/8
+             // N=1 D=256, 4000 keys in pages of 4; each scale by its own word spills more.)
+             if constexpr (D == 256 && FULL)
+               if (before == 3) before = at.back;
+             x.bit[i % (kBits + 1)] = 8u * before;
+             uint32_t w;
+             __builtin_memcpy(&w, word - before, 4);
+             return w;
            });
     };
     // Block j's K or V, or, where it is not live, a row of its memory, not used: a branch
@@ -618,7 +628,8 @@ hipError_t launch_paged4_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
     d.scale_head = a.scales.head_stride;
     d.scale_row = a.scales.row_stride;
     // Tiles go by 32-bit places in a kv head's rows, and by words of scales that begin at the
-    // same bits in every tile (a lane of width 256 takes two scales, of one word).
+    // same bits in every tile (a lane of width 256 takes two scales, of one word: from an even
+    // byte). Else row by row, by words that hold each row's scales wherever they begin.
     const auto& sc = a.scales;
     const long long code_bytes = (a.pool.pages - 1LL) * a.pool.page_stride +
                                  ((1LL << a.pool.page_shift) - 1) * a.pool.row_stride + a.D / 2;
