@@ -890,9 +890,13 @@ int fa_paged_evict(const fa_paged_cache* cache, const fa_paged_scales* scales, f
     return FA_ERR_NULL;
   if (workspace_bytes < fa::evict_workspace_bytes(B, Hkv, cache->table_width, cache->page_size))
     return FA_ERR_WORKSPACE;
-  // (the lengths are read after the new ones are written)
-  const long long apart = (const char*)new_len - (const char*)cache->kv_len;
-  if (apart > -4LL * B && apart < 4LL * B) return FA_ERR_PAGES;
+  // (Lengths and budgets are read after new lengths are written. A budget that its own new
+  // length has replaced still gives that; another request's does not.)
+  auto apart = [&](const int* p) {
+    const long long bytes = (const char*)new_len - (const char*)p;
+    return bytes <= -4LL * B || bytes >= 4LL * B;
+  };
+  if (!apart(cache->kv_len) || (new_len != max_len && !apart(max_len))) return FA_ERR_PAGES;
   const int pages = a.pool.pages, rows = cache->page_size;
   if (w_stride_page < 0 || w_stride_head < 0 || w_stride_row < 0 ||
       (reinterpret_cast<uintptr_t>(workspace) & 3u) ||

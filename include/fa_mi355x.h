@@ -72,8 +72,8 @@ enum {
                                 sizes are not positive, whose rows are not 16-byte aligned or
                                 (where they are written) overlap, or with an option that paged
                                 attention does not take, or a buffer of its that is not
-                                16-byte aligned; weights that overlap, lengths that eviction
-                                would write where it reads them */
+                                16-byte aligned; weights that overlap, lengths or budgets that
+                                eviction would write where it reads them */
 };
 
 /* Memory layouts of the 16-bit tensors, for the entry points that take one:
@@ -624,9 +624,10 @@ int fa_paged_weights(const void* q, const float* lse, const fa_paged_cache* cach
  * largest weights (of equal ones the older; NaN above all, keys in pages outside the pool
  * below all). What is kept moves to the front of the request's pages in its order, rows,
  * scales and weights alike (places in pages outside the pool are left out); rows behind it
- * keep what they hold. new_len[b], not in kv_len's place, becomes min(kv_len[b],
- * max_len[b]); a call of fa_paged_tables with these as new lengths gives the pages back.
- * Tokens of different kv heads in a row of the pool then differ, and a key's row no longer
+ * keep what they hold. new_len[b] becomes min(kv_len[b], max_len[b]) (kv_len[b] as it is
+ * clamped, at least 0). It may take max_len's own place (new_len == max_len), and lies apart
+ * from kv_len and max_len otherwise. A call of fa_paged_tables with these as new lengths
+ * gives the pages back. Tokens of different kv heads in a row of the pool then differ, and a key's row no longer
  * says its position: what counts distances (windows, ALiBi) counts kept tokens. scales NULL:
  * rows of 16 bits, else of 4. The pools' rows, the scales and the weights must lie apart; a page is one
  * request's. `workspace` has fa_paged_evict_workspace_bytes() bytes, 4-byte aligned (a

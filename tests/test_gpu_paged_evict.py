@@ -2,6 +2,7 @@
 float64 with their bound, evictions bit for bit (paged4_ref.py), and all operators of the
 smaller caches together as a serving loop runs them. No counterpart in the reference, which
 has no cache."""
+import ctypes
 import math
 
 import pytest
@@ -420,3 +421,29 @@ def test_a_serving_loop_with_a_budget(four, dtype):
         assert torch.equal(lens, cut)
     held = sum(-(-int(n) // page) for n in lens)
     assert int(ring[1]) == P - held
+
+
+@pytest.mark.parametrize("width", [1, 4000])
+def test_new_lengths_in_the_budgets_place(width):
+    """By the C entry: in one launch and in three, with several kv heads to a request."""
+    from test_paged4_cpu import capi4
+    from test_paged_cpu import Cache
+    lens, budget = [700, 3, 0, 650, 64, 900], [100, 40, 5, 64, -3, 899]
+    B, Hkv, D, page = len(lens), 3, 64, 16
+    arrays, w, table = evict_case(False, B, Hkv, D, page, lens, 21)
+    table = torch.nn.functional.pad(table, (0, width), value=2 ** 30)
+    want, want_w = [a.cpu() for a in arrays], w.cpu()
+    new = paged4_ref.evict(want, want_w, table, lens, budget, 16)
+    n, both = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (lens, budget))
+    t = table.to(DEV)
+    lib = capi4()
+    nbytes = lib.fa_paged_evict_workspace_bytes(B, Hkv, t.size(1), page)
+    ws = torch.full((nbytes,), 0x7f, dtype=torch.uint8, device=DEV)
+    cache = Cache(arrays[0].data_ptr(), arrays[1].data_ptr(), *arrays[0].stride()[:3], arrays[0].size(0), page,
+                  t.data_ptr(), t.size(1), t.size(1), n.data_ptr())
+    assert lib.fa_paged_evict(ctypes.byref(cache), None, w.data_ptr(), *w.stride(), both.data_ptr(), 16,
+                              both.data_ptr(), ws.data_ptr(), nbytes, B, Hkv, D,
+                              torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(both.cpu(), new)
+    for a, b in zip((*arrays, w), (*want, want_w)):
+        assert torch.equal(a.cpu(), b)

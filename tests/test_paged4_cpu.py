@@ -165,6 +165,23 @@ def test_evict_refusals():
         assert lib.fa_paged_evict_workspace_bytes(*bad) == 0, bad
 
 
+def test_evict_refuses_new_lengths_across_the_budgets():
+    """Budgets are read by all kv heads while new lengths are written: these may lie in their
+    place, which changes nothing that is read, but not shifted against them."""
+    lib = capi4()
+    B = 4
+
+    def call(max_len, new, kv_len=1 << 27):
+        return lib.fa_paged_evict(cache4(kv_len=kv_len), scales(), 16, 32, 16, 1, max_len, 0, new, 16,
+                                  1 << 40, B, 2, 64, None)
+
+    at = 1 << 26
+    for off in range(4, 4 * B, 4):
+        assert call(at, at + off) == 10019 and call(at, at - off) == 10019, off
+    for off in (0, 4 * B - 4, -4):  # in the lengths' place, or across it
+        assert call(1 << 28, at + off, kv_len=at) == 10019, off
+
+
 def test_binding_refuses_host_tensors_and_bad_arguments():
     import fa_p100
     ints, lens = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
