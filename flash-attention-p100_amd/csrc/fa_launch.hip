@@ -4,6 +4,7 @@
 #include <limits.h>
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "fa_device.h"
@@ -397,15 +398,25 @@ hipError_t launch_bwd_main(const BwdArgs& a) {
   });
 }
 
-size_t paged_workspace_bytes(int rows, int D) {
+// A workspace that holds what either format's kernels lay out in it: of(width, bf) is a
+// format's size. (The size is asked for without a format.)
+template <typename Of>
+static size_t larger_format(int D, const Of& of) {
   FwdArgs a{};
   a.D = D;
   size_t n = 0;
-  (void)by_width(a, false, [&](auto w, auto bf, const FwdArgs&) {
-    n = paged_workspace_w<decltype(w)::value, decltype(bf)::value>(rows);
-    return hipSuccess;
-  });
+  for (const bool bf : {false, true})
+    (void)by_width(a, bf, [&](auto w, auto bf, const FwdArgs&) {
+      n = std::max(n, of(w, bf));
+      return hipSuccess;
+    });
   return n;
+}
+
+size_t paged_workspace_bytes(int rows, int D) {
+  return larger_format(D, [&](auto w, auto bf) {
+    return paged_workspace_w<decltype(w)::value, decltype(bf)::value>(rows);
+  });
 }
 
 hipError_t launch_paged(const PagedArgs& a) {
@@ -414,16 +425,10 @@ hipError_t launch_paged(const PagedArgs& a) {
   });
 }
 
-// (bf16's: its tiles hold as many rows as fp16's or more)
 size_t paged4_workspace_bytes(int rows, int D) {
-  FwdArgs a{};
-  a.D = D;
-  size_t n = 0;
-  (void)by_width(a, true, [&](auto w, auto bf, const FwdArgs&) {
-    n = paged4_workspace_w<decltype(w)::value, decltype(bf)::value>(rows);
-    return hipSuccess;
+  return larger_format(D, [&](auto w, auto bf) {
+    return paged4_workspace_w<decltype(w)::value, decltype(bf)::value>(rows);
   });
-  return n;
 }
 
 hipError_t launch_paged4(const PagedArgs& a) {

@@ -1,12 +1,14 @@
 """The smaller paged caches' argument checks that need no GPU (nothing is launched), and
 their plain restatements against second ones. No counterpart in the reference."""
 import ctypes
+import subprocess
+import sys
 
 import pytest
 import torch
 
 import paged4_ref
-from helpers import fa_opts
+from helpers import LIB, fa_opts
 from test_paged_cpu import cache, capi
 
 
@@ -117,6 +119,21 @@ def test_attn_refusals():
     # what the header says that it is at most
     most = max(lib.fa_paged4_attn_workspace_bytes(1, 64, 1, n, D) for n in (1, 2) for D in (32, 64, 96, 128, 160, 256))
     assert most <= 68.5e6
+
+
+@pytest.mark.parametrize("entry,units", [("fa_paged_attn", "17paged_workspace_w"), ("fa_paged4_attn", "18paged4_workspace_w")])
+@pytest.mark.parametrize("bf", [0, 1])
+def test_workspace_is_the_larger_format_s(entry, units, bf, tmp_path):
+    """Each format's kernels lay the workspace out for themselves, and the size that a caller
+    asks for holds either: where one format's needs more, that (here what a stub in the place of
+    that format's answer says, loaded ahead of the library in a process of its own)."""
+    stub, need = tmp_path / "stub.so", 1 << 40
+    code = f'extern "C" unsigned long _ZN2fa{units}ILi128ELb{bf}EEEmi(int) {{ return {need}ul; }}'
+    subprocess.run(["g++", "-shared", "-fPIC", "-x", "c++", "-", "-o", stub], input=code.encode(), check=True)
+    ask = (f"import ctypes; ctypes.CDLL({str(stub)!r}, ctypes.RTLD_GLOBAL); "
+           f"f = ctypes.CDLL({LIB!r}).{entry}_workspace_bytes; f.restype = ctypes.c_size_t; "
+           "print(f(1, 4, 2, 1, 128))")
+    assert int(subprocess.run([sys.executable, "-c", ask], check=True, capture_output=True).stdout) == need
 
 
 def test_weights_refusals():
