@@ -14,10 +14,11 @@
 //   * tokens from within the kept length L, by a workgroup per pool and slice of a row;
 //   * tokens from behind L: nothing writes there, and what their places held has moved,
 //     so all of them move at once.
-// Bound by HBM where many rows move: 32 requests of 8 kv heads of about 1024 rows of 256
-// bytes, 270 MB read and written, take 50 to 80 us, 10 of them selecting; 4 requests of
-// 16384 to 32768 tokens of which 4096 stay, 26 us of selecting (half of that reading 2 MB
-// of weights and counting: one CU to a kv head) and 45 us of moving 134 MB.
+// Bound by HBM where many rows move: 32 requests of 8 kv heads of 1100 rows of 256 bytes of
+// which 1024 stay, 270 MB read and written, take 54 us, 10 of them selecting (in 4 bits, 71
+// MB: 22 us); 4 requests of 16384 to 32768 tokens of which 4096 stay, 28 us of selecting
+// (half of that reading 3 MB of weights and counting: one CU to a kv head) and 12 + 43 us of
+// moving 134 MB (in 4 bits, 36 MB: 27, 10 + 26).
 #include <algorithm>
 
 #include "fa_device.h"
@@ -71,7 +72,10 @@ struct Table {
   }
 };
 
-// HOLD: up to kHeld tokens, whose keys are made once and stay in registers.
+// HOLD: up to kHeld tokens, whose keys are made once and stay in registers, 32 a thread. Of
+// longer requests weights are read again for each of the four digits and for the list, a
+// chunk at a time: two kv heads of 32768 tokens are selected in 26 us, of 33000 in 50, of
+// 65536 in 84, of 131072 in 166. (More registers, or several chunks in flight there: not tried.)
 constexpr int kHeldChunks = 8, kChunk = kSelThreads * kPer, kHeld = kHeldChunks * kChunk;
 struct SelectLds {
   __attribute__((aligned(16))) int hist[256 * kCopies];

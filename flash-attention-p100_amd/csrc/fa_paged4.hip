@@ -644,7 +644,8 @@ hipError_t launch_paged4_w<FA_WIDTH, FA_BF>(const PagedArgs& a) {
       d.scale_bytes = (uint32_t)(scale_bytes + 6) & ~3u;  // (of whole words, from the first's)
     }
     // Where a table holds two blocks of a request for each of a workgroup's waves at most, and
-    // the card has a CU for every item: an item to a workgroup, and no parts to join. (H=16/8
+    // the card has a CU for every item: an item to a workgroup, and no parts to join. (It is the
+    // table that counts, 1024 tokens at D <= 128 and 512 above: lengths are the device's. H=16/8
     // D=128, us with the call's host, against the line: one request of 200 keys 7.9 and 10.6, of
     // 1021 10.8 and 11.6, of 1500 13.3 and 10.9; 32 of 1000 13.2 and 17.8, 128 of 500 34.7
     // and 26.0.)

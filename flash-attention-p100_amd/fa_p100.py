@@ -545,7 +545,8 @@ def paged_append(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None):
 
     With k_scale and v_scale the cache is of 4 bits, about a quarter of the size: k_cache
     and v_cache are then uint8 (pages, Hkv, page_size, D / 2), D a multiple of 32, and
-    k_scale and v_scale uint8 (pages, Hkv, page_size, D / 32), laid out alike. Value d of a
+    k_scale and v_scale uint8 (pages, Hkv, page_size, D / 32), laid out alike (rows of the
+    codes on 16-byte boundaries, of the scales at any byte). Value d of a
     row is in the low (d even) or high half of byte d // 2: a sign and one of 0, 0.5, 1,
     1.5, 2, 3, 4, 6, times 2^(s - 127) for the scale byte s of its 32 values (255: NaN).
     The scale of 32 values is the least power of two of which their largest magnitude is 7
@@ -679,13 +680,15 @@ def paged_evict(k_cache, v_cache, weights, block_table, kv_len, max_len, recent=
     keeps its newest min(recent, max_len[b]) tokens and, of the others, those of the
     largest weights (paged_weights; of equal ones the older, NaN above all). They move to
     the front of the request's pages, in their order, with their weights and, in a cache of
-    4 bits, scales; the rows behind them keep what they held. The pages they no longer need go back with
+    4 bits, scales; the rows behind them keep what they held. The pages they no longer need
+    go back with
     paged_tables(block_table, kv_len, new_len, free_pages, ring, page_size, max_new=0).
 
     Kept tokens then differ between kv heads, and a key's index no longer is its position:
     keys are cached with their positions already applied, and sliding windows and ALiBi
-    count kept tokens. HIP kernels without a copy to the host; a page is one request's. No
-    gradient, as paged_append.
+    count kept tokens. HIP kernels without a copy to the host, and a workspace during the
+    call of 4 bytes for each request, kv head and token that block_table has room for; a page
+    is one request's. No gradient, as paged_append.
     """
     _paged_inputs("paged_evict", k_cache, v_cache, weights, block_table, kv_len,
                   *_scales(k_scale, v_scale))

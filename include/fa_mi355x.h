@@ -550,8 +550,8 @@ int fa_paged_attn(const void* q, void* o, float* lse, const fa_paged_cache* cach
  * (bits 2 .. 0), a scale byte x stands for 2^(x - 127), 255 for NaN, and is that of 32
  * values in a row (the E2M1 and E8M0 of the OCP microscaling formats). The codes lie in
  * the pools of a struct fa_paged_cache, whose strides then count bytes and are multiples
- * of 16; the scales in two pools of their own, byte strides, the same for both, below
- * 2^31.
+ * of 16; the scales in two pools of their own, which may begin at any byte, byte strides,
+ * the same for both, below 2^31.
  */
 typedef struct fa_paged_scales {
   uint8_t* k;
@@ -631,7 +631,8 @@ int fa_paged_weights(const void* q, const float* lse, const fa_paged_cache* cach
  * says its position: what counts distances (windows, ALiBi) counts kept tokens. scales NULL:
  * rows of 16 bits, else of 4. The pools' rows, the scales and the weights must lie apart; a page is one
  * request's. `workspace` has fa_paged_evict_workspace_bytes() bytes, 4-byte aligned (a
- * token list per request and kv head, for all that a table holds), may hold anything, and
+ * token list per request and kv head, 4 bytes for each token that a table has room for:
+ * 1.07 GB for 256 requests of 8 kv heads with tables of 131072), may hold anything, and
  * serves one call at a time. B * Hkv <= 2^21.
  */
 size_t fa_paged_evict_workspace_bytes(int B, int Hkv, int table_width, int page_size);
